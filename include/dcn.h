@@ -36,10 +36,11 @@
 extern "C" {
 #endif
 
-#define DCN_ABI_VERSION 5 /* 2: dcn_allreduce_grads takes a dtype; dcn_set_comm, dcn_set_grad_stream;
+#define DCN_ABI_VERSION 6 /* 2: dcn_allreduce_grads takes a dtype; dcn_set_comm, dcn_set_grad_stream;
                              3: dcn_backward_host_ex; 4: dcn_host_state, dcn_host_alloc;
                              5: dcn_forward_ex (DCN_FWD_NO_COLUMNS), dcn_get_fwd_path,
-                                dcn_workspace_bytes(DCN_WS_FORWARD_NO_COLUMNS) */
+                                dcn_workspace_bytes(DCN_WS_FORWARD_NO_COLUMNS);
+                             6: dcn_dropout_* */
 
 typedef enum {
   DCN_OK = 0,
@@ -281,6 +282,44 @@ int dcn_roi_pool_fwd_host(dcn_handle* h, const dcn_roi_desc* d, const float* fea
 int dcn_roi_pool_bwd_host(dcn_handle* h, const dcn_roi_desc* d, const float* features,
                           const float* rois, const float* offsets, const float* grad_out,
                           float* grad_features, float* grad_offsets);
+
+/* ---- residual block around a DeformConv2d ------------------------------------- *
+ * What stands between two blocks of a network. No counterpart in the reference, whose
+ * network is DeformConv2d + BatchNorm + ReLU (train.py:304-337).
+ *
+ * Tensors are dense, of the descriptor's dtype (parameters and gradients too), caller-owned
+ * and on the handle's device. A map tensor is DCN_NCHW [B][C][P] or DCN_NHWC [B][P][C]
+ * (token rows: B sequences of P tokens). Sums, statistics and everything between the loads
+ * and the stores are fp32; each output is rounded once. Outputs are bitwise reproducible.
+ * Every call may be captured into a graph. Unlike the entry points above, these leave the
+ * thread's current device as they found it. */
+typedef enum { DCN_NCHW = 0, DCN_NHWC = 1 } dcn_layout;
+
+/* Random bits. Element i draws the 16-bit half (i & 7) of the four words that
+ * Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3")
+ * gives for key = seed and counter = (i >> 3, offset), each 64 bits as two words, low
+ * first. It is dropped where the draw is below T = floor(65536 p + 1/2); what is kept is
+ * scaled by 65536 / (65536 - T), so p is taken to the nearest 1/65536 and the mean stays. A
+ * dropped value is 0 whatever it was (NaN and infinities too). The mask is never stored:
+ * the backward draws it again from the same seed and offset. `rng`, where not NULL, is a
+ * device pointer to two uint64 {seed, offset} (8-byte aligned) read when the kernel runs,
+ * in place of the descriptor's: a captured graph draws new masks by writing them between
+ * replays. */
+typedef struct {
+  long long n;     /* elements */
+  long long group; /* neighbouring elements (in memory order) that share one draw: draw
+                      i / group. 1 = dropout, P on DCN_NCHW = whole channel maps,
+                      C*P = whole images (stochastic depth) */
+  uint64_t seed, offset;
+  int dtype; /* dcn_dtype */
+  float p;   /* 0 <= p <= 1 */
+} dcn_dropout_desc;
+/* y = residual + drop(x) (residual may be NULL: y = drop(x)). y may be x or residual. */
+int dcn_dropout_fwd(dcn_handle* h, const dcn_dropout_desc* d, const void* x,
+                    const void* residual, void* y, const void* rng);
+/* grad_x = drop(grad_y) (the residual's gradient is grad_y). grad_x may be grad_y. */
+int dcn_dropout_bwd(dcn_handle* h, const dcn_dropout_desc* d, const void* grad_y,
+                    void* grad_x, const void* rng);
 
 /* ---- in-library kernel timing (HIP events on the handle's stream) ---------- */
 typedef enum {

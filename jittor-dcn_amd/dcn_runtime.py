@@ -15,7 +15,7 @@ import threading
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DCN_LIB", os.path.join(HERE, "lib", "libdcn.so"))
 
-ABI_VERSION = 5  # include/dcn.h DCN_ABI_VERSION
+ABI_VERSION = 6  # include/dcn.h DCN_ABI_VERSION
 HOST_REUSE_FWD = 2  # include/dcn.h DCN_HOST_REUSE_FWD
 DCN_F32, DCN_BF16 = 0, 1
 DCN_BWD_COL_IN_WS = 1
@@ -42,6 +42,13 @@ class RoiDesc(ctypes.Structure):
                                             "part_w")] + \
                [("spatial_scale", ctypes.c_float), ("trans_std", ctypes.c_float),
                 ("ps", ctypes.c_int), ("no_trans", ctypes.c_int)]
+
+
+class DropoutDesc(ctypes.Structure):
+    """dcn_dropout_desc (include/dcn.h)."""
+    _fields_ = [("n", ctypes.c_longlong), ("group", ctypes.c_longlong),
+                ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
+                ("dtype", ctypes.c_int), ("p", ctypes.c_float)]
 
 
 _vp = ctypes.c_void_p
@@ -113,6 +120,8 @@ SIGNATURES = {
     "dcn_roi_pool_bwd": [_vp, ctypes.POINTER(RoiDesc), _vp, _vp, _vp, _vp, _vp, _vp],
     "dcn_roi_pool_fwd_host": [_vp, ctypes.POINTER(RoiDesc), _vp, _vp, _vp, _vp],
     "dcn_roi_pool_bwd_host": [_vp, ctypes.POINTER(RoiDesc), _vp, _vp, _vp, _vp, _vp, _vp],
+    "dcn_dropout_fwd": [_vp, ctypes.POINTER(DropoutDesc), _vp, _vp, _vp, _vp],
+    "dcn_dropout_bwd": [_vp, ctypes.POINTER(DropoutDesc), _vp, _vp, _vp],
 }
 _RESTYPES = {"dcn_last_error": ctypes.c_char_p}
 
