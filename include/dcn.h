@@ -40,7 +40,7 @@ extern "C" {
                              3: dcn_backward_host_ex; 4: dcn_host_state, dcn_host_alloc;
                              5: dcn_forward_ex (DCN_FWD_NO_COLUMNS), dcn_get_fwd_path,
                                 dcn_workspace_bytes(DCN_WS_FORWARD_NO_COLUMNS);
-                             6: dcn_dropout_* */
+                             6: dcn_dropout_*, dcn_block_norm_* */
 
 typedef enum {
   DCN_OK = 0,
@@ -320,6 +320,53 @@ int dcn_dropout_fwd(dcn_handle* h, const dcn_dropout_desc* d, const void* x,
 /* grad_x = drop(grad_y) (the residual's gradient is grad_y). grad_x may be grad_y. */
 int dcn_dropout_bwd(dcn_handle* h, const dcn_dropout_desc* d, const void* grad_y,
                     void* grad_x, const void* rng);
+
+/* Block norms. Per position (b, p), over its C channels:
+ *   t   = drop(alpha · scale[c] · act(gate) · N_post(x))
+ *   out = residual + t
+ *   y   = N_pre(out)
+ *   N(v) = (v - m) / sqrt(var + eps) · w[c] + b[c];  DCN_NORM_LAYER: m = mean, var =
+ *   mean((v - m)²); DCN_NORM_RMS: m = 0, var = mean(v²); DCN_NORM_NONE: N_post(x) = x, and
+ *   no y. */
+typedef enum { DCN_NORM_NONE = 0, DCN_NORM_RMS = 1, DCN_NORM_LAYER = 2 } dcn_norm_kind;
+/* DCN_GATE_FULL: a gate of x's shape; DCN_GATE_IMAGE: gate[B][C], one per image and channel */
+typedef enum { DCN_GATE_NONE = 0, DCN_GATE_FULL = 1, DCN_GATE_IMAGE = 2 } dcn_gate_kind;
+typedef enum { DCN_ACT_LINEAR = 0, DCN_ACT_SIGMOID = 1, DCN_ACT_SILU = 2 } dcn_gate_act;
+typedef struct {
+  int B, C, P;         /* images, channels, positions of an image */
+  int layout, dtype;   /* dcn_layout, dcn_dtype */
+  int post, pre;       /* dcn_norm_kind of N_post and N_pre */
+  int gate, gate_act;  /* dcn_gate_kind, dcn_gate_act */
+  float eps_post, eps_pre;
+  float alpha;
+  float drop_p;        /* 0 = no dropout */
+  int drop_image;      /* 0: every element draws (memory order); 1: every image draws once */
+  uint64_t seed, offset;
+} dcn_block_desc;
+/* The tensors of one call; one that the descriptor leaves unused is NULL. scale and the
+ * w_* may be NULL (= 1), the b_* too (= 0). */
+typedef struct {
+  const void *x, *residual; /* x NULL: only y = N_pre(residual) (no post, gate, scale, drop);
+                               residual NULL: out = t */
+  const void *gate, *scale, *w_post, *b_post, *w_pre, *b_pre;
+  const void* rng;          /* as in dcn_dropout_desc */
+  /* forward results. out may be NULL where only y is wanted (x NULL: it has to be), and may
+   * be `residual` itself; y is required with pre, else NULL */
+  void *out, *y;
+  /* backward: gradients of out and y (either may be NULL = zero; not both), then the
+   * gradients wanted (NULL: not computed), overwritten */
+  const void *grad_out, *grad_y;
+  void *grad_x, *grad_residual, *grad_gate, *grad_scale;
+  void *grad_w_post, *grad_b_post, *grad_w_pre, *grad_b_pre;
+} dcn_block_io;
+int dcn_block_norm_fwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_io* io);
+/* Reads the forward's inputs (x, residual, gate, parameters, rng), never its results, and
+ * grad_out / grad_y. ws: dcn_block_norm_workspace bytes (256-byte aligned), one per call in
+ * flight: calls that may run at the same time (other streams, other graphs) each need their
+ * own. */
+int dcn_block_norm_workspace(const dcn_block_desc* d, size_t* bytes);
+int dcn_block_norm_bwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_io* io, void* ws,
+                       size_t ws_bytes);
 
 /* ---- in-library kernel timing (HIP events on the handle's stream) ---------- */
 typedef enum {

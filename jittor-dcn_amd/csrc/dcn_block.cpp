@@ -82,9 +82,149 @@ int dropout(dcn_handle* h, const dcn_dropout_desc* d, const void* x, const void*
               "dropout");
 }
 
+// The checks that need no tensor; fills the geometry of `a`.
+int block_geo(const dcn_block_desc* d, dcn::BlockArgs* a) {
+  if (!d) return fail(DCN_ERR_INVALID, "null descriptor");
+  *a = dcn::BlockArgs{};
+  if (d->B <= 0 || d->C <= 0 || d->P <= 0) return fail(DCN_ERR_INVALID, "B, C, P must be positive");
+  if (!dtype_ok(d->dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
+  if (d->layout != DCN_NCHW && d->layout != DCN_NHWC) return fail(DCN_ERR_INVALID, "unknown layout");
+  if ((double)d->B * d->C * d->P > (double)(1LL << 40) || (long long)d->B * d->P > (1LL << 34))
+    return fail(DCN_ERR_UNSUPPORTED, "more than 2^40 elements or 2^34 positions");
+  for (int k : {d->post, d->pre})
+    if (k < DCN_NORM_NONE || k > DCN_NORM_LAYER) return fail(DCN_ERR_INVALID, "unknown norm");
+  if (d->gate < DCN_GATE_NONE || d->gate > DCN_GATE_IMAGE)
+    return fail(DCN_ERR_INVALID, "unknown gate kind");
+  if (d->gate_act < DCN_ACT_LINEAR || d->gate_act > DCN_ACT_SILU)
+    return fail(DCN_ERR_INVALID, "unknown gate activation");
+  for (float e : {d->eps_post, d->eps_pre})
+    if (!(e >= 0.f && std::isfinite(e))) return fail(DCN_ERR_INVALID, "eps must be finite and >= 0");
+  if (d->drop_image != 0 && d->drop_image != 1) return fail(DCN_ERR_INVALID, "drop_image is 0 or 1");
+  a->B = d->B; a->C = d->C; a->P = d->P;
+  a->layout = d->layout; a->dtype = d->dtype;
+  a->post = d->post; a->pre = d->pre;
+  a->gate_kind = d->gate; a->act = d->gate_act;
+  a->drop_image = d->drop_image;
+  a->eps1 = d->eps_post; a->eps2 = d->eps_pre; a->alpha = d->alpha;
+  return DCN_OK;
+}
+
+// The inputs of either direction.
+int block_inputs(const dcn_block_desc* d, const dcn_block_io* io, dcn::BlockArgs* a) {
+  if (int rc = block_geo(d, a)) return rc;
+  if (!io) return fail(DCN_ERR_INVALID, "null tensor list");
+  if (!drop_args(d->drop_p, d->seed, d->offset, io->rng, &a->drop))
+    return fail(DCN_ERR_INVALID, "dropout needs 0 <= p <= 1");
+  if (!aligned(io->rng, 8)) return fail(DCN_ERR_INVALID, "rng must be 8-byte aligned");
+  if (!io->x && !io->residual) return fail(DCN_ERR_INVALID, "neither x nor a residual");
+  if (!io->x && (d->post || d->gate || io->scale || io->w_post || io->b_post || d->drop_p > 0.f))
+    return fail(DCN_ERR_INVALID, "post norm, gate, scale and dropout need x");
+  if (!io->x && !d->pre) return fail(DCN_ERR_INVALID, "nothing to compute: no x and no pre norm");
+  if ((io->w_post || io->b_post) && !d->post) return fail(DCN_ERR_INVALID, "w_post / b_post without a post norm");
+  if ((io->w_pre || io->b_pre) && !d->pre) return fail(DCN_ERR_INVALID, "w_pre / b_pre without a pre norm");
+  if ((io->gate != nullptr) != (d->gate != DCN_GATE_NONE))
+    return fail(DCN_ERR_INVALID, "the gate tensor and the gate kind must come together");
+  a->x = io->x; a->res = io->residual; a->gate = io->gate; a->scale = io->scale;
+  a->w1 = io->w_post; a->b1 = io->b_post; a->w2 = io->w_pre; a->b2 = io->b_pre;
+  return DCN_OK;
+}
+
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+
+// Every output apart from every input and every other output; `same` may equal `inplace` whole.
+int block_spans(const Span* in, int nin, const Span* out, int nout, size_t es,
+                const void* inplace_out, const void* inplace_in) {
+  for (int i = 0; i < nin; ++i)
+    if (!aligned(in[i].p, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
+  for (int i = 0; i < nout; ++i) {
+    if (!aligned(out[i].p, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
+    for (int j = 0; j < nin; ++j) {
+      if (out[i].p && out[i].p == inplace_out && in[j].p == inplace_in && out[i].p == in[j].p)
+        continue;
+      if (overlap(out[i].p, out[i].bytes, in[j].p, in[j].bytes))
+        return fail(DCN_ERR_INVALID, "an output overlaps an input");
+    }
+    for (int j = 0; j < i; ++j)
+      if (overlap(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
+        return fail(DCN_ERR_INVALID, "two outputs overlap");
+  }
+  return DCN_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int dcn_block_norm_fwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_io* io) {
+  dcn::BlockArgs a;
+  if (int rc = block_inputs(d, io, &a)) return rc;
+  if ((io->y != nullptr) != (d->pre != DCN_NORM_NONE))
+    return fail(DCN_ERR_INVALID, "y and the pre norm must come together");
+  if (!io->x && io->out) return fail(DCN_ERR_INVALID, "without x there is no out");
+  if (!io->y && !io->out) return fail(DCN_ERR_INVALID, "no output");
+  a.out = io->out; a.y = io->y;
+  const size_t es = dtype_bytes(d->dtype), full = (size_t)d->B * d->C * d->P * es,
+               vec = (size_t)d->C * es;
+  const size_t gate = d->gate == DCN_GATE_FULL ? full : (size_t)d->B * d->C * es;
+  const Span in[] = {{io->x, full}, {io->residual, full}, {io->gate, gate}, {io->scale, vec},
+                     {io->w_post, vec}, {io->b_post, vec}, {io->w_pre, vec}, {io->b_pre, vec},
+                     {io->rng, 16}};
+  const Span out[] = {{io->out, full}, {io->y, full}};
+  if (int rc = block_spans(in, 9, out, 2, es, io->out, io->residual)) return rc;
+  DeviceScope ds;
+  if (int rc = ds.bind(h)) return rc;
+  return done(dcn::launch_block_norm_fwd(a, ds.stream), "block_norm forward");
+}
+
+int dcn_block_norm_workspace(const dcn_block_desc* d, size_t* bytes) {
+  dcn::BlockArgs a;
+  if (int rc = block_geo(d, &a)) return rc;
+  if (!bytes) return fail(DCN_ERR_INVALID, "null out pointer");
+  *bytes = dcn::block_norm_ws_floats(a) * sizeof(float);
+  return DCN_OK;
+}
+
+int dcn_block_norm_bwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_io* io, void* ws,
+                       size_t ws_bytes) {
+  dcn::BlockArgs a;
+  if (int rc = block_inputs(d, io, &a)) return rc;
+  if (!io->grad_out && !io->grad_y) return fail(DCN_ERR_INVALID, "neither grad_out nor grad_y");
+  if (io->grad_y && !d->pre) return fail(DCN_ERR_INVALID, "grad_y without a pre norm");
+  if (!io->x && (io->grad_out || io->grad_x || io->grad_gate || io->grad_scale ||
+                 io->grad_w_post || io->grad_b_post))
+    return fail(DCN_ERR_INVALID, "without x there is no out and no gradient of the block");
+  if (io->grad_gate && !d->gate) return fail(DCN_ERR_INVALID, "grad_gate without a gate");
+  if ((io->grad_w_post || io->grad_b_post) && !d->post)
+    return fail(DCN_ERR_INVALID, "grad_w_post / grad_b_post without a post norm");
+  if ((io->grad_w_pre || io->grad_b_pre) && !d->pre)
+    return fail(DCN_ERR_INVALID, "grad_w_pre / grad_b_pre without a pre norm");
+  if (!(io->grad_x || io->grad_residual || io->grad_gate || io->grad_scale || io->grad_w_post ||
+        io->grad_b_post || io->grad_w_pre || io->grad_b_pre))
+    return fail(DCN_ERR_INVALID, "no gradient wanted");
+  a.go = io->grad_out; a.gy = io->grad_y;
+  a.gx = io->grad_x; a.gr = io->grad_residual; a.gg = io->grad_gate; a.gs = io->grad_scale;
+  a.gw1 = io->grad_w_post; a.gb1 = io->grad_b_post; a.gw2 = io->grad_w_pre; a.gb2 = io->grad_b_pre;
+  const size_t need = dcn::block_norm_ws_floats(a) * sizeof(float);
+  if (!ws || ws_bytes < need) return fail(DCN_ERR_WORKSPACE, "block_norm workspace too small");
+  if (!aligned(ws, 256)) return fail(DCN_ERR_INVALID, "workspace must be 256-byte aligned");
+  const size_t es = dtype_bytes(d->dtype), full = (size_t)d->B * d->C * d->P * es,
+               vec = (size_t)d->C * es;
+  const size_t gate = d->gate == DCN_GATE_FULL ? full : (size_t)d->B * d->C * es;
+  const Span in[] = {{io->x, full}, {io->residual, full}, {io->gate, gate}, {io->scale, vec},
+                     {io->w_post, vec}, {io->b_post, vec}, {io->w_pre, vec}, {io->b_pre, vec},
+                     {io->grad_out, full}, {io->grad_y, full}, {io->rng, 16}};
+  const Span out[] = {{io->grad_x, full}, {io->grad_residual, full}, {io->grad_gate, gate},
+                      {io->grad_scale, vec}, {io->grad_w_post, vec}, {io->grad_b_post, vec},
+                      {io->grad_w_pre, vec}, {io->grad_b_pre, vec}, {ws, need}};
+  if (int rc = block_spans(in, 11, out, 9, es, nullptr, nullptr)) return rc;
+  a.ws = static_cast<float*>(ws);
+  DeviceScope ds;
+  if (int rc = ds.bind(h)) return rc;
+  return done(dcn::launch_block_norm_bwd(a, ds.stream), "block_norm backward");
+}
 
 int dcn_dropout_fwd(dcn_handle* h, const dcn_dropout_desc* d, const void* x, const void* residual,
                     void* y, const void* rng) {

@@ -3,12 +3,27 @@
 // dcn_block.cpp holds the entry points and their checks.
 #pragma once
 #include "dcn_internal.h"
+#include "dcn_philox.h"
 
 namespace dcn {
 
-struct DropArgs;
 // y = res + drop(x) (res may be null); n elements, `group` to a draw
 hipError_t launch_dropout(const DropArgs& a, int dtype, const void* x, const void* res, void* y,
                           uint64_t n, uint64_t group, hipStream_t s);
+
+// One block-norm call (dcn_block_desc / dcn_block_io): 1 = post, 2 = pre.
+struct BlockArgs {
+  const void *x, *res, *gate, *scale, *w1, *b1, *w2, *b2;
+  void *out, *y;
+  const void *go, *gy;
+  void *gx, *gr, *gg, *gs, *gw1, *gb1, *gw2, *gb2;
+  float* ws;
+  DropArgs drop;
+  int B, C, P, layout, dtype, post, pre, gate_kind, act, drop_image;
+  float eps1, eps2, alpha;
+};
+size_t block_norm_ws_floats(const BlockArgs& a);
+hipError_t launch_block_norm_fwd(const BlockArgs& a, hipStream_t s);
+hipError_t launch_block_norm_bwd(const BlockArgs& a, hipStream_t s);
 
 }  // namespace dcn

@@ -22,6 +22,10 @@ DCN_BWD_COL_IN_WS = 1
 DCN_FWD_NO_COLUMNS = 1  # dcn_forward_ex flag
 DCN_WS_FORWARD_NO_COLUMNS = 2  # dcn_workspace_bytes(with_backward=2)
 DCN_FWD_AUTO, DCN_FWD_UNFUSED, DCN_FWD_FUSED, DCN_FWD_FUSED_NOCOL = 0, 1, 2, 3
+DCN_NCHW, DCN_NHWC = 0, 1
+DCN_NORM_NONE, DCN_NORM_RMS, DCN_NORM_LAYER = 0, 1, 2
+DCN_GATE_NONE, DCN_GATE_FULL, DCN_GATE_IMAGE = 0, 1, 2
+DCN_ACT_LINEAR, DCN_ACT_SIGMOID, DCN_ACT_SILU = 0, 1, 2
 DCN_MATH_F32, DCN_MATH_F32_BF16X3, DCN_MATH_F32_BF16X6, DCN_MATH_F32_BF16X9 = 0, 3, 6, 9
 KERNEL_IDS = {
     "offset_fwd": 0, "im2col": 1, "gemm_fwd": 2, "bias_fwd": 3, "bwd_bias": 4,
@@ -49,6 +53,23 @@ class DropoutDesc(ctypes.Structure):
     _fields_ = [("n", ctypes.c_longlong), ("group", ctypes.c_longlong),
                 ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
                 ("dtype", ctypes.c_int), ("p", ctypes.c_float)]
+
+
+class BlockDesc(ctypes.Structure):
+    """dcn_block_desc (include/dcn.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("B", "C", "P", "layout", "dtype", "post", "pre",
+                                            "gate", "gate_act")] + \
+               [(n, ctypes.c_float) for n in ("eps_post", "eps_pre", "alpha", "drop_p")] + \
+               [("drop_image", ctypes.c_int), ("seed", ctypes.c_uint64),
+                ("offset", ctypes.c_uint64)]
+
+
+class BlockIO(ctypes.Structure):
+    """dcn_block_io (include/dcn.h): device pointers, 0 / None where absent."""
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("x", "residual", "gate", "scale", "w_post", "b_post", "w_pre", "b_pre", "rng",
+                 "out", "y", "grad_out", "grad_y", "grad_x", "grad_residual", "grad_gate",
+                 "grad_scale", "grad_w_post", "grad_b_post", "grad_w_pre", "grad_b_pre")]
 
 
 _vp = ctypes.c_void_p
@@ -122,6 +143,9 @@ SIGNATURES = {
     "dcn_roi_pool_bwd_host": [_vp, ctypes.POINTER(RoiDesc), _vp, _vp, _vp, _vp, _vp, _vp],
     "dcn_dropout_fwd": [_vp, ctypes.POINTER(DropoutDesc), _vp, _vp, _vp, _vp],
     "dcn_dropout_bwd": [_vp, ctypes.POINTER(DropoutDesc), _vp, _vp, _vp],
+    "dcn_block_norm_fwd": [_vp, ctypes.POINTER(BlockDesc), ctypes.POINTER(BlockIO)],
+    "dcn_block_norm_workspace": [ctypes.POINTER(BlockDesc), ctypes.POINTER(_sz)],
+    "dcn_block_norm_bwd": [_vp, ctypes.POINTER(BlockDesc), ctypes.POINTER(BlockIO), _vp, _sz],
 }
 _RESTYPES = {"dcn_last_error": ctypes.c_char_p}
 

@@ -161,3 +161,144 @@ class DropPath(Dropout):
 
     def __init__(self, p=0.1, rng=None):
         super().__init__(p, "image", rng)
+
+
+# ---------------------------------------------------------------------------- block norms
+_NORM = {None: rt.DCN_NORM_NONE, "rms": rt.DCN_NORM_RMS, "layer": rt.DCN_NORM_LAYER}
+_ACT = {"linear": rt.DCN_ACT_LINEAR, "sigmoid": rt.DCN_ACT_SIGMOID, "silu": rt.DCN_ACT_SILU}
+
+
+def _layout(x):
+    """(layout, B, C, P, memory format) of a map tensor: [B, C, H, W] (channels-last memory
+    stays channels-last) or token rows [..., C]."""
+    if x.dim() == 4:
+        B, C, H, W = x.shape
+        if not x.is_contiguous() and x.is_contiguous(memory_format=torch.channels_last):
+            return rt.DCN_NHWC, B, C, H * W, torch.channels_last
+        return rt.DCN_NCHW, B, C, H * W, torch.contiguous_format
+    C = x.shape[-1]
+    B = x.shape[0] if x.dim() > 2 else 1
+    return rt.DCN_NHWC, B, C, x.numel() // max(B * C, 1), torch.contiguous_format
+
+
+_GRADS = ("x", "residual", "gate", "scale", "w_post", "b_post", "w_pre", "b_pre")
+
+
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, gate, scale, w_post, b_post, w_pre, b_pre, desc, mf, dev_rng):
+        ref = residual if x is None else x
+        full = lambda t: None if t is None else t.contiguous(memory_format=mf)
+        x, residual = full(x), full(residual)
+        gate = full(gate) if desc.gate == rt.DCN_GATE_FULL else gate
+        gate, scale, w_post, b_post, w_pre, b_pre = (
+            t if t is None or t is gate and desc.gate == rt.DCN_GATE_FULL else t.contiguous()
+            for t in (gate, scale, w_post, b_post, w_pre, b_pre))
+        out = torch.empty_like(x, memory_format=mf) if x is not None else None
+        y = torch.empty_like(ref, memory_format=mf) if desc.pre else None
+        if ref.numel():
+            io = rt.BlockIO(*map(_ptr, (x, residual, gate, scale, w_post, b_post, w_pre, b_pre,
+                                        dev_rng, out, y)))
+            _call(ref.device, "dcn_block_norm_fwd", desc, io)
+        ctx.desc, ctx.mf = desc, mf
+        ctx.save_for_backward(x, residual, gate, scale, w_post, b_post, w_pre, b_pre, dev_rng)
+        ctx.set_materialize_grads(False)
+        return out, y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_y):
+        *inputs, dev_rng = ctx.saved_tensors
+        need = ctx.needs_input_grad[:8]
+        if grad_out is None and grad_y is None:
+            return (None,) * 11
+        full = lambda t: None if t is None else t.contiguous(memory_format=ctx.mf)
+        grad_out, grad_y = full(grad_out), full(grad_y)
+        ref = inputs[0] if inputs[0] is not None else inputs[1]
+        if not ref.numel():
+            return (*(torch.zeros_like(t) if n else None for t, n in zip(inputs, need)),
+                    None, None, None)
+        grads = [torch.empty_like(t) if n else None for t, n in zip(inputs, need)]
+        nbytes = ctypes.c_size_t()
+        rt.check(rt.load().dcn_block_norm_workspace(ctx.desc, ctypes.byref(nbytes)),
+                 "dcn_block_norm_workspace")
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=ref.device)
+        io = rt.BlockIO(*map(_ptr, (*inputs, dev_rng, None, None, grad_out, grad_y, *grads)))
+        _call(ref.device, "dcn_block_norm_bwd", ctx.desc, io, ws.data_ptr(), nbytes.value)
+        return (*grads, None, None, None)
+
+
+def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=None, alpha=1.0,
+               post=None, post_weight=None, post_bias=None, pre=None, pre_weight=None,
+               pre_bias=None, eps=1e-6, drop_p=0.0, drop="element", rng=None):
+    """The operator between two residual blocks: returns (out, y),
+
+        t = dropout(alpha * scale * act(gate) * N_post(x));  out = residual + t;  y = N_pre(out)
+
+    with the norms over the channels: dim 1 of a 4-d tensor (NCHW, or channels-last memory as
+    it is), else the last. post / pre: None, "rms" or "layer" (None: no norm after the block;
+    no y); eps: one number, or (post, pre). gate: of x's shape, or [B, C] for one per image
+    and channel, through gate_act "linear", "sigmoid" or "silu". scale, *_weight, *_bias: [C].
+    drop: "element" (elements count in memory order) or "image". Without a residual out = t;
+    without x the operator is the pre norm alone and out is the residual. All tensors have
+    x's dtype; everything but the rounding of the results is fp32."""
+    ref = residual if x is None else x
+    if ref is None:
+        raise ValueError("block_norm: neither x nor a residual")
+    dt = _dtype(ref, "block_norm")
+    if post not in _NORM or pre not in _NORM or gate_act not in _ACT:
+        raise ValueError("block_norm: norms are None, 'rms' or 'layer'; gate_act is 'linear', "
+                         "'sigmoid' or 'silu'")
+    if drop not in ("element", "image") or not 0.0 <= drop_p <= 1.0:
+        raise ValueError("block_norm: drop is 'element' or 'image' and 0 <= drop_p <= 1")
+    layout, B, C, P, mf = _layout(ref)
+    if ref.dim() == 0 or C == 0:
+        raise ValueError("block_norm: no channels")
+    kind = rt.DCN_GATE_NONE
+    if gate is not None:
+        image = gate.dim() == 2 and tuple(gate.shape) == (B, C) and gate.shape != ref.shape
+        kind = rt.DCN_GATE_IMAGE if image else rt.DCN_GATE_FULL
+        _same(ref, gate, "block_norm", "gate", (B, C) if image else None)
+    if x is not None:
+        _same(x, residual, "block_norm", "residual")
+    for name, t in (("scale", scale), ("post_weight", post_weight), ("post_bias", post_bias),
+                    ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
+        _same(ref, t, "block_norm", name, (C,))
+    e1, e2 = eps if isinstance(eps, (tuple, list)) else (eps, eps)
+    seed, offset, dev_rng = _rng(rng, ref.device, "block_norm") if drop_p > 0 else (0, 0, None)
+    desc = rt.BlockDesc(B, C, P, layout, dt, _NORM[post], _NORM[pre], kind, _ACT[gate_act], e1, e2,
+                        alpha, drop_p, int(drop == "image"), seed, offset)
+    out, y = _BlockNorm.apply(x, residual, gate, scale, post_weight, post_bias, pre_weight,
+                              pre_bias, desc, mf, dev_rng)
+    return (residual if x is None else out), y
+
+
+class BlockNorm(torch.nn.Module):
+    """block_norm() with its parameters: (x, residual, gate=None) -> (out, y).
+
+    post / pre: None, "rms" (weight) or "layer" (weight and bias); layer_scale: the residual
+    scale's initial value per channel, or None for no scale; alpha: a fixed factor; drop_p:
+    dropout of the block's result in training, per element or per image ("image": stochastic
+    depth), seeded like Dropout."""
+
+    def __init__(self, channels, post="rms", pre="rms", layer_scale=None, alpha=1.0, gate_act="linear",
+                 drop_p=0.0, drop="element", eps=1e-6, rng=None):
+        super().__init__()
+        self.channels, self.post, self.pre, self.alpha, self.gate_act = (channels, post, pre,
+                                                                         alpha, gate_act)
+        self.drop_p, self.drop, self.eps, self.rng = drop_p, drop, eps, rng
+
+        def vec(on, value):
+            return torch.nn.Parameter(torch.full((channels,), float(value))) if on else None
+
+        self.scale = vec(layer_scale is not None, layer_scale or 0.0)
+        self.post_weight, self.post_bias = vec(post, 1.0), vec(post == "layer", 0.0)
+        self.pre_weight, self.pre_bias = vec(pre, 1.0), vec(pre == "layer", 0.0)
+
+    def forward(self, x, residual=None, gate=None):
+        p = self.drop_p if self.training else 0.0
+        return block_norm(x, residual, gate=gate, gate_act=self.gate_act, scale=self.scale,
+                          alpha=self.alpha, post=self.post, post_weight=self.post_weight,
+                          post_bias=self.post_bias, pre=self.pre, pre_weight=self.pre_weight,
+                          pre_bias=self.pre_bias, eps=self.eps, drop_p=p, drop=self.drop,
+                          rng=_fresh_rng(self.rng) if p > 0 else None)

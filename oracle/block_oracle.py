@@ -40,3 +40,99 @@ def drop_factor(n, group, p, seed, offset):
     nd = -(-n // group)
     f = np.where(draws(0, nd, seed, offset) < t, 0.0, 65536.0 / max(65536 - t, 1))
     return np.repeat(f, group)[:n]
+
+
+# ---- block norms ---------------------------------------------------------------------------
+ACTS = {"linear": lambda g: g, "sigmoid": torch.sigmoid, "silu": lambda g: g * torch.sigmoid(g)}
+
+
+def norm(v, kind, w, b, eps):
+    """N over the last axis, any float dtype."""
+    if kind is None:
+        return v
+    if kind == "layer":
+        v = v - v.mean(-1, keepdim=True)
+    h = v / torch.sqrt((v * v).mean(-1, keepdim=True) + eps)
+    h = h if w is None else h * w
+    return h if b is None else h + b
+
+
+def block_forward(t, *, post=None, pre=None, act="linear", alpha=1.0, eps=1e-6, factor=None):
+    """(out, y) of tensors t["x"], t["residual"], ... all [B][P][C] (gate [B][C] per image);
+    factor: the dropout factor [B][P][C] or None. x absent: out is the residual."""
+    if t.get("x") is None:
+        return t["residual"], norm(t["residual"], pre, t.get("w_pre"), t.get("b_pre"), eps)
+    v = norm(t["x"], post, t.get("w_post"), t.get("b_post"), eps)
+    if t.get("gate") is not None:
+        g = t["gate"]
+        v = v * ACTS[act](g[:, None] if g.dim() == 2 else g)
+    if t.get("scale") is not None:
+        v = v * t["scale"]
+    v = v * alpha
+    if factor is not None:
+        v = torch.where(factor == 0, torch.zeros_like(v), v * factor)
+    out = v if t.get("residual") is None else t["residual"] + v
+    return out, norm(out, pre, t.get("w_pre"), t.get("b_pre"), eps) if pre else None
+
+
+def block_bounds(t, go, gy, *, post=None, pre=None, act="linear", alpha=1.0, eps=1e-6,
+                 factor=None):
+    """For every output, the value of its formula with every term replaced by its magnitude
+    (no cancellation): a result computed with sums of n fp32 terms is within a small multiple
+    of n · 2^-24 of it. A norm's r amplifies by mean(d²) r² >= 1 where its mean cancels."""
+    one = torch.ones((), dtype=torch.float64)
+    a = {k: v.abs() for k, v in t.items() if v is not None}
+    g = t.get("gate")
+
+    def mag(m, v, kind, w, b):  # magnitudes of N's output and of its normalised value; r
+        if kind is None:
+            return m, None, one
+        mean = m.mean(-1, keepdim=True) if kind == "layer" else 0.0
+        c = v - v.mean(-1, keepdim=True) if kind == "layer" else v
+        r = 1 / torch.sqrt((c * c).mean(-1, keepdim=True) + eps)
+        d = m + mean
+        q = ((d * d).mean(-1, keepdim=True) * r * r).clamp(min=1.0)
+        h = d * r * q
+        return h * a.get(w, one) + a.get(b, torch.zeros(())), h, r * q
+
+    def back(m, kind, w, h, r):
+        m = m * a.get(w, one)
+        mean = m.mean(-1, keepdim=True) if kind == "layer" else 0.0
+        return r * (m + mean + h * (m * h).mean(-1, keepdim=True))
+
+    out, _ = block_forward(t, post=post, pre=pre, act=act, alpha=alpha, eps=eps, factor=factor)
+    f = one if factor is None else factor
+    lead = tuple(range(out.dim() - 1))
+    res = {}
+    if t.get("x") is not None:
+        mv, h1, r1 = mag(a["x"], t["x"], post, "w_post", "b_post")
+        av = ad = one
+        if g is not None:
+            gg = g[:, None] if g.dim() == 2 else g
+            s = torch.sigmoid(gg)
+            av, ad = {"linear": (gg.abs(), one), "sigmoid": (s, s * (1 + s)),
+                      "silu": (gg.abs() * s, s * (1 + gg.abs() * (1 + s)))}[act]
+        ms = a.get("scale", one) * abs(alpha)
+        mo = a.get("residual", torch.zeros(())) + mv * ms * av * f
+    else:
+        mo = a["residual"]
+    res["out"] = mo
+    mg = torch.zeros_like(out) if go is None else go.abs()
+    if pre:
+        res["y"], h2, r2 = mag(mo, out, pre, "w_pre", "b_pre")
+        m = torch.zeros_like(out) if gy is None else gy.abs()
+        mg = mg + back(m, pre, "w_pre", h2, r2)
+        res["w_pre"], res["b_pre"] = (m * h2).sum(lead), m.sum(lead)
+    res["residual"] = mg
+    if t.get("x") is not None:
+        md = mg * f
+        res["scale"] = (md * mv * av).sum(lead) * abs(alpha)
+        if g is not None:
+            m = md * mv * ms * ad
+            res["gate"] = m.sum(1) if g.dim() == 2 else m
+        m = md * ms * av
+        if post:
+            res["w_post"], res["b_post"] = (m * h1).sum(lead), m.sum(lead)
+            m = back(m, post, "w_post", h1, r1)
+        res["x"] = m
+    return res

@@ -68,3 +68,92 @@ def test_drop_factor_mean():
     sd = (p * (1 - p) / n) ** 0.5
     assert abs(np.mean(f > 0) - (1 - p)) < 5 * sd + 1 / 65536
     assert abs(f.mean() - 1) < 5 * sd / (1 - p)
+
+
+# ---- block norms
+def _block(L, io=None, fwd=True, ws=OK_PTR * 64, ws_bytes=1 << 30, **kw):
+    d = rt.BlockDesc(**{**dict(B=2, C=8, P=6, layout=0, dtype=0, post=1, pre=1, gate=0,
+                               gate_act=0, eps_post=1e-6, eps_pre=1e-6, alpha=1.0, drop_p=0.0),
+                        **kw})
+    t = {n: OK_PTR * (i + 1) for i, n in enumerate(
+        ("x", "residual", "out", "y") if fwd else ("x", "residual", "grad_out", "grad_y",
+                                                   "grad_x", "grad_residual"))}
+    t.update(io or {})
+    t = rt.BlockIO(**t)
+    if fwd:
+        return L.dcn_block_norm_fwd(None, ctypes.byref(d), ctypes.byref(t))
+    return L.dcn_block_norm_bwd(None, ctypes.byref(d), ctypes.byref(t), ws, ws_bytes)
+
+
+FAR = OK_PTR * 100
+
+
+@pytest.mark.parametrize("kw,io,msg", [
+    (dict(B=0), {}, "positive"), (dict(C=-1), {}, "positive"), (dict(P=0), {}, "positive"),
+    (dict(dtype=3), {}, "dtype"), (dict(layout=2), {}, "layout"), (dict(post=3), {}, "norm"),
+    (dict(pre=-1), {}, "norm"), (dict(gate=4), {}, "gate kind"), (dict(gate_act=3), {}, "activ"),
+    (dict(eps_pre=-1.0), {}, "eps"), (dict(eps_post=float("nan")), {}, "eps"),
+    (dict(eps_post=float("inf")), {}, "eps"), (dict(drop_p=2.0), {}, "p <= 1"),
+    (dict(drop_image=2), {}, "drop_image"), (dict(gate=1), {}, "come together"),
+    (dict(), dict(gate=FAR), "come together"), (dict(), dict(x=None, residual=None), "neither"),
+    (dict(), dict(x=None, out=None), "need x"), (dict(post=0, pre=0), dict(x=None), "nothing"),
+    (dict(post=0), dict(w_post=FAR), "without a post"), (dict(pre=0), dict(b_pre=FAR), "a pre"),
+    (dict(pre=0), {}, "come together"), (dict(), dict(y=None), "come together"),
+    (dict(post=0), dict(x=None), "no out"), (dict(pre=0), dict(y=None, out=None), "no output"),
+    (dict(), dict(rng=FAR + 4), "8-byte"), (dict(), dict(x=OK_PTR + 2), "aligned"),
+    (dict(), dict(out=OK_PTR + 64), "overlaps"), (dict(), dict(out=OK_PTR), "overlaps"),
+    (dict(), dict(y=OK_PTR * 2), "overlaps"), (dict(), dict(y=OK_PTR * 3 + 380), "two outputs"),
+    (dict(), dict(w_pre=OK_PTR * 4), "overlaps"),
+    (dict(B=1 << 20, C=1 << 20, P=2), {}, "2\\^40"),
+    (dict(), {}, "null handle"), (dict(), dict(out=OK_PTR * 2), "null handle"),
+    (dict(post=0), dict(x=None, out=None), "null handle"),
+])
+def test_block_norm_forward_refusals(kw, io, msg):
+    assert _block(rt.load(), io, **kw) < 0
+    import re
+    assert re.search(msg, rt.last_error()), rt.last_error()
+
+
+@pytest.mark.parametrize("kw,io,ws,msg", [
+    (dict(), dict(grad_out=None, grad_y=None), {}, "neither"),
+    (dict(pre=0), {}, {}, "without a pre"), (dict(), dict(grad_gate=FAR), {}, "without a gate"),
+    (dict(post=0), dict(grad_w_post=FAR), {}, "without a post"),
+    (dict(pre=0), dict(grad_y=None, grad_b_pre=FAR), {}, "without a pre"),
+    (dict(), dict(grad_x=None, grad_residual=None), {}, "no gradient"),
+    (dict(post=0), dict(x=None, grad_x=None), {}, "without x"),
+    (dict(), {}, dict(ws=None), "workspace"), (dict(), {}, dict(ws_bytes=16), "workspace"),
+    (dict(), {}, dict(ws=OK_PTR * 64 + 8), "256-byte"),
+    (dict(), dict(grad_x=OK_PTR * 3), {}, "overlaps"),
+    (dict(), dict(grad_x=OK_PTR * 6), {}, "two outputs"),
+    (dict(), {}, dict(ws=OK_PTR), "overlaps"), (dict(), {}, {}, "null handle"),
+])
+def test_block_norm_backward_refusals(kw, io, ws, msg):
+    assert _block(rt.load(), io, fwd=False, **ws, **kw) < 0
+    assert msg in rt.last_error()
+
+
+@pytest.mark.parametrize("post,pre,gate", [("layer", "layer", 3), ("rms", "layer", 2),
+                                           (None, "rms", 3), ("layer", None, 0)])
+def test_block_oracle_gradients_against_differences(post, pre, gate):
+    """The oracle's autograd gradients against central differences (float64 gradcheck)."""
+    import torch
+    g = torch.Generator().manual_seed(1)
+    B, P, C = 2, 3, 5
+    t = {"x": torch.randn(B, P, C, generator=g, dtype=torch.float64),
+         "residual": torch.randn(B, P, C, generator=g, dtype=torch.float64),
+         "scale": torch.rand(C, generator=g, dtype=torch.float64) + 0.5}
+    if gate:
+        t["gate"] = torch.randn(*((B, P, C) if gate == 3 else (B, C)), generator=g,
+                                dtype=torch.float64)
+    for k, on in (("w_post", post), ("b_post", post == "layer"), ("w_pre", pre),
+                  ("b_pre", pre == "layer")):
+        if on:
+            t[k] = torch.randn(C, generator=g, dtype=torch.float64)
+    f = torch.from_numpy(BO.drop_factor(B * P * C, 1, 0.3, 1, 2)).reshape(B, P, C)
+    names = list(t)
+
+    def fn(*v):
+        o, y = BO.block_forward(dict(zip(names, v)), post=post, pre=pre, act="silu", factor=f)
+        return (o, y) if pre else o
+
+    assert torch.autograd.gradcheck(fn, [t[k].requires_grad_() for k in names])

@@ -1,0 +1,359 @@
+"""GPU: the block norms (torch_block.block_norm, dcn_block_norm_*) against the 64-bit oracle.
+
+Tolerances: with M the output's formula in magnitudes (block_oracle.block_bounds), n the number
+of terms of its longest sum and u = 2^-24, |Δ| <= 16 n' u M + eps/2 |ref|, n' = n + 64. A sum of
+n fp32 terms is off by at most n u of its magnitudes whatever its order; two norms forward and
+two backward chain at most a dozen such sums and products of them (16), 64 covers the
+elementwise roundings, eps/2 the store in the tensor's type."""
+import itertools
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import block_oracle as BO  # noqa: E402
+
+SEED, OFF = 77, 0x123456789A
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def tb():
+    import torch_block
+    return torch_block
+
+
+def tensors(layout, B, C, P, dt, post, pre, gate, seed=0, x=True, residual=True, params=True,
+            shift=0.0):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=g)
+    shape = (B, C, P, 1) if layout == "nchw" else (B, P, C)
+    t = {}
+    if x:
+        t["x"] = rnd(*shape) * 0.7 + shift
+        if gate == "full":
+            t["gate"] = rnd(*shape)
+        elif gate == "image":
+            t["gate"] = rnd(B, C)
+        if params:
+            t["scale"] = rnd(C) * 0.1 + 0.5
+            if post:
+                t["w_post"] = 1 + 0.2 * rnd(C)
+            if post == "layer":
+                t["b_post"] = 0.2 * rnd(C)
+    if residual:
+        t["residual"] = rnd(*shape) * 2 + shift
+    if params and pre:
+        t["w_pre"] = 1 + 0.2 * rnd(C)
+        if pre == "layer":
+            t["b_pre"] = 0.2 * rnd(C)
+    t = {k: v.to(dt).cuda() for k, v in t.items()}
+    return t, rnd(*shape).to(dt).cuda(), rnd(*shape).to(dt).cuda()
+
+
+def rows(v, layout):
+    """float64 on the CPU, [B][P][C] for a map tensor."""
+    if v is None:
+        return None
+    v = v.detach().cpu().double()
+    return v[..., 0].transpose(1, 2) if layout == "nchw" and v.dim() == 4 else v
+
+
+def call(tb, t, post, pre, act, p=0.0, drop="element", rng=(SEED, OFF), **kw):
+    return tb.block_norm(t.get("x"), t.get("residual"), gate=t.get("gate"), gate_act=act,
+                         scale=t.get("scale"), post=post, post_weight=t.get("w_post"),
+                         post_bias=t.get("b_post"), pre=pre, pre_weight=t.get("w_pre"),
+                         pre_bias=t.get("b_pre"), drop_p=p, drop=drop, rng=rng, **kw)
+
+
+def run_and_check(tb, layout, B, C, P, dt, post, pre, gate="none", act="linear", p=0.0,
+                  drop="element", alpha=1.0, eps=1e-6, use=("out", "y"), **mk):
+    t, go, gy = tensors(layout, B, C, P, dt, post, pre, gate, **mk)
+    for v in t.values():
+        v.requires_grad_()
+    out, y = call(tb, t, post, pre, act, p, drop, alpha=alpha, eps=eps)
+    ref = {k: rows(v, layout).requires_grad_() for k, v in t.items()}
+    factor = None
+    if p > 0:
+        n = B * C * P
+        f = torch.from_numpy(BO.drop_factor(n, C * P if drop == "image" else 1, p, SEED, OFF))
+        factor = f.reshape(B, C, P).transpose(1, 2) if layout == "nchw" else f.reshape(B, P, C)
+    kw = dict(post=post, pre=pre, act=act, alpha=alpha, eps=eps, factor=factor)
+    rout, ry = BO.block_forward(ref, **kw)
+    use = [u for u in use if not (u == "y" and not pre) and not (u == "out" and "x" not in t)]
+    g64 = {"out": rows(go, layout), "y": rows(gy, layout)}
+    pick = {"out": (out, go, rout), "y": (y, gy, ry)}
+    grads = torch.autograd.grad([pick[u][0] for u in use], list(t.values()),
+                                [pick[u][1] for u in use], allow_unused=True)
+    refg = torch.autograd.grad([pick[u][2] for u in use], list(ref.values()),
+                               [g64[u] for u in use], allow_unused=True)
+    with torch.no_grad():
+        bounds = BO.block_bounds({k: v.detach() for k, v in ref.items()},
+                                 g64["out"] if "out" in use else None,
+                                 g64["y"] if "y" in use else None, **kw)
+    half = torch.finfo(dt).eps / 2 if dt == torch.bfloat16 else 0.0
+    got = {"out": (out, rout, C)} if "x" in t else {}
+    if pre:
+        got["y"] = (y, ry, C)
+    for k, a, r in zip(t, grads, refg):
+        if r is None:  # a gradient that no output reaches
+            assert a is None or not a.any()
+            continue
+        n = C if k in ("x", "residual") or (k == "gate" and gate == "full") else \
+            (P if k == "gate" else B * P) + C
+        got["grad " + k] = (a, r, n)
+    for name, (a, r, n) in got.items():
+        m = bounds[name.replace("grad ", "")]
+        a, r = rows(a, layout), r.detach()
+        assert a.shape == r.shape, name
+        tol = 16 * (n + 64) * U * m + half * r.abs() + 1e-37
+        err = (a - r).abs()
+        bad = ~(err <= tol)
+        assert not bad.any(), (f"{name}: {int(bad.sum())} / {bad.numel()} off, worst "
+                               f"{float((err / tol).max()):.2f} x tolerance")
+
+
+NORMS = [None, "rms", "layer"]
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+@pytest.mark.parametrize("post,pre", [p for p in itertools.product(NORMS, NORMS)])
+@pytest.mark.parametrize("gate,act", [("none", "linear"), ("full", "silu"), ("image", "sigmoid")])
+def test_variants(tb, dt, layout, post, pre, gate, act):
+    run_and_check(tb, layout, 3, 40, 29, dt, post, pre, gate, act, p=0.1)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+@pytest.mark.parametrize("C", [1, 2, 3, 7, 8, 9, 15, 16, 17, 31, 33, 63, 64, 65, 100, 127, 128, 129,
+                               255, 256, 257, 511, 513, 1000, 1023, 1025])
+def test_channel_counts(tb, dt, layout, C):
+    run_and_check(tb, layout, 2, C, 11, dt, "layer", "rms", "full", "silu", p=0.25, seed=C)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout,B,C,P", [
+    ("rows", 1, 64, 1), ("rows", 1, 4096, 1), ("nchw", 1, 64, 1), ("nchw", 5, 33, 1),
+    ("rows", 5, 33, 1), ("rows", 1, 2047, 3), ("rows", 2, 2048, 5), ("rows", 1, 4097, 4),
+    ("rows", 1, 8192, 3), ("rows", 1, 16384, 2), ("rows", 1, 16385, 2), ("rows", 1, 20000, 2),
+    ("nchw", 1, 2048, 7), ("nchw", 1, 2049, 9), ("nchw", 1, 4099, 8), ("nchw", 2, 600, 49),
+    ("nchw", 300, 8, 4), ("rows", 300, 8, 4), ("nchw", 2, 256, 784), ("rows", 2, 256, 784),
+    ("nchw", 3, 64, 31), ("nchw", 3, 64, 32), ("nchw", 3, 64, 33), ("nchw", 2, 16, 3137),
+    ("rows", 3, 24, 1601)])
+@pytest.mark.parametrize("gate", ["none", "image"])
+def test_shapes(tb, dt, layout, B, C, P, gate):
+    run_and_check(tb, layout, B, C, P, dt, "rms", "layer", gate, "silu", seed=C + P)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+def test_parts(tb, dt, layout):
+    """Absent pieces: the pre norm alone, no residual, no parameters, no pre norm, a gradient of
+    one output only, per-image dropout, another alpha and eps."""
+    base = (tb, layout, 4, 50, 37, dt)
+    for pre in ("rms", "layer"):
+        run_and_check(*base, None, pre, x=False)
+        run_and_check(*base, None, pre, x=False, params=False)
+    run_and_check(*base, "layer", "layer", residual=False)
+    run_and_check(*base, "rms", "layer", params=False, gate="full", act="linear")
+    run_and_check(*base, "rms", None, p=0.5)
+    run_and_check(*base, None, None, gate="image", act="silu")
+    run_and_check(*base, "layer", "rms", use=("out",))
+    run_and_check(*base, "layer", "rms", use=("y",), gate="full", act="sigmoid")
+    run_and_check(*base, "layer", "rms", p=0.4, drop="image", alpha=-0.5, eps=1e-2)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+def test_large_mean(tb, dt, layout):
+    """Means far above the spread: the variance is taken about the mean."""
+    run_and_check(tb, layout, 2, 300, 21, dt, "layer", "layer", shift=64.0)
+
+
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+def test_zero_rows_and_non_finite(tb, layout):
+    """A row of zeros normalises to zero; a NaN or infinity stays in its own position."""
+    t, _, _ = tensors(layout, 2, 48, 10, torch.float32, "rms", "rms", "none")
+    x, res = t["x"], t["residual"]
+    put = (lambda v, b, p, c, w: v.__setitem__((b, c, p, 0), w)) if layout == "nchw" else \
+        (lambda v, b, p, c, w: v.__setitem__((b, p, c), w))
+    clean_out, clean_y = call(tb, t, "rms", "rms", "linear")
+    for c in range(48):
+        put(x, 0, 3, c, 0.0)
+        put(res, 0, 3, c, 0.0)
+    put(x, 1, 5, 7, float("nan"))
+    put(res, 1, 8, 2, float("inf"))
+    out, y = call(tb, t, "rms", "rms", "linear")
+    ro, rc, ry, rcy = (rows(v, layout) for v in (out, clean_out, y, clean_y))
+    assert not ro[0, 3].any() and not ry[0, 3].any()
+    assert torch.isnan(ro[1, 5]).all() and torch.isnan(ry[1, 5]).all()
+    assert torch.isinf(ro[1, 8, 2]) and torch.isnan(ry[1, 8, 2])
+    keep = torch.ones(2, 10, dtype=torch.bool)
+    keep[0, 3] = keep[1, 5] = keep[1, 8] = False
+    assert torch.equal(ro[keep], rc[keep]) and torch.equal(ry[keep], rcy[keep])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_layouts_and_strides_agree(tb, dt):
+    """Channels-last memory, transposed and sliced inputs give the results of dense copies (no
+    dropout, whose elements count in memory order), each gradient in its input's shape."""
+    t, go, gy = tensors("nchw", 3, 24, 35, dt, "layer", "rms", "full")
+    t = {k: v.reshape(3, 24, 5, 7) if v.dim() == 4 else v for k, v in t.items()}
+    go, gy = go.reshape(3, 24, 5, 7), gy.reshape(3, 24, 5, 7)
+
+    def run(conv, names):
+        u = {k: (conv(v) if k in names else v.clone()).requires_grad_() for k, v in t.items()}
+        o, y = call(tb, u, "layer", "rms", "silu")
+        g = torch.autograd.grad((o, y), list(u.values()), (go, gy))
+        return [o, y, *g]
+
+    cl = lambda v: v.contiguous(memory_format=torch.channels_last) if v.dim() == 4 else v
+
+    def odd(v):  # one element off the allocation's start
+        w = torch.empty(v.numel() + 1, dtype=v.dtype, device=v.device)[1:].view(v.shape)
+        return w.copy_(v)
+
+    def wide(v):  # every second column of a larger tensor
+        w = torch.zeros(*v.shape[:-1], 2 * v.shape[-1], dtype=v.dtype, device=v.device)
+        w[..., ::2] = v
+        return w[..., ::2]
+
+    want = run(torch.clone, ())
+    for conv, names in ((wide, list(t)), (odd, list(t)), (cl, ["residual", "gate"])):
+        got = run(lambda v: conv(v.detach()).detach(), names)
+        for a, b in zip(got, want):
+            assert a.shape == b.shape and torch.equal(a, b)
+    got = run(lambda v: cl(v.detach()), list(t))  # runs as token rows: another summation order
+    tol = 2.0 ** -7 if dt == torch.bfloat16 else 1e-4
+    for a, b in zip(got, want):
+        assert a.shape == b.shape
+        assert float((a - b).abs().max()) <= tol * float(b.abs().max())
+
+
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+def test_bitwise_reproducible_and_graph(tb, layout):
+    t, go, gy = tensors(layout, 8, 96, 333, torch.bfloat16, "layer", "layer", "image")
+    for v in t.values():
+        v.requires_grad_()
+    rng = torch.tensor([3, 4], dtype=torch.int64, device="cuda")
+
+    def step():
+        o, y = call(tb, t, "layer", "layer", "sigmoid", p=0.2, rng=rng)
+        return [o.detach(), y.detach(), *torch.autograd.grad((o, y), list(t.values()), (go, gy))]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a = step()
+        b = step()
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        r1 = step()
+    with torch.cuda.graph(g2):
+        r2 = step()
+    for off in (4, 9, 4):
+        rng.copy_(torch.tensor([3, off]))
+        g1.replay()
+        e1 = step()
+        g2.replay()
+        torch.cuda.synchronize()
+        for u, v, w in zip(r1, r2, e1):
+            assert torch.equal(u, w) and torch.equal(v, w)
+
+
+def test_in_place_out(tb):
+    """dcn_block_norm_fwd with out = residual gives the bits of separate tensors."""
+    import dcn_runtime as rt
+    for layout in ("nchw", "rows"):
+        for C in (96, 5000, 20000):
+            t, _, _ = tensors(layout, 2, C, 7, torch.bfloat16, "rms", "layer", "none")
+            out, y = call(tb, t, "rms", "layer", "linear")
+            d = rt.BlockDesc(2, C, 7, 0 if layout == "nchw" else 1, rt.DCN_BF16, 1, 2, 0, 0,
+                             1e-6, 1e-6, 1.0, 0.0, 0, 0, 0)
+            r, y2 = t["residual"].clone(), torch.empty_like(y)
+            io = rt.BlockIO(x=t["x"].data_ptr(), residual=r.data_ptr(),
+                            scale=t["scale"].data_ptr(), w_post=t["w_post"].data_ptr(),
+                            w_pre=t["w_pre"].data_ptr(), b_pre=t["b_pre"].data_ptr(),
+                            out=r.data_ptr(), y=y2.data_ptr())
+            tb._call(r.device, "dcn_block_norm_fwd", d, io)
+            assert torch.equal(r, out) and torch.equal(y2, y)
+
+
+def test_directional_difference(tb):
+    """Gradients against central differences of the operator itself (fp32): the sum of the
+    outputs along go, gy changes by the gradients along a direction. The oracle's difference
+    with the same step has the same truncation; the operator's own rounding is below
+    16 (C + 64) u of the outputs' magnitudes, divided by the step."""
+    layout, B, C, P = "nchw", 2, 24, 15
+    t, go, gy = tensors(layout, B, C, P, torch.float32, "layer", "rms", "image")
+    d = {k: torch.randn(v.shape, generator=torch.Generator().manual_seed(9)).cuda()
+         for k, v in t.items()}
+    u = {k: v.clone().requires_grad_() for k, v in t.items()}
+    grads = torch.autograd.grad(call(tb, u, "layer", "rms", "silu"), list(u.values()), (go, gy))
+    along = sum(float((g.double() * d[k].double()).sum()) for g, k in zip(grads, u))
+    h, s = 2.0 ** -8, []
+    mag = 0.0
+    for sign in (1, -1):
+        v = {k: t[k] + sign * h * d[k] for k in t}
+        o, y = call(tb, v, "layer", "rms", "silu")
+        s.append(float((o.double() * go).sum() + (y.double() * gy).sum()))
+        b = BO.block_bounds({k: rows(w, layout) for k, w in v.items()}, None, None, post="layer",
+                            pre="rms", act="silu")
+        mag += float((b["out"] * rows(go, layout).abs()).sum() +
+                     (b["y"] * rows(gy, layout).abs()).sum())
+    diff = (s[0] - s[1]) / (2 * h)
+
+    def oracle(sign):
+        v = {k: rows(t[k], layout) + sign * h * rows(d[k], layout) for k in t}
+        o, y = BO.block_forward(v, post="layer", pre="rms", act="silu")
+        return float((o * rows(go, layout)).sum() + (y * rows(gy, layout)).sum())
+
+    trunc = abs((oracle(1) - oracle(-1)) / (2 * h) - along)
+    assert abs(diff - along) <= trunc + 16 * (C + 64) * U * mag / (2 * h)
+    assert trunc <= 0.02 * abs(along) + 0.05
+
+
+def test_refusals(tb):
+    t, _, _ = tensors("nchw", 2, 8, 6, torch.float32, "rms", "rms", "full")
+    ok = dict(x=t["x"], residual=t["residual"])
+    tb.block_norm(**ok, pre="rms")
+    for kw, err in [(dict(pre="batch"), ValueError), (dict(gate_act="relu"), ValueError),
+                    (dict(drop="row", drop_p=0.1), ValueError), (dict(drop_p=1.1), ValueError),
+                    (dict(drop_p=0.1), ValueError), (dict(scale=t["x"]), ValueError),
+                    (dict(gate=t["x"][:1]), ValueError),
+                    (dict(pre_weight=torch.ones(8, device="cuda")), RuntimeError),
+                    (dict(post_weight=torch.ones(8, device="cuda"), pre="rms"), RuntimeError),
+                    (dict(pre="rms", eps=float("nan")), RuntimeError),
+                    (dict(pre="rms", eps=-1.0), RuntimeError),
+                    (dict(scale=torch.ones(8, device="cuda").bfloat16()), ValueError)]:
+        with pytest.raises(err):
+            tb.block_norm(**ok, **kw)
+    with pytest.raises(ValueError):
+        tb.block_norm()
+    with pytest.raises(ValueError):
+        tb.block_norm(t["x"], t["residual"].bfloat16())
+    with pytest.raises(RuntimeError):
+        tb.block_norm(None, t["residual"])
+
+
+def test_empty_and_modules(tb):
+    m = tb.BlockNorm(16, post="layer", pre="layer", layer_scale=0.5, drop_p=0.3).cuda()
+    x = torch.randn(4, 16, 6, 6, device="cuda", requires_grad=True)
+    out, y = m(x, x * 2)
+    (out.sum() + (y * y).sum()).backward()
+    assert all(p.grad is not None for p in m.parameters()) and x.grad is not None
+    m.eval()
+    a, b = m(x, x), m(x, x)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    e = x.detach()[:0].requires_grad_()
+    out, y = m(e, e)
+    assert out.shape == y.shape == (0, 16, 6, 6)
+    for p in m.parameters():
+        p.grad = None
+    y.sum().backward()
+    assert not m.pre_weight.grad.any()
