@@ -40,7 +40,7 @@ extern "C" {
                              3: dcn_backward_host_ex; 4: dcn_host_state, dcn_host_alloc;
                              5: dcn_forward_ex (DCN_FWD_NO_COLUMNS), dcn_get_fwd_path,
                                 dcn_workspace_bytes(DCN_WS_FORWARD_NO_COLUMNS);
-                             6: dcn_dropout_*, dcn_block_norm_* */
+                             6: dcn_dropout_*, dcn_block_norm_*, dcn_fp8_* */
 
 typedef enum {
   DCN_OK = 0,
@@ -284,8 +284,10 @@ int dcn_roi_pool_bwd_host(dcn_handle* h, const dcn_roi_desc* d, const float* fea
                           float* grad_features, float* grad_offsets);
 
 /* ---- residual block around a DeformConv2d ------------------------------------- *
- * What stands between two blocks of a network. No counterpart in the reference, whose
- * network is DeformConv2d + BatchNorm + ReLU (train.py:304-337).
+ * What stands between two blocks of a network: the norm after a block, its gate, its
+ * residual scale, dropout, the residual sum and the norm before the next block, as one
+ * operator; dropout alone; and pointwise (1x1) products in 8 bits. No counterpart in the
+ * reference, whose network is DeformConv2d + BatchNorm + ReLU (train.py:304-337).
  *
  * Tensors are dense, of the descriptor's dtype (parameters and gradients too), caller-owned
  * and on the handle's device. A map tensor is DCN_NCHW [B][C][P] or DCN_NHWC [B][P][C]
@@ -367,6 +369,42 @@ int dcn_block_norm_fwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_i
 int dcn_block_norm_workspace(const dcn_block_desc* d, size_t* bytes);
 int dcn_block_norm_bwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_io* io, void* ws,
                        size_t ws_bytes);
+
+/* 8-bit pointwise products. A quantised matrix is q[rows][K] e4m3 bytes (OCP, 448 largest),
+ * K a multiple of 128 (padded with zeros), 16-byte aligned, with exponent bytes
+ * s[K / 128][stride], biased by 127: the value of q[r][k] is q · 2^(s[k / 128][r / block] - 127).
+ * block = 1: stride = rows rounded up to 128; block = 128: stride = rows / 128 rounded up;
+ * s is 4-byte aligned. The exponent of a block is the smallest e >= -126 with max|v| <=
+ * 448 · 2^e over its finite values; the bytes are round-to-nearest-even of v · 2^-e; an
+ * infinity or NaN becomes NaN. */
+typedef struct {
+  int B, C, P;        /* a map tensor */
+  int layout, dtype;
+} dcn_fp8_desc;
+/* Quantise a map tensor, either way or both in one read (NULL: not wanted):
+ *   by token:   q_tok[B*P][Cp], Cp = C rounded up to 128, s_tok[Cp/128][B*P up to 128]
+ *   by channel: q_ch[C][Kt], the tokens as columns: DCN_NHWC Kt = B*P rounded up to 128;
+ *               DCN_NCHW Kt = B * Pp, Pp = P rounded up to 128 (an image's blocks end with
+ *               it), s_ch[Kt/128][C up to 128] */
+int dcn_fp8_quantize(dcn_handle* h, const dcn_fp8_desc* d, const void* v, void* q_tok,
+                     void* s_tok, void* q_ch, void* s_ch);
+/* Quantise a weight w[O][C] in blocks of 128 x 128, as it stands (q[O][Cp], s[Cp/128][ceil(O/128)])
+ * and transposed (qT[C][Op], sT[Op/128][ceil(C/128)]; NULL: not wanted). */
+int dcn_fp8_quantize_weight(dcn_handle* h, int O, int C, int dtype, const void* w, void* q,
+                            void* s, void* qT, void* sT);
+typedef struct {
+  int M, N, K;          /* a[M][K], b[N][K]; K a multiple of 128 */
+  int a_block, b_block; /* rows that share an exponent: 1 or 128 */
+  int layout;           /* DCN_NHWC: out[M][N]; DCN_NCHW: b's rows are the tokens of N / P
+                           images and out is [N / P][M][P] */
+  int P;                /* DCN_NCHW only */
+  int out_dtype;        /* dcn_dtype */
+} dcn_fp8_matmul_desc;
+/* out = a · bᵀ with fp32 accumulation. ws: dcn_fp8_matmul_workspace bytes (may be 0, then
+ * NULL), one per call in flight. */
+int dcn_fp8_matmul_workspace(const dcn_fp8_matmul_desc* d, size_t* bytes);
+int dcn_fp8_matmul(dcn_handle* h, const dcn_fp8_matmul_desc* d, const void* a, const void* sa,
+                   const void* b, const void* sb, void* out, void* ws, size_t ws_bytes);
 
 /* ---- in-library kernel timing (HIP events on the handle's stream) ---------- */
 typedef enum {

@@ -154,9 +154,122 @@ int block_spans(const Span* in, int nin, const Span* out, int nout, size_t es,
   return DCN_OK;
 }
 
+size_t up128(size_t v) { return (v + 127) / 128 * 128; }
+
+// Bytes of an 8-bit matrix of `rows` x K (K a multiple of 128) and of its exponents.
+size_t fp8_bytes(size_t rows, size_t k) { return rows * k; }
+size_t exp_bytes(size_t rows, size_t k, int block) {
+  return k / 128 * (block == 128 ? (rows + 127) / 128 : up128(rows));
+}
+
+int fp8_pair(const void* q, const void* s, const char* what) {
+  if ((q != nullptr) != (s != nullptr))
+    return fail(DCN_ERR_INVALID, (std::string(what) + ": bytes and exponents come together").c_str());
+  if (!aligned(q, 16) || !aligned(s, 4))
+    return fail(DCN_ERR_INVALID,
+                (std::string(what) + ": bytes 16-byte, exponents 4-byte aligned").c_str());
+  return DCN_OK;
+}
+
+// At most 2^31 - 1 tiles of 128 x 128 (one workgroup each).
+bool tiles_ok(double a, double b, double images) {
+  return std::ceil(a / 128) * std::ceil(b / 128) * images < 2147483647.0;
+}
+
+int fp8_matmul_check(const dcn_fp8_matmul_desc* d) {
+  if (!d) return fail(DCN_ERR_INVALID, "null descriptor");
+  if (d->M <= 0 || d->N <= 0 || d->K <= 0) return fail(DCN_ERR_INVALID, "M, N, K must be positive");
+  if (d->K % 128) return fail(DCN_ERR_INVALID, "K must be a multiple of 128");
+  for (int b : {d->a_block, d->b_block})
+    if (b != 1 && b != 128) return fail(DCN_ERR_INVALID, "exponents are per 1 or 128 rows");
+  if (d->layout != DCN_NCHW && d->layout != DCN_NHWC) return fail(DCN_ERR_INVALID, "unknown layout");
+  if (d->layout == DCN_NCHW && (d->P <= 0 || d->N % d->P))
+    return fail(DCN_ERR_INVALID, "DCN_NCHW needs N a multiple of P");
+  if (!dtype_ok(d->out_dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
+  if (d->M > (1 << 30) || d->N > (1 << 30) || d->K > (1 << 30) || !tiles_ok(d->M, d->N, 1))
+    return fail(DCN_ERR_UNSUPPORTED, "M, N or K above 2^30, or 2^31 tiles of the product");
+  return DCN_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int dcn_fp8_quantize(dcn_handle* h, const dcn_fp8_desc* d, const void* v, void* q_tok, void* s_tok,
+                     void* q_ch, void* s_ch) {
+  if (!d) return fail(DCN_ERR_INVALID, "null descriptor");
+  if (d->B <= 0 || d->C <= 0 || d->P <= 0) return fail(DCN_ERR_INVALID, "B, C, P must be positive");
+  if (!dtype_ok(d->dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
+  if (d->layout != DCN_NCHW && d->layout != DCN_NHWC) return fail(DCN_ERR_INVALID, "unknown layout");
+  const bool maps = d->layout == DCN_NCHW;
+  const size_t T = (size_t)d->B * d->P, C = d->C;
+  const size_t kt = maps ? d->B * up128(d->P) : up128(T);
+  if (T > (1u << 30) || kt > (1u << 30) || C > (1u << 30) ||
+      !tiles_ok(maps ? d->C : (double)T, maps ? d->P : d->C, maps ? d->B : 1))
+    return fail(DCN_ERR_UNSUPPORTED, "tensor too large");
+  if (int rc = fp8_pair(q_tok, s_tok, "by token")) return rc;
+  if (int rc = fp8_pair(q_ch, s_ch, "by channel")) return rc;
+  if (!v || !(q_tok || q_ch)) return fail(DCN_ERR_INVALID, "null tensor");
+  const size_t es = dtype_bytes(d->dtype);
+  const Span in[] = {{v, T * C * es}};
+  if (!aligned(v, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
+  const Span out[] = {{q_tok, fp8_bytes(T, up128(C))}, {s_tok, exp_bytes(T, up128(C), 1)},
+                      {q_ch, fp8_bytes(C, kt)}, {s_ch, exp_bytes(C, kt, 1)}};
+  if (int rc = block_spans(in, 1, out, 4, 1, nullptr, nullptr)) return rc;
+  DeviceScope ds;
+  if (int rc = ds.bind(h)) return rc;
+  return done(dcn::launch_fp8_quantize(d->B, d->C, d->P, d->layout, d->dtype, v, q_tok, s_tok, q_ch,
+                                       s_ch, ds.stream),
+              "fp8_quantize");
+}
+
+int dcn_fp8_quantize_weight(dcn_handle* h, int O, int C, int dtype, const void* w, void* q, void* s,
+                            void* qT, void* sT) {
+  if (O <= 0 || C <= 0) return fail(DCN_ERR_INVALID, "O, C must be positive");
+  if (!dtype_ok(dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
+  if (O > (1 << 30) || C > (1 << 30) || !tiles_ok(O, C, 1))
+    return fail(DCN_ERR_UNSUPPORTED, "weight too large");
+  if (int rc = fp8_pair(q, s, "weight")) return rc;
+  if (int rc = fp8_pair(qT, sT, "transposed weight")) return rc;
+  if (!w || !(q || qT)) return fail(DCN_ERR_INVALID, "null tensor");
+  const size_t es = dtype_bytes(dtype);
+  if (!aligned(w, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
+  const Span in[] = {{w, (size_t)O * C * es}};
+  const Span out[] = {{q, fp8_bytes(O, up128(C))}, {s, exp_bytes(O, up128(C), 128)},
+                      {qT, fp8_bytes(C, up128(O))}, {sT, exp_bytes(C, up128(O), 128)}};
+  if (int rc = block_spans(in, 1, out, 4, 1, nullptr, nullptr)) return rc;
+  DeviceScope ds;
+  if (int rc = ds.bind(h)) return rc;
+  return done(dcn::launch_fp8_quantize_weight(O, C, dtype, w, q, s, qT, sT, ds.stream),
+              "fp8_quantize_weight");
+}
+
+int dcn_fp8_matmul_workspace(const dcn_fp8_matmul_desc* d, size_t* bytes) {
+  if (int rc = fp8_matmul_check(d)) return rc;
+  if (!bytes) return fail(DCN_ERR_INVALID, "null out pointer");
+  *bytes = dcn::fp8_matmul_ws_bytes(*d);
+  return DCN_OK;
+}
+
+int dcn_fp8_matmul(dcn_handle* h, const dcn_fp8_matmul_desc* d, const void* a, const void* sa,
+                   const void* b, const void* sb, void* out, void* ws, size_t ws_bytes) {
+  if (int rc = fp8_matmul_check(d)) return rc;
+  if (!a || !b || !out) return fail(DCN_ERR_INVALID, "null tensor");
+  if (int rc = fp8_pair(a, sa, "a")) return rc;
+  if (int rc = fp8_pair(b, sb, "b")) return rc;
+  const size_t es = dtype_bytes(d->out_dtype), need = dcn::fp8_matmul_ws_bytes(*d);
+  if (need && (!ws || ws_bytes < need))
+    return fail(DCN_ERR_WORKSPACE, "fp8_matmul workspace too small");
+  if (!aligned(ws, 256)) return fail(DCN_ERR_INVALID, "workspace must be 256-byte aligned");
+  if (!aligned(out, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
+  const Span in[] = {{a, fp8_bytes(d->M, d->K)}, {sa, exp_bytes(d->M, d->K, d->a_block)},
+                     {b, fp8_bytes(d->N, d->K)}, {sb, exp_bytes(d->N, d->K, d->b_block)}};
+  const Span outs[] = {{out, (size_t)d->M * d->N * es}, {need ? ws : nullptr, need}};
+  if (int rc = block_spans(in, 4, outs, 2, 1, nullptr, nullptr)) return rc;
+  DeviceScope ds;
+  if (int rc = ds.bind(h)) return rc;
+  return done(dcn::launch_fp8_matmul(*d, a, sa, b, sb, out, ws, ds.stream), "fp8_matmul");
+}
 
 int dcn_block_norm_fwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_io* io) {
   dcn::BlockArgs a;

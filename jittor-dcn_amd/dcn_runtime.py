@@ -72,6 +72,17 @@ class BlockIO(ctypes.Structure):
                  "grad_scale", "grad_w_post", "grad_b_post", "grad_w_pre", "grad_b_pre")]
 
 
+class Fp8Desc(ctypes.Structure):
+    """dcn_fp8_desc (include/dcn.h): a map tensor to quantise."""
+    _fields_ = [(n, ctypes.c_int) for n in ("B", "C", "P", "layout", "dtype")]
+
+
+class Fp8MatmulDesc(ctypes.Structure):
+    """dcn_fp8_matmul_desc (include/dcn.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("M", "N", "K", "a_block", "b_block", "layout", "P",
+                                            "out_dtype")]
+
+
 _vp = ctypes.c_void_p
 _ip = ctypes.POINTER(ctypes.c_int)
 _dp = ctypes.POINTER(Desc)
@@ -146,6 +157,11 @@ SIGNATURES = {
     "dcn_block_norm_fwd": [_vp, ctypes.POINTER(BlockDesc), ctypes.POINTER(BlockIO)],
     "dcn_block_norm_workspace": [ctypes.POINTER(BlockDesc), ctypes.POINTER(_sz)],
     "dcn_block_norm_bwd": [_vp, ctypes.POINTER(BlockDesc), ctypes.POINTER(BlockIO), _vp, _sz],
+    "dcn_fp8_quantize": [_vp, ctypes.POINTER(Fp8Desc), _vp, _vp, _vp, _vp, _vp],
+    "dcn_fp8_quantize_weight": [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp,
+                                _vp],
+    "dcn_fp8_matmul_workspace": [ctypes.POINTER(Fp8MatmulDesc), ctypes.POINTER(_sz)],
+    "dcn_fp8_matmul": [_vp, ctypes.POINTER(Fp8MatmulDesc), _vp, _vp, _vp, _vp, _vp, _vp, _sz],
 }
 _RESTYPES = {"dcn_last_error": ctypes.c_char_p}
 

@@ -302,3 +302,198 @@ class BlockNorm(torch.nn.Module):
                           post_bias=self.post_bias, pre=self.pre, pre_weight=self.pre_weight,
                           pre_bias=self.pre_bias, eps=self.eps, drop_p=p, drop=self.drop,
                           rng=_fresh_rng(self.rng) if p > 0 else None)
+
+
+# ---------------------------------------------------------------------------- 8-bit products
+def _up(n, m=128):
+    return (n + m - 1) // m * m
+
+
+def _bytes(dev, *shape):
+    return torch.empty(shape, dtype=torch.uint8, device=dev)
+
+
+class Fp8Weight:
+    """A weight [O, C] kept in 8 bits: q [O, C up to 128s] e4m3 bytes and exponents
+    [C / 128, O / 128] (each up; bias 127), one per 128 x 128 block (include/dcn.h). What a
+    server keeps instead of the weight; fp8_quantize_weight makes one."""
+
+    def __init__(self, q, exponents, in_features):
+        O, C = q.shape[0], int(in_features)
+        for t, shape in ((q, (O, _up(C))), (exponents, (_up(C) // 128, -(-O // 128)))):
+            if t.dtype != torch.uint8 or not t.is_cuda or tuple(t.shape) != shape or \
+                    t.device != q.device:
+                raise ValueError(f"Fp8Weight: expected uint8 {shape} on a GPU, not "
+                                 f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        self.q, self.exponents = _at16(q), _at16(exponents)
+        self.out_features, self.in_features = O, C
+
+
+def _at16(t):
+    """Dense and 16-byte aligned (a slice of a larger buffer may not be)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _quantize_weight(w, plain, transposed):
+    O, C = w.shape
+    w, dev = w.contiguous(), w.device
+    q = e = qt = et = None
+    if plain:
+        q, e = _bytes(dev, O, _up(C)), _bytes(dev, _up(C) // 128, -(-O // 128))
+    if transposed:
+        qt, et = _bytes(dev, C, _up(O)), _bytes(dev, _up(O) // 128, -(-C // 128))
+    _call(dev, "dcn_fp8_quantize_weight", O, C, _DT[w.dtype], _ptr(w), _ptr(q), _ptr(e),
+          _ptr(qt), _ptr(et))
+    return q, e, qt, et
+
+
+def fp8_quantize_weight(w):
+    """Fp8Weight of a float32 or bfloat16 weight [O, C] (or [O, C, 1, 1])."""
+    _dtype(w, "fp8_quantize_weight")
+    if w.dim() == 4 and w.shape[2:] == (1, 1):
+        w = w.flatten(1)
+    if w.dim() != 2 or not w.numel():
+        raise ValueError(f"fp8_quantize_weight: a weight is [O, C], not {tuple(w.shape)}")
+    q, e, _, _ = _quantize_weight(w.detach(), True, False)
+    return Fp8Weight(q, e, w.shape[1])
+
+
+def _quantize(v, geo, tokens, channels):
+    """(bytes, exponents) by token and by channel of a map tensor in `geo`'s layout."""
+    layout, B, C, P, _ = geo
+    T, dev = B * P, v.device
+    kt = B * _up(P) if layout == rt.DCN_NCHW else _up(T)
+    q = e = qc = ec = None
+    if tokens:
+        q, e = _bytes(dev, T, _up(C)), _bytes(dev, _up(C) // 128, _up(T))
+    if channels:
+        qc, ec = _bytes(dev, C, kt), _bytes(dev, kt // 128, _up(C))
+    _call(dev, "dcn_fp8_quantize", rt.Fp8Desc(B, C, P, layout, _DT[v.dtype]), _ptr(v), _ptr(q),
+          _ptr(e), _ptr(qc), _ptr(ec))
+    return q, e, qc, ec
+
+
+def _matmul(desc, a, sa, b, sb, out):
+    nbytes = ctypes.c_size_t()
+    rt.check(rt.load().dcn_fp8_matmul_workspace(desc, ctypes.byref(nbytes)),
+             "dcn_fp8_matmul_workspace")
+    ws = _bytes(out.device, nbytes.value) if nbytes.value else None
+    _call(out.device, "dcn_fp8_matmul", desc, _ptr(a), _ptr(sa), _ptr(b), _ptr(sb), _ptr(out),
+          _ptr(ws), nbytes.value)
+
+
+def _pointwise(geo, O, q, e, wq, we, like):
+    """The map tensor [.., O, ..] of tokens q and a 128 x 128 blocked weight wq [O][K]."""
+    layout, B, _, P, mf = geo
+    T, K, dt = B * P, q.shape[1], _DT[like.dtype]
+    if like.dim() == 4:
+        shape = (B, O, *like.shape[2:])
+        out = torch.empty(shape, dtype=like.dtype, device=like.device, memory_format=mf)
+    else:
+        out = torch.empty((*like.shape[:-1], O), dtype=like.dtype, device=like.device)
+    if layout == rt.DCN_NCHW:
+        d = rt.Fp8MatmulDesc(O, T, K, 128, 1, layout, P, dt)
+        _matmul(d, wq, we, q, e, out)
+    else:
+        d = rt.Fp8MatmulDesc(T, O, K, 1, 128, layout, 0, dt)
+        _matmul(d, q, e, wq, we, out)
+    return out
+
+
+class _Fp8Pointwise(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, geo):
+        mf = geo[-1]
+        x = x.contiguous(memory_format=mf)
+        O = w.shape[0]
+        need_x, need_w = ctx.needs_input_grad[:2]
+        wq, we, wqt, wet = _quantize_weight(w, True, need_x)
+        q, e, qc, ec = _quantize(x, geo, True, need_w)
+        y = _pointwise(geo, O, q, e, wq, we, x)
+        ctx.geo, ctx.shapes = geo, (x.shape, w.shape, x.dtype)
+        ctx.save_for_backward(wqt, wet, qc, ec)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        (layout, B, C, P, mf), (xs, wshape, dt) = ctx.geo, ctx.shapes
+        wqt, wet, qc, ec = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        gy = gy.contiguous(memory_format=mf)
+        O = wshape[0]
+        geo = (layout, B, O, P, mf)
+        q, e, gc, gec = _quantize(gy, geo, need_x, need_w)
+        gx = gw = None
+        if need_x:
+            gx = _pointwise(geo, C, q, e, wqt, wet, gy)
+        if need_w:
+            gw = torch.empty(wshape, dtype=dt, device=gy.device)
+            d = rt.Fp8MatmulDesc(O, C, gc.shape[1], 1, 1, rt.DCN_NHWC, 0, _DT[dt])
+            _matmul(d, gc, gec, qc, ec, gw)
+        return gx, gw, None
+
+
+def fp8_pointwise(x, weight):
+    """x · weightᵀ over the channels (dim 1 of a 4-d tensor, else the last): a linear layer of
+    token rows or a 1x1 convolution of maps, its products in 8 bits with one power-of-two scale
+    per 128 channels of a token (128 tokens of a channel in the weight's gradient; 128 x 128 of
+    the weight) and fp32 sums.
+
+    weight: [O, C] (or [O, C, 1, 1]) of x's dtype, rounded in the call, gradients for both; or an
+    Fp8Weight (no gradients), as a server keeps it."""
+    dt = _dtype(x, "fp8_pointwise")
+    geo = _layout(x)
+    C = geo[2]
+    if x.dim() == 0 or C == 0:
+        raise ValueError("fp8_pointwise: no channels")
+    if isinstance(weight, Fp8Weight):
+        if weight.in_features != C or weight.q.device != x.device:
+            raise ValueError(f"fp8_pointwise: the weight takes {weight.in_features} channels on "
+                             f"{weight.q.device}, x has {C} on {x.device}")
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("fp8_pointwise: an Fp8Weight is for inference (no gradients)")
+        O = weight.out_features
+    else:
+        O = weight.shape[0] if weight.dim() else 0
+        if weight.dim() == 4 and tuple(weight.shape[2:]) == (1, 1):
+            weight = weight.flatten(1)
+        _same(x, weight, "fp8_pointwise", "weight", (O, C))
+        if O == 0:
+            raise ValueError("fp8_pointwise: no output channels")
+    if not x.numel():  # no tokens
+        shape = (x.shape[0], O, *x.shape[2:]) if x.dim() == 4 else (*x.shape[:-1], O)
+        y = x.new_empty(shape)
+        return y if isinstance(weight, Fp8Weight) else y + 0 * (x.sum() + weight.sum())
+    if isinstance(weight, Fp8Weight):
+        xc = x.contiguous(memory_format=geo[-1])
+        q, e, _, _ = _quantize(xc, geo, True, False)
+        return _pointwise(geo, O, q, e, weight.q, weight.exponents, xc)
+    return _Fp8Pointwise.apply(x, weight, geo)
+
+
+class Fp8Pointwise(torch.nn.Module):
+    """fp8_pointwise with its weight [out, in] (no bias: a norm or a residual scale follows it in
+    a block). serve() replaces the weight by its 8-bit form for inference."""
+
+    def __init__(self, in_channels, out_channels):
+        super().__init__()
+        self.in_channels, self.out_channels = in_channels, out_channels
+        self.weight = torch.nn.Parameter(torch.randn(out_channels, in_channels) *
+                                         in_channels ** -0.5)
+        self.weight8 = None
+
+    def serve(self):
+        self.weight8 = fp8_quantize_weight(self.weight)
+        return self
+
+    def train(self, mode=True):
+        if mode:
+            self.weight8 = None
+        return super().train(mode)
+
+    def forward(self, x):
+        if self.weight8 is not None and not (torch.is_grad_enabled() and x.requires_grad):
+            return fp8_pointwise(x, self.weight8)
+        return fp8_pointwise(x, self.weight)

@@ -136,3 +136,44 @@ def block_bounds(t, go, gy, *, post=None, pre=None, act="linear", alpha=1.0, eps
             m = back(m, post, "w_post", h1, r1)
         res["x"] = m
     return res
+
+
+# ---- 8-bit blocks --------------------------------------------------------------------------
+def fp8_round(v, rows, cols):
+    """(bytes' values, exponents) of v [R][C] (float64, dims multiples of rows / cols) in blocks of
+    rows x cols: exponent e = the smallest integer >= -126 with max|v| <= 448 * 2^e over the
+    finite values, value = e4m3(v * 2^-e) by round-half-even on a grid of 2^(x - 3), x the
+    value's exponent, at least -6; non-finite values become NaN."""
+    v = np.asarray(v, np.float64)
+    R, C = v.shape
+    blk = v.reshape(R // rows, rows, C // cols, cols)
+    mag = np.where(np.isfinite(blk), np.abs(blk), 0.0).max((1, 3), keepdims=True)
+    m, x = np.frexp(mag)  # mag = m * 2^x
+    e = np.where(mag > 0, x - 9 + (m > 0.875), -126)
+    e = np.maximum(e, -126)
+    with np.errstate(invalid="ignore"):
+        s = np.ldexp(blk, -e)
+        _, x = np.frexp(s)
+        step = np.ldexp(1.0, np.maximum(x - 1, -6) - 3)
+        q = np.rint(s / step) * step
+    q = np.where(np.isfinite(blk), q, np.nan)
+    return q.reshape(R, C), e[:, 0, :, 0]
+
+
+def fp8_value(v, rows, cols):
+    """The values that v [R][C] (any size) stands for after the rounding."""
+    v = np.asarray(v, np.float64)
+    R, C = v.shape
+    p = np.zeros((-(-R // rows) * rows, -(-C // cols) * cols))
+    p[:R, :C] = v
+    q, e = fp8_round(p, rows, cols)
+    return np.ldexp(q, np.repeat(np.repeat(e, rows, 0), cols, 1))[:R, :C]
+
+
+def e4m3_decode(b):
+    """Values of OCP e4m3 bytes."""
+    b = np.asarray(b, np.uint8).astype(np.int64)
+    s, x, m = b >> 7, (b >> 3) & 15, b & 7
+    v = np.where(x == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (x - 10.0))
+    v = np.where((x == 15) & (m == 7), np.nan, v)
+    return np.where(s == 1, -v, v)

@@ -157,3 +157,69 @@ def test_block_oracle_gradients_against_differences(post, pre, gate):
         return (o, y) if pre else o
 
     assert torch.autograd.gradcheck(fn, [t[k].requires_grad_() for k in names])
+
+
+# ---- 8-bit products
+def test_fp8_rounding_is_the_nearest():
+    """fp8_round picks, for each value, a nearest multiple the byte format holds."""
+    g = np.random.default_rng(3)
+    v = g.standard_normal((4, 256)) * np.exp2(g.integers(-12, 9, (4, 256)))
+    v[0, :128] = 0
+    q, e = BO.fp8_round(v, 1, 128)
+    grid = np.unique(BO.e4m3_decode(np.arange(256))[~np.isnan(BO.e4m3_decode(np.arange(256)))])
+    s = np.ldexp(v, -np.repeat(e, 128, 1))
+    assert np.isin(q, grid).all() and np.abs(s).max() <= 448
+    assert np.array_equal(np.abs(s - q), np.abs(s[..., None] - grid).min(-1))
+    assert e[0, 0] == -126 and all(448 * 2.0 ** (e[i, 1] - 1) < np.abs(v[i, 128:]).max()
+                                   for i in range(4))
+
+
+A = OK_PTR
+
+
+@pytest.mark.parametrize("kw,ptr,msg", [
+    (dict(B=0), {}, "positive"), (dict(dtype=5), {}, "dtype"), (dict(layout=3), {}, "layout"),
+    (dict(), dict(s_tok=None), "come together"), (dict(), dict(q_ch=A * 9), "come together"),
+    (dict(), dict(q_tok=A * 2 + 8), "16-byte"), (dict(), dict(s_tok=A * 3 + 2), "4-byte"),
+    (dict(), dict(q_tok=None, s_tok=None), "null tensor"), (dict(), dict(v=None), "null tensor"),
+    (dict(), dict(v=A + 2), "aligned"), (dict(), dict(q_tok=A + 16), "overlaps"),
+    (dict(), dict(s_tok=A * 2), "two outputs"), (dict(B=1 << 20, P=1 << 20), {}, "too large"),
+    (dict(), {}, "null handle"),
+])
+def test_fp8_quantize_refusals(kw, ptr, msg):
+    d = rt.Fp8Desc(**{**dict(B=2, C=8, P=6, layout=0, dtype=0), **kw})
+    p = {**dict(v=A, q_tok=A * 2, s_tok=A * 3, q_ch=None, s_ch=None), **ptr}
+    assert rt.load().dcn_fp8_quantize(None, ctypes.byref(d), *p.values()) < 0
+    assert msg in rt.last_error()
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(O=0), "positive"), (dict(C=-3), "positive"), (dict(dtype=2), "dtype"),
+    (dict(w=None), "null tensor"), (dict(q=None, s=None), "null tensor"),
+    (dict(s=None), "come together"), (dict(qT=A * 5), "come together"),
+    (dict(q=A + 64), "overlaps"), (dict(w=A + 1), "aligned"), (dict(O=1 << 30, C=1 << 30), "large"),
+    (dict(), "null handle"),
+])
+def test_fp8_quantize_weight_refusals(kw, msg):
+    p = {**dict(O=20, C=30, dtype=0, w=A, q=A * 2, s=A * 3, qT=None, sT=None), **kw}
+    assert rt.load().dcn_fp8_quantize_weight(None, *p.values()) < 0
+    assert msg in rt.last_error()
+
+
+@pytest.mark.parametrize("kw,ptr,msg", [
+    (dict(M=0), {}, "positive"), (dict(K=-128), {}, "positive"), (dict(K=100), {}, "multiple of 128"),
+    (dict(a_block=64), {}, "1 or 128"), (dict(b_block=0), {}, "1 or 128"),
+    (dict(layout=2), {}, "layout"), (dict(layout=0, P=0), {}, "multiple of P"),
+    (dict(layout=0, P=7), {}, "multiple of P"), (dict(out_dtype=9), {}, "dtype"),
+    (dict(M=1 << 30, N=1 << 30), {}, "2^31 tiles"),
+    (dict(), dict(a=None), "null tensor"), (dict(), dict(sb=None), "come together"),
+    (dict(), dict(b=A * 3 + 4), "16-byte"), (dict(), dict(sa=A * 2 + 1), "4-byte"),
+    (dict(), dict(out=A * 5 + 2), "aligned"), (dict(), dict(out=A * 3), "overlaps"),
+    (dict(), dict(ws=A * 6 + 16), "256-byte"), (dict(), {}, "null handle"),
+])
+def test_fp8_matmul_refusals(kw, ptr, msg):
+    d = rt.Fp8MatmulDesc(**{**dict(M=16, N=24, K=256, a_block=1, b_block=128, layout=1, P=0,
+                                   out_dtype=0), **kw})
+    p = {**dict(a=A, sa=A * 2, b=A * 3, sb=A * 4, out=A * 5, ws=None, n=0), **ptr}
+    assert rt.load().dcn_fp8_matmul(None, ctypes.byref(d), *p.values()) < 0
+    assert msg in rt.last_error()

@@ -1,0 +1,306 @@
+"""GPU: 8-bit pointwise products (torch_block.fp8_*, dcn_fp8_*) against the 64-bit oracle.
+
+The rounding to 8 bits is exact arithmetic, so bytes (as values) and exponents must be the
+oracle's. Products: each e4m3 product and its power-of-two scale are exact in fp32 and a sum of K
+fp32 terms is off by at most K u of its magnitudes, u = 2^-24: |Δ| <= (K + 128) u Σ|a b| +
+eps/2 |ref|, the 128 for sums over parts of K joined later and a step of the result's exponent.
+That is the bound of fp32 results. bf16 results come from the 8-bit MFMA, which cuts the products
+of 8 neighbouring k's below 2^-13 of the largest one's power of two (measured on the instruction
+with single pairs of products): each of the other 7 loses less than 2^-13 max|a b|, so a group
+loses less than 7 2^-13 of its Σ|a b|, and so does the whole sum; that is added for bf16."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import block_oracle as BO  # noqa: E402
+
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def tb():
+    import torch_block
+    return torch_block
+
+
+def make(shape, dt, seed=0, spread=1.0):
+    """Normal values whose magnitudes vary by 2^±(4 spread) between the elements."""
+    g = torch.Generator().manual_seed(seed)
+    v = torch.randn(shape, generator=g) * torch.exp2(4 * spread * torch.randn(shape, generator=g))
+    return v.to(dt).cuda()
+
+
+def up(n):
+    return -(-n // 128) * 128
+
+
+def np64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def check_blocks(v, q, e, K):
+    """Bytes q [R][Kp] and exponents e [Kp/128][>= R] of v [R][K'] (oracle layout: K' = Kp)."""
+    R = v.shape[0]
+    want, we = BO.fp8_round(v, 1, 128)
+    got = BO.e4m3_decode(q.cpu().numpy())
+    assert np.array_equal(e.cpu().numpy()[:, :R].T.astype(int) - 127, we)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(np.nan_to_num(got), np.nan_to_num(want))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+@pytest.mark.parametrize("B,C,P", [(1, 1, 1), (2, 3, 5), (1, 128, 128), (2, 127, 129), (3, 129, 127),
+                                   (2, 260, 49), (2, 64, 784), (1, 1000, 77), (5, 16, 1),
+                                   (1, 256, 300)])
+def test_quantize(tb, dt, layout, B, C, P):
+    shape = (B, C, P, 1) if layout == "nchw" else (B, P, C)
+    x = make(shape, dt, seed=C + P)
+    if P > 4:  # an infinity, a NaN, a block of zeros and values far below the block's largest
+        f = x.view(-1)
+        f[0], f[min(7, f.numel() - 1)] = float("inf"), float("nan")
+        f[f.numel() // 2:f.numel() // 2 + 40] = 0.0
+    geo = tb._layout(x)
+    q, e, qc, ec = tb._quantize(x, geo, True, True)
+    img = np64(x).reshape(B, C, P) if layout == "nchw" else np64(x).reshape(B, P, C).transpose(0, 2, 1)
+    tok = np.zeros((B * P, up(C)))
+    tok[:, :C] = img.transpose(0, 2, 1).reshape(B * P, C)
+    check_blocks(tok, q, e, up(C))
+    if layout == "nchw":
+        ch = np.zeros((C, B, up(P)))
+        ch[:, :, :P] = img.transpose(1, 0, 2)
+        ch = ch.reshape(C, -1)
+    else:
+        ch = np.zeros((C, up(B * P)))
+        ch[:, :B * P] = tok[:, :C].T
+    check_blocks(ch, qc, ec, ch.shape[1])
+    # either alone gives the same bytes
+    assert torch.equal(tb._quantize(x, geo, True, False)[0], q)
+    assert torch.equal(tb._quantize(x, geo, False, True)[2], qc)
+
+
+def test_rounding_of_every_half_step(tb):
+    """Every e4m3 value, the midpoints between neighbours (ties to even) and their neighbours in
+    fp32, under a block maximum of 448, 1.75 * 2^k and just above it."""
+    grid = np.unique(np.abs(BO.e4m3_decode(np.arange(256)))[~np.isnan(BO.e4m3_decode(np.arange(256)))])
+    mid = (grid[:-1] + grid[1:]) / 2
+    vals = np.concatenate([grid, mid, np.nextafter(mid.astype(np.float32), np.float32(1e9)),
+                           np.nextafter(mid.astype(np.float32), np.float32(0))])
+    vals = np.concatenate([vals, -vals]).astype(np.float32)
+    rows = []
+    for top in (448.0, np.nextafter(np.float32(448), np.float32(1e9)), 449.0, 1.75 * 2.0 ** -20,
+                2.0 ** -126, 2.0 ** -140, 3e38):
+        for i in range(0, len(vals), 127):
+            r = np.zeros(128, np.float32)
+            part = vals[i:i + 127] * np.float32(top / 448.0 if top < 1 else 1.0)
+            r[:len(part)] = np.clip(part, -top, top)
+            r[127] = top
+            rows.append(r)
+    v = torch.from_numpy(np.stack(rows)).cuda()
+    q, e, _, _ = tb._quantize(v, tb._layout(v), True, False)
+    check_blocks(np64(v), q, e, 128)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("O,C", [(1, 1), (5, 130), (128, 128), (127, 300), (300, 127), (640, 256)])
+def test_quantize_weight(tb, dt, O, C):
+    w = make((O, C), dt, seed=O)
+    q, e, qt, et = tb._quantize_weight(w, True, True)
+    p = np.zeros((up(O), up(C)))
+    p[:O, :C] = np64(w)
+    want, we = BO.fp8_round(p, 128, 128)
+    assert np.array_equal(e.cpu().numpy().astype(int) - 127, we.T)
+    assert np.array_equal(et.cpu().numpy().astype(int) - 127, we)
+    assert np.array_equal(BO.e4m3_decode(q.cpu().numpy()), want[:O])
+    assert np.array_equal(BO.e4m3_decode(qt.cpu().numpy()), want[:, :C].T)
+
+
+def tok(v):
+    """[tokens][channels] float64 of a map tensor."""
+    v = np64(v)
+    return v.reshape(*v.shape[:2], -1).transpose(0, 2, 1).reshape(-1, v.shape[1]) if v.ndim == 4 \
+        else v.reshape(-1, v.shape[-1])
+
+
+def by_channel(v):
+    """The values of v's blocks of 128 tokens, [channels][tokens]."""
+    a = np64(v)
+    if a.ndim != 4:
+        return BO.fp8_value(a.reshape(-1, a.shape[-1]).T, 1, 128)
+    B, C = a.shape[:2]
+    return np.concatenate([BO.fp8_value(a[i].reshape(C, -1), 1, 128) for i in range(B)], 1)
+
+
+def close(got, a, b, dt, what):
+    """got against a · bᵀ in 64 bits."""
+    ref, mag = a @ b.T, np.abs(a) @ np.abs(b).T
+    half, cut = (2.0 ** -8, 7 * 2.0 ** -13) if dt == torch.bfloat16 else (0.0, 0.0)
+    tol = ((a.shape[1] + 128) * U + cut) * mag + half * np.abs(ref) + 1e-37
+    err = np.abs(got - ref)
+    assert got.shape == ref.shape, what
+    assert (err <= tol).all(), f"{what}: {(err / tol).max():.2f} x tolerance"
+
+
+def run_pointwise(tb, x, w, gy, dt):
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    y = tb.fp8_pointwise(x, w)
+    assert y.dtype == dt and y.shape == gy.shape
+    gx, gw = torch.autograd.grad(y, (x, w), gy)
+    xt, wq, gt = (BO.fp8_value(tok(x), 1, 128), BO.fp8_value(np64(w).reshape(w.shape[0], -1), 128, 128),
+                  BO.fp8_value(tok(gy), 1, 128))
+    close(tok(y), xt, wq, dt, "y")
+    close(tok(gx), gt, wq.T, dt, "grad x")
+    close(np64(gw).reshape(w.shape[0], -1), by_channel(gy), by_channel(x), dt, "grad w")
+    return y, gx, gw
+
+
+SIZES = [(1, 1, 1, 1), (1, 1, 128, 128), (1, 5, 130, 70), (2, 49, 100, 300), (3, 128, 256, 129),
+         (1, 1, 1000, 500), (1, 17, 4096, 33), (2, 333, 65, 64), (1, 130, 257, 640),
+         (64, 1, 40, 24), (2, 784, 256, 1024), (1, 16, 300, 2050), (1, 33, 520, 40),
+         (1, 65, 128, 260), (1, 2000, 16, 16)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+@pytest.mark.parametrize("B,P,C,O", SIZES)
+def test_pointwise(tb, dt, layout, B, P, C, O):
+    sh = lambda c: (B, c, P, 1) if layout == "nchw" else (B, P, c)
+    x, w, gy = make(sh(C), dt, 1, 0.3), make((O, C), dt, 2, 0.1), make(sh(O), dt, 3, 0.3)
+    y, gx, gw = run_pointwise(tb, x, w, gy, dt)
+    # the same bits again, and from a kept weight
+    xr, wr = x.detach().requires_grad_(), w.detach().requires_grad_()
+    y2 = tb.fp8_pointwise(xr, wr)
+    g2 = torch.autograd.grad(y2, (xr, wr), gy)
+    assert torch.equal(y2, y) and torch.equal(g2[0], gx) and torch.equal(g2[1], gw)
+    with torch.no_grad():
+        assert torch.equal(tb.fp8_pointwise(x, tb.fp8_quantize_weight(w)), y)
+
+
+def test_asymmetric_identity(tb):
+    """Each weight row picks one channel: every output element is one input value, so a row, a
+    column or an exponent out of place shows at once."""
+    T, C, O = 200, 384, 300
+    x = torch.arange(T * C, dtype=torch.float32).reshape(T, C) % 13 + 1
+    x = (x * torch.exp2((torch.arange(T) % 9 - 4).float())[:, None] *
+         torch.exp2((torch.arange(C) // 128 * 3).float())).cuda()
+    pick = (torch.arange(O) * 7) % C
+    w = torch.zeros(O, C)
+    w[torch.arange(O), pick] = torch.exp2((torch.arange(O) // 128).float())
+    y = tb.fp8_pointwise(x, w.cuda())
+    want = x[:, pick.cuda()] * torch.exp2((torch.arange(O) // 128).float()).cuda()
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_channels_last_and_strides(tb, dt):
+    x, w, gy = make((2, 70, 6, 9), dt, 1), make((50, 70, 1, 1), dt, 2, 0.1), make((2, 50, 6, 9), dt, 3)
+    y, gx, gw = run_pointwise(tb, x, w, gy, dt)
+    cl = torch.channels_last
+    xl, wl = x.contiguous(memory_format=cl).requires_grad_(), w.clone().requires_grad_()
+    yl = tb.fp8_pointwise(xl, wl)
+    assert yl.is_contiguous(memory_format=cl) and torch.equal(yl, y)
+    gl = torch.autograd.grad(yl, (xl, wl), gy)
+    assert torch.equal(gl[0], gx) and gl[1].shape == gw.shape
+    flat = make((10001,), dt, 5)[1:1 + 100 * 70].view(100, 70)
+    wt = w.flatten(1).t().contiguous().t()
+    with torch.no_grad():
+        assert torch.equal(tb.fp8_pointwise(flat, wt), tb.fp8_pointwise(flat.clone(), w))
+
+
+def test_nan_stays_in_its_row(tb):
+    x, w = make((40, 300), torch.float32, 1), make((90, 300), torch.float32, 2, 0.1)
+    clean = tb.fp8_pointwise(x, w)
+    x[7, 200], x[20, 3] = float("nan"), float("-inf")
+    y = tb.fp8_pointwise(x, w)
+    bad = torch.zeros(40, dtype=torch.bool)
+    bad[7] = bad[20] = True
+    assert torch.isnan(y[bad]).all() and torch.equal(y[~bad], clean[~bad])
+
+
+def test_graph_and_side_stream(tb):
+    x, w, gy = (make(s, torch.bfloat16, i, 0.2) for i, s in enumerate(((300, 520), (200, 520), (300, 200))))
+    x.requires_grad_(), w.requires_grad_()
+
+    def step():
+        y = tb.fp8_pointwise(x, w)
+        return [y.detach(), *torch.autograd.grad(y, (x, w), gy)]
+
+    want = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = step()
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(side, want))
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        r1 = step()
+    with torch.cuda.graph(g2):
+        r2 = step()
+    for k in range(3):
+        with torch.no_grad():
+            x.mul_(1.5)
+        g1.replay()
+        eager = step()
+        g2.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip(r1, r2, eager):
+            assert torch.equal(a, c) and torch.equal(b, c)
+
+
+def test_gradient_against_differences(tb):
+    """The 8-bit product is piecewise constant, so differences are taken of the oracle: with
+    inputs that e4m3 holds exactly, the gradients are the exact bilinear form's."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randint(-8, 9, (70, 140), generator=g).float().cuda().requires_grad_()
+    w = torch.randint(-8, 9, (60, 140), generator=g).float().cuda().requires_grad_()
+    gy = torch.randint(-8, 9, (70, 60), generator=g).float().cuda()
+    y = tb.fp8_pointwise(x, w)
+    gx, gw = torch.autograd.grad(y, (x, w), gy)
+    xd, wd, gd = x.detach().double(), w.detach().double(), gy.double()
+    f = lambda a, b: float(((a @ b.t()) * gd).sum())
+    assert torch.equal(y.double(), xd @ wd.t())
+    for i, j in ((0, 0), (13, 139), (69, 70)):
+        d = torch.zeros_like(xd)
+        d[i, j] = 1.0
+        assert float(gx[i, j]) == (f(xd + d, wd) - f(xd - d, wd)) / 2
+    for i, j in ((0, 0), (59, 139), (31, 128)):
+        d = torch.zeros_like(wd)
+        d[i, j] = 1.0
+        assert float(gw[i, j]) == (f(xd, wd + d) - f(xd, wd - d)) / 2
+
+
+def test_refusals_and_modules(tb):
+    x, w = make((4, 10), torch.float32), make((6, 10), torch.float32)
+    for bad in (w.bfloat16(), w[:, :9], w.cpu(), w[None]):
+        with pytest.raises(ValueError):
+            tb.fp8_pointwise(x, bad)
+    with pytest.raises(TypeError):
+        tb.fp8_pointwise(x.half(), w)
+    with pytest.raises(RuntimeError):
+        tb.fp8_pointwise(x.cpu(), w)
+    qw = tb.fp8_quantize_weight(w)
+    with pytest.raises(RuntimeError):
+        tb.fp8_pointwise(x.clone().requires_grad_(), qw)
+    with pytest.raises(ValueError):
+        tb.fp8_pointwise(make((4, 11), torch.float32), qw)
+    with pytest.raises(ValueError):
+        tb.Fp8Weight(qw.q, qw.exponents, 200)
+    with pytest.raises(ValueError):
+        tb.fp8_quantize_weight(x[0])
+    assert tb.fp8_pointwise(x[:0], w).shape == (0, 6)
+    assert tb.fp8_pointwise(make((2, 10, 3, 0), torch.float32), w).shape == (2, 6, 3, 0)
+    e = x[:0].requires_grad_()
+    wr = w.clone().requires_grad_()
+    tb.fp8_pointwise(e, wr).sum().backward()
+    assert not wr.grad.any() and e.grad.shape == (0, 10)
+    m = tb.Fp8Pointwise(10, 6).cuda()
+    y = m(x)
+    y.sum().backward()
+    assert m.weight.grad is not None
+    with torch.no_grad():
+        assert torch.equal(m.eval().serve()(x), y)
+    assert m.train().weight8 is None
