@@ -256,6 +256,495 @@ __global__ __launch_bounds__(kThreads) void block_any_params(BlockArgs a) {
   }
 }
 
+// ---- one pass: the channels of a tile of positions stay in registers ----------------------
+// Both layouts share the plan: work is cut into tiles (maps: TP neighbouring positions of an
+// image, rows: one row per LPR lanes), the tiles of one workgroup are neighbours, and a thread
+// keeps the same channels in every tile, so its parameter gradients add up in registers. They
+// leave once per workgroup as partials [workgroup][5][C] (scale, w1, b1, w2, b2), an image
+// gate's once per workgroup and image, and block_fold adds them in workgroup order.
+struct Plan {
+  int tpi;            // tiles of an image
+  long tiles;         // of the call
+  int wgs;            // workgroups; workgroup w takes tiles [w · tiles / wgs, (w + 1) · tiles / wgs)
+  int images, P;      // rows without an image gate count as one image
+  bool image_gate;    // ∂gate sums over positions
+  float *part, *gpart;  // [wgs][5][C], [wgs + images][C]: slot wg + image is written once
+};
+
+__device__ __forceinline__ long first_tile(const Plan& q, int w) { return q.tiles * w / q.wgs; }
+
+// the workgroups that share an XCD (equal index mod 8) take neighbouring ranges
+__device__ __forceinline__ int xcd_wg(int n) {
+  const int bid = blockIdx.x, q = n >> 3, r = n & 7, x = bid & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
+}
+
+// Σ over the lanes that share (lane % STRIDE), or over aligned groups of LPR lanes; every lane
+// gets the sum. VALU only (DPP rotations and mirrors, lane-row swaps), fixed order.
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (LPR >= 2) v += dpp_f<0xB1>(v);
+  if constexpr (LPR >= 4) v += dpp_f<0x4E>(v);
+  if constexpr (LPR >= 8) v += dpp_f<0x141>(v);
+  if constexpr (LPR >= 16) v += dpp_f<0x140>(v);
+  if constexpr (LPR >= 32) v = swap_fold16(v);
+  if constexpr (LPR >= 64) v = swap_fold32(v);
+  return v;
+}
+template <int STRIDE>
+__device__ __forceinline__ float stride_sum(float v) {
+  if constexpr (STRIDE <= 2) v += dpp_f<0x122>(v);  // row_ror:2
+  if constexpr (STRIDE <= 4) v += dpp_f<0x124>(v);
+  if constexpr (STRIDE <= 8) v += dpp_f<0x128>(v);
+  if constexpr (STRIDE <= 16) v = swap_fold16(v);
+  return swap_fold32(v);
+}
+
+// keep bits of the V elements from i
+template <int V>
+__device__ __forceinline__ unsigned keepv(uint64_t i, const PhiloxKey& k, unsigned thr) {
+  const unsigned s = (unsigned)(i & 7);
+  unsigned m = keep8(i >> 3, k, thr) >> s;
+  if (s + V > 8) m |= keep8((i >> 3) + 1, k, thr) << (8 - s);
+  return m;
+}
+
+// ---- maps [B][C][P]: PL lanes of one vector along the positions, NT / PL channel groups, channels
+// cg + CG · i of a thread, i < CPT.
+template <int NT, int PL, int V>
+struct MapSums {
+  static constexpr int TP = PL * V, NW = NT / 64, GPW = 64 / PL, CG = NT / PL;
+  float (*buf)[NW][2][TP];  // two buffers: a round's readers are done when the next but one writes
+  int phase = 0, w, pl, lane, C;
+  __device__ float count(int wave, int cpt) const {  // channels of a wave
+    int n = 0;
+    for (int i = 0; i < cpt; ++i) n += min(max(C - (CG * i + wave * GPW), 0), GPW);
+    return (float)n;
+  }
+  // wave-level sums of two rows of V values, exchanged: out of the buffer every thread reads
+  // the waves' values of its positions
+  __device__ void put(const float (&a)[V], const float (&b)[V]) {
+    phase ^= 1;
+    if (lane < PL) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        buf[phase][w][0][pl * V + e] = a[e];
+        buf[phase][w][1][pl * V + e] = b[e];
+      }
+    }
+    lds_barrier();
+  }
+  __device__ float at(int wave, int k, int e) const { return buf[phase][wave][k][pl * V + e]; }
+  __device__ void sum2(float (&a)[V], float (&b)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      a[e] = stride_sum<PL>(a[e]);
+      b[e] = stride_sum<PL>(b[e]);
+    }
+    if constexpr (NW > 1) {
+      put(a, b);
+#pragma unroll
+      for (int e = 0; e < V; ++e) a[e] = b[e] = 0.f;
+#pragma unroll 1  // unrolled, the reads of all waves' values at once would need the registers
+      for (int v = 0; v < NW; ++v)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          a[e] += at(v, 0, e);
+          b[e] += at(v, 1, e);
+        }
+    }
+  }
+  // Mean and 1/sqrt(var + eps) of each position. Layer: every wave takes its own mean and the
+  // squares about it; the waves' are joined about the whole mean, so large means cancel nowhere.
+  template <int CPT>
+  __device__ void moments(const float (&v)[CPT][V], const bool (&ok)[CPT], int kind, float eps,
+                          float (&m)[V], float (&r)[V]) {
+    float s[V], q[V];
+    const float nw = count(w, CPT), inw = nw > 0.f ? 1.f / nw : 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float t = 0.f, u = 0.f;
+      if (kind == DCN_NORM_LAYER) {
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) t += v[i][e];
+        t = stride_sum<PL>(t);
+      }
+      const float mu = t * inw;
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        const float d = ok[i] ? v[i][e] - mu : 0.f;
+        u = fmaf(d, d, u);
+      }
+      s[e] = t;
+      q[e] = stride_sum<PL>(u);
+    }
+    const float ic = 1.f / (float)C;
+    if constexpr (NW > 1) {
+      put(s, q);
+      float ts[V], tq[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) ts[e] = tq[e] = 0.f;
+#pragma unroll 1
+      for (int wv = 0; wv < NW; ++wv)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          ts[e] += at(wv, 0, e);
+          tq[e] += at(wv, 1, e);
+        }
+      if (kind == DCN_NORM_LAYER) {
+#pragma unroll 1
+        for (int wv = 0; wv < NW; ++wv) {
+          const float n = count(wv, CPT), in = n > 0.f ? 1.f / n : 0.f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float d = at(wv, 0, e) * in - ts[e] * ic;
+            tq[e] = fmaf(n * d, d, tq[e]);
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        s[e] = ts[e];
+        q[e] = tq[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      m[e] = s[e] * ic;
+      r[e] = 1.f / sqrtf(q[e] * ic + eps);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float par(const void* t, int c, float none) {
+  return t ? to_f32(static_cast<const T*>(t)[c]) : none;
+}
+
+template <typename T, int NT, int PL, int CPT, bool BWD, bool FULL>
+__global__ __launch_bounds__(NT) void block_map(BlockArgs a, Plan q) {
+  constexpr int V = ElemVec<T>::N, TP = PL * V, CG = NT / PL;
+  __shared__ __attribute__((aligned(16))) float buf[2][NT / 64][2][TP];
+  const PhiloxKey key = philox_key(a.drop);
+  const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
+  MapSums<NT, PL, V> sums;
+  sums.buf = buf;
+  sums.w = threadIdx.x >> 6;
+  sums.lane = threadIdx.x & 63;
+  sums.pl = pl;
+  sums.C = a.C;
+  const int wg = xcd_wg(q.wgs);
+  const T *xp = static_cast<const T*>(a.x), *rp = static_cast<const T*>(a.res);
+  const T* gp = static_cast<const T*>(a.gate);
+
+  bool inc[CPT];
+  float sc[CPT], w1[CPT], b1[CPT], w2[CPT], b2[CPT];
+  float acc[5][CPT], accg[CPT];
+#pragma unroll
+  for (int i = 0; i < CPT; ++i) {
+    const int c = cg + CG * i;
+    inc[i] = c < a.C;
+    sc[i] = a.alpha * (inc[i] ? par<T>(a.scale, c, 1.f) : 0.f);
+    w1[i] = inc[i] ? par<T>(a.w1, c, 1.f) : 0.f;
+    b1[i] = inc[i] ? par<T>(a.b1, c, 0.f) : 0.f;
+    w2[i] = inc[i] ? par<T>(a.w2, c, 1.f) : 0.f;
+    b2[i] = inc[i] ? par<T>(a.b2, c, 0.f) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) acc[k][i] = 0.f;
+    accg[i] = 0.f;
+  }
+  const long t0 = first_tile(q, wg), t1 = first_tile(q, wg + 1);
+  for (long t = t0; t < t1; ++t) {
+    const int b = (int)(t / q.tpi), p = (int)(t % q.tpi) * TP + pl * V, valid = a.P - p;
+    const size_t base = (size_t)b * a.C * a.P + p;
+    bool ok[CPT];
+    size_t at[CPT];
+    u32x4 xr[CPT], rr[CPT], gr[CPT], yr[CPT], orr[CPT];
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      ok[i] = inc[i] && valid > 0;
+      at[i] = base + (size_t)(cg + CG * i) * a.P;
+      xr[i] = ok[i] && xp ? ldv_raw(xp + at[i], valid) : zero;
+      rr[i] = ok[i] && rp ? ldv_raw(rp + at[i], valid) : zero;
+      if constexpr (FULL) gr[i] = ok[i] ? ldv_raw(gp + at[i], valid) : zero;
+      if constexpr (BWD) {
+        yr[i] = ok[i] && a.gy ? ldv_raw(static_cast<const T*>(a.gy) + at[i], valid) : zero;
+        orr[i] = ok[i] && a.go ? ldv_raw(static_cast<const T*>(a.go) + at[i], valid) : zero;
+      }
+    }
+    float gv[CPT], gd[CPT];  // an image gate's act and act'
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      gv[i] = 1.f;
+      gd[i] = 0.f;
+      if (a.gate_kind == DCN_GATE_IMAGE && inc[i])
+        gate_act_grad(to_f32(gp[(size_t)b * a.C + cg + CG * i]), a.act, gv[i], gd[i]);
+    }
+    unsigned keep[CPT];
+    const bool img_keep = !a.drop_image || !a.drop.thr || keep1(b, key, a.drop.thr);
+#pragma unroll
+    for (int i = 0; i < CPT; ++i)
+      keep[i] = !a.drop.thr ? 0xffu
+                : a.drop_image ? (img_keep ? 0xffu : 0u)
+                               : keepv<V>(at[i], key, a.drop.thr);
+    const float ds = a.drop.thr ? a.drop.scale : 1.f;
+
+    float m1[V], r1[V], m2[V], r2[V];
+    float o[CPT][V];
+    if (xp) {
+      if (a.post) {
+        float xv[CPT][V];
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) unpack<T>(xr[i], xv[i]);
+        sums.template moments<CPT>(xv, inc, a.post, a.eps1, m1, r1);
+      }
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        float xv[V], rv[V], fv[V];
+        unpack<T>(xr[i], xv);
+        unpack<T>(rr[i], rv);
+        if constexpr (FULL) unpack<T>(gr[i], fv);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float v = a.post ? fmaf((xv[e] - m1[e]) * r1[e], w1[i], b1[i]) : xv[e];
+          const float act = FULL ? gate_act(fv[e], a.act) : gv[i];
+          const float tt = v * (sc[i] * act);
+          o[i][e] = rv[e] + ((keep[i] >> e) & 1u ? tt * ds : 0.f);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) unpack<T>(rr[i], o[i]);
+    }
+    if (a.pre) sums.template moments<CPT>(o, inc, a.pre, a.eps2, m2, r2);
+
+    if constexpr (!BWD) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        if (!ok[i]) continue;
+        if (a.pre) {
+          float y[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) y[e] = fmaf((o[i][e] - m2[e]) * r2[e], w2[i], b2[i]);
+          stv(static_cast<T*>(a.y) + at[i], valid, y);
+        }
+        if (a.out) stv(static_cast<T*>(a.out) + at[i], valid, o[i]);
+      }
+    } else {
+      // G into o
+      if (a.pre) {
+        float s1[V], s2[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          float gy[V];
+          unpack<T>(yr[i], gy);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float h = (o[i][e] - m2[e]) * r2[e], w = gy[e] * w2[i];
+            o[i][e] = h;
+            s1[e] += w;
+            s2[e] = fmaf(w, h, s2[e]);
+            if (ok[i] && e < valid) {
+              acc[3][i] = fmaf(gy[e], h, acc[3][i]);
+              acc[4][i] += gy[e];
+            }
+          }
+        }
+        sums.sum2(s1, s2);
+        const float ic = 1.f / (float)a.C;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          s1[e] = a.pre == DCN_NORM_LAYER ? s1[e] * ic : 0.f;
+          s2[e] *= ic;
+        }
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          float gy[V], go[V];
+          unpack<T>(yr[i], gy);
+          unpack<T>(orr[i], go);
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            o[i][e] = fmaf(r2[e], gy[e] * w2[i] - s1[e] - o[i][e] * s2[e], go[e]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) unpack<T>(orr[i], o[i]);
+      }
+      if (a.gr) {
+#pragma unroll
+        for (int i = 0; i < CPT; ++i)
+          if (ok[i]) stv(static_cast<T*>(a.gr) + at[i], valid, o[i]);
+      }
+      if (xp) {
+        // dt, ∂gate, ∂scale; dv into o
+        float s3[V], s4[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s3[e] = s4[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          float xv[V], fv[V], gg[V];
+          unpack<T>(xr[i], xv);
+          if constexpr (FULL) unpack<T>(gr[i], fv);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float h = a.post ? (xv[e] - m1[e]) * r1[e] : 0.f;
+            const float v = a.post ? fmaf(h, w1[i], b1[i]) : xv[e];
+            float av = gv[i], ad = gd[i];
+            if constexpr (FULL) gate_act_grad(fv[e], a.act, av, ad);
+            const float dt = (keep[i] >> e) & 1u ? o[i][e] * ds : 0.f;
+            const float dtv = dt * v, dv = dt * (sc[i] * av);
+            gg[e] = dtv * sc[i] * ad;
+            if (ok[i] && e < valid) {
+              acc[0][i] = fmaf(dtv, a.alpha * av, acc[0][i]);
+              acc[1][i] = fmaf(dv, h, acc[1][i]);
+              acc[2][i] += dv;
+              accg[i] += gg[e];
+            }
+            o[i][e] = dv;
+            const float w = dv * w1[i];
+            s3[e] += w;
+            s4[e] = fmaf(w, h, s4[e]);
+          }
+          if (a.gg && FULL && ok[i])
+            stv(static_cast<T*>(a.gg) + at[i], valid, gg);
+        }
+        if (a.gx) {
+          if (a.post) {
+            sums.sum2(s3, s4);
+            const float ic = 1.f / (float)a.C;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              s3[e] = a.post == DCN_NORM_LAYER ? s3[e] * ic : 0.f;
+              s4[e] *= ic;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < CPT; ++i) {
+            if (!ok[i]) continue;
+            if (a.post) {
+              float xv[V];
+              unpack<T>(xr[i], xv);
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                const float h = (xv[e] - m1[e]) * r1[e];
+                o[i][e] = r1[e] * (o[i][e] * w1[i] - s3[e] - h * s4[e]);
+              }
+            }
+            stv(static_cast<T*>(a.gx) + at[i], valid, o[i]);
+          }
+        }
+        if (q.image_gate && (t + 1 == t1 || (t + 1) % q.tpi == 0)) {
+#pragma unroll
+          for (int i = 0; i < CPT; ++i) {
+            const float g = group_sum<PL>(accg[i]);
+            if (inc[i] && pl == 0) q.gpart[(size_t)(wg + b) * a.C + cg + CG * i] = g;
+            accg[i] = 0.f;
+          }
+        }
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (!q.part) return;
+#pragma unroll
+    for (int i = 0; i < CPT; ++i)
+#pragma unroll
+      for (int k = 0; k < 5; ++k) {
+        const float g = group_sum<PL>(acc[k][i]);
+        if (inc[i] && pl == 0) q.part[((size_t)wg * 5 + k) * a.C + cg + CG * i] = g;
+      }
+  }
+}
+
+// The partials of one parameter (blockIdx.y < 5) or of one image's gate (5 + image), 64 channels
+// per workgroup, added in workgroup order: 16 threads a channel, then a tree over them.
+template <typename T>
+__global__ __launch_bounds__(1024) void block_fold(BlockArgs a, Plan q) {
+  __shared__ float red[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6, k = blockIdx.y;
+  void* dst[5] = {a.gs, a.gw1, a.gb1, a.gw2, a.gb2};
+  T* out = k < 5 ? static_cast<T*>(dst[k]) : static_cast<T*>(a.gg) + (size_t)(k - 5) * a.C;
+  if (k < 5 && !dst[k]) return;
+  float s = 0.f;
+  if (c < a.C) {
+    if (k < 5) {
+#pragma unroll 4
+      for (int w = g; w < q.wgs; w += 16) s += q.part[((size_t)w * 5 + k) * a.C + c];
+    } else {
+      // workgroups whose range meets this image's tiles
+      const long lo = (long)(k - 5) * q.tpi, hi = lo + q.tpi;
+      int w0 = (int)(lo * q.wgs / q.tiles);
+      while (w0 > 0 && first_tile(q, w0) > lo) --w0;
+      while (first_tile(q, w0 + 1) <= lo) ++w0;
+      for (int w = w0 + g; w < q.wgs && first_tile(q, w) < hi; w += 16)
+        if (first_tile(q, w + 1) > first_tile(q, w)) s += q.gpart[(size_t)(w + k - 5) * a.C + c];
+    }
+  }
+  red[g][threadIdx.x & 63] = s;
+  __syncthreads();
+  for (int o = 8; o > 0; o >>= 1) {
+    if (g < o) red[g][threadIdx.x & 63] += red[g + o][threadIdx.x & 63];
+    __syncthreads();
+  }
+  if (g == 0 && c < a.C) out[c] = from_f32(red[0][threadIdx.x], T());
+}
+
+constexpr int kMaxWgs = 1024;
+
+// floats of the partials, then the gate's
+size_t plan_floats(const BlockArgs& a) {
+  return (size_t)kMaxWgs * 5 * a.C + (size_t)(kMaxWgs + a.B) * a.C;
+}
+
+template <typename T, int NT, int PL, int CPT, bool BWD>
+hipError_t run_map(const BlockArgs& a, hipStream_t s) {
+  constexpr int TP = PL * ElemVec<T>::N;
+  Plan q{};
+  q.tpi = (a.P + TP - 1) / TP;
+  q.tiles = (long)q.tpi * a.B;
+  q.images = a.B;
+  q.P = a.P;
+  const bool params = BWD && (a.gs || a.gw1 || a.gb1 || a.gw2 || a.gb2);
+  q.image_gate = BWD && a.gg && a.gate_kind == DCN_GATE_IMAGE;
+  q.wgs = (int)std::min<long>(q.tiles, params || q.image_gate ? kMaxWgs : 1 << 20);
+  if (params) q.part = a.ws;
+  if (q.image_gate) q.gpart = a.ws + (size_t)kMaxWgs * 5 * a.C;
+  if (a.gate_kind == DCN_GATE_FULL)
+    hipLaunchKernelGGL((block_map<T, NT, PL, CPT, BWD, true>), dim3(q.wgs), dim3(NT), 0, s, a, q);
+  else
+    hipLaunchKernelGGL((block_map<T, NT, PL, CPT, BWD, false>), dim3(q.wgs), dim3(NT), 0, s, a, q);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !(params || q.image_gate)) return e;
+  // without parameter gradients the first five rows have no destination and end at once
+  hipLaunchKernelGGL((block_fold<T>), dim3((a.C + 63) / 64, 5 + (q.image_gate ? a.B : 0)),
+                     dim3(1024), 0, s, a, q);
+  return hipGetLastError();
+}
+
+// false: no register-resident variant for this many channels
+template <bool BWD>
+bool map_variant(const BlockArgs& a, hipStream_t s, hipError_t* e) {
+  if (a.dtype == DCN_BF16) {
+    if (a.C <= 64) *e = run_map<bf16_t, 256, 8, 2, BWD>(a, s);
+    else if (a.C <= 128) *e = run_map<bf16_t, 256, 8, 4, BWD>(a, s);
+    else if (a.C <= 256) *e = run_map<bf16_t, 512, 8, 4, BWD>(a, s);
+    else if (a.C <= 512) *e = run_map<bf16_t, 512, 4, 4, BWD>(a, s);
+    else if (a.C <= 1024) *e = run_map<bf16_t, 512, 2, 4, BWD>(a, s);
+    else return false;
+  } else {
+    if (a.C <= 64) *e = run_map<float, 256, 8, 2, BWD>(a, s);
+    else if (a.C <= 128) *e = run_map<float, 256, 8, 4, BWD>(a, s);
+    else if (a.C <= 256) *e = run_map<float, 256, 8, 8, BWD>(a, s);
+    else if (a.C <= 512) *e = run_map<float, 512, 8, 8, BWD>(a, s);
+    else if (a.C <= 1024) *e = run_map<float, 512, 4, 8, BWD>(a, s);
+    else return false;
+  }
+  return true;
+}
+
 template <typename T, int LP>
 hipError_t any_fwd(const BlockArgs& a, hipStream_t s) {
   const size_t rows = (size_t)a.B * a.P, per = kThreads / LP;
@@ -277,15 +766,21 @@ hipError_t any_bwd(const BlockArgs& a, hipStream_t s) {
 
 }  // namespace
 
-size_t block_norm_ws_floats(const BlockArgs& a) { return 6 * (size_t)a.B * a.P; }
+size_t block_norm_ws_floats(const BlockArgs& a) {
+  return std::max(6 * (size_t)a.B * a.P, plan_floats(a));
+}
 
 hipError_t launch_block_norm_fwd(const BlockArgs& a, hipStream_t s) {
+  hipError_t e;
+  if (a.layout == DCN_NCHW && map_variant<false>(a, s, &e)) return e;
   if (a.layout == DCN_NCHW)
     return a.dtype == DCN_BF16 ? any_fwd<bf16_t, 1>(a, s) : any_fwd<float, 1>(a, s);
   return a.dtype == DCN_BF16 ? any_fwd<bf16_t, 64>(a, s) : any_fwd<float, 64>(a, s);
 }
 
 hipError_t launch_block_norm_bwd(const BlockArgs& a, hipStream_t s) {
+  hipError_t e;
+  if (a.layout == DCN_NCHW && map_variant<true>(a, s, &e)) return e;
   if (a.layout == DCN_NCHW)
     return a.dtype == DCN_BF16 ? any_bwd<bf16_t, 1>(a, s) : any_bwd<float, 1>(a, s);
   return a.dtype == DCN_BF16 ? any_bwd<bf16_t, 64>(a, s) : any_bwd<float, 64>(a, s);
