@@ -279,8 +279,8 @@ __device__ __forceinline__ int xcd_wg(int n) {
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
 }
 
-// Σ over the lanes that share (lane % STRIDE), or over aligned groups of LPR lanes; every lane
-// gets the sum. VALU only (DPP rotations and mirrors, lane-row swaps), fixed order.
+// Σ over aligned groups of LPR lanes; every lane gets the sum. VALU only (DPP mirrors and
+// lane-row swaps), fixed order.
 template <int LPR>
 __device__ __forceinline__ float group_sum(float v) {
   if constexpr (LPR >= 2) v += dpp_f<0xB1>(v);
@@ -291,15 +291,6 @@ __device__ __forceinline__ float group_sum(float v) {
   if constexpr (LPR >= 64) v = swap_fold32(v);
   return v;
 }
-template <int STRIDE>
-__device__ __forceinline__ float stride_sum(float v) {
-  if constexpr (STRIDE <= 2) v += dpp_f<0x122>(v);  // row_ror:2
-  if constexpr (STRIDE <= 4) v += dpp_f<0x124>(v);
-  if constexpr (STRIDE <= 8) v += dpp_f<0x128>(v);
-  if constexpr (STRIDE <= 16) v = swap_fold16(v);
-  return swap_fold32(v);
-}
-
 // keep bits of the V elements from i
 template <int V>
 __device__ __forceinline__ unsigned keepv(uint64_t i, const PhiloxKey& k, unsigned thr) {
@@ -311,108 +302,178 @@ __device__ __forceinline__ unsigned keepv(uint64_t i, const PhiloxKey& k, unsign
 
 // ---- maps [B][C][P]: PL lanes of one vector along the positions, NT / PL channel groups, channels
 // cg + CG · i of a thread, i < CPT.
-template <int NT, int PL, int V>
+//
+// Sums over the channels of every position. A thread's partial sums of its V positions go
+// through LDS twice: inside the wave (its GPW channel groups x TP positions, each lane then adds
+// a column's share), then between the waves; finally every wave finishes all TP positions for
+// itself, one lane each, and the threads read their V results back. Done in registers instead
+// (V values through DPP rotations, every thread finishing all its positions) the same sums took
+// two thirds of the kernel's instructions.
+template <int NT, int PL, int V, int CPT>
 struct MapSums {
   static constexpr int TP = PL * V, NW = NT / 64, GPW = 64 / PL, CG = NT / PL;
-  float (*buf)[NW][2][TP];  // two buffers: a round's readers are done when the next but one writes
-  int phase = 0, w, pl, lane, C;
-  __device__ float count(int wave, int cpt) const {  // channels of a wave
+  static constexpr int SHARE = 64 / TP, EACH = GPW / SHARE;  // lanes a position, groups a lane
+  static_assert(TP <= 64 && SHARE * TP == 64 && EACH * SHARE == GPW, "lanes cover the positions");
+  struct Shared {
+    float wave[NW][2][GPW][TP];  // a wave's partials (two quantities)
+    float join[2][NW][2][TP];    // waves' sums, alternating: read in a round, written in the next
+                                 // but one
+    float res[NW][2][TP];        // a wave's copy of the results
+    float2 num[NW];              // channels of every wave and 1 / that (0 of 0)
+  };
+  Shared& sh;
+  int w, lane, pl, gl, C, phase = 0;
+  float inw;  // 1 / channels of this wave
+  __device__ MapSums(Shared& s, int c) : sh(s), C(c) {
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    pl = threadIdx.x % PL;
+    gl = lane / PL;
+    const float n = count(w);
+    inw = n > 0.f ? 1.f / n : 0.f;
+    if (lane == 0) sh.num[w] = make_float2(n, inw);  // read behind the first join's barrier
+  }
+  __device__ float count(int wave) const {  // channels of a wave
     int n = 0;
-    for (int i = 0; i < cpt; ++i) n += min(max(C - (CG * i + wave * GPW), 0), GPW);
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) n += min(max(C - (CG * i + wave * GPW), 0), GPW);
     return (float)n;
   }
-  // wave-level sums of two rows of V values, exchanged: out of the buffer every thread reads
-  // the waves' values of its positions
-  __device__ void put(const float (&a)[V], const float (&b)[V]) {
-    phase ^= 1;
-    if (lane < PL) {
+  // LDS accesses of one wave happen in order; this keeps the compiler to it
+  static __device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __device__ void put(int k, const float (&v)[V]) {
+    float* d = &sh.wave[w][k][gl][pl * V];
+#pragma unroll
+    for (int e = 0; e < V; e += 4)
+      *reinterpret_cast<float4*>(d + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  }
+  // the wave's sum of quantity k at position lane % TP
+  __device__ float column(int k) const {
+    const float* d = &sh.wave[w][k][(lane / TP) * EACH][lane % TP];
+    float t = d[0];
+#pragma unroll
+    for (int i = 1; i < EACH; ++i) t += d[i * TP];
+    if constexpr (SHARE >= 2) t = swap_fold32(t);
+    if constexpr (SHARE >= 4) t = swap_fold16(t);
+    return t;
+  }
+  __device__ void get(int k, float (&v)[V]) const {
+    const float* d = &sh.res[w][k][pl * V];
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(d + e);
+      v[e] = f.x;
+      v[e + 1] = f.y;
+      v[e + 2] = f.z;
+      v[e + 3] = f.w;
+    }
+  }
+  __device__ void give(int k, float v) {
+    if (lane < TP) sh.res[w][k][lane] = v;
+  }
+  // Σ over all channels, a times fa, b times fb
+  __device__ void sum2(float (&a)[V], float (&b)[V], float fa, float fb) {
+    put(0, a);
+    put(1, b);
+    wave_order();
+    float ta = column(0), tb = column(1);
+    if constexpr (NW > 1) {
+      phase ^= 1;
+      if (lane < TP) {
+        sh.join[phase][w][0][lane] = ta;
+        sh.join[phase][w][1][lane] = tb;
+      }
+      lds_barrier();
+      ta = tb = 0.f;
+#pragma unroll
+      for (int v = 0; v < NW; ++v) {
+        ta += sh.join[phase][v][0][lane % TP];
+        tb += sh.join[phase][v][1][lane % TP];
+      }
+    }
+    give(0, ta * fa);
+    give(1, tb * fb);
+    wave_order();
+    get(0, a);
+    get(1, b);
+    wave_order();
+  }
+  // Mean and 1/sqrt(var + eps) of each position (0 past the map's end, `left` = positions of
+  // the tile, so that nothing from there reaches the parameter sums); mk: 1 for a channel, 0
+  // past the last (its v is 0). Layer: every wave takes its own mean and the squares about it;
+  // the waves' are joined about the whole mean, so large means cancel nowhere.
+  __device__ void moments(const float (&v)[CPT][V], const float (&mk)[CPT], int kind, float eps,
+                          int left, float (&m)[V], float (&r)[V]) {
+    float t[V], s = 0.f, q;
+    if (kind == DCN_NORM_LAYER) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        buf[phase][w][0][pl * V + e] = a[e];
-        buf[phase][w][1][pl * V + e] = b[e];
+        t[e] = v[0][e];
+#pragma unroll
+        for (int i = 1; i < CPT; ++i) t[e] += v[i][e];
       }
-    }
-    lds_barrier();
-  }
-  __device__ float at(int wave, int k, int e) const { return buf[phase][wave][k][pl * V + e]; }
-  __device__ void sum2(float (&a)[V], float (&b)[V]) {
+      put(0, t);
+      wave_order();
+      s = column(0);
+      give(0, s * inw);
+      wave_order();
+      get(0, m);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      a[e] = stride_sum<PL>(a[e]);
-      b[e] = stride_sum<PL>(b[e]);
-    }
-    if constexpr (NW > 1) {
-      put(a, b);
+      for (int e = 0; e < V; ++e) {
+        t[e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) a[e] = b[e] = 0.f;
-#pragma unroll 1  // unrolled, the reads of all waves' values at once would need the registers
-      for (int v = 0; v < NW; ++v)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          a[e] += at(v, 0, e);
-          b[e] += at(v, 1, e);
+        for (int i = 0; i < CPT; ++i) {
+          const float d = fmaf(-m[e], mk[i], v[i][e]);
+          t[e] = fmaf(d, d, t[e]);
         }
-    }
-  }
-  // Mean and 1/sqrt(var + eps) of each position. Layer: every wave takes its own mean and the
-  // squares about it; the waves' are joined about the whole mean, so large means cancel nowhere.
-  template <int CPT>
-  __device__ void moments(const float (&v)[CPT][V], const bool (&ok)[CPT], int kind, float eps,
-                          float (&m)[V], float (&r)[V]) {
-    float s[V], q[V];
-    const float nw = count(w, CPT), inw = nw > 0.f ? 1.f / nw : 0.f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float t = 0.f, u = 0.f;
-      if (kind == DCN_NORM_LAYER) {
-#pragma unroll
-        for (int i = 0; i < CPT; ++i) t += v[i][e];
-        t = stride_sum<PL>(t);
       }
-      const float mu = t * inw;
+    } else {
 #pragma unroll
-      for (int i = 0; i < CPT; ++i) {
-        const float d = ok[i] ? v[i][e] - mu : 0.f;
-        u = fmaf(d, d, u);
+      for (int e = 0; e < V; ++e) {
+        t[e] = v[0][e] * v[0][e];
+#pragma unroll
+        for (int i = 1; i < CPT; ++i) t[e] = fmaf(v[i][e], v[i][e], t[e]);
       }
-      s[e] = t;
-      q[e] = stride_sum<PL>(u);
     }
+    put(1, t);
+    wave_order();
+    q = column(1);
     const float ic = 1.f / (float)C;
     if constexpr (NW > 1) {
-      put(s, q);
-      float ts[V], tq[V];
+      phase ^= 1;
+      if (lane < TP) {
+        sh.join[phase][w][0][lane] = s;
+        sh.join[phase][w][1][lane] = q;
+      }
+      lds_barrier();
+      q = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) ts[e] = tq[e] = 0.f;
-#pragma unroll 1
-      for (int wv = 0; wv < NW; ++wv)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          ts[e] += at(wv, 0, e);
-          tq[e] += at(wv, 1, e);
-        }
+      for (int x = 0; x < NW; ++x) q += sh.join[phase][x][1][lane % TP];
       if (kind == DCN_NORM_LAYER) {
-#pragma unroll 1
-        for (int wv = 0; wv < NW; ++wv) {
-          const float n = count(wv, CPT), in = n > 0.f ? 1.f / n : 0.f;
+        float sx[NW];
+        s = 0.f;
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float d = at(wv, 0, e) * in - ts[e] * ic;
-            tq[e] = fmaf(n * d, d, tq[e]);
-          }
+        for (int x = 0; x < NW; ++x) {
+          sx[x] = sh.join[phase][x][0][lane % TP];
+          s += sx[x];
+        }
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+          const float2 n = sh.num[x];
+          const float d = fmaf(sx[x], n.y, -s * ic);  // a wave without channels: s and n are 0
+          q = fmaf(n.x * d, d, q);
         }
       }
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        s[e] = ts[e];
-        q[e] = tq[e];
-      }
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      m[e] = s[e] * ic;
-      r[e] = 1.f / sqrtf(q[e] * ic + eps);
-    }
+    give(0, s * ic);
+    give(1, lane % TP < left ? rsqrtf(fmaf(q, ic, eps)) : 0.f);
+    wave_order();
+    get(0, m);
+    get(1, r);
+    wave_order();
   }
 };
 
@@ -421,29 +482,27 @@ __device__ __forceinline__ float par(const void* t, int c, float none) {
   return t ? to_f32(static_cast<const T*>(t)[c]) : none;
 }
 
-template <typename T, int NT, int PL, int CPT, bool BWD, bool FULL>
-__global__ __launch_bounds__(NT) void block_map(BlockArgs a, Plan q) {
+template <typename T, int NT, int PL, int CPT, int WPE, bool AHEAD, bool BWD, bool FULL, bool DROP>
+__global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
   constexpr int V = ElemVec<T>::N, TP = PL * V, CG = NT / PL;
-  __shared__ __attribute__((aligned(16))) float buf[2][NT / 64][2][TP];
+  using Sums = MapSums<NT, PL, V, CPT>;
+  __shared__ __attribute__((aligned(16))) typename Sums::Shared shared;
   const PhiloxKey key = philox_key(a.drop);
   const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
-  MapSums<NT, PL, V> sums;
-  sums.buf = buf;
-  sums.w = threadIdx.x >> 6;
-  sums.lane = threadIdx.x & 63;
-  sums.pl = pl;
-  sums.C = a.C;
+  Sums sums(shared, a.C);
   const int wg = xcd_wg(q.wgs);
   const T *xp = static_cast<const T*>(a.x), *rp = static_cast<const T*>(a.res);
   const T* gp = static_cast<const T*>(a.gate);
 
   bool inc[CPT];
+  float mk[CPT];
   float sc[CPT], w1[CPT], b1[CPT], w2[CPT], b2[CPT];
   float acc[5][CPT], accg[CPT];
 #pragma unroll
   for (int i = 0; i < CPT; ++i) {
     const int c = cg + CG * i;
     inc[i] = c < a.C;
+    mk[i] = inc[i] ? 1.f : 0.f;
     sc[i] = a.alpha * (inc[i] ? par<T>(a.scale, c, 1.f) : 0.f);
     w1[i] = inc[i] ? par<T>(a.w1, c, 1.f) : 0.f;
     b1[i] = inc[i] ? par<T>(a.b1, c, 0.f) : 0.f;
@@ -454,25 +513,41 @@ __global__ __launch_bounds__(NT) void block_map(BlockArgs a, Plan q) {
     accg[i] = 0.f;
   }
   const long t0 = first_tile(q, wg), t1 = first_tile(q, wg + 1);
+  struct Raw {
+    u32x4 x[CPT], r[CPT], g[CPT], y[CPT], o[CPT];
+  } nx;
+  auto load = [&](long t, Raw& w) {
+    const int p = (int)(t % q.tpi) * TP + pl * V, valid = a.P - p;
+    const size_t base = (size_t)(t / q.tpi) * a.C * a.P + p;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      const bool ok = inc[i] && valid > 0;
+      const size_t at = base + (size_t)(cg + CG * i) * a.P;
+      w.x[i] = ok && xp ? ldv_raw(xp + at, valid) : zero;
+      w.r[i] = ok && rp ? ldv_raw(rp + at, valid) : zero;
+      if constexpr (FULL) w.g[i] = ok ? ldv_raw(gp + at, valid) : zero;
+      if constexpr (BWD) {
+        w.y[i] = ok && a.gy ? ldv_raw(static_cast<const T*>(a.gy) + at, valid) : zero;
+        w.o[i] = ok && a.go ? ldv_raw(static_cast<const T*>(a.go) + at, valid) : zero;
+      }
+    }
+  };
+  if (AHEAD && t0 < t1) load(t0, nx);
   for (long t = t0; t < t1; ++t) {
     const int b = (int)(t / q.tpi), p = (int)(t % q.tpi) * TP + pl * V, valid = a.P - p;
+    const int left = a.P - (int)(t % q.tpi) * TP;
     const size_t base = (size_t)b * a.C * a.P + p;
     bool ok[CPT];
     size_t at[CPT];
-    u32x4 xr[CPT], rr[CPT], gr[CPT], yr[CPT], orr[CPT];
-    const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
       ok[i] = inc[i] && valid > 0;
       at[i] = base + (size_t)(cg + CG * i) * a.P;
-      xr[i] = ok[i] && xp ? ldv_raw(xp + at[i], valid) : zero;
-      rr[i] = ok[i] && rp ? ldv_raw(rp + at[i], valid) : zero;
-      if constexpr (FULL) gr[i] = ok[i] ? ldv_raw(gp + at[i], valid) : zero;
-      if constexpr (BWD) {
-        yr[i] = ok[i] && a.gy ? ldv_raw(static_cast<const T*>(a.gy) + at[i], valid) : zero;
-        orr[i] = ok[i] && a.go ? ldv_raw(static_cast<const T*>(a.go) + at[i], valid) : zero;
-      }
     }
+    if (!AHEAD) load(t, nx);
+    const Raw in = nx;
+    if (AHEAD && t + 1 < t1) load(t + 1, nx);
     float gv[CPT], gd[CPT];  // an image gate's act and act'
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
@@ -482,42 +557,48 @@ __global__ __launch_bounds__(NT) void block_map(BlockArgs a, Plan q) {
         gate_act_grad(to_f32(gp[(size_t)b * a.C + cg + CG * i]), a.act, gv[i], gd[i]);
     }
     unsigned keep[CPT];
-    const bool img_keep = !a.drop_image || !a.drop.thr || keep1(b, key, a.drop.thr);
+    if constexpr (DROP) {
+      const unsigned img = a.drop_image && keep1(b, key, a.drop.thr) ? 0xffu : 0u;
 #pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      keep[i] = !a.drop.thr ? 0xffu
-                : a.drop_image ? (img_keep ? 0xffu : 0u)
-                               : keepv<V>(at[i], key, a.drop.thr);
-    const float ds = a.drop.thr ? a.drop.scale : 1.f;
+      for (int i = 0; i < CPT; ++i) keep[i] = a.drop_image ? img : keepv<V>(at[i], key, a.drop.thr);
+    }
+    auto drop = [&](int i, int e, float t) {
+      if constexpr (DROP) return (keep[i] >> e) & 1u ? t * a.drop.scale : 0.f;
+      return t;
+    };
 
     float m1[V], r1[V], m2[V], r2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {  // no post norm: N_post(x) = x
+      m1[e] = 0.f;
+      r1[e] = 1.f;
+    }
     float o[CPT][V];
     if (xp) {
       if (a.post) {
         float xv[CPT][V];
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) unpack<T>(xr[i], xv[i]);
-        sums.template moments<CPT>(xv, inc, a.post, a.eps1, m1, r1);
+        for (int i = 0; i < CPT; ++i) unpack<T>(in.x[i], xv[i]);
+        sums.moments(xv, mk, a.post, a.eps1, left, m1, r1);
       }
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
         float xv[V], rv[V], fv[V];
-        unpack<T>(xr[i], xv);
-        unpack<T>(rr[i], rv);
-        if constexpr (FULL) unpack<T>(gr[i], fv);
+        const float k = sc[i] * gv[i];
+        unpack<T>(in.x[i], xv);
+        unpack<T>(in.r[i], rv);
+        if constexpr (FULL) unpack<T>(in.g[i], fv);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float v = a.post ? fmaf((xv[e] - m1[e]) * r1[e], w1[i], b1[i]) : xv[e];
-          const float act = FULL ? gate_act(fv[e], a.act) : gv[i];
-          const float tt = v * (sc[i] * act);
-          o[i][e] = rv[e] + ((keep[i] >> e) & 1u ? tt * ds : 0.f);
+          const float v = fmaf((xv[e] - m1[e]) * r1[e], w1[i], b1[i]);
+          o[i][e] = rv[e] + drop(i, e, v * (FULL ? sc[i] * gate_act(fv[e], a.act) : k));
         }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < CPT; ++i) unpack<T>(rr[i], o[i]);
+      for (int i = 0; i < CPT; ++i) unpack<T>(in.r[i], o[i]);
     }
-    if (a.pre) sums.template moments<CPT>(o, inc, a.pre, a.eps2, m2, r2);
+    if (a.pre) sums.moments(o, mk, a.pre, a.eps2, left, m2, r2);
 
     if constexpr (!BWD) {
 #pragma unroll
@@ -540,38 +621,31 @@ __global__ __launch_bounds__(NT) void block_map(BlockArgs a, Plan q) {
 #pragma unroll
         for (int i = 0; i < CPT; ++i) {
           float gy[V];
-          unpack<T>(yr[i], gy);
+          unpack<T>(in.y[i], gy);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float h = (o[i][e] - m2[e]) * r2[e], w = gy[e] * w2[i];
             o[i][e] = h;
             s1[e] += w;
             s2[e] = fmaf(w, h, s2[e]);
-            if (ok[i] && e < valid) {
-              acc[3][i] = fmaf(gy[e], h, acc[3][i]);
-              acc[4][i] += gy[e];
-            }
+            acc[3][i] = fmaf(gy[e], h, acc[3][i]);
+            acc[4][i] += gy[e];
           }
         }
-        sums.sum2(s1, s2);
         const float ic = 1.f / (float)a.C;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          s1[e] = a.pre == DCN_NORM_LAYER ? s1[e] * ic : 0.f;
-          s2[e] *= ic;
-        }
+        sums.sum2(s1, s2, a.pre == DCN_NORM_LAYER ? ic : 0.f, ic);
 #pragma unroll
         for (int i = 0; i < CPT; ++i) {
           float gy[V], go[V];
-          unpack<T>(yr[i], gy);
-          unpack<T>(orr[i], go);
+          unpack<T>(in.y[i], gy);
+          unpack<T>(in.o[i], go);
 #pragma unroll
           for (int e = 0; e < V; ++e)
             o[i][e] = fmaf(r2[e], gy[e] * w2[i] - s1[e] - o[i][e] * s2[e], go[e]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) unpack<T>(orr[i], o[i]);
+        for (int i = 0; i < CPT; ++i) unpack<T>(in.o[i], o[i]);
       }
       if (a.gr) {
 #pragma unroll
@@ -586,47 +660,46 @@ __global__ __launch_bounds__(NT) void block_map(BlockArgs a, Plan q) {
 #pragma unroll
         for (int i = 0; i < CPT; ++i) {
           float xv[V], fv[V], gg[V];
-          unpack<T>(xr[i], xv);
-          if constexpr (FULL) unpack<T>(gr[i], fv);
+          const float ka = a.alpha * gv[i], kd = sc[i] * gd[i], k = sc[i] * gv[i];
+          unpack<T>(in.x[i], xv);
+          if constexpr (FULL) unpack<T>(in.g[i], fv);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float h = a.post ? (xv[e] - m1[e]) * r1[e] : 0.f;
-            const float v = a.post ? fmaf(h, w1[i], b1[i]) : xv[e];
-            float av = gv[i], ad = gd[i];
-            if constexpr (FULL) gate_act_grad(fv[e], a.act, av, ad);
-            const float dt = (keep[i] >> e) & 1u ? o[i][e] * ds : 0.f;
-            const float dtv = dt * v, dv = dt * (sc[i] * av);
-            gg[e] = dtv * sc[i] * ad;
-            if (ok[i] && e < valid) {
+            const float h = (xv[e] - m1[e]) * r1[e], v = fmaf(h, w1[i], b1[i]);
+            const float dt = drop(i, e, o[i][e]), dtv = dt * v;
+            float dv;
+            if constexpr (FULL) {
+              float av, ad;
+              gate_act_grad(fv[e], a.act, av, ad);
+              dv = dt * (sc[i] * av);
+              gg[e] = dtv * (sc[i] * ad);
               acc[0][i] = fmaf(dtv, a.alpha * av, acc[0][i]);
-              acc[1][i] = fmaf(dv, h, acc[1][i]);
-              acc[2][i] += dv;
-              accg[i] += gg[e];
+            } else {
+              dv = dt * k;
+              accg[i] = fmaf(dtv, kd, accg[i]);
+              acc[0][i] = fmaf(dtv, ka, acc[0][i]);
             }
+            acc[1][i] = fmaf(dv, h, acc[1][i]);
+            acc[2][i] += dv;
             o[i][e] = dv;
             const float w = dv * w1[i];
             s3[e] += w;
             s4[e] = fmaf(w, h, s4[e]);
           }
-          if (a.gg && FULL && ok[i])
+          if (FULL && a.gg && ok[i])
             stv(static_cast<T*>(a.gg) + at[i], valid, gg);
         }
         if (a.gx) {
           if (a.post) {
-            sums.sum2(s3, s4);
             const float ic = 1.f / (float)a.C;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              s3[e] = a.post == DCN_NORM_LAYER ? s3[e] * ic : 0.f;
-              s4[e] *= ic;
-            }
+            sums.sum2(s3, s4, a.post == DCN_NORM_LAYER ? ic : 0.f, ic);
           }
 #pragma unroll
           for (int i = 0; i < CPT; ++i) {
             if (!ok[i]) continue;
             if (a.post) {
               float xv[V];
-              unpack<T>(xr[i], xv);
+              unpack<T>(in.x[i], xv);
 #pragma unroll
               for (int e = 0; e < V; ++e) {
                 const float h = (xv[e] - m1[e]) * r1[e];
@@ -699,7 +772,7 @@ size_t plan_floats(const BlockArgs& a) {
   return (size_t)kMaxWgs * 5 * a.C + (size_t)(kMaxWgs + a.B) * a.C;
 }
 
-template <typename T, int NT, int PL, int CPT, bool BWD>
+template <typename T, int NT, int PL, int CPT, int WPE, int WGS, bool BWD>
 hipError_t run_map(const BlockArgs& a, hipStream_t s) {
   constexpr int TP = PL * ElemVec<T>::N;
   Plan q{};
@@ -709,13 +782,19 @@ hipError_t run_map(const BlockArgs& a, hipStream_t s) {
   q.P = a.P;
   const bool params = BWD && (a.gs || a.gw1 || a.gb1 || a.gw2 || a.gb2);
   q.image_gate = BWD && a.gg && a.gate_kind == DCN_GATE_IMAGE;
-  q.wgs = (int)std::min<long>(q.tiles, params || q.image_gate ? kMaxWgs : 1 << 20);
+  q.wgs = (int)std::min<long>(q.tiles, WGS ? WGS : params || q.image_gate ? kMaxWgs : 1 << 20);
   if (params) q.part = a.ws;
   if (q.image_gate) q.gpart = a.ws + (size_t)kMaxWgs * 5 * a.C;
-  if (a.gate_kind == DCN_GATE_FULL)
-    hipLaunchKernelGGL((block_map<T, NT, PL, CPT, BWD, true>), dim3(q.wgs), dim3(NT), 0, s, a, q);
+  const bool full = a.gate_kind == DCN_GATE_FULL, drop = a.drop.thr != 0;
+  const dim3 grid(q.wgs), block(NT);
+  if (full && drop)
+    hipLaunchKernelGGL((block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, true, true>), grid, block, 0, s, a, q);
+  else if (full)
+    hipLaunchKernelGGL((block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, true, false>), grid, block, 0, s, a, q);
+  else if (drop)
+    hipLaunchKernelGGL((block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, false, true>), grid, block, 0, s, a, q);
   else
-    hipLaunchKernelGGL((block_map<T, NT, PL, CPT, BWD, false>), dim3(q.wgs), dim3(NT), 0, s, a, q);
+    hipLaunchKernelGGL((block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, false, false>), grid, block, 0, s, a, q);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !(params || q.image_gate)) return e;
   // without parameter gradients the first five rows have no destination and end at once
@@ -724,22 +803,39 @@ hipError_t run_map(const BlockArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// false: no register-resident variant for this many channels
+// Threads, lanes along the positions, channels a thread, waves per SIMD and workgroups that
+// prefetch their next tile (0: a workgroup per tile, or 1024 of them where parameters add up)
+// by channels and direction, the fastest of those tried at 64 images (us, the best two):
+//   bf16 forward   64x3136: 30, 44    128x784: 23, 25    256x784: 35, 35   512x196: 32, 36
+//   bf16 backward  64x3136: 52, 79    128x784: 42, 47    256x784: 72, 89   512x196: 62, 147
+//   f32 forward    64x3136: 46, 55    128x784: 31, 34    256x784: 57, 66   512x196: 46, 52
+//   f32 backward   64x3136: 83, 108   128x784: 61, 100   256x784: 112, 191 512x196: 103, 168
+// More channels than a workgroup's registers hold take narrower tiles (32-byte runs of a
+// channel at 1024), which costs less than a second pass. false: no variant (C > 2048).
 template <bool BWD>
 bool map_variant(const BlockArgs& a, hipStream_t s, hipError_t* e) {
+  const int C = a.C;
   if (a.dtype == DCN_BF16) {
-    if (a.C <= 64) *e = run_map<bf16_t, 256, 8, 2, BWD>(a, s);
-    else if (a.C <= 128) *e = run_map<bf16_t, 256, 8, 4, BWD>(a, s);
-    else if (a.C <= 256) *e = run_map<bf16_t, 512, 8, 4, BWD>(a, s);
-    else if (a.C <= 512) *e = run_map<bf16_t, 512, 4, 4, BWD>(a, s);
-    else if (a.C <= 1024) *e = run_map<bf16_t, 512, 2, 4, BWD>(a, s);
+    if (C <= 32) *e = run_map<bf16_t, 256, 8, 1, 3, 0, BWD>(a, s);
+    else if (C <= 64) *e = run_map<bf16_t, 256, 8, 2, 2, 512, BWD>(a, s);
+    else if (C <= 128) *e = run_map<bf16_t, 256, 4, 2, 2, 512, BWD>(a, s);
+    else if (C <= 256 && !BWD) *e = run_map<bf16_t, 512, 4, 2, 4, 0, false>(a, s);
+    else if (C <= 256) *e = run_map<bf16_t, 512, 4, 2, 2, 256, BWD>(a, s);
+    else if (C <= 512 && !BWD) *e = run_map<bf16_t, 1024, 4, 2, 4, 0, false>(a, s);
+    else if (C <= 512) *e = run_map<bf16_t, 512, 2, 2, 2, 256, BWD>(a, s);
+    else if (C <= 1024) *e = run_map<bf16_t, 512, 2, 4, 2, 256, BWD>(a, s);
+    else if (C <= 2048) *e = run_map<bf16_t, 1024, 2, 4, 4, 256, BWD>(a, s);
     else return false;
   } else {
-    if (a.C <= 64) *e = run_map<float, 256, 8, 2, BWD>(a, s);
-    else if (a.C <= 128) *e = run_map<float, 256, 8, 4, BWD>(a, s);
-    else if (a.C <= 256) *e = run_map<float, 256, 8, 8, BWD>(a, s);
-    else if (a.C <= 512) *e = run_map<float, 512, 8, 8, BWD>(a, s);
-    else if (a.C <= 1024) *e = run_map<float, 512, 4, 8, BWD>(a, s);
+    if (C <= 32) *e = run_map<float, 256, 8, 1, 3, 0, BWD>(a, s);
+    else if (C <= 64) *e = run_map<float, 256, 8, 2, 4, 0, BWD>(a, s);
+    else if (C <= 128) *e = run_map<float, 256, 8, 4, 2, 512, BWD>(a, s);
+    else if (C <= 256 && !BWD) *e = run_map<float, 512, 8, 4, 4, 0, false>(a, s);
+    else if (C <= 256) *e = run_map<float, 512, 8, 4, 2, 256, BWD>(a, s);
+    else if (C <= 512) *e = run_map<float, 512, 4, 4, 2, 256, BWD>(a, s);
+    else if (C <= 1024 && !BWD) *e = run_map<float, 512, 4, 8, 2, 256, false>(a, s);
+    else if (C <= 1024) *e = run_map<float, 1024, 4, 4, 4, 0, BWD>(a, s);
+    else if (C <= 2048) *e = run_map<float, 1024, 4, 8, 4, 256, BWD>(a, s);
     else return false;
   }
   return true;

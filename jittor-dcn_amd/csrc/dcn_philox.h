@@ -80,6 +80,7 @@ __device__ __forceinline__ unsigned keep8_from(uint64_t i, const PhiloxKey& k, u
 // Vectors of 16 bytes at any element alignment: global memory takes unaligned accesses, so rows
 // of odd length and sliced tensors need no scalar path (only their last partial vector does).
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16v2 __attribute__((ext_vector_type(2)));
 typedef u32x4 u32x4_any __attribute__((aligned(2), may_alias));
 
 template <typename T>
@@ -128,8 +129,10 @@ __device__ __forceinline__ u32x4 pack(const float (&v)[ElemVec<T>::N]) {
   u32x4 r;
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      r[j] = (unsigned)f2bf(v[2 * j]) | ((unsigned)f2bf(v[2 * j + 1]) << 16);
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 p = {v[2 * j], v[2 * j + 1]};
+      r[j] = __builtin_bit_cast(unsigned, __builtin_convertvector(p, bf16v2));  // one cvt_pk
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = __float_as_uint(v[j]);
