@@ -1,0 +1,992 @@
+// dcn_block_norm.h — kernels of the operator between two residual blocks (include/dcn.h, block norms):
+//   t = drop(alpha · scale[c] · act(gate) · N_post(x)), out = residual + t, y = N_pre(out)
+// over the C channels of every position, and its backward.
+//
+// Backward, with h = (v - m) · r the normalised values of a norm and a = g · w:
+//   N'(g) = r · (a - [layer] mean(a) - h · mean(a h)),  ∂w = Σ g h,  ∂b = Σ g
+//   G  = ∂out + N_pre'(∂y)                 (= ∂residual)
+//   dt = keep ? G · drop scale : 0
+//   ∂gate = dt · N_post(x) · alpha · scale · act'(gate),  ∂scale = Σ dt · N_post(x) · alpha · act
+//   ∂x = N_post'(dt · alpha · scale · act)
+// out and the statistics are computed again from x and the residual (the residual is read
+// instead of out, so that costs no bytes), which keeps the backward free of out's rounding.
+#pragma once
+#include "dcn_block.h"
+#include "dcn_philox.h"
+
+namespace dcn {
+
+// register-resident variants (dcn_block_map_*.hip, dcn_block_row_*.hip): false where there is
+// none for this many channels, else *e is the launch's result
+bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e);
+bool block_map_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e);
+bool block_row_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e);
+bool block_row_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e);
+
+namespace {
+
+// act(g) and act'(g)
+__device__ __forceinline__ float gate_act(float g, int act) {
+  if (act == DCN_ACT_LINEAR) return g;
+  const float s = 1.f / (1.f + expf(-g));
+  return act == DCN_ACT_SIGMOID ? s : g * s;
+}
+__device__ __forceinline__ void gate_act_grad(float g, int act, float& a, float& d) {
+  a = g;
+  d = 1.f;
+  if (act == DCN_ACT_LINEAR) return;
+  const float s = 1.f / (1.f + expf(-g));
+  a = act == DCN_ACT_SIGMOID ? s : g * s;
+  d = act == DCN_ACT_SIGMOID ? s * (1.f - s) : s * (1.f + g * (1.f - s));
+}
+
+// ---- one pass: the channels of a tile of positions stay in registers ----------------------
+// Both layouts share the plan: work is cut into tiles (maps: TP neighbouring positions of an
+// image, rows: one row per LPR lanes), the tiles of one workgroup are neighbours, and a thread
+// keeps the same channels in every tile, so its parameter gradients add up in registers. They
+// leave once per workgroup as partials [workgroup][5][C] (scale, w1, b1, w2, b2), an image
+// gate's once per workgroup and image, and block_fold adds them in workgroup order.
+struct Plan {
+  int tpi;            // tiles of an image
+  long tiles;         // of the call
+  int wgs;            // workgroups; workgroup w takes tiles [w · tiles / wgs, (w + 1) · tiles / wgs)
+  int images, P;      // rows without an image gate count as one image
+  bool image_gate;    // ∂gate sums over positions
+  float *part, *gpart;  // [wgs][5][C], [wgs + images][C]: slot wg + image is written once
+};
+
+__device__ __forceinline__ long first_tile(const Plan& q, int w) { return q.tiles * w / q.wgs; }
+
+// the workgroups that share an XCD (equal index mod 8) take neighbouring ranges
+__device__ __forceinline__ int xcd_wg(int n) {
+  const int bid = blockIdx.x, q = n >> 3, r = n & 7, x = bid & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
+}
+
+// Σ over aligned groups of LPR lanes; every lane gets the sum. VALU only (DPP mirrors and
+// lane-row swaps), fixed order.
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (LPR >= 2) v += dpp_f<0xB1>(v);
+  if constexpr (LPR >= 4) v += dpp_f<0x4E>(v);
+  if constexpr (LPR >= 8) v += dpp_f<0x141>(v);
+  if constexpr (LPR >= 16) v += dpp_f<0x140>(v);
+  if constexpr (LPR >= 32) v = swap_fold16(v);
+  if constexpr (LPR >= 64) v = swap_fold32(v);
+  return v;
+}
+// keep bits of the V elements from i
+template <int V>
+__device__ __forceinline__ unsigned keepv(uint64_t i, const PhiloxKey& k, unsigned thr) {
+  const unsigned s = (unsigned)(i & 7);
+  unsigned m = keep8(i >> 3, k, thr) >> s;
+  if (s + V > 8) m |= keep8((i >> 3) + 1, k, thr) << (8 - s);
+  return m;
+}
+
+// ---- maps [B][C][P]: PL lanes of one vector along the positions, NT / PL channel groups, channels
+// cg + CG · i of a thread, i < CPT.
+//
+// Sums over the channels of every position. A thread's partial sums of its V positions go
+// through LDS twice: inside the wave (its GPW channel groups x TP positions, each lane then adds
+// a column's share), then between the waves; finally every wave finishes all TP positions for
+// itself, one lane each, and the threads read their V results back. Done in registers instead
+// (V values through DPP rotations, every thread finishing all its positions) the same sums took
+// two thirds of the kernel's instructions.
+template <int NT, int PL, int V, int CPT>
+struct MapSums {
+  static constexpr int TP = PL * V, NW = NT / 64, GPW = 64 / PL, CG = NT / PL;
+  static constexpr int SHARE = 64 / TP, EACH = GPW / SHARE;  // lanes a position, groups a lane
+  static_assert(TP <= 64 && SHARE * TP == 64 && EACH * SHARE == GPW, "lanes cover the positions");
+  struct Shared {
+    float wave[NW][2][GPW][TP];  // a wave's partials (two quantities)
+    float join[2][NW][2][TP];    // waves' sums, alternating: read in a round, written in the next
+                                 // but one
+    float res[NW][2][TP];        // a wave's copy of the results
+    float2 num[NW];              // channels of every wave and 1 / that (0 of 0)
+  };
+  Shared& sh;
+  int w, lane, pl, gl, C, phase = 0;
+  float inw;  // 1 / channels of this wave
+  __device__ MapSums(Shared& s, int c) : sh(s), C(c) {
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    pl = threadIdx.x % PL;
+    gl = lane / PL;
+    const float n = count(w);
+    inw = n > 0.f ? 1.f / n : 0.f;
+    if (lane == 0) sh.num[w] = make_float2(n, inw);  // read behind the first join's barrier
+  }
+  __device__ float count(int wave) const {  // channels of a wave
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) n += min(max(C - (CG * i + wave * GPW), 0), GPW);
+    return (float)n;
+  }
+  // LDS accesses of one wave happen in order; this keeps the compiler to it
+  static __device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __device__ void put(int k, const float (&v)[V]) {
+    float* d = &sh.wave[w][k][gl][pl * V];
+#pragma unroll
+    for (int e = 0; e < V; e += 4)
+      *reinterpret_cast<float4*>(d + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  }
+  // the wave's sum of quantity k at position lane % TP
+  __device__ float column(int k) const {
+    const float* d = &sh.wave[w][k][(lane / TP) * EACH][lane % TP];
+    float t = d[0];
+#pragma unroll
+    for (int i = 1; i < EACH; ++i) t += d[i * TP];
+    if constexpr (SHARE >= 2) t = swap_fold32(t);
+    if constexpr (SHARE >= 4) t = swap_fold16(t);
+    return t;
+  }
+  __device__ void get(int k, float (&v)[V]) const {
+    const float* d = &sh.res[w][k][pl * V];
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(d + e);
+      v[e] = f.x;
+      v[e + 1] = f.y;
+      v[e + 2] = f.z;
+      v[e + 3] = f.w;
+    }
+  }
+  __device__ void give(int k, float v) {
+    if (lane < TP) sh.res[w][k][lane] = v;
+  }
+  // Σ over all channels, a times fa, b times fb
+  __device__ void sum2(float (&a)[V], float (&b)[V], float fa, float fb) {
+    put(0, a);
+    put(1, b);
+    wave_order();
+    float ta = column(0), tb = column(1);
+    if constexpr (NW > 1) {
+      phase ^= 1;
+      if (lane < TP) {
+        sh.join[phase][w][0][lane] = ta;
+        sh.join[phase][w][1][lane] = tb;
+      }
+      lds_barrier();
+      ta = tb = 0.f;
+#pragma unroll
+      for (int v = 0; v < NW; ++v) {
+        ta += sh.join[phase][v][0][lane % TP];
+        tb += sh.join[phase][v][1][lane % TP];
+      }
+    }
+    give(0, ta * fa);
+    give(1, tb * fb);
+    wave_order();
+    get(0, a);
+    get(1, b);
+    wave_order();
+  }
+  // Mean and 1/sqrt(var + eps) of each position (0 past the map's end, `left` = positions of
+  // the tile, so that nothing from there reaches the parameter sums); mk: 1 for a channel, 0
+  // past the last (its v is 0). Layer: every wave takes its own mean and the squares about it;
+  // the waves' are joined about the whole mean, so large means cancel nowhere.
+  __device__ void moments(const float (&v)[CPT][V], const float (&mk)[CPT], int kind, float eps,
+                          int left, float (&m)[V], float (&r)[V]) {
+    float t[V], s = 0.f, q;
+    if (kind == DCN_NORM_LAYER) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        t[e] = v[0][e];
+#pragma unroll
+        for (int i = 1; i < CPT; ++i) t[e] += v[i][e];
+      }
+      put(0, t);
+      wave_order();
+      s = column(0);
+      give(0, s * inw);
+      wave_order();
+      get(0, m);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        t[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          const float d = fmaf(-m[e], mk[i], v[i][e]);
+          t[e] = fmaf(d, d, t[e]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        t[e] = v[0][e] * v[0][e];
+#pragma unroll
+        for (int i = 1; i < CPT; ++i) t[e] = fmaf(v[i][e], v[i][e], t[e]);
+      }
+    }
+    put(1, t);
+    wave_order();
+    q = column(1);
+    const float ic = 1.f / (float)C;
+    if constexpr (NW > 1) {
+      phase ^= 1;
+      if (lane < TP) {
+        sh.join[phase][w][0][lane] = s;
+        sh.join[phase][w][1][lane] = q;
+      }
+      lds_barrier();
+      q = 0.f;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) q += sh.join[phase][x][1][lane % TP];
+      if (kind == DCN_NORM_LAYER) {
+        float sx[NW];
+        s = 0.f;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+          sx[x] = sh.join[phase][x][0][lane % TP];
+          s += sx[x];
+        }
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+          const float2 n = sh.num[x];
+          const float d = fmaf(sx[x], n.y, -s * ic);  // a wave without channels: s and n are 0
+          q = fmaf(n.x * d, d, q);
+        }
+      }
+    }
+    give(0, s * ic);
+    give(1, lane % TP < left ? rsqrtf(fmaf(q, ic, eps)) : 0.f);
+    wave_order();
+    get(0, m);
+    get(1, r);
+    wave_order();
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float par(const void* t, int c, float none) {
+  return t ? to_f32(static_cast<const T*>(t)[c]) : none;
+}
+
+template <typename T, int NT, int PL, int CPT, int WPE, bool AHEAD, bool BWD, bool FULL, bool DROP>
+__global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
+  constexpr int V = ElemVec<T>::N, TP = PL * V, CG = NT / PL;
+  using Sums = MapSums<NT, PL, V, CPT>;
+  __shared__ __attribute__((aligned(16))) typename Sums::Shared shared;
+  const PhiloxKey key = philox_key(a.drop);
+  const int pl = threadIdx.x % PL, cg = threadIdx.x / PL;
+  Sums sums(shared, a.C);
+  const int wg = xcd_wg(q.wgs);
+  const T *xp = static_cast<const T*>(a.x), *rp = static_cast<const T*>(a.res);
+  const T* gp = static_cast<const T*>(a.gate);
+
+  bool inc[CPT];
+  float mk[CPT];
+  float sc[CPT], w1[CPT], b1[CPT], w2[CPT], b2[CPT];
+  float acc[5][CPT], accg[CPT];
+#pragma unroll
+  for (int i = 0; i < CPT; ++i) {
+    const int c = cg + CG * i;
+    inc[i] = c < a.C;
+    mk[i] = inc[i] ? 1.f : 0.f;
+    sc[i] = a.alpha * (inc[i] ? par<T>(a.scale, c, 1.f) : 0.f);
+    w1[i] = inc[i] ? par<T>(a.w1, c, 1.f) : 0.f;
+    b1[i] = inc[i] ? par<T>(a.b1, c, 0.f) : 0.f;
+    w2[i] = inc[i] ? par<T>(a.w2, c, 1.f) : 0.f;
+    b2[i] = inc[i] ? par<T>(a.b2, c, 0.f) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) acc[k][i] = 0.f;
+    accg[i] = 0.f;
+  }
+  const long t0 = first_tile(q, wg), t1 = first_tile(q, wg + 1);
+  struct Raw {
+    u32x4 x[CPT], r[CPT], g[CPT], y[CPT], o[CPT];
+  } nx;
+  auto load = [&](long t, Raw& w) {
+    const int p = (int)(t % q.tpi) * TP + pl * V, valid = a.P - p;
+    const size_t base = (size_t)(t / q.tpi) * a.C * a.P + p;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      const bool ok = inc[i] && valid > 0;
+      const size_t at = base + (size_t)(cg + CG * i) * a.P;
+      w.x[i] = ok && xp ? ldv_raw(xp + at, valid) : zero;
+      w.r[i] = ok && rp ? ldv_raw(rp + at, valid) : zero;
+      if constexpr (FULL) w.g[i] = ok ? ldv_raw(gp + at, valid) : zero;
+      if constexpr (BWD) {
+        w.y[i] = ok && a.gy ? ldv_raw(static_cast<const T*>(a.gy) + at, valid) : zero;
+        w.o[i] = ok && a.go ? ldv_raw(static_cast<const T*>(a.go) + at, valid) : zero;
+      }
+    }
+  };
+  if (AHEAD && t0 < t1) load(t0, nx);
+  for (long t = t0; t < t1; ++t) {
+    const int b = (int)(t / q.tpi), p = (int)(t % q.tpi) * TP + pl * V, valid = a.P - p;
+    const int left = a.P - (int)(t % q.tpi) * TP;
+    const size_t base = (size_t)b * a.C * a.P + p;
+    bool ok[CPT];
+    size_t at[CPT];
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      ok[i] = inc[i] && valid > 0;
+      at[i] = base + (size_t)(cg + CG * i) * a.P;
+    }
+    if (!AHEAD) load(t, nx);
+    const Raw in = nx;
+    if (AHEAD && t + 1 < t1) load(t + 1, nx);
+    float gv[CPT], gd[CPT];  // an image gate's act and act'
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      gv[i] = 1.f;
+      gd[i] = 0.f;
+      if (a.gate_kind == DCN_GATE_IMAGE && inc[i])
+        gate_act_grad(to_f32(gp[(size_t)b * a.C + cg + CG * i]), a.act, gv[i], gd[i]);
+    }
+    unsigned keep[CPT];
+    if constexpr (DROP) {
+      const unsigned img = a.drop_image && keep1(b, key, a.drop.thr) ? 0xffu : 0u;
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) keep[i] = a.drop_image ? img : keepv<V>(at[i], key, a.drop.thr);
+    }
+    auto drop = [&](int i, int e, float t) {
+      if constexpr (DROP) return (keep[i] >> e) & 1u ? t * a.drop.scale : 0.f;
+      return t;
+    };
+
+    float m1[V], r1[V], m2[V], r2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {  // no post norm: N_post(x) = x
+      m1[e] = 0.f;
+      r1[e] = 1.f;
+    }
+    float o[CPT][V];
+    if (xp) {
+      if (a.post) {
+        float xv[CPT][V];
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) unpack<T>(in.x[i], xv[i]);
+        sums.moments(xv, mk, a.post, a.eps1, left, m1, r1);
+      }
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        float xv[V], rv[V], fv[V];
+        const float k = sc[i] * gv[i];
+        unpack<T>(in.x[i], xv);
+        unpack<T>(in.r[i], rv);
+        if constexpr (FULL) unpack<T>(in.g[i], fv);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float v = fmaf((xv[e] - m1[e]) * r1[e], w1[i], b1[i]);
+          o[i][e] = rv[e] + drop(i, e, v * (FULL ? sc[i] * gate_act(fv[e], a.act) : k));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) unpack<T>(in.r[i], o[i]);
+    }
+    if (a.pre) sums.moments(o, mk, a.pre, a.eps2, left, m2, r2);
+
+    if constexpr (!BWD) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        if (!ok[i]) continue;
+        if (a.pre) {
+          float y[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) y[e] = fmaf((o[i][e] - m2[e]) * r2[e], w2[i], b2[i]);
+          stv(static_cast<T*>(a.y) + at[i], valid, y);
+        }
+        if (a.out) stv(static_cast<T*>(a.out) + at[i], valid, o[i]);
+      }
+    } else {
+      // G into o
+      if (a.pre) {
+        float s1[V], s2[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          float gy[V];
+          unpack<T>(in.y[i], gy);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float h = (o[i][e] - m2[e]) * r2[e], w = gy[e] * w2[i];
+            o[i][e] = h;
+            s1[e] += w;
+            s2[e] = fmaf(w, h, s2[e]);
+            acc[3][i] = fmaf(gy[e], h, acc[3][i]);
+            acc[4][i] += gy[e];
+          }
+        }
+        const float ic = 1.f / (float)a.C;
+        sums.sum2(s1, s2, a.pre == DCN_NORM_LAYER ? ic : 0.f, ic);
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          float gy[V], go[V];
+          unpack<T>(in.y[i], gy);
+          unpack<T>(in.o[i], go);
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            o[i][e] = fmaf(r2[e], gy[e] * w2[i] - s1[e] - o[i][e] * s2[e], go[e]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) unpack<T>(in.o[i], o[i]);
+      }
+      if (a.gr) {
+#pragma unroll
+        for (int i = 0; i < CPT; ++i)
+          if (ok[i]) stv(static_cast<T*>(a.gr) + at[i], valid, o[i]);
+      }
+      if (xp) {
+        // dt, ∂gate, ∂scale; dv into o
+        float s3[V], s4[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s3[e] = s4[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          float xv[V], fv[V], gg[V];
+          const float ka = a.alpha * gv[i], kd = sc[i] * gd[i], k = sc[i] * gv[i];
+          unpack<T>(in.x[i], xv);
+          if constexpr (FULL) unpack<T>(in.g[i], fv);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float h = (xv[e] - m1[e]) * r1[e], v = fmaf(h, w1[i], b1[i]);
+            const float dt = drop(i, e, o[i][e]), dtv = dt * v;
+            float dv;
+            if constexpr (FULL) {
+              float av, ad;
+              gate_act_grad(fv[e], a.act, av, ad);
+              dv = dt * (sc[i] * av);
+              gg[e] = dtv * (sc[i] * ad);
+              acc[0][i] = fmaf(dtv, a.alpha * av, acc[0][i]);
+            } else {
+              dv = dt * k;
+              accg[i] = fmaf(dtv, kd, accg[i]);
+              acc[0][i] = fmaf(dtv, ka, acc[0][i]);
+            }
+            acc[1][i] = fmaf(dv, h, acc[1][i]);
+            acc[2][i] += dv;
+            o[i][e] = dv;
+            const float w = dv * w1[i];
+            s3[e] += w;
+            s4[e] = fmaf(w, h, s4[e]);
+          }
+          if (FULL && a.gg && ok[i])
+            stv(static_cast<T*>(a.gg) + at[i], valid, gg);
+        }
+        if (a.gx) {
+          if (a.post) {
+            const float ic = 1.f / (float)a.C;
+            sums.sum2(s3, s4, a.post == DCN_NORM_LAYER ? ic : 0.f, ic);
+          }
+#pragma unroll
+          for (int i = 0; i < CPT; ++i) {
+            if (!ok[i]) continue;
+            if (a.post) {
+              float xv[V];
+              unpack<T>(in.x[i], xv);
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                const float h = (xv[e] - m1[e]) * r1[e];
+                o[i][e] = r1[e] * (o[i][e] * w1[i] - s3[e] - h * s4[e]);
+              }
+            }
+            stv(static_cast<T*>(a.gx) + at[i], valid, o[i]);
+          }
+        }
+        if (q.image_gate && (t + 1 == t1 || (t + 1) % q.tpi == 0)) {
+#pragma unroll
+          for (int i = 0; i < CPT; ++i) {
+            const float g = group_sum<PL>(accg[i]);
+            if (inc[i] && pl == 0) q.gpart[(size_t)(wg + b) * a.C + cg + CG * i] = g;
+            accg[i] = 0.f;
+          }
+        }
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (!q.part) return;
+#pragma unroll
+    for (int i = 0; i < CPT; ++i)
+#pragma unroll
+      for (int k = 0; k < 5; ++k) {
+        const float g = group_sum<PL>(acc[k][i]);
+        if (inc[i] && pl == 0) q.part[((size_t)wg * 5 + k) * a.C + cg + CG * i] = g;
+      }
+  }
+}
+
+// ---- rows [B][P][C]: LPR lanes a row, NV vectors a lane (channels (lane + LPR · j) · V ..), NT / LPR
+// rows of one image at a time. LPR <= 64: a row stays inside a wave and its sums are lane
+// exchanges; above, a workgroup holds one row and the waves join through LDS.
+template <int NT, int LPR, int V, int NV>
+struct RowSums {
+  static constexpr int NW = LPR > 64 ? LPR / 64 : 1, GR = NT / LPR;
+  struct Shared {
+    float join[2][GR][NW][2];  // alternating, as in MapSums
+    float2 num[NW];
+  };
+  Shared& sh;
+  int lane, g, w, C, phase = 0;
+  float inw = 0.f;
+  bool tail;  // some lane's last vector is not full
+  __device__ RowSums(Shared& s, int c) : sh(s), C(c) {
+    lane = threadIdx.x % LPR;
+    g = threadIdx.x / LPR;
+    w = lane >> 6;
+    tail = c != LPR * NV * V;
+    if constexpr (NW > 1) {
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) n += min(max(c - (LPR * j + w * 64) * V, 0), 64 * V);
+      inw = n > 0 ? 1.f / (float)n : 0.f;
+      if ((lane & 63) == 0) sh.num[w] = make_float2((float)n, inw);
+    }
+  }
+  __device__ void sum2(float& a, float& b) {
+    constexpr int G = LPR < 64 ? LPR : 64;
+    a = group_sum<G>(a);
+    b = group_sum<G>(b);
+    if constexpr (NW > 1) {
+      phase ^= 1;
+      if ((lane & 63) == 0) {
+        sh.join[phase][g][w][0] = a;
+        sh.join[phase][g][w][1] = b;
+      }
+      lds_barrier();
+      a = b = 0.f;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) {
+        a += sh.join[phase][g][x][0];
+        b += sh.join[phase][g][x][1];
+      }
+    }
+  }
+  // v is 0 past the last channel
+  __device__ void moments(const float (&v)[NV][V], int kind, float eps, bool live, float& m,
+                          float& r) {
+    constexpr int G = LPR < 64 ? LPR : 64;
+    const float ic = 1.f / (float)C;
+    float s = 0.f, q = 0.f, mu = 0.f;
+    if (kind == DCN_NORM_LAYER) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += v[j][e];
+      s = group_sum<G>(s);
+      mu = s * (NW > 1 ? inw : ic);
+    }
+    if (tail && kind == DCN_NORM_LAYER) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = (lane + LPR * j) * V + e < C ? v[j][e] - mu : 0.f;
+          q = fmaf(d, d, q);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = v[j][e] - mu;
+          q = fmaf(d, d, q);
+        }
+    }
+    q = group_sum<G>(q);
+    m = mu;
+    if constexpr (NW > 1) {
+      phase ^= 1;
+      if ((lane & 63) == 0) {
+        sh.join[phase][g][w][0] = s;
+        sh.join[phase][g][w][1] = q;
+      }
+      lds_barrier();
+      s = q = 0.f;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) {
+        s += sh.join[phase][g][x][0];
+        q += sh.join[phase][g][x][1];
+      }
+      m = s * ic;
+      if (kind == DCN_NORM_LAYER) {
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+          const float2 n = sh.num[x];
+          const float d = fmaf(sh.join[phase][g][x][0], n.y, -m);
+          q = fmaf(n.x * d, d, q);
+        }
+      }
+    }
+    r = live ? rsqrtf(fmaf(q, ic, eps)) : 0.f;
+  }
+};
+
+template <typename T, int NT, int LPR, int NV, int WPE, bool AHEAD, bool BWD, bool FULL, bool DROP>
+__global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
+  constexpr int V = ElemVec<T>::N, GR = NT / LPR;
+  using Sums = RowSums<NT, LPR, V, NV>;
+  __shared__ __attribute__((aligned(16))) typename Sums::Shared shared;
+  __shared__ float fold[BWD ? GR : 1][BWD ? LPR * NV * V : 1];
+  const PhiloxKey key = philox_key(a.drop);
+  Sums sums(shared, a.C);
+  const int lane = sums.lane, g = threadIdx.x / LPR;
+  const int wg = xcd_wg(q.wgs);
+  auto ptr = [](const void* p) { return static_cast<const T*>(p); };
+
+  int cv[NV];  // valid elements of a vector
+  u32x4 psc[NV], pw1[NV], pb1[NV], pw2[NV], pb2[NV];
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  u32x4 one;
+  {
+    float t[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[e] = 1.f;
+    one = pack<T>(t);
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (lane + LPR * j) * V;
+    cv[j] = a.C - c;
+    auto get = [&](const void* p, u32x4 none) {
+      return cv[j] <= 0 ? zero : p ? ldv_raw(ptr(p) + c, cv[j]) : none;
+    };
+    psc[j] = get(a.scale, one);
+    pw1[j] = get(a.w1, one);
+    pb1[j] = get(a.b1, zero);
+    pw2[j] = get(a.w2, one);
+    pb2[j] = BWD ? zero : get(a.b2, zero);
+  }
+  float acc[BWD ? 5 : 1][NV][V], accg[BWD && !FULL ? NV : 1][V];
+  if constexpr (BWD) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) acc[k][j][e] = 0.f;
+        if constexpr (!FULL) accg[j][e] = 0.f;
+      }
+  }
+  // Σ of v over the row groups of the workgroup, to dst[C]
+  auto fold_groups = [&](const float (&v)[NV][V], float* dst) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) fold[g][(lane + LPR * j) * V + e] = v[j][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.C; c += NT) {
+      float s = fold[0][c];
+#pragma unroll
+      for (int x = 1; x < GR; ++x) s += fold[x][c];
+      dst[c] = s;
+    }
+  };
+
+  const long t0 = first_tile(q, wg), t1 = first_tile(q, wg + 1);
+  struct Raw {
+    u32x4 x[NV], r[NV], g[NV], y[NV], o[NV];
+  } nx;
+  auto load = [&](long t, Raw& w) {
+    const int b = (int)(t / q.tpi), p = (int)(t % q.tpi) * GR + g;
+    const size_t base = ((size_t)b * q.P + p) * a.C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const bool ok = p < q.P && cv[j] > 0;
+      const size_t at = base + (lane + LPR * j) * V;
+      w.x[j] = ok && a.x ? ldv_raw(ptr(a.x) + at, cv[j]) : zero;
+      w.r[j] = ok && a.res ? ldv_raw(ptr(a.res) + at, cv[j]) : zero;
+      if constexpr (FULL) w.g[j] = ok ? ldv_raw(ptr(a.gate) + at, cv[j]) : zero;
+      if constexpr (BWD) {
+        w.y[j] = ok && a.gy ? ldv_raw(ptr(a.gy) + at, cv[j]) : zero;
+        w.o[j] = ok && a.go ? ldv_raw(ptr(a.go) + at, cv[j]) : zero;
+      }
+    }
+  };
+  if (AHEAD && t0 < t1) load(t0, nx);
+  for (long t = t0; t < t1; ++t) {
+    const int b = (int)(t / q.tpi), p = (int)(t % q.tpi) * GR + g;
+    const bool live = p < q.P;
+    const size_t base = ((size_t)b * q.P + p) * a.C;
+    if (!AHEAD) load(t, nx);
+    const Raw in = nx;
+    if (AHEAD && t + 1 < t1) load(t + 1, nx);
+
+    unsigned keep[NV];
+    if constexpr (DROP) {
+      const int image = q.images == a.B ? b : (int)(((size_t)b * q.P + p) / a.P);
+      const unsigned img = a.drop_image && keep1(image, key, a.drop.thr) ? 0xffu : 0u;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        keep[j] = a.drop_image ? img
+                               : keepv<V>(base + (lane + LPR * j) * V, key, a.drop.thr);
+    }
+    auto drop = [&](int j, int e, float v) {
+      if constexpr (DROP) return (keep[j] >> e) & 1u ? v * a.drop.scale : 0.f;
+      return v;
+    };
+    // the gate's value and slope; an image's gate is read here (the same row for all positions)
+    auto gate = [&](int j, float (&av)[V], float (&ad)[V]) {
+      float f[V];
+      if constexpr (FULL) {
+        unpack<T>(in.g[j], f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          av[e] = 1.f;
+          ad[e] = 0.f;
+        }
+        if (a.gate_kind == DCN_GATE_NONE || cv[j] <= 0) return;
+        ldv(ptr(a.gate) + (size_t)b * a.C + (lane + LPR * j) * V, cv[j], f);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) gate_act_grad(f[e], a.act, av[e], ad[e]);
+    };
+
+    float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
+    float o[NV][V];
+    if (a.x) {
+      if (a.post) {
+        float xv[NV][V];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) unpack<T>(in.x[j], xv[j]);
+        sums.moments(xv, a.post, a.eps1, live, m1, r1);
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float xv[V], rv[V], sc[V], w1[V], b1[V], av[V], ad[V];
+        unpack<T>(in.x[j], xv);
+        unpack<T>(in.r[j], rv);
+        unpack<T>(psc[j], sc);
+        unpack<T>(pw1[j], w1);
+        unpack<T>(pb1[j], b1);
+        gate(j, av, ad);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float v = fmaf((xv[e] - m1) * r1, w1[e], b1[e]);
+          o[j][e] = rv[e] + drop(j, e, v * (a.alpha * sc[e] * av[e]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) unpack<T>(in.r[j], o[j]);
+    }
+    if (a.pre) sums.moments(o, a.pre, a.eps2, live, m2, r2);
+
+    if constexpr (!BWD) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (!live || cv[j] <= 0) continue;
+        const size_t at = base + (lane + LPR * j) * V;
+        if (a.pre) {
+          float w2[V], b2[V], y[V];
+          unpack<T>(pw2[j], w2);
+          unpack<T>(pb2[j], b2);
+#pragma unroll
+          for (int e = 0; e < V; ++e) y[e] = fmaf((o[j][e] - m2) * r2, w2[e], b2[e]);
+          stv(static_cast<T*>(a.y) + at, cv[j], y);
+        }
+        if (a.out) stv(static_cast<T*>(a.out) + at, cv[j], o[j]);
+      }
+    } else {
+      const float ic = 1.f / (float)a.C;
+      // G into o
+      if (a.pre) {
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          float gy[V], w2[V];
+          unpack<T>(in.y[j], gy);
+          unpack<T>(pw2[j], w2);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float h = (o[j][e] - m2) * r2, w = gy[e] * w2[e];
+            o[j][e] = h;
+            s1 += w;
+            s2 = fmaf(w, h, s2);
+            acc[3][j][e] = fmaf(gy[e], h, acc[3][j][e]);
+            acc[4][j][e] += gy[e];
+          }
+        }
+        sums.sum2(s1, s2);
+        s1 = a.pre == DCN_NORM_LAYER ? s1 * ic : 0.f;
+        s2 *= ic;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          float gy[V], go[V], w2[V];
+          unpack<T>(in.y[j], gy);
+          unpack<T>(in.o[j], go);
+          unpack<T>(pw2[j], w2);
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            o[j][e] = fmaf(r2, gy[e] * w2[e] - s1 - o[j][e] * s2, go[e]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) unpack<T>(in.o[j], o[j]);
+      }
+      if (a.gr) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (live && cv[j] > 0)
+            stv(static_cast<T*>(a.gr) + base + (lane + LPR * j) * V, cv[j], o[j]);
+      }
+      if (a.x) {
+        float s3 = 0.f, s4 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          float xv[V], sc[V], w1[V], b1[V], av[V], ad[V], gg[V];
+          unpack<T>(in.x[j], xv);
+          unpack<T>(psc[j], sc);
+          unpack<T>(pw1[j], w1);
+          unpack<T>(pb1[j], b1);
+          gate(j, av, ad);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float h = (xv[e] - m1) * r1, v = fmaf(h, w1[e], b1[e]);
+            const float dt = drop(j, e, o[j][e]), dtv = dt * v, k = a.alpha * sc[e];
+            const float dv = dt * (k * av[e]);
+            gg[e] = dtv * (k * ad[e]);
+            acc[0][j][e] = fmaf(dtv, a.alpha * av[e], acc[0][j][e]);
+            acc[1][j][e] = fmaf(dv, h, acc[1][j][e]);
+            acc[2][j][e] += dv;
+            if constexpr (!FULL) accg[j][e] += gg[e];
+            o[j][e] = dv;
+            const float w = dv * w1[e];
+            s3 += w;
+            s4 = fmaf(w, h, s4);
+          }
+          if (FULL && a.gg && live && cv[j] > 0)
+            stv(static_cast<T*>(a.gg) + base + (lane + LPR * j) * V, cv[j], gg);
+        }
+        if (a.gx) {
+          if (a.post) {
+            sums.sum2(s3, s4);
+            s3 = a.post == DCN_NORM_LAYER ? s3 * ic : 0.f;
+            s4 *= ic;
+          }
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            if (!live || cv[j] <= 0) continue;
+            if (a.post) {
+              float xv[V], w1[V];
+              unpack<T>(in.x[j], xv);
+              unpack<T>(pw1[j], w1);
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                const float h = (xv[e] - m1) * r1;
+                o[j][e] = r1 * (o[j][e] * w1[e] - s3 - h * s4);
+              }
+            }
+            stv(static_cast<T*>(a.gx) + base + (lane + LPR * j) * V, cv[j], o[j]);
+          }
+        }
+        if constexpr (!FULL) {
+          if (q.image_gate && (t + 1 == t1 || (t + 1) % q.tpi == 0)) {
+            fold_groups(accg, q.gpart + (size_t)(wg + b) * a.C);
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+              for (int e = 0; e < V; ++e) accg[j][e] = 0.f;
+          }
+        }
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (!q.part) return;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) fold_groups(acc[k], q.part + ((size_t)wg * 5 + k) * a.C);
+  }
+}
+
+// The partials of one parameter (k < 5) or of one image's gate (k = 5 + image), 64 channels
+// per workgroup, added in workgroup order: 16 threads a channel, then a tree over them.
+template <typename T>
+__global__ __launch_bounds__(1024) void block_fold(BlockArgs a, Plan q, int k0) {
+  __shared__ float red[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6, k = k0 + blockIdx.y;
+  void* dst[5] = {a.gs, a.gw1, a.gb1, a.gw2, a.gb2};
+  T* out = k < 5 ? static_cast<T*>(dst[k]) : static_cast<T*>(a.gg) + (size_t)(k - 5) * a.C;
+  if (k < 5 && !dst[k]) return;
+  float s = 0.f;
+  if (c < a.C) {
+    if (k < 5) {
+#pragma unroll 4
+      for (int w = g; w < q.wgs; w += 16) s += q.part[((size_t)w * 5 + k) * a.C + c];
+    } else {
+      // workgroups whose range meets this image's tiles
+      const long lo = (long)(k - 5) * q.tpi, hi = lo + q.tpi;
+      int w0 = (int)(lo * q.wgs / q.tiles);
+      while (w0 > 0 && first_tile(q, w0) > lo) --w0;
+      while (first_tile(q, w0 + 1) <= lo) ++w0;
+      for (int w = w0 + g; w < q.wgs && first_tile(q, w) < hi; w += 16)
+        if (first_tile(q, w + 1) > first_tile(q, w)) s += q.gpart[(size_t)(w + k - 5) * a.C + c];
+    }
+  }
+  red[g][threadIdx.x & 63] = s;
+  __syncthreads();
+  for (int o = 8; o > 0; o >>= 1) {
+    if (g < o) red[g][threadIdx.x & 63] += red[g + o][threadIdx.x & 63];
+    __syncthreads();
+  }
+  if (g == 0 && c < a.C) out[c] = from_f32(red[0][threadIdx.x], T());
+}
+
+constexpr int kMaxWgs = 1024;  // workgroups with partials
+
+// Fills the plan for tiles of `per` positions, launches `kernel(full gate, dropout)` and the fold.
+template <typename T, bool BWD, typename K>
+hipError_t run_tiles(const BlockArgs& a, int images, int P, int per, int wgs, int threads, K kernel,
+                     hipStream_t s) {
+  Plan q{};
+  q.images = images;
+  q.P = P;
+  q.tpi = (P + per - 1) / per;
+  q.tiles = (long)q.tpi * images;
+  const bool params = BWD && (a.gs || a.gw1 || a.gb1 || a.gw2 || a.gb2);
+  q.image_gate = BWD && a.gg && a.gate_kind == DCN_GATE_IMAGE;
+  q.wgs = (int)std::min<long>(q.tiles, wgs ? wgs : params || q.image_gate ? kMaxWgs : 1 << 20);
+  if (params) q.part = a.ws;
+  if (q.image_gate) q.gpart = a.ws + (size_t)kMaxWgs * 5 * a.C;
+  auto* fn = kernel(a.gate_kind == DCN_GATE_FULL, a.drop.thr != 0);
+  hipLaunchKernelGGL(fn, dim3(q.wgs), dim3(threads), 0, s, a, q);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !(params || q.image_gate)) return e;
+  // (a parameter without a destination ends at once; an image gate's rows start at 5)
+  for (int k = params ? 0 : 5, n; k < 5 + (q.image_gate ? a.B : 0); k += n) {
+    n = std::min(5 + (q.image_gate ? a.B : 0) - k, 32768);
+    hipLaunchKernelGGL((block_fold<T>), dim3((a.C + 63) / 64, n), dim3(1024), 0, s, a, q, k);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <typename T, int NT, int PL, int CPT, int WPE, int WGS, bool BWD>
+hipError_t run_map(const BlockArgs& a, hipStream_t s) {
+  auto pick = [](bool full, bool drop) {
+    return full ? (drop ? block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, true, true>
+                        : block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, true, false>)
+                : (drop ? block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, false, true>
+                        : block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, false, false>);
+  };
+  return run_tiles<T, BWD>(a, a.B, a.P, PL * ElemVec<T>::N, WGS, NT, pick, s);
+}
+
+template <typename T, int NT, int LPR, int NV, int WPE, int WGS, bool BWD>
+hipError_t run_row(const BlockArgs& a, hipStream_t s) {
+  auto pick = [](bool full, bool drop) {
+    return full ? (drop ? block_row<T, NT, LPR, NV, WPE, WGS != 0, BWD, true, true>
+                        : block_row<T, NT, LPR, NV, WPE, WGS != 0, BWD, true, false>)
+                : (drop ? block_row<T, NT, LPR, NV, WPE, WGS != 0, BWD, false, true>
+                        : block_row<T, NT, LPR, NV, WPE, WGS != 0, BWD, false, false>);
+  };
+  // images matter to an image gate only; else all rows are one run (up to int)
+  const bool one = a.gate_kind != DCN_GATE_IMAGE && (size_t)a.B * a.P < (1u << 30);
+  return run_tiles<T, BWD>(a, one ? 1 : a.B, one ? a.B * a.P : a.P, NT / LPR, WGS, NT, pick, s);
+}
+
+}  // namespace
+
+}  // namespace dcn
