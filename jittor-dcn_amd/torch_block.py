@@ -14,7 +14,6 @@ tensor is updated between replays). The backward draws the same mask again.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 
@@ -26,22 +25,48 @@ import dcn_runtime as rt
 _DT = {torch.float32: rt.DCN_F32, torch.bfloat16: rt.DCN_BF16}
 _handles = {}
 _lock = threading.Lock()  # a handle takes one caller at a time: stream and launch belong together
-_null = contextlib.nullcontext()
+_fns = {}
 
 
-def _call(dev: torch.device, fn: str, *args):
+def _fn(name):
+    """The entry point, bound so that the call keeps the GIL: these calls only enqueue, and
+    giving the GIL up and taking it back around each costs more than the call itself (a
+    backward runs beside the thread that waits for it)."""
+    f = _fns.get(name)
+    if f is None:
+        lib = rt.load()
+        f = getattr(ctypes.PyDLL(lib._name, handle=lib._handle), name)
+        f.argtypes, f.restype = rt.SIGNATURES[name], ctypes.c_int
+        _fns[name] = f
+    return f
+
+
+def _call(dev: torch.device, name: str, *args):
     """One libdcn call on torch's current stream of `dev`, whatever device is current."""
-    here = torch.cuda.current_device()
-    idx = dev.index if dev.index is not None else here
-    with (_null if idx == here else torch.cuda.device(idx)), _lock:
+    idx = dev.index
+    if idx != torch._C._cuda_getDevice():
+        with torch.cuda.device(idx):
+            return _call(dev, name, *args)
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    with _lock:
         h = _handles.get(idx)
         if h is None:
             h = _handles[idx] = rt.Handle(idx)
-        stream = torch.cuda.current_stream(idx).cuda_stream
-        if getattr(h, "bound", -1) != stream:
+            h.bound = None
+        if h.bound != stream:
             h.set_stream(stream)
             h.bound = stream
-        rt.check(getattr(h.lib, fn)(h.h, *args), fn)
+        rc = _fn(name)(h.h, *args)
+    if rc:
+        rt.check(rc, name)
+
+
+def _wants_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _ptr(t):
@@ -90,17 +115,21 @@ def _fresh_rng(rng):
 
 
 # ---------------------------------------------------------------------------- dropout
+def _drop(x, residual, p, rng, group):
+    seed, offset, dev_rng = _rng(rng, x.device, "dropout")
+    d = rt.DropoutDesc(x.numel(), group, seed, offset, _DT[x.dtype], p)
+    x = x.contiguous()
+    residual = residual.contiguous() if residual is not None else None
+    y = torch.empty_like(x)
+    if d.n:
+        _call(x.device, "dcn_dropout_fwd", d, _ptr(x), _ptr(residual), _ptr(y), _ptr(dev_rng))
+    return y, d, dev_rng
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, rng, group):
-        seed, offset, dev_rng = _rng(rng, x.device, "dropout")
-        d = rt.DropoutDesc(x.numel(), group, seed, offset, _DT[x.dtype], p)
-        x = x.contiguous()
-        residual = residual.contiguous() if residual is not None else None
-        y = torch.empty_like(x)
-        if x.numel():
-            _call(x.device, "dcn_dropout_fwd", d, _ptr(x), _ptr(residual), _ptr(y), _ptr(dev_rng))
-        ctx.desc = d
+        y, ctx.desc, dev_rng = _drop(x, residual, p, rng, group)
         ctx.save_for_backward(dev_rng)
         return y
 
@@ -137,7 +166,8 @@ def dropout(x, p, rng, group="element", residual=None):
             group *= s
     if group < 1 and x.numel():
         raise ValueError("dropout: group must be positive")
-    return _Dropout.apply(x, residual, float(p), rng, max(int(group), 1))
+    args = (x, residual, float(p), rng, max(int(group), 1))
+    return _Dropout.apply(*args) if _wants_grad(x, residual) else _drop(*args)[0]
 
 
 class Dropout(torch.nn.Module):
@@ -181,27 +211,27 @@ def _layout(x):
     return rt.DCN_NHWC, B, C, x.numel() // max(B * C, 1), torch.contiguous_format
 
 
-_GRADS = ("x", "residual", "gate", "scale", "w_post", "b_post", "w_pre", "b_pre")
+def _block(tensors, desc, mf, dev_rng):
+    """(out, y) and the dense tensors behind them."""
+    x, residual, gate = tensors[:3]
+    full = (True, True, desc.gate == rt.DCN_GATE_FULL)
+    tensors = [t if t is None else t.contiguous(memory_format=mf) if i < 3 and full[i]
+               else t.contiguous() for i, t in enumerate(tensors)]
+    x, ref = tensors[0], tensors[1] if tensors[0] is None else tensors[0]
+    out = torch.empty_like(x, memory_format=mf) if x is not None else None
+    y = torch.empty_like(ref, memory_format=mf) if desc.pre else None
+    if ref.numel():
+        _call(ref.device, "dcn_block_norm_fwd", desc,
+              rt.BlockIO(*map(_ptr, (*tensors, dev_rng, out, y))))
+    return out, y, tensors
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, gate, scale, w_post, b_post, w_pre, b_pre, desc, mf, dev_rng):
-        ref = residual if x is None else x
-        full = lambda t: None if t is None else t.contiguous(memory_format=mf)
-        x, residual = full(x), full(residual)
-        gate = full(gate) if desc.gate == rt.DCN_GATE_FULL else gate
-        gate, scale, w_post, b_post, w_pre, b_pre = (
-            t if t is None or t is gate and desc.gate == rt.DCN_GATE_FULL else t.contiguous()
-            for t in (gate, scale, w_post, b_post, w_pre, b_pre))
-        out = torch.empty_like(x, memory_format=mf) if x is not None else None
-        y = torch.empty_like(ref, memory_format=mf) if desc.pre else None
-        if ref.numel():
-            io = rt.BlockIO(*map(_ptr, (x, residual, gate, scale, w_post, b_post, w_pre, b_pre,
-                                        dev_rng, out, y)))
-            _call(ref.device, "dcn_block_norm_fwd", desc, io)
+    def forward(ctx, desc, mf, dev_rng, *tensors):
+        out, y, tensors = _block(tensors, desc, mf, dev_rng)
         ctx.desc, ctx.mf = desc, mf
-        ctx.save_for_backward(x, residual, gate, scale, w_post, b_post, w_pre, b_pre, dev_rng)
+        ctx.save_for_backward(*tensors, dev_rng)
         ctx.set_materialize_grads(False)
         return out, y
 
@@ -209,23 +239,22 @@ class _BlockNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out, grad_y):
         *inputs, dev_rng = ctx.saved_tensors
-        need = ctx.needs_input_grad[:8]
+        need = ctx.needs_input_grad[3:]
         if grad_out is None and grad_y is None:
             return (None,) * 11
         full = lambda t: None if t is None else t.contiguous(memory_format=ctx.mf)
         grad_out, grad_y = full(grad_out), full(grad_y)
         ref = inputs[0] if inputs[0] is not None else inputs[1]
         if not ref.numel():
-            return (*(torch.zeros_like(t) if n else None for t, n in zip(inputs, need)),
-                    None, None, None)
+            return (None, None, None,
+                    *(torch.zeros_like(t) if n else None for t, n in zip(inputs, need)))
         grads = [torch.empty_like(t) if n else None for t, n in zip(inputs, need)]
         nbytes = ctypes.c_size_t()
-        rt.check(rt.load().dcn_block_norm_workspace(ctx.desc, ctypes.byref(nbytes)),
-                 "dcn_block_norm_workspace")
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=ref.device)
+        rt.check(_fn("dcn_block_norm_workspace")(ctx.desc, nbytes), "dcn_block_norm_workspace")
+        ws = _bytes(ref.device, nbytes.value)
         io = rt.BlockIO(*map(_ptr, (*inputs, dev_rng, None, None, grad_out, grad_y, *grads)))
         _call(ref.device, "dcn_block_norm_bwd", ctx.desc, io, ws.data_ptr(), nbytes.value)
-        return (*grads, None, None, None)
+        return (None, None, None, *grads)
 
 
 def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=None, alpha=1.0,
@@ -268,8 +297,11 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     seed, offset, dev_rng = _rng(rng, ref.device, "block_norm") if drop_p > 0 else (0, 0, None)
     desc = rt.BlockDesc(B, C, P, layout, dt, _NORM[post], _NORM[pre], kind, _ACT[gate_act], e1, e2,
                         alpha, drop_p, int(drop == "image"), seed, offset)
-    out, y = _BlockNorm.apply(x, residual, gate, scale, post_weight, post_bias, pre_weight,
-                              pre_bias, desc, mf, dev_rng)
+    tensors = (x, residual, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
+    if _wants_grad(*tensors):
+        out, y = _BlockNorm.apply(desc, mf, dev_rng, *tensors)
+    else:
+        out, y, _ = _block(tensors, desc, mf, dev_rng)
     return (residual if x is None else out), y
 
 
@@ -376,8 +408,7 @@ def _quantize(v, geo, tokens, channels):
 
 def _matmul(desc, a, sa, b, sb, out):
     nbytes = ctypes.c_size_t()
-    rt.check(rt.load().dcn_fp8_matmul_workspace(desc, ctypes.byref(nbytes)),
-             "dcn_fp8_matmul_workspace")
+    rt.check(_fn("dcn_fp8_matmul_workspace")(desc, nbytes), "dcn_fp8_matmul_workspace")
     ws = _bytes(out.device, nbytes.value) if nbytes.value else None
     _call(out.device, "dcn_fp8_matmul", desc, _ptr(a), _ptr(sa), _ptr(b), _ptr(sb), _ptr(out),
           _ptr(ws), nbytes.value)
