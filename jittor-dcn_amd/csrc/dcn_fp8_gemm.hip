@@ -17,6 +17,8 @@
 // Rows of a 64-row group are dealt to the fragments in turn (fragment f, lane r = row 4r + f):
 // one aligned dword of exponents then serves a lane's four fragments (the instruction picks the
 // byte), and a lane's four columns of the result are neighbours, stored as one vector.
+#include <type_traits>
+
 #include "dcn_block.h"
 #include "dcn_philox.h"
 
@@ -31,15 +33,15 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(1))) void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;
 
-constexpr int kT = 128;  // tile rows of either operand, and K per stage
-constexpr int kThreads = 256;
-constexpr int kStage = 2 * kT * 128;  // bytes: a's rows, then b's
-
 struct GemmArgs {
   const unsigned char *a, *sa, *b, *sb;
   void* out;
-  int M, N, K, P, nchw, a_shift, b_shift;  // shift: log2 of rows per exponent
-  long sa_str, sb_str;
+  float* part;  // split K: fp32 partials [split][M][N]
+  int M, N, nkb, P, nchw, a_shift, b_shift;  // shift: log2 of rows per exponent
+  long K, sa_str, sb_str;
+  int vec;         // four neighbouring columns may be stored at once
+  int kb_split;    // k blocks of a split
+  int tiles_m, tiles_n;
 };
 
 // row of a tile that LDS row `slot` holds
@@ -55,9 +57,9 @@ __device__ __forceinline__ int exps4(const unsigned char* s, long str, int shift
   return *reinterpret_cast<const int*>(p + min((long)(row0 + 4 * r), str - 4));
 }
 
-// eight bytes (dwords 2p, 2p + 1 of a fragment) as bf16, with the exponent in byte f of e4
-__device__ __forceinline__ bf16x8 widen(const i32x8& v, int p, int e4, int f) {
-  const float sc = __uint_as_float((((unsigned)e4 >> (8 * f)) & 255u) << 23);
+// eight bytes (dwords 2p, 2p + 1 of a fragment) as bf16, with the exponent `e`
+__device__ __forceinline__ bf16x8 widen(const i32x8& v, int p, unsigned e) {
+  const float sc = __uint_as_float(e << 23);
   bf16x2 w[4];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -67,113 +69,351 @@ __device__ __forceinline__ bf16x8 widen(const i32x8& v, int p, int e4, int f) {
   return bf16x8{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
 }
 
-template <bool WIDE>
-__global__ __launch_bounds__(kThreads) void fp8_gemm(GemmArgs g) {
-  __shared__ __attribute__((aligned(1024))) char ring0[kStage], ring1[kStage];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned tiles_m = (g.M + kT - 1) / kT;
-  const int m0 = (blockIdx.x % tiles_m) * kT, n0 = (blockIdx.x / tiles_m) * kT;
-  const int nkb = g.K / 128;
+template <int I, int J>
+__device__ __forceinline__ f32x4 mfma8(const i32x8& a, const i32x8& b, f32x4 c, int ea, int eb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, I, ea, J, eb);
+}
 
-  // 1 KiB per instruction: 8 LDS rows of 128 bytes; 16-byte chunk c of row t sits at c ^ (t >> 1)
+// four fragments of a times four of b (one 64-row group of either)
+template <bool WIDE>
+__device__ __forceinline__ void quad(const i32x8 (&a)[4], const i32x8 (&b)[4], int ea, int eb,
+                                     f32x4 (&c)[4][4]) {
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      bf16x8 xa[4], xb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        xa[i] = widen(a[i], p, ((unsigned)ea >> (8 * i)) & 255u);
+        xb[i] = widen(b[i], p, ((unsigned)eb >> (8 * i)) & 255u);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          c[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[i], xb[j], c[i][j], 0, 0, 0);
+    }
+  } else {
+#define DCN_ROW(i)                                \
+  c[i][0] = mfma8<i, 0>(a[i], b[0], c[i][0], ea, eb); \
+  c[i][1] = mfma8<i, 1>(a[i], b[1], c[i][1], ea, eb); \
+  c[i][2] = mfma8<i, 2>(a[i], b[2], c[i][2], ea, eb); \
+  c[i][3] = mfma8<i, 3>(a[i], b[3], c[i][3], ea, eb);
+    DCN_ROW(0)
+    DCN_ROW(1)
+    DCN_ROW(2)
+    DCN_ROW(3)
+#undef DCN_ROW
+  }
+}
+
+// where element (m, n) of the result lies
+__device__ __forceinline__ size_t out_at(const GemmArgs& g, int m, int n) {
+  if (!g.nchw) return (size_t)m * g.N + n;
+  const int b = n / g.P;
+  return ((size_t)b * g.M + m) * g.P + (n - b * g.P);
+}
+template <bool WIDE>
+__device__ __forceinline__ void put(const GemmArgs& g, size_t at, float v) {
+  if constexpr (WIDE)
+    static_cast<float*>(g.out)[at] = v;
+  else
+    static_cast<bf16_t*>(g.out)[at] = f2bf(v);
+}
+// columns n .. n + 3 of row m
+template <bool WIDE>
+__device__ __forceinline__ void put4(const GemmArgs& g, int m, int n, f32x4 v) {
+  if (g.vec && n + 4 <= g.N) {
+    const size_t at = out_at(g, m, n);
+    if constexpr (WIDE) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + at) = v;
+    } else {
+      const float t[4] = {v[0], v[1], v[2], v[3]};
+      uint2 u;
+      u.x = (unsigned)f2bf(t[0]) | ((unsigned)f2bf(t[1]) << 16);
+      u.y = (unsigned)f2bf(t[2]) | ((unsigned)f2bf(t[3]) << 16);
+      *reinterpret_cast<uint2*>(static_cast<bf16_t*>(g.out) + at) = u;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (n + j < g.N) put<WIDE>(g, out_at(g, m, n + j), v[j]);
+}
+
+// ---- tiles: WM x WN waves, each GA x GB groups of 64 x 64, K in stages of 128 through two LDS
+// buffers: while one is multiplied, LDS-DMA fills the other.
+template <int GA, int GB, int WM, int WN, int WPE, bool WIDE, bool SPLIT>
+__global__ __launch_bounds__(WM* WN * 64, WPE) void fp8_gemm(GemmArgs g) {
+  constexpr int BM = WM * GA * 64, BN = WN * GB * 64, NW = WM * WN, STAGE = (BM + BN) * 128;
+  constexpr int PER = STAGE / 1024 / NW;  // 1 KiB DMA instructions of a wave and stage
+  __shared__ __attribute__((aligned(1024))) char ring0[STAGE], ring1[STAGE];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // neighbouring tiles on one XCD, in bands of 8 tile rows, share their operands through its L2
+  const int nwg = g.tiles_m * g.tiles_n, bid = blockIdx.x, xcd = bid & 7, q8 = nwg >> 3, r8 = nwg & 7;
+  const int lid = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (bid >> 3);
+  const int width = 8 * g.tiles_n, band = lid / width, in = lid % width;
+  const int rows = min(8, g.tiles_m - band * 8);
+  const int m0 = (band * 8 + in % rows) * BM, n0 = in / rows * BN;
+  const int k0 = SPLIT ? (int)blockIdx.y * g.kb_split : 0;
+  const int nkb = SPLIT ? min(g.kb_split, g.nkb - k0) : g.nkb;
+
+  // LDS rows of 128 bytes, a's then b's; 16-byte chunk c of row t sits at c ^ (t >> 1)
+  const unsigned char* src[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int i = u * NW + w, t = i * 8 + (lane >> 3), c = (lane & 7) ^ ((t >> 1) & 7);
+    const bool isb = i >= BM / 8;
+    const int row = isb ? min(n0 + slot_row(t - BM), g.N - 1) : min(m0 + slot_row(t), g.M - 1);
+    src[u] = (isb ? g.b : g.a) + (size_t)row * g.K + (size_t)k0 * 128 + c * 16;
+  }
   auto issue = [&](int kb, char* slot) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = u * 4 + w;  // 0..15: a, 16..31: b
-      const int t = (i & 15) * 8 + (lane >> 3), c = (lane & 7) ^ ((t >> 1) & 7);
-      const bool isb = i >= 16;
-      const int row = isb ? min(n0 + slot_row(t), g.N - 1) : min(m0 + slot_row(t), g.M - 1);
-      const unsigned char* src = (isb ? g.b : g.a) + (size_t)row * g.K + kb * 128 + c * 16;
-      __builtin_amdgcn_global_load_lds((gvoid*)src, (lvoid*)(slot + i * 1024), 16, 0, 0);
-    }
+    for (int u = 0; u < PER; ++u)
+      __builtin_amdgcn_global_load_lds((gvoid*)(src[u] + (size_t)kb * 128),
+                                       (lvoid*)(slot + (u * NW + w) * 1024), 16, 0, 0);
   };
-  const int wm = w >> 1, wn = w & 1, r = lane & 15, q = lane >> 4;
+  const int wm = w / WN, wn = w % WN, r = lane & 15, q = lane >> 4, x = (r >> 1) & 7;
+  const int lo = r * 128 + ((q ^ x) << 4), hi = r * 128 + (((q + 4) ^ x) << 4);
   auto frag = [&](const char* base, int f) {  // f: fragment of 16 LDS rows
-    const int t = f * 16 + r, x = (t >> 1) & 7;
-    const i32x4 lo = *reinterpret_cast<const i32x4*>(base + t * 128 + ((q ^ x) << 4));
-    const i32x4 hi = *reinterpret_cast<const i32x4*>(base + t * 128 + (((q + 4) ^ x) << 4));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    const i32x4 l = *reinterpret_cast<const i32x4*>(base + f * 2048 + lo);
+    const i32x4 h = *reinterpret_cast<const i32x4*>(base + f * 2048 + hi);
+    return __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  f32x4 acc[4][4];
+  f32x4 acc[GA][GB][4][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < GA * GB * 16; ++i)
+    (&acc[0][0][0][0])[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-#define MFMA(i, j) \
-  acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa[i], fb[j], acc[i][j], 0, 0, i, ea, j, eb)
-#define MFMA_ROW(i) MFMA(i, 0); MFMA(i, 1); MFMA(i, 2); MFMA(i, 3)
-  auto compute = [&](int kb, const char* slot) {
-    const int ea = exps4(g.sa, g.sa_str, g.a_shift, kb, m0 + wm * 64, r);
-    const int eb = exps4(g.sb, g.sb_str, g.b_shift, kb, n0 + wn * 64, r);
-    i32x8 fa[4], fb[4];
+  int ea[GA], eb[GB], na[GA], nb[GB];  // this stage's exponents and the next's
+  auto exps = [&](int kb) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) fa[i] = frag(slot, wm * 4 + i);
+    for (int i = 0; i < GA; ++i)
+      na[i] = exps4(g.sa, g.sa_str, g.a_shift, k0 + kb, m0 + (wm * GA + i) * 64, r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) fb[i] = frag(slot + kT * 128, wn * 4 + i);
-    if constexpr (WIDE) {
+    for (int j = 0; j < GB; ++j)
+      nb[j] = exps4(g.sb, g.sb_str, g.b_shift, k0 + kb, n0 + (wn * GB + j) * 64, r);
+  };
+  auto compute = [&](const char* slot) {
+    i32x8 fb[GB][4];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        bf16x8 xa[4], xb[4];
+    for (int j = 0; j < GB; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          xa[i] = widen(fa[i], p, ea, i);
-          xb[i] = widen(fb[i], p, eb, i);
-        }
+      for (int f = 0; f < 4; ++f) fb[j][f] = frag(slot + BM * 128, (wn * GB + j) * 4 + f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < GA; ++i) {
+      i32x8 fa[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[i], xb[j], acc[i][j], 0, 0, 0);
-      }
-    } else {
-      MFMA_ROW(0);
-      MFMA_ROW(1);
-      MFMA_ROW(2);
-      MFMA_ROW(3);
+      for (int f = 0; f < 4; ++f) fa[f] = frag(slot, (wm * GA + i) * 4 + f);
+#pragma unroll
+      for (int j = 0; j < GB; ++j) quad<WIDE>(fa, fb[j], ea[i], eb[j], acc[i][j]);
     }
   };
+  auto step = [&](int kb, const char* cur, char* other) {
+    __syncthreads();  // stage kb and its exponents landed; every wave is done with `other`
+#pragma unroll
+    for (int i = 0; i < GA; ++i) ea[i] = na[i];
+#pragma unroll
+    for (int j = 0; j < GB; ++j) eb[j] = nb[j];
+    if (kb + 1 < nkb) {
+      exps(kb + 1);
+      issue(kb + 1, other);
+    }
+    compute(cur);
+  };
+  exps(0);
   issue(0, ring0);
   for (int kb = 0; kb < nkb; kb += 2) {
-    __syncthreads();  // stage kb landed (the barrier waits for this wave's own loads)
-    if (kb + 1 < nkb) issue(kb + 1, ring1);
-    compute(kb, ring0);
-    if (kb + 1 >= nkb) break;
-    __syncthreads();
-    if (kb + 2 < nkb) issue(kb + 2, ring0);
-    compute(kb + 1, ring1);
+    step(kb, ring0, ring1);
+    if (kb + 1 < nkb) step(kb + 1, ring1, ring0);
   }
 
-  // acc[i][j][e]: row 4 · (4q + e) + i, column 4r + j of the wave's 64 x 64
+  // acc[..][i][j][e]: row 4 (4q + e) + i, column 4r + j of its 64 x 64
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int ga = 0; ga < GA; ++ga)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int m = m0 + wm * 64 + 4 * (4 * q + e) + i, n = n0 + wn * 64 + 4 * r;
-      if (m >= g.M) continue;
+    for (int gb = 0; gb < GB; ++gb)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (n + j >= g.N) continue;
-        size_t at = (size_t)m * g.N + n + j;
-        if (g.nchw) {
-          const int b = (n + j) / g.P;
-          at = ((size_t)b * g.M + m) * g.P + (n + j - b * g.P);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = m0 + (wm * GA + ga) * 64 + 4 * (4 * q + e) + i;
+          const int n = n0 + (wn * GB + gb) * 64 + 4 * r;
+          if (m >= g.M || n >= g.N) continue;
+          const f32x4 v = {acc[ga][gb][i][0][e], acc[ga][gb][i][1][e], acc[ga][gb][i][2][e],
+                           acc[ga][gb][i][3][e]};
+          if constexpr (SPLIT) {
+            float* p = g.part + ((size_t)blockIdx.y * g.M + m) * g.N + n;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (n + j < g.N) p[j] = v[j];
+          } else {
+            put4<WIDE>(g, m, n, v);
+          }
         }
-        const float v = acc[i][j][e];
-        if constexpr (WIDE)
-          static_cast<float*>(g.out)[at] = v;
-        else
-          static_cast<bf16_t*>(g.out)[at] = f2bf(v);
+}
+
+// the splits' partials, added in order
+template <bool WIDE>
+__global__ __launch_bounds__(256) void fp8_gemm_join(GemmArgs g, int splits) {
+  const size_t total = (size_t)g.M * g.N;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+    float s = g.part[i];
+#pragma unroll 8
+    for (int k = 1; k < splits; ++k) s += g.part[i + k * total];
+    const int m = (int)(i / g.N);
+    put<WIDE>(g, out_at(g, m, (int)(i - (size_t)m * g.N)), s);
+  }
+}
+
+// ---- few rows on one side (tokens being served): nothing to reuse, so no LDS for the operands.
+// A workgroup takes 16 rows of the long side and all of K; its waves take the k blocks in
+// turn, each lane loading its 32 bytes of a block straight into MFMA operands (whole 128-byte
+// lines per four lanes), AHEAD blocks in flight; the waves' sums meet in LDS, in wave order.
+template <int F, bool WIDE>  // F: fragments of the short side
+__global__ __launch_bounds__(512) void fp8_gemm_few(GemmArgs g, int swap) {
+  constexpr int NW = 8, AHEAD = F == 1 ? 4 : 2;
+  __shared__ float sum[NW][F][256];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  // short side s (F * 16 rows), long side l
+  const unsigned char *sp = swap ? g.b : g.a, *lp = swap ? g.a : g.b;
+  const unsigned char *se = swap ? g.sb : g.sa, *le = swap ? g.sa : g.sb;
+  const long sstr = swap ? g.sb_str : g.sa_str, lstr = swap ? g.sa_str : g.sb_str;
+  const int ssh = swap ? g.b_shift : g.a_shift, lsh = swap ? g.a_shift : g.b_shift;
+  const int S = swap ? g.N : g.M, L = swap ? g.M : g.N;
+  const int l0 = blockIdx.x * 16, lrow = min(l0 + r, L - 1);
+  const unsigned char* lsrc = lp + (size_t)lrow * g.K + q * 16;
+  const unsigned char* lexp = le + (lrow >> lsh);
+  const unsigned char *ssrc[F], *sexp[F];
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const int row = min(f * 16 + r, S - 1);
+    ssrc[f] = sp + (size_t)row * g.K + q * 16;
+    sexp[f] = se + (row >> ssh);
+  }
+  f32x4 acc[F];
+#pragma unroll
+  for (int f = 0; f < F; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto ld = [](const unsigned char* p) {
+    const i32x4 l = *reinterpret_cast<const i32x4*>(p);
+    const i32x4 h = *reinterpret_cast<const i32x4*>(p + 64);
+    return __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // U blocks from kb0: all their loads, then their products
+  auto blocks = [&](int kb0, auto count) {
+    constexpr int U = decltype(count)::value;
+    i32x8 lv[U], sv[U][F];
+    int el[U], es[U][F];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      lv[u] = ld(lsrc + (size_t)(kb0 + u) * 128);
+      el[u] = lexp[(size_t)(kb0 + u) * lstr];
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        sv[u][f] = ld(ssrc[f] + (size_t)(kb0 + u) * 128);
+        es[u][f] = sexp[f][(size_t)(kb0 + u) * sstr];
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                widen(sv[u][f], p, es[u][f]), widen(lv[u], p, el[u]), acc[f], 0, 0, 0);
+        } else {
+          acc[f] = mfma8<0, 0>(sv[u][f], lv[u], acc[f], es[u][f], el[u]);
+        }
+      }
+  };
+  const int whole = g.nkb / AHEAD;
+  for (int c = w; c < whole; c += NW) blocks(c * AHEAD, std::integral_constant<int, AHEAD>());
+  for (int kb = whole * AHEAD; kb < g.nkb; ++kb)
+    if ((whole + kb) % NW == w) blocks(kb, std::integral_constant<int, 1>());
+#pragma unroll
+  for (int f = 0; f < F; ++f)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[w][f][(4 * q + e) * 16 + r] = acc[f][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < F * 256; i += 512) {
+    float t = 0.f;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) t += sum[v][i >> 8][i & 255];
+    const int s = i >> 4, l = l0 + (i & 15);
+    if (s < S && l < L) put<WIDE>(g, swap ? out_at(g, l, s) : out_at(g, s, l), t);
+  }
+}
+
+// How a product runs; the same for the workspace query and the call.
+struct Plan {
+  enum { FEW, TILE128, TILE256 } kind;
+  int splits, kb_split;
+};
+
+Plan plan(const dcn_fp8_matmul_desc& d) {
+  const int few = std::min(d.M, d.N), nkb = d.K / 128;
+  if (few <= 64) return {Plan::FEW, 1, nkb};
+  auto tiles = [&](int b) { return (long)((d.M + b - 1) / b) * ((d.N + b - 1) / b); };
+  if (tiles(256) >= 192) return {Plan::TILE256, 1, nkb};
+  // too few tiles for the card: parts of K, at least four k blocks each, two workgroups a CU
+  const long t = tiles(128);
+  int splits = (int)std::min<long>(std::max<long>(1, 512 / t), std::max(1, nkb / 4));
+  const int kb = (nkb + splits - 1) / splits;
+  splits = (nkb + kb - 1) / kb;
+  return {Plan::TILE128, splits, kb};
+}
+
+template <int GA, int GB, int WM, int WN, int WPE>
+hipError_t run_tiles(GemmArgs g, const Plan& p, bool wide, hipStream_t s) {
+  g.tiles_m = (g.M + WM * GA * 64 - 1) / (WM * GA * 64);
+  g.tiles_n = (g.N + WN * GB * 64 - 1) / (WN * GB * 64);
+  g.kb_split = p.kb_split;
+  const dim3 grid((unsigned)g.tiles_m * g.tiles_n, p.splits), block(WM * WN * 64);
+  if (p.splits == 1) {
+    if (wide)
+      hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, true, false>), grid, block, 0, s, g);
+    else
+      hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, false, false>), grid, block, 0, s, g);
+    return hipGetLastError();
+  }
+  if (wide)
+    hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, true, true>), grid, block, 0, s, g);
+  else
+    hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, false, true>), grid, block, 0, s, g);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const unsigned n = (unsigned)std::min<size_t>(((size_t)g.M * g.N + 255) / 256, 4096);
+  if (wide)
+    hipLaunchKernelGGL(fp8_gemm_join<true>, dim3(n), dim3(256), 0, s, g, p.splits);
+  else
+    hipLaunchKernelGGL(fp8_gemm_join<false>, dim3(n), dim3(256), 0, s, g, p.splits);
+  return hipGetLastError();
+}
+
+template <int F>
+hipError_t run_few(const GemmArgs& g, bool wide, hipStream_t s) {
+  const int swap = g.N < g.M, longest = swap ? g.M : g.N;
+  const dim3 grid((longest + 15) / 16), block(512);
+  if (wide)
+    hipLaunchKernelGGL((fp8_gemm_few<F, true>), grid, block, 0, s, g, swap);
+  else
+    hipLaunchKernelGGL((fp8_gemm_few<F, false>), grid, block, 0, s, g, swap);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-size_t fp8_matmul_ws_bytes(const dcn_fp8_matmul_desc&) { return 0; }
+size_t fp8_matmul_ws_bytes(const dcn_fp8_matmul_desc& d) {
+  const Plan p = plan(d);
+  return p.splits > 1 ? (size_t)p.splits * d.M * d.N * sizeof(float) : 0;
+}
 
 hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const void* sa,
-                             const void* b, const void* sb, void* out, void*, hipStream_t s) {
+                             const void* b, const void* sb, void* out, void* ws, hipStream_t s) {
   GemmArgs g{};
   auto u8 = [](const void* p) { return static_cast<const unsigned char*>(p); };
   g.a = u8(a);
@@ -181,21 +421,28 @@ hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const 
   g.b = u8(b);
   g.sb = u8(sb);
   g.out = out;
+  g.part = static_cast<float*>(ws);
   g.M = d.M;
   g.N = d.N;
   g.K = d.K;
+  g.nkb = d.K / 128;
   g.P = d.P;
   g.nchw = d.layout == DCN_NCHW;
   g.a_shift = d.a_block == 128 ? 7 : 0;
   g.b_shift = d.b_block == 128 ? 7 : 0;
   g.sa_str = d.a_block == 128 ? (d.M + 127) / 128 : (d.M + 127) / 128 * 128;
   g.sb_str = d.b_block == 128 ? (d.N + 127) / 128 : (d.N + 127) / 128 * 128;
-  const dim3 grid((unsigned)((d.N + kT - 1) / kT) * (unsigned)((d.M + kT - 1) / kT));
-  if (d.out_dtype == DCN_BF16)
-    hipLaunchKernelGGL(fp8_gemm<false>, grid, dim3(kThreads), 0, s, g);
-  else
-    hipLaunchKernelGGL(fp8_gemm<true>, grid, dim3(kThreads), 0, s, g);
-  return hipGetLastError();
+  const bool wide = d.out_dtype == DCN_F32;
+  g.vec = (g.nchw ? g.P : g.N) % 4 == 0 &&
+          reinterpret_cast<uintptr_t>(out) % (wide ? 16 : 8) == 0;
+  const Plan p = plan(d);
+  if (p.kind == Plan::FEW) {
+    const int few = std::min(d.M, d.N);
+    return few <= 16 ? run_few<1>(g, wide, s) : few <= 32 ? run_few<2>(g, wide, s)
+                                                          : run_few<4>(g, wide, s);
+  }
+  if (p.kind == Plan::TILE256) return run_tiles<2, 1, 2, 4, 2>(g, p, wide, s);
+  return run_tiles<1, 1, 2, 2, 2>(g, p, wide, s);
 }
 
 }  // namespace dcn

@@ -179,6 +179,19 @@ def test_pointwise(tb, dt, layout, B, P, C, O):
         assert torch.equal(tb.fp8_pointwise(x, tb.fp8_quantize_weight(w)), y)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout,B,P,C,O", [("rows", 1, 3601, 200, 3503), ("nchw", 5, 723, 129, 3330),
+                                            ("nchw", 4, 900, 384, 3588), ("rows", 1, 3700, 520, 3396)])
+def test_large_tiles(tb, dt, layout, B, P, C, O):
+    """Results of about 200 tiles of 256 x 256 and more, with ragged edges, an odd and an even
+    number of k blocks; forward only (the gradients run the same kernels)."""
+    sh = lambda c: (B, c, P, 1) if layout == "nchw" else (B, P, c)
+    x, w = make(sh(C), dt, 1, 0.3), make((O, C), dt, 2, 0.1)
+    with torch.no_grad():
+        y = tb.fp8_pointwise(x, w)
+    close(tok(y), BO.fp8_value(tok(x), 1, 128), BO.fp8_value(np64(w), 128, 128), dt, "y")
+
+
 def test_asymmetric_identity(tb):
     """Each weight row picks one channel: every output element is one input value, so a row, a
     column or an exponent out of place shows at once."""
