@@ -39,7 +39,6 @@ struct GemmArgs {
   float* part;  // split K: fp32 partials [split][M][N]
   int M, N, nkb, P, nchw, a_shift, b_shift;  // shift: log2 of rows per exponent
   long K, sa_str, sb_str;
-  int vec;         // four neighbouring columns may be stored at once
   int kb_split;    // k blocks of a split
   int tiles_m, tiles_n;
 };
@@ -120,19 +119,30 @@ __device__ __forceinline__ void put(const GemmArgs& g, size_t at, float v) {
   else
     static_cast<bf16_t*>(g.out)[at] = f2bf(v);
 }
-// columns n .. n + 3 of row m
+typedef f32x4 f32x4_any __attribute__((aligned(4), may_alias));
+typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(2), may_alias));
+// columns n .. n + 3 of row m, one store where they are neighbours (any alignment will do)
+struct Column {  // column n's place in row 0, the rows' stride, and whether n .. n + 3 are neighbours
+  size_t at, stride;
+  bool four;
+};
+__device__ __forceinline__ Column column(const GemmArgs& g, int n) {
+  if (!g.nchw) return {(size_t)n, (size_t)g.N, n + 4 <= g.N};
+  const int b = n / g.P, p = n - b * g.P;
+  return {(size_t)b * g.M * g.P + p, (size_t)g.P, n + 4 <= g.N && p + 4 <= g.P};
+}
 template <bool WIDE>
-__device__ __forceinline__ void put4(const GemmArgs& g, int m, int n, f32x4 v) {
-  if (g.vec && n + 4 <= g.N) {
-    const size_t at = out_at(g, m, n);
+__device__ __forceinline__ void put4(const GemmArgs& g, const Column& c, int m, int n, f32x4 v) {
+  if (c.four) {
+    const size_t at = c.at + m * c.stride;
     if constexpr (WIDE) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + at) = v;
+      *reinterpret_cast<f32x4_any*>(static_cast<float*>(g.out) + at) = v;
     } else {
-      const float t[4] = {v[0], v[1], v[2], v[3]};
-      uint2 u;
-      u.x = (unsigned)f2bf(t[0]) | ((unsigned)f2bf(t[1]) << 16);
-      u.y = (unsigned)f2bf(t[2]) | ((unsigned)f2bf(t[3]) << 16);
-      *reinterpret_cast<uint2*>(static_cast<bf16_t*>(g.out) + at) = u;
+      const u32x2_any u = {__builtin_bit_cast(unsigned, __builtin_convertvector(
+                               __builtin_shufflevector(v, v, 0, 1), bf16x2)),
+                           __builtin_bit_cast(unsigned, __builtin_convertvector(
+                               __builtin_shufflevector(v, v, 2, 3), bf16x2))};
+      *reinterpret_cast<u32x2_any*>(static_cast<bf16_t*>(g.out) + at) = u;
     }
     return;
   }
@@ -143,11 +153,11 @@ __device__ __forceinline__ void put4(const GemmArgs& g, int m, int n, f32x4 v) {
 
 // ---- tiles: WM x WN waves, each GA x GB groups of 64 x 64, K in stages of 128 through two LDS
 // buffers: while one is multiplied, LDS-DMA fills the other.
-template <int GA, int GB, int WM, int WN, int WPE, bool WIDE, bool SPLIT>
+template <int GA, int GB, int WM, int WN, int WPE, int STAGES, bool WIDE, bool SPLIT>
 __global__ __launch_bounds__(WM* WN * 64, WPE) void fp8_gemm(GemmArgs g) {
   constexpr int BM = WM * GA * 64, BN = WN * GB * 64, NW = WM * WN, STAGE = (BM + BN) * 128;
   constexpr int PER = STAGE / 1024 / NW;  // 1 KiB DMA instructions of a wave and stage
-  __shared__ __attribute__((aligned(1024))) char ring0[STAGE], ring1[STAGE];
+  __shared__ __attribute__((aligned(1024))) char ring0[STAGE], ring1[STAGES == 2 ? STAGE : 16];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // neighbouring tiles on one XCD, in bands of 8 tile rows, share their operands through its L2
   const int nwg = g.tiles_m * g.tiles_n, bid = blockIdx.x, xcd = bid & 7, q8 = nwg >> 3, r8 = nwg & 7;
@@ -223,46 +233,79 @@ __global__ __launch_bounds__(WM* WN * 64, WPE) void fp8_gemm(GemmArgs g) {
   };
   exps(0);
   issue(0, ring0);
-  for (int kb = 0; kb < nkb; kb += 2) {
-    step(kb, ring0, ring1);
-    if (kb + 1 < nkb) step(kb + 1, ring1, ring0);
+  if constexpr (STAGES == 2) {
+    for (int kb = 0; kb < nkb; kb += 2) {
+      step(kb, ring0, ring1);
+      if (kb + 1 < nkb) step(kb + 1, ring1, ring0);
+    }
+  } else {
+    for (int kb = 0; kb < nkb; ++kb) {
+      __syncthreads();  // the stage landed
+#pragma unroll
+      for (int i = 0; i < GA; ++i) ea[i] = na[i];
+#pragma unroll
+      for (int j = 0; j < GB; ++j) eb[j] = nb[j];
+      compute(ring0);
+      if (kb + 1 == nkb) break;
+      __syncthreads();  // every wave has read it
+      exps(kb + 1);
+      issue(kb + 1, ring0);
+    }
   }
 
   // acc[..][i][j][e]: row 4 (4q + e) + i, column 4r + j of its 64 x 64
 #pragma unroll
   for (int ga = 0; ga < GA; ++ga)
 #pragma unroll
-    for (int gb = 0; gb < GB; ++gb)
+    for (int gb = 0; gb < GB; ++gb) {
+      const int n = n0 + (wn * GB + gb) * 64 + 4 * r;
+      const Column col = column(g, n);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int m = m0 + (wm * GA + ga) * 64 + 4 * (4 * q + e) + i;
-          const int n = n0 + (wn * GB + gb) * 64 + 4 * r;
           if (m >= g.M || n >= g.N) continue;
           const f32x4 v = {acc[ga][gb][i][0][e], acc[ga][gb][i][1][e], acc[ga][gb][i][2][e],
                            acc[ga][gb][i][3][e]};
           if constexpr (SPLIT) {
             float* p = g.part + ((size_t)blockIdx.y * g.M + m) * g.N + n;
+            if (n + 4 <= g.N) {
+              *reinterpret_cast<f32x4_any*>(p) = v;
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (n + j < g.N) p[j] = v[j];
+              for (int j = 0; j < 4; ++j)
+                if (n + j < g.N) p[j] = v[j];
+            }
           } else {
-            put4<WIDE>(g, m, n, v);
+            put4<WIDE>(g, col, m, n, v);
           }
         }
+    }
 }
 
-// the splits' partials, added in order
+// the splits' partials, added in order, four columns a thread
 template <bool WIDE>
 __global__ __launch_bounds__(256) void fp8_gemm_join(GemmArgs g, int splits) {
   const size_t total = (size_t)g.M * g.N;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-    float s = g.part[i];
-#pragma unroll 8
-    for (int k = 1; k < splits; ++k) s += g.part[i + k * total];
-    const int m = (int)(i / g.N);
-    put<WIDE>(g, out_at(g, m, (int)(i - (size_t)m * g.N)), s);
+  const unsigned quads = (g.N + 3) / 4;
+  const size_t all = (size_t)g.M * quads;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+    const int m = (int)(i / quads), n = 4 * (int)(i - (size_t)m * quads);
+    const float* p = g.part + (size_t)m * g.N + n;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (n + 4 <= g.N) {
+      s = *reinterpret_cast<const f32x4_any*>(p);
+#pragma unroll 4
+      for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const f32x4_any*>(p + k * total);
+    } else {
+      for (int j = 0; n + j < g.N; ++j) {
+        float t = p[j];
+        for (int k = 1; k < splits; ++k) t += p[j + k * total];
+        s[j] = t;
+      }
+    }
+    put4<WIDE>(g, column(g, n), m, n, s);
   }
 }
 
@@ -350,7 +393,7 @@ __global__ __launch_bounds__(512) void fp8_gemm_few(GemmArgs g, int swap) {
 
 // How a product runs; the same for the workspace query and the call.
 struct Plan {
-  enum { FEW, TILE128, TILE256 } kind;
+  enum { FEW, SHORT, TILE128, TILE256 } kind;
   int splits, kb_split;
 };
 
@@ -358,8 +401,15 @@ Plan plan(const dcn_fp8_matmul_desc& d) {
   const int few = std::min(d.M, d.N), nkb = d.K / 128;
   if (few <= 64) return {Plan::FEW, 1, nkb};
   auto tiles = [&](int b) { return (long)((d.M + b - 1) / b) * ((d.N + b - 1) / b); };
+  // A short K is all prologue and epilogue: three small workgroups a CU that take turns at them
+  // beat one large one that overlaps its own stages (50176 x 1024 bf16 results, K = 256 / 512 /
+  // 1024: 31.6 / 44 / 71 us, one stage in LDS; two stages 35 / 49 / 78; 256 x 256 tiles 52 /
+  // 57 / 85).
+  if (nkb <= 8 && tiles(128) >= 768) return {Plan::SHORT, 1, nkb};
+  // 256 x 256: half the LDS reads per product (16384 x 8192 x 8192: 1.0 ms; 128 x 128 1.7 ms)
   if (tiles(256) >= 192) return {Plan::TILE256, 1, nkb};
-  // too few tiles for the card: parts of K, at least four k blocks each, two workgroups a CU
+  // Too few tiles for the card: parts of K, at least four k blocks each, two workgroups a CU
+  // (2048 x 2048 x 2048 in two parts: 18 us, and 7 us to join them)
   const long t = tiles(128);
   int splits = (int)std::min<long>(std::max<long>(1, 512 / t), std::max(1, nkb / 4));
   const int kb = (nkb + splits - 1) / splits;
@@ -367,7 +417,7 @@ Plan plan(const dcn_fp8_matmul_desc& d) {
   return {Plan::TILE128, splits, kb};
 }
 
-template <int GA, int GB, int WM, int WN, int WPE>
+template <int GA, int GB, int WM, int WN, int WPE, int STAGES>
 hipError_t run_tiles(GemmArgs g, const Plan& p, bool wide, hipStream_t s) {
   g.tiles_m = (g.M + WM * GA * 64 - 1) / (WM * GA * 64);
   g.tiles_n = (g.N + WN * GB * 64 - 1) / (WN * GB * 64);
@@ -375,18 +425,18 @@ hipError_t run_tiles(GemmArgs g, const Plan& p, bool wide, hipStream_t s) {
   const dim3 grid((unsigned)g.tiles_m * g.tiles_n, p.splits), block(WM * WN * 64);
   if (p.splits == 1) {
     if (wide)
-      hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, true, false>), grid, block, 0, s, g);
+      hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, STAGES, true, false>), grid, block, 0, s, g);
     else
-      hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, false, false>), grid, block, 0, s, g);
+      hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, STAGES, false, false>), grid, block, 0, s, g);
     return hipGetLastError();
   }
   if (wide)
-    hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, true, true>), grid, block, 0, s, g);
+    hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, STAGES, true, true>), grid, block, 0, s, g);
   else
-    hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, false, true>), grid, block, 0, s, g);
+    hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, STAGES, false, true>), grid, block, 0, s, g);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const unsigned n = (unsigned)std::min<size_t>(((size_t)g.M * g.N + 255) / 256, 4096);
+  const unsigned n = (unsigned)std::min<size_t>(((size_t)g.M * ((g.N + 3) / 4) + 255) / 256, 4096);
   if (wide)
     hipLaunchKernelGGL(fp8_gemm_join<true>, dim3(n), dim3(256), 0, s, g, p.splits);
   else
@@ -433,16 +483,15 @@ hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const 
   g.sa_str = d.a_block == 128 ? (d.M + 127) / 128 : (d.M + 127) / 128 * 128;
   g.sb_str = d.b_block == 128 ? (d.N + 127) / 128 : (d.N + 127) / 128 * 128;
   const bool wide = d.out_dtype == DCN_F32;
-  g.vec = (g.nchw ? g.P : g.N) % 4 == 0 &&
-          reinterpret_cast<uintptr_t>(out) % (wide ? 16 : 8) == 0;
   const Plan p = plan(d);
   if (p.kind == Plan::FEW) {
     const int few = std::min(d.M, d.N);
     return few <= 16 ? run_few<1>(g, wide, s) : few <= 32 ? run_few<2>(g, wide, s)
                                                           : run_few<4>(g, wide, s);
   }
-  if (p.kind == Plan::TILE256) return run_tiles<2, 1, 2, 4, 2>(g, p, wide, s);
-  return run_tiles<1, 1, 2, 2, 2>(g, p, wide, s);
+  if (p.kind == Plan::TILE256) return run_tiles<2, 1, 2, 4, 2, 2>(g, p, wide, s);
+  if (p.kind == Plan::SHORT) return run_tiles<1, 1, 2, 2, 3, 1>(g, p, wide, s);
+  return run_tiles<1, 1, 2, 2, 2, 2>(g, p, wide, s);
 }
 
 }  // namespace dcn
