@@ -360,10 +360,14 @@ typedef struct {
   const void *grad_out, *grad_y;
   void *grad_x, *grad_residual, *grad_gate, *grad_scale;
   void *grad_w_post, *grad_b_post, *grad_w_pre, *grad_b_pre;
+  /* 4 * B * P floats (16-byte aligned) or NULL. The forward writes each position's mean and
+   * 1 / sqrt(var + eps) of both norms there; a backward given them (of the same inputs) does
+   * not compute them again */
+  float* stats;
 } dcn_block_io;
 int dcn_block_norm_fwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_io* io);
-/* Reads the forward's inputs (x, residual, gate, parameters, rng), never its results, and
- * grad_out / grad_y. ws: dcn_block_norm_workspace bytes (256-byte aligned), one per call in
+/* Reads the forward's inputs (x, residual, gate, parameters, rng) and stats, not its results,
+ * and grad_out / grad_y. ws: dcn_block_norm_workspace bytes (256-byte aligned), one per call in
  * flight: calls that may run at the same time (other streams, other graphs) each need their
  * own. */
 int dcn_block_norm_workspace(const dcn_block_desc* d, size_t* bytes);

@@ -125,6 +125,8 @@ int block_inputs(const dcn_block_desc* d, const dcn_block_io* io, dcn::BlockArgs
   if ((io->gate != nullptr) != (d->gate != DCN_GATE_NONE))
     return fail(DCN_ERR_INVALID, "the gate tensor and the gate kind must come together");
   a->x = io->x; a->res = io->residual; a->gate = io->gate; a->scale = io->scale;
+  if (!aligned(io->stats, 16)) return fail(DCN_ERR_INVALID, "stats must be 16-byte aligned");
+  a->stats = io->stats;
   a->w1 = io->w_post; a->b1 = io->b_post; a->w2 = io->w_pre; a->b2 = io->b_pre;
   return DCN_OK;
 }
@@ -285,8 +287,8 @@ int dcn_block_norm_fwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_i
   const Span in[] = {{io->x, full}, {io->residual, full}, {io->gate, gate}, {io->scale, vec},
                      {io->w_post, vec}, {io->b_post, vec}, {io->w_pre, vec}, {io->b_pre, vec},
                      {io->rng, 16}};
-  const Span out[] = {{io->out, full}, {io->y, full}};
-  if (int rc = block_spans(in, 9, out, 2, es, io->out, io->residual)) return rc;
+  const Span out[] = {{io->out, full}, {io->y, full}, {io->stats, (size_t)d->B * d->P * 16}};
+  if (int rc = block_spans(in, 9, out, 3, es, io->out, io->residual)) return rc;
   DeviceScope ds;
   if (int rc = ds.bind(h)) return rc;
   return done(dcn::launch_block_norm_fwd(a, ds.stream), "block_norm forward");
@@ -328,11 +330,12 @@ int dcn_block_norm_bwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_i
   const size_t gate = d->gate == DCN_GATE_FULL ? full : (size_t)d->B * d->C * es;
   const Span in[] = {{io->x, full}, {io->residual, full}, {io->gate, gate}, {io->scale, vec},
                      {io->w_post, vec}, {io->b_post, vec}, {io->w_pre, vec}, {io->b_pre, vec},
-                     {io->grad_out, full}, {io->grad_y, full}, {io->rng, 16}};
+                     {io->grad_out, full}, {io->grad_y, full}, {io->rng, 16},
+                     {io->stats, (size_t)d->B * d->P * 16}};
   const Span out[] = {{io->grad_x, full}, {io->grad_residual, full}, {io->grad_gate, gate},
                       {io->grad_scale, vec}, {io->grad_w_post, vec}, {io->grad_b_post, vec},
                       {io->grad_w_pre, vec}, {io->grad_b_pre, vec}, {ws, need}};
-  if (int rc = block_spans(in, 11, out, 9, es, nullptr, nullptr)) return rc;
+  if (int rc = block_spans(in, 12, out, 9, es, nullptr, nullptr)) return rc;
   a.ws = static_cast<float*>(ws);
   DeviceScope ds;
   if (int rc = ds.bind(h)) return rc;

@@ -18,6 +18,7 @@ struct BlockArgs {
   const void *go, *gy;
   void *gx, *gr, *gg, *gs, *gw1, *gb1, *gw2, *gb2;
   float* ws;
+  float* stats;  // [4][B · P]: m1, r1, m2, r2 of every position, or null
   DropArgs drop;
   int B, C, P, layout, dtype, post, pre, gate_kind, act, drop_image;
   float eps1, eps2, alpha;

@@ -8,8 +8,10 @@
 //   dt = keep ? G · drop scale : 0
 //   ∂gate = dt · N_post(x) · alpha · scale · act'(gate),  ∂scale = Σ dt · N_post(x) · alpha · act
 //   ∂x = N_post'(dt · alpha · scale · act)
-// out and the statistics are computed again from x and the residual (the residual is read
-// instead of out, so that costs no bytes), which keeps the backward free of out's rounding.
+// out is computed again from x and the residual (the residual is read instead of out, so that
+// costs no bytes), which keeps the backward free of out's rounding. The statistics come from
+// the forward where the caller kept them: 16 bytes a position, against two of the four rounds
+// of sums that a position's workgroup goes through.
 #pragma once
 #include "dcn_block.h"
 #include "dcn_philox.h"
@@ -102,7 +104,7 @@ struct MapSums {
     float wave[NW][2][GPW][TP];  // a wave's partials (two quantities)
     float join[2][NW][2][TP];    // waves' sums, alternating: read in a round, written in the next
                                  // but one
-    float res[NW][2][TP];        // a wave's copy of the results
+    float res[NW][6][TP];        // a wave's copy of m1, r1, m2, r2 and of a pair of sums
     float2 num[NW];              // channels of every wave and 1 / that (0 of 0)
   };
   Shared& sh;
@@ -178,20 +180,21 @@ struct MapSums {
         tb += sh.join[phase][v][1][lane % TP];
       }
     }
-    give(0, ta * fa);
-    give(1, tb * fb);
+    give(4, ta * fa);
+    give(5, tb * fb);
     wave_order();
-    get(0, a);
-    get(1, b);
+    get(4, a);
+    get(5, b);
     wave_order();
   }
   // Mean and 1/sqrt(var + eps) of each position (0 past the map's end, `left` = positions of
   // the tile, so that nothing from there reaches the parameter sums); mk: 1 for a channel, 0
   // past the last (its v is 0). Layer: every wave takes its own mean and the squares about it;
   // the waves' are joined about the whole mean, so large means cancel nowhere.
+  // The results go to rows k and k + 1 of the wave's copies, and to `stats` where wanted.
   __device__ void moments(const float (&v)[CPT][V], const float (&mk)[CPT], int kind, float eps,
-                          int left, float (&m)[V], float (&r)[V]) {
-    float t[V], s = 0.f, q;
+                          int left, int k, float* stats, size_t rows) {
+    float t[V], m[V], s = 0.f, q;
     if (kind == DCN_NORM_LAYER) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -202,9 +205,9 @@ struct MapSums {
       put(0, t);
       wave_order();
       s = column(0);
-      give(0, s * inw);
+      give(4, s * inw);
       wave_order();
-      get(0, m);
+      get(4, m);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         t[e] = 0.f;
@@ -252,11 +255,30 @@ struct MapSums {
         }
       }
     }
-    give(0, s * ic);
-    give(1, lane % TP < left ? rsqrtf(fmaf(q, ic, eps)) : 0.f);
+    const float mean = s * ic, rs = lane % TP < left ? rsqrtf(fmaf(q, ic, eps)) : 0.f;
+    give(k, mean);
+    give(k + 1, rs);
     wave_order();
-    get(0, m);
-    get(1, r);
+    if (stats && w == 0 && lane < TP && lane < left) {
+      stats[k * rows + lane] = mean;
+      stats[(k + 1) * rows + lane] = rs;
+    }
+  }
+  // kept statistics of a tile: lane + 64 i of the 4 x TP values, fetched ahead of their use
+  static constexpr int KEPT = TP / 16;
+  __device__ void fetch(const float* stats, size_t rows, int left, float (&st)[KEPT]) const {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+      const int j = lane + 64 * i, p = j % TP;
+      st[i] = p < left ? stats[(j / TP) * rows + p] : 0.f;
+    }
+  }
+  __device__ void keep(const float (&st)[KEPT]) {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+      const int j = lane + 64 * i;
+      sh.res[w][j / TP][j % TP] = st[i];
+    }
     wave_order();
   }
 };
@@ -299,9 +321,14 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
   const long t0 = first_tile(q, wg), t1 = first_tile(q, wg + 1);
   struct Raw {
     u32x4 x[CPT], r[CPT], g[CPT], y[CPT], o[CPT];
+    float st[Sums::KEPT];
   } nx;
+  const size_t rows = (size_t)a.B * a.P;
   auto load = [&](long t, Raw& w) {
     const int p = (int)(t % q.tpi) * TP + pl * V, valid = a.P - p;
+    if (BWD && a.stats)
+      sums.fetch(a.stats + (t / q.tpi) * a.P + t % q.tpi * TP, rows,
+                 a.P - (int)(t % q.tpi) * TP, w.st);
     const size_t base = (size_t)(t / q.tpi) * a.C * a.P + p;
     const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -351,20 +378,31 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
       return t;
     };
 
-    float m1[V], r1[V], m2[V], r2[V];
+    float* st = a.stats && !BWD ? a.stats + (size_t)b * a.P + (t % q.tpi) * TP : nullptr;
+    const bool known = BWD && a.stats;
+    if (known) sums.keep(in.st);
+    auto post = [&](float (&m)[V], float (&r)[V]) {
+      if (a.post) {
+        sums.get(0, m);
+        sums.get(1, r);
+        return;
+      }
 #pragma unroll
-    for (int e = 0; e < V; ++e) {  // no post norm: N_post(x) = x
-      m1[e] = 0.f;
-      r1[e] = 1.f;
-    }
+      for (int e = 0; e < V; ++e) {  // no post norm: N_post(x) = x
+        m[e] = 0.f;
+        r[e] = 1.f;
+      }
+    };
     float o[CPT][V];
     if (xp) {
-      if (a.post) {
+      if (a.post && !known) {
         float xv[CPT][V];
 #pragma unroll
         for (int i = 0; i < CPT; ++i) unpack<T>(in.x[i], xv[i]);
-        sums.moments(xv, mk, a.post, a.eps1, left, m1, r1);
+        sums.moments(xv, mk, a.post, a.eps1, left, 0, st, rows);
       }
+      float m1[V], r1[V];
+      post(m1, r1);
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
         float xv[V], rv[V], fv[V];
@@ -382,9 +420,15 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
 #pragma unroll
       for (int i = 0; i < CPT; ++i) unpack<T>(in.r[i], o[i]);
     }
-    if (a.pre) sums.moments(o, mk, a.pre, a.eps2, left, m2, r2);
+    if (a.pre && !known) sums.moments(o, mk, a.pre, a.eps2, left, 2, st, rows);
 
     if constexpr (!BWD) {
+      float m2[V], r2[V];
+      if (a.pre) {
+        sums.get(2, m2);
+        sums.get(3, r2);
+      }
+      Sums::wave_order();  // read before the next tile's are written
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
         if (!ok[i]) continue;
@@ -399,7 +443,9 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
     } else {
       // G into o
       if (a.pre) {
-        float s1[V], s2[V];
+        float s1[V], s2[V], m2[V], r2[V];
+        sums.get(2, m2);
+        sums.get(3, r2);
 #pragma unroll
         for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
 #pragma unroll
@@ -438,7 +484,9 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
       }
       if (xp) {
         // dt, ∂gate, ∂scale; dv into o
-        float s3[V], s4[V];
+        float s3[V], s4[V], m1[V], r1[V];
+        post(m1, r1);
+        Sums::wave_order();  // read before the next tile's are written
 #pragma unroll
         for (int e = 0; e < V; ++e) s3[e] = s4[e] = 0.f;
 #pragma unroll
@@ -687,10 +735,17 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
   const long t0 = first_tile(q, wg), t1 = first_tile(q, wg + 1);
   struct Raw {
     u32x4 x[NV], r[NV], g[NV], y[NV], o[NV];
+    float st[4];
   } nx;
+  const size_t rows = (size_t)q.images * q.P;
   auto load = [&](long t, Raw& w) {
     const int b = (int)(t / q.tpi), p = (int)(t % q.tpi) * GR + g;
     const size_t base = ((size_t)b * q.P + p) * a.C;
+    if (BWD && a.stats) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)  // 0 past the last row: nothing there may reach the sums
+        w.st[k] = p < q.P ? a.stats[k * rows + (size_t)b * q.P + p] : 0.f;
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const bool ok = p < q.P && cv[j] > 0;
@@ -745,9 +800,18 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
     };
 
     float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
+    const bool known = BWD && a.stats;
+    if (known) {
+      if (a.post) {
+        m1 = in.st[0];
+        r1 = in.st[1];
+      }
+      m2 = in.st[2];
+      r2 = in.st[3];
+    }
     float o[NV][V];
     if (a.x) {
-      if (a.post) {
+      if (a.post && !known) {
         float xv[NV][V];
 #pragma unroll
         for (int j = 0; j < NV; ++j) unpack<T>(in.x[j], xv[j]);
@@ -772,9 +836,16 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) unpack<T>(in.r[j], o[j]);
     }
-    if (a.pre) sums.moments(o, a.pre, a.eps2, live, m2, r2);
+    if (a.pre && !known) sums.moments(o, a.pre, a.eps2, live, m2, r2);
 
     if constexpr (!BWD) {
+      if (a.stats && live && lane == 0) {
+        float* st = a.stats + (size_t)b * q.P + p;
+        st[0] = m1;
+        st[rows] = r1;
+        st[2 * rows] = m2;
+        st[3 * rows] = r2;
+      }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (!live || cv[j] <= 0) continue;

@@ -77,8 +77,20 @@ __device__ __forceinline__ void moments(F f, int lane, int C, int kind, float ep
 }
 
 template <typename T, int LP>
-__device__ __forceinline__ void pos_moments(Pos<T>& q, int lane) {
+__device__ __forceinline__ void pos_moments(Pos<T>& q, int lane, size_t row, bool known) {
   const BlockArgs& a = q.a;
+  const size_t rows = (size_t)a.B * a.P;
+  if (known) {
+    if (a.x && a.post) {
+      q.m1 = a.stats[row];
+      q.r1 = a.stats[rows + row];
+    }
+    if (a.pre) {
+      q.m2 = a.stats[2 * rows + row];
+      q.r2 = a.stats[3 * rows + row];
+    }
+    return;
+  }
   if (a.x && a.post)
     moments<LP>([&](int c) { return q.x(c); }, lane, a.C, a.post, a.eps1, q.m1, q.r1);
   if (a.pre) moments<LP>([&](int c) { return q.out(c); }, lane, a.C, a.pre, a.eps2, q.m2, q.r2);
@@ -92,7 +104,12 @@ __global__ __launch_bounds__(kThreads) void block_any_fwd(BlockArgs a) {
   for (size_t row = (size_t)blockIdx.x * (kThreads / LP) + threadIdx.x / LP; row < rows;
        row += step) {
     Pos<T> q(a, key, (int)(row / a.P), (int)(row % a.P));
-    pos_moments<T, LP>(q, lane);
+    pos_moments<T, LP>(q, lane, row, false);
+    if (a.stats && lane == 0) {
+      const float st[4] = {q.m1, q.r1, q.m2, q.r2};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a.stats[k * rows + row] = st[k];
+    }
     for (int c = lane; c < a.C; c += LP) {
       const float o = q.out(c);
       const size_t i = q.base + c * q.cs;
@@ -114,7 +131,7 @@ __global__ __launch_bounds__(kThreads) void block_any_bwd(BlockArgs a) {
   for (size_t row = (size_t)blockIdx.x * (kThreads / LP) + threadIdx.x / LP; row < rows;
        row += step) {
     Pos<T> q(a, key, (int)(row / a.P), (int)(row % a.P));
-    pos_moments<T, LP>(q, lane);
+    pos_moments<T, LP>(q, lane, row, a.stats != nullptr);
     float s1 = 0.f, s2 = 0.f;
     if (a.pre) {
       for (int c = lane; c < a.C; c += LP) {

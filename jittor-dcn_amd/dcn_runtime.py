@@ -69,7 +69,7 @@ class BlockIO(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in
                 ("x", "residual", "gate", "scale", "w_post", "b_post", "w_pre", "b_pre", "rng",
                  "out", "y", "grad_out", "grad_y", "grad_x", "grad_residual", "grad_gate",
-                 "grad_scale", "grad_w_post", "grad_b_post", "grad_w_pre", "grad_b_pre")]
+                 "grad_scale", "grad_w_post", "grad_b_post", "grad_w_pre", "grad_b_pre", "stats")]
 
 
 class Fp8Desc(ctypes.Structure):

@@ -211,8 +211,8 @@ def _layout(x):
     return rt.DCN_NHWC, B, C, x.numel() // max(B * C, 1), torch.contiguous_format
 
 
-def _block(tensors, desc, mf, dev_rng):
-    """(out, y) and the dense tensors behind them."""
+def _block(tensors, desc, mf, dev_rng, keep=False):
+    """(out, y), the dense tensors behind them and, with keep, the norms' statistics."""
     x, residual, gate = tensors[:3]
     full = (True, True, desc.gate == rt.DCN_GATE_FULL)
     tensors = [t if t is None else t.contiguous(memory_format=mf) if i < 3 and full[i]
@@ -220,25 +220,28 @@ def _block(tensors, desc, mf, dev_rng):
     x, ref = tensors[0], tensors[1] if tensors[0] is None else tensors[0]
     out = torch.empty_like(x, memory_format=mf) if x is not None else None
     y = torch.empty_like(ref, memory_format=mf) if desc.pre else None
+    stats = None
     if ref.numel():
+        if keep and (desc.post or desc.pre):
+            stats = torch.empty(4 * desc.B * desc.P, dtype=torch.float32, device=ref.device)
         _call(ref.device, "dcn_block_norm_fwd", desc,
-              rt.BlockIO(*map(_ptr, (*tensors, dev_rng, out, y))))
-    return out, y, tensors
+              rt.BlockIO(*map(_ptr, (*tensors, dev_rng, out, y)), stats=_ptr(stats)))
+    return out, y, tensors, stats
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, desc, mf, dev_rng, *tensors):
-        out, y, tensors = _block(tensors, desc, mf, dev_rng)
+        out, y, tensors, stats = _block(tensors, desc, mf, dev_rng, keep=True)
         ctx.desc, ctx.mf = desc, mf
-        ctx.save_for_backward(*tensors, dev_rng)
+        ctx.save_for_backward(*tensors, dev_rng, stats)
         ctx.set_materialize_grads(False)
         return out, y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_y):
-        *inputs, dev_rng = ctx.saved_tensors
+        *inputs, dev_rng, stats = ctx.saved_tensors
         need = ctx.needs_input_grad[3:]
         if grad_out is None and grad_y is None:
             return (None,) * 11
@@ -252,7 +255,7 @@ class _BlockNorm(torch.autograd.Function):
         nbytes = ctypes.c_size_t()
         rt.check(_fn("dcn_block_norm_workspace")(ctx.desc, nbytes), "dcn_block_norm_workspace")
         ws = _bytes(ref.device, nbytes.value)
-        io = rt.BlockIO(*map(_ptr, (*inputs, dev_rng, None, None, grad_out, grad_y, *grads)))
+        io = rt.BlockIO(*map(_ptr, (*inputs, dev_rng, None, None, grad_out, grad_y, *grads, stats)))
         _call(ref.device, "dcn_block_norm_bwd", ctx.desc, io, ws.data_ptr(), nbytes.value)
         return (None, None, None, *grads)
 
@@ -301,7 +304,7 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     if _wants_grad(*tensors):
         out, y = _BlockNorm.apply(desc, mf, dev_rng, *tensors)
     else:
-        out, y, _ = _block(tensors, desc, mf, dev_rng)
+        out, y, _, _ = _block(tensors, desc, mf, dev_rng)
     return (residual if x is None else out), y
 
 
