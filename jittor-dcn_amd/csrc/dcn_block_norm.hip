@@ -269,8 +269,11 @@ hipError_t any_bwd(const BlockArgs& a, hipStream_t s) {
 }  // namespace
 
 size_t block_norm_ws_floats(const BlockArgs& a) {
-  // partials of the parameters and of an image gate, or six numbers a position
-  const size_t partials = (size_t)kMaxWgs * 5 * a.C + (size_t)(kMaxWgs + a.B) * a.C;
+  // partials of the parameters and of an image gate (interleaved where an image has
+  // kInterleave tiles, of 16 positions at least), or six numbers a position
+  size_t partials = (size_t)kMaxWgs * 5 * a.C;
+  if (a.gate_kind == DCN_GATE_IMAGE)
+    partials += (kMaxWgs + (size_t)a.B * (a.P > 16 * (kInterleave - 1) ? kInterleave : 1)) * a.C;
   return std::max(6 * (size_t)a.B * a.P, partials);
 }
 

@@ -149,6 +149,48 @@ def test_shapes(tb, dt, layout, B, C, P, gate):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout,B,C,P", [
+    ("nchw", 16, 256, 784), ("nchw", 24, 128, 1003), ("nchw", 8, 512, 300), ("nchw", 300, 16, 260),
+    ("nchw", 2, 64, 8193), ("rows", 16, 256, 784), ("rows", 700, 40, 5), ("rows", 3, 1024, 700)])
+@pytest.mark.parametrize("gate", ["none", "image"])
+def test_many_tiles(tb, dt, layout, B, C, P, gate):
+    """Enough tiles that workgroups take several, in turn, over image borders: every workgroup's
+    share of the parameter and gate gradients has to arrive once."""
+    run_and_check(tb, layout, B, C, P, dt, "layer", "rms", gate, "silu", seed=B + P)
+
+
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+@pytest.mark.parametrize("C", [48, 300, 3000])
+def test_backward_without_kept_statistics(tb, layout, C):
+    """dcn_block_norm_bwd computes the statistics again where it gets none: the kept ones are the
+    same numbers up to the summation order of the same kernel, so the gradients agree to fp32
+    rounding (16 (C + 64) u of their magnitudes on either side)."""
+    import ctypes
+
+    import dcn_runtime as rt
+    t, go, gy = tensors(layout, 3, C, 70, torch.float32, "layer", "rms", "full")
+    names = list(t)
+    for v in t.values():
+        v.requires_grad_()
+    want = torch.autograd.grad(call(tb, t, "layer", "rms", "silu"), list(t.values()), (go, gy))
+    d = rt.BlockDesc(3, C, 70, 0 if layout == "nchw" else 1, rt.DCN_F32, 2, 1, 1, 2, 1e-6, 1e-6,
+                     1.0, 0.0, 0, 0, 0)
+    n = ctypes.c_size_t()
+    rt.check(rt.load().dcn_block_norm_workspace(d, n))
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    got = {k: torch.full_like(v, float("nan")) for k, v in t.items()}
+    io = rt.BlockIO(**{k: v.data_ptr() for k, v in t.items()}, grad_out=go.data_ptr(),
+                    grad_y=gy.data_ptr(), **{"grad_" + k: v.data_ptr() for k, v in got.items()})
+    tb._call(ws.device, "dcn_block_norm_bwd", d, io, ws.data_ptr(), n.value)
+    ref = {k: rows(v, layout) for k, v in t.items()}
+    b = BO.block_bounds(ref, rows(go, layout), rows(gy, layout), post="layer", pre="rms", act="silu")
+    for k, w in zip(names, want):
+        terms = C if k in ("x", "residual", "gate") else 3 * 70 + C
+        err = (rows(got[k], layout) - rows(w, layout)).abs()
+        assert bool((err <= 2 * 16 * (terms + 64) * U * b[k] + 1e-37).all()), k
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("layout", ["nchw", "rows"])
 def test_parts(tb, dt, layout):
     """Absent pieces: the pre norm alone, no residual, no parameters, no pre norm, a gradient of
