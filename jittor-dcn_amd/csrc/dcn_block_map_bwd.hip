@@ -4,12 +4,11 @@
 namespace dcn {
 
 // Threads, lanes along the positions, channels a thread, waves per SIMD and workgroups that
-// prefetch their next tile (0: a workgroup per tile, or 1024 of them where parameters add up)
-// by channels, the fastest of those tried at 64 images (us, the best two):
-//   bf16 backward  64x3136: 52, 79    128x784: 42, 47    256x784: 72, 89   512x196: 62, 147
-//   f32 backward   64x3136: 83, 108   128x784: 61, 100   256x784: 112, 191 512x196: 103, 168
-// More channels than a workgroup's registers hold take narrower tiles (32-byte runs of a
-// channel at 1024), which costs less than a second pass. false: no variant (C > 2048).
+// prefetch their next tile (0: up to 1024 that do not) by channels; the fastest of those tried
+// at 64 images (us, the best two, tiles not yet interleaved):
+//   bf16  64x3136: 52, 79   128x784: 42, 47   256x784: 72, 89   512x196: 62, 147
+//   fp32  64x3136: 83, 108  128x784: 61, 100  256x784: 112, 191  512x196: 103, 168
+// false: no variant (C > 2048).
 bool block_map_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
   const int C = a.C;
   if (a.dtype == DCN_BF16) {

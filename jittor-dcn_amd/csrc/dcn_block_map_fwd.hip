@@ -4,10 +4,11 @@
 namespace dcn {
 
 // Threads, lanes along the positions, channels a thread, waves per SIMD and workgroups that
-// prefetch their next tile (0: a workgroup per tile, or 1024 of them where parameters add up)
-// by channels, the fastest of those tried at 64 images (us, the best two):
-//   bf16 forward   64x3136: 30, 44    128x784: 23, 25    256x784: 35, 35   512x196: 32, 36
-//   f32 forward    64x3136: 46, 55    128x784: 31, 34    256x784: 57, 66   512x196: 46, 52
+// prefetch their next tile (0: one workgroup per tile) by channels; the fastest of those tried
+// at 64 images (us, the best two):
+//   bf16  64x3136: 30, 44   128x784: 23, 25   256x784: 31, 34   512x196: 28, 36
+//   fp32  64x3136: 46, 55   128x784: 31, 34   256x3136: 178, 179   512x196: 35, 52
+// With dropout 256 bf16 channels want four waves per SIMD more than the prefetch (49 us, 55).
 // More channels than a workgroup's registers hold take narrower tiles (32-byte runs of a
 // channel at 1024), which costs less than a second pass. false: no variant (C > 2048).
 bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
@@ -16,7 +17,8 @@ bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     if (C <= 32) *e = run_map<bf16_t, 256, 8, 1, 3, 0, false>(a, s);
     else if (C <= 64) *e = run_map<bf16_t, 256, 8, 2, 2, 512, false>(a, s);
     else if (C <= 128) *e = run_map<bf16_t, 256, 4, 2, 2, 512, false>(a, s);
-    else if (C <= 256) *e = run_map<bf16_t, 512, 4, 2, 4, 0, false>(a, s);
+    else if (C <= 256 && a.drop.thr) *e = run_map<bf16_t, 512, 4, 2, 4, 0, false>(a, s);
+    else if (C <= 256) *e = run_map<bf16_t, 512, 4, 2, 2, 256, false>(a, s);
     else if (C <= 512) *e = run_map<bf16_t, 1024, 4, 2, 4, 0, false>(a, s);
     else if (C <= 1024) *e = run_map<bf16_t, 512, 2, 4, 2, 256, false>(a, s);
     else if (C <= 2048) *e = run_map<bf16_t, 1024, 2, 4, 4, 256, false>(a, s);
@@ -25,7 +27,7 @@ bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     if (C <= 32) *e = run_map<float, 256, 8, 1, 3, 0, false>(a, s);
     else if (C <= 64) *e = run_map<float, 256, 8, 2, 4, 0, false>(a, s);
     else if (C <= 128) *e = run_map<float, 256, 8, 4, 2, 512, false>(a, s);
-    else if (C <= 256) *e = run_map<float, 512, 8, 4, 4, 0, false>(a, s);
+    else if (C <= 256) *e = run_map<float, 512, 8, 4, 2, 256, false>(a, s);
     else if (C <= 512) *e = run_map<float, 512, 4, 4, 2, 256, false>(a, s);
     else if (C <= 1024) *e = run_map<float, 512, 4, 8, 2, 256, false>(a, s);
     else if (C <= 2048) *e = run_map<float, 1024, 4, 8, 4, 256, false>(a, s);

@@ -13,6 +13,9 @@
 // the forward where the caller kept them: 16 bytes a position, against two of the four rounds
 // of sums that a position's workgroup goes through.
 #pragma once
+#include <algorithm>
+#include <cstdlib>
+
 #include "dcn_block.h"
 #include "dcn_philox.h"
 
@@ -27,17 +30,22 @@ bool block_row_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e);
 
 namespace {
 
-// act(g) and act'(g)
+// act(g) and act'(g). The sigmoid from the hardware's exp2 and reciprocal, 1 ulp each, and an
+// argument rounded once: about (2 + |g|) 2^-24 of its value, an order below the sums' error and
+// a third of the instructions of the exact ones.
+__device__ __forceinline__ float sigmoid(float g) {
+  return __builtin_amdgcn_rcpf(1.f + __expf(-g));
+}
 __device__ __forceinline__ float gate_act(float g, int act) {
   if (act == DCN_ACT_LINEAR) return g;
-  const float s = 1.f / (1.f + expf(-g));
+  const float s = sigmoid(g);
   return act == DCN_ACT_SIGMOID ? s : g * s;
 }
 __device__ __forceinline__ void gate_act_grad(float g, int act, float& a, float& d) {
   a = g;
   d = 1.f;
   if (act == DCN_ACT_LINEAR) return;
-  const float s = 1.f / (1.f + expf(-g));
+  const float s = sigmoid(g);
   a = act == DCN_ACT_SIGMOID ? s : g * s;
   d = act == DCN_ACT_SIGMOID ? s * (1.f - s) : s * (1.f + g * (1.f - s));
 }
@@ -694,28 +702,35 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
   auto ptr = [](const void* p) { return static_cast<const T*>(p); };
 
   int cv[NV];  // valid elements of a vector
-  u32x4 psc[NV], pw1[NV], pb1[NV], pw2[NV], pb2[NV];
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  u32x4 one;
-  {
+  // The parameters of this lane's channels: kept beside a prefetched row, read again (from the
+  // caches) for every row where the registers are needed for the sums.
+  const void* const pars[5] = {a.scale, a.w1, a.b1, a.w2, a.b2};
+  u32x4 kept[AHEAD ? (BWD ? 4 : 5) : 1][NV];
+  auto fetch = [&](int k, int j) {
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    if (cv[j] <= 0) return zero;
+    if (pars[k]) return ldv_raw(ptr(pars[k]) + (lane + LPR * j) * V, cv[j]);
     float t[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) t[e] = 1.f;
-    one = pack<T>(t);
-  }
+    for (int e = 0; e < V; ++e) t[e] = k == 2 || k == 4 ? 0.f : 1.f;
+    return pack<T>(t);
+  };
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = (lane + LPR * j) * V;
-    cv[j] = a.C - c;
-    auto get = [&](const void* p, u32x4 none) {
-      return cv[j] <= 0 ? zero : p ? ldv_raw(ptr(p) + c, cv[j]) : none;
-    };
-    psc[j] = get(a.scale, one);
-    pw1[j] = get(a.w1, one);
-    pb1[j] = get(a.b1, zero);
-    pw2[j] = get(a.w2, one);
-    pb2[j] = BWD ? zero : get(a.b2, zero);
+    cv[j] = a.C - (lane + LPR * j) * V;
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int k = 0; k < (BWD ? 4 : 5); ++k) kept[k][j] = fetch(k, j);
+    }
   }
+  enum { SC, W1, B1, W2, B2 };
+  auto param = [&](int k, int j, float (&v)[V]) {
+    if constexpr (AHEAD)
+      unpack<T>(kept[k][j], v);
+    else
+      unpack<T>(fetch(k, j), v);
+  };
+  const u32x4 zero = {0u, 0u, 0u, 0u};
   float acc[BWD ? 5 : 1][NV][V], accg[BWD && !FULL ? NV : 1][V];
   if constexpr (BWD) {
 #pragma unroll
@@ -833,9 +848,9 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
         float xv[V], rv[V], sc[V], w1[V], b1[V], av[V], ad[V];
         unpack<T>(in.x[j], xv);
         unpack<T>(in.r[j], rv);
-        unpack<T>(psc[j], sc);
-        unpack<T>(pw1[j], w1);
-        unpack<T>(pb1[j], b1);
+        param(SC, j, sc);
+        param(W1, j, w1);
+        param(B1, j, b1);
         gate(j, av, ad);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -863,8 +878,8 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
         const size_t at = base + (lane + LPR * j) * V;
         if (a.pre) {
           float w2[V], b2[V], y[V];
-          unpack<T>(pw2[j], w2);
-          unpack<T>(pb2[j], b2);
+          param(W2, j, w2);
+          param(B2, j, b2);
 #pragma unroll
           for (int e = 0; e < V; ++e) y[e] = fmaf((o[j][e] - m2) * r2, w2[e], b2[e]);
           stv(static_cast<T*>(a.y) + at, cv[j], y);
@@ -880,7 +895,7 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
         for (int j = 0; j < NV; ++j) {
           float gy[V], w2[V];
           unpack<T>(in.y[j], gy);
-          unpack<T>(pw2[j], w2);
+          param(W2, j, w2);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float h = (o[j][e] - m2) * r2, w = gy[e] * w2[e];
@@ -899,7 +914,7 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
           float gy[V], go[V], w2[V];
           unpack<T>(in.y[j], gy);
           unpack<T>(in.o[j], go);
-          unpack<T>(pw2[j], w2);
+          param(W2, j, w2);
 #pragma unroll
           for (int e = 0; e < V; ++e)
             o[j][e] = fmaf(r2, gy[e] * w2[e] - s1 - o[j][e] * s2, go[e]);
@@ -920,9 +935,9 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
         for (int j = 0; j < NV; ++j) {
           float xv[V], sc[V], w1[V], b1[V], av[V], ad[V], gg[V];
           unpack<T>(in.x[j], xv);
-          unpack<T>(psc[j], sc);
-          unpack<T>(pw1[j], w1);
-          unpack<T>(pb1[j], b1);
+          param(SC, j, sc);
+          param(W1, j, w1);
+          param(B1, j, b1);
           gate(j, av, ad);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
@@ -954,7 +969,7 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
             if (a.post) {
               float xv[V], w1[V];
               unpack<T>(in.x[j], xv);
-              unpack<T>(pw1[j], w1);
+              param(W1, j, w1);
 #pragma unroll
               for (int e = 0; e < V; ++e) {
                 const float h = (xv[e] - m1) * r1;
@@ -1036,7 +1051,9 @@ hipError_t run_tiles(const BlockArgs& a, int images, int P, int per, int wgs, in
   q.tiles = (long)q.tpi * images;
   const bool params = BWD && (a.gs || a.gw1 || a.gb1 || a.gw2 || a.gb2);
   q.image_gate = BWD && a.gg && a.gate_kind == DCN_GATE_IMAGE;
-  q.wgs = (int)std::min<long>(q.tiles, wgs ? wgs : params || q.image_gate ? kMaxWgs : 1 << 20);
+  // wgs: > 0 with a prefetch, < 0 without, 0 one a tile as far as partials allow
+  q.wgs = (int)std::min<long>(
+      q.tiles, wgs ? std::abs(wgs) : params || q.image_gate ? kMaxWgs : 1 << 20);
   q.group = maps && q.tpi >= kInterleave && q.wgs % kInterleave == 0 ? kInterleave : 1;
   if (params) q.part = a.ws;
   if (q.image_gate) q.gpart = a.ws + (size_t)kMaxWgs * 5 * a.C;
@@ -1056,10 +1073,10 @@ hipError_t run_tiles(const BlockArgs& a, int images, int P, int per, int wgs, in
 template <typename T, int NT, int PL, int CPT, int WPE, int WGS, bool BWD>
 hipError_t run_map(const BlockArgs& a, hipStream_t s) {
   auto pick = [](bool full, bool drop) {
-    return full ? (drop ? block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, true, true>
-                        : block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, true, false>)
-                : (drop ? block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, false, true>
-                        : block_map<T, NT, PL, CPT, WPE, WGS != 0, BWD, false, false>);
+    return full ? (drop ? block_map<T, NT, PL, CPT, WPE, (WGS > 0), BWD, true, true>
+                        : block_map<T, NT, PL, CPT, WPE, (WGS > 0), BWD, true, false>)
+                : (drop ? block_map<T, NT, PL, CPT, WPE, (WGS > 0), BWD, false, true>
+                        : block_map<T, NT, PL, CPT, WPE, (WGS > 0), BWD, false, false>);
   };
   return run_tiles<T, BWD>(a, a.B, a.P, PL * ElemVec<T>::N, WGS, NT, true, pick, s);
 }
@@ -1067,10 +1084,10 @@ hipError_t run_map(const BlockArgs& a, hipStream_t s) {
 template <typename T, int NT, int LPR, int NV, int WPE, int WGS, bool BWD>
 hipError_t run_row(const BlockArgs& a, hipStream_t s) {
   auto pick = [](bool full, bool drop) {
-    return full ? (drop ? block_row<T, NT, LPR, NV, WPE, WGS != 0, BWD, true, true>
-                        : block_row<T, NT, LPR, NV, WPE, WGS != 0, BWD, true, false>)
-                : (drop ? block_row<T, NT, LPR, NV, WPE, WGS != 0, BWD, false, true>
-                        : block_row<T, NT, LPR, NV, WPE, WGS != 0, BWD, false, false>);
+    return full ? (drop ? block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, true, true>
+                        : block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, true, false>)
+                : (drop ? block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, false, true>
+                        : block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, false, false>);
   };
   // images matter to an image gate only; else all rows are one run (up to int)
   const bool one = a.gate_kind != DCN_GATE_IMAGE && (size_t)a.B * a.P < (1u << 30);
