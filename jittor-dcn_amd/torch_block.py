@@ -531,3 +531,40 @@ class Fp8Pointwise(torch.nn.Module):
         if self.weight8 is not None and not (torch.is_grad_enabled() and x.requires_grad):
             return fp8_pointwise(x, self.weight8)
         return fp8_pointwise(x, self.weight)
+
+
+# ---------------------------------------------------------------------------- a block
+class DeformBlock(torch.nn.Module):
+    """A residual block around torch_dcn.DeformConv2d and a channel MLP in 8 bits:
+
+        x1, y1 = block_norm(dcn(N(x)), x)      # norm after, layer scale, stochastic depth, norm
+        out    = x1 + drop(scale * N(fc2(act(fc1(y1)))))
+
+    on [B, C, H, W] maps, C as torch_dcn.DeformConv2d takes it (bfloat16: a multiple of 4 up
+    to 256). `rng`: as in Dropout (two tensors, one per join) for captured steps."""
+
+    def __init__(self, channels, expand=4, layer_scale=0.1, drop_path=0.0, kernel_size=3,
+                 act=torch.nn.functional.silu, rng=(None, None)):
+        super().__init__()
+        import torch_dcn
+        pad = kernel_size // 2
+        self.norm = BlockNorm(channels, post=None, pre="layer")
+        self.dcn = torch_dcn.DeformConv2d(channels, channels, kernel_size, 1, pad)
+        self.join = BlockNorm(channels, post="rms", pre="layer", layer_scale=layer_scale,
+                              drop_p=drop_path, drop="image", rng=rng[0])
+        self.fc1 = Fp8Pointwise(channels, expand * channels)
+        self.fc2 = Fp8Pointwise(expand * channels, channels)
+        self.act = act
+        self.leave = BlockNorm(channels, post="rms", pre=None, layer_scale=layer_scale,
+                               drop_p=drop_path, drop="image", rng=rng[1])
+
+    def serve(self):
+        """For inference: the MLP's weights in 8 bits."""
+        self.fc1.serve()
+        self.fc2.serve()
+        return self
+
+    def forward(self, x):
+        _, y = self.norm(None, x)
+        x, y = self.join(self.dcn(y), x)
+        return self.leave(self.fc2(self.act(self.fc1(y))), x)[0]
