@@ -410,6 +410,31 @@ int dcn_fp8_matmul_workspace(const dcn_fp8_matmul_desc* d, size_t* bytes);
 int dcn_fp8_matmul(dcn_handle* h, const dcn_fp8_matmul_desc* d, const void* a, const void* sa,
                    const void* b, const void* sb, void* out, void* ws, size_t ws_bytes);
 
+/* A pointwise product of a map tensor in one call: y[.., O, ..] = w · x over the channels (a
+ * linear layer of token rows, a 1x1 convolution of maps), both rounded as above (x by token,
+ * w in 128 x 128 blocks), and its gradients
+ *   grad_x = wᵀ · grad_y (grad_y by token),  grad_w = grad_y · xᵀ (both by channel). */
+typedef struct {
+  int B, C, P, O;     /* x is a map tensor of C channels, y of O */
+  int layout, dtype;
+} dcn_fp8_pointwise_desc;
+#define DCN_FP8_GRAD_X 1
+#define DCN_FP8_GRAD_W 2
+/* Bytes of the workspaces of the forward and the backward (one per call in flight) and of what
+ * the forward leaves for a backward that computes `grads` (DCN_FP8_GRAD_* bits; 0: none). */
+int dcn_fp8_pointwise_workspace(const dcn_fp8_pointwise_desc* d, int grads, size_t* fwd_ws,
+                                size_t* saved, size_t* bwd_ws);
+/* w[O][C], or w NULL and its 8-bit form q[O][Cp], s (then grads is 0: a served weight). saved
+ * holds the 8-bit forms that the backward multiplies: wᵀ for grad_x, x by channel for grad_w
+ * (half of keeping bf16 x and w, a quarter of fp32). All buffers 256-byte aligned. */
+int dcn_fp8_pointwise_fwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int grads, const void* x,
+                          const void* w, const void* q, const void* s, void* y, void* saved,
+                          size_t saved_bytes, void* ws, size_t ws_bytes);
+/* grads: as given to the forward; saved: what it left. A gradient that is NULL is not computed. */
+int dcn_fp8_pointwise_bwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int grads,
+                          const void* grad_y, const void* saved, size_t saved_bytes, void* grad_x,
+                          void* grad_w, void* ws, size_t ws_bytes);
+
 /* ---- in-library kernel timing (HIP events on the handle's stream) ---------- */
 typedef enum {
   DCN_K_OFFSET_FWD = 0,

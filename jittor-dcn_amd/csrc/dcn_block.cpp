@@ -1,6 +1,7 @@
 // dcn_block.cpp — entry points of the residual block's operators (include/dcn.h): argument
 // checks, then one launcher each. Nothing here allocates, synchronises or keeps state, so every
 // call can be captured into a graph.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -193,9 +194,177 @@ int fp8_matmul_check(const dcn_fp8_matmul_desc* d) {
   return DCN_OK;
 }
 
+// One pointwise product: where its 8-bit operands lie in the workspaces and in `saved`.
+struct Pointwise {
+  size_t T, cp, op, kt;                       // tokens; C, O and the tokens by channel, up to 128s
+  size_t wq, ws, xq, xs, mm, fwd;             // forward workspace
+  size_t wt, wts, xc, xcs, saved;             // saved
+  size_t gq, gs, gc, gcs, mmb, bwd;           // backward workspace
+  dcn_fp8_matmul_desc y, gx, gw;
+};
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+int pointwise(const dcn_fp8_pointwise_desc* d, int grads, Pointwise* p) {
+  if (!d) return fail(DCN_ERR_INVALID, "null descriptor");
+  if (d->B <= 0 || d->C <= 0 || d->P <= 0 || d->O <= 0)
+    return fail(DCN_ERR_INVALID, "B, C, P, O must be positive");
+  if (!dtype_ok(d->dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
+  if (d->layout != DCN_NCHW && d->layout != DCN_NHWC) return fail(DCN_ERR_INVALID, "unknown layout");
+  if (grads & ~(DCN_FP8_GRAD_X | DCN_FP8_GRAD_W)) return fail(DCN_ERR_INVALID, "unknown gradient");
+  const bool maps = d->layout == DCN_NCHW;
+  p->T = (size_t)d->B * d->P;
+  p->cp = up128(d->C);
+  p->op = up128(d->O);
+  p->kt = maps ? d->B * up128(d->P) : up128(p->T);
+  const double widest = std::max(d->C, d->O);
+  if (p->T > (1u << 30) || p->kt > (1u << 30) || widest > (1 << 30) ||
+      !tiles_ok(maps ? widest : (double)p->T, maps ? d->P : widest, maps ? d->B : 1) ||
+      !tiles_ok(d->O, d->C, 1) || !tiles_ok((double)p->T, widest, 1))
+    return fail(DCN_ERR_UNSUPPORTED, "tensor too large");
+  const int T = (int)p->T;
+  if (maps) {
+    p->y = {d->O, T, (int)p->cp, 128, 1, DCN_NCHW, d->P, d->dtype};
+    p->gx = {d->C, T, (int)p->op, 128, 1, DCN_NCHW, d->P, d->dtype};
+  } else {
+    p->y = {T, d->O, (int)p->cp, 1, 128, DCN_NHWC, 0, d->dtype};
+    p->gx = {T, d->C, (int)p->op, 1, 128, DCN_NHWC, 0, d->dtype};
+  }
+  p->gw = {d->O, d->C, (int)p->kt, 1, 1, DCN_NHWC, 0, d->dtype};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += up256(bytes);
+    return o;
+  };
+  p->wq = take(fp8_bytes(d->O, p->cp));
+  p->ws = take(exp_bytes(d->O, p->cp, 128));
+  p->xq = take(fp8_bytes(p->T, p->cp));
+  p->xs = take(exp_bytes(p->T, p->cp, 1));
+  p->mm = take(dcn::fp8_matmul_ws_bytes(p->y));
+  p->fwd = at;
+  at = 0;
+  if (grads & DCN_FP8_GRAD_X) {
+    p->wt = take(fp8_bytes(d->C, p->op));
+    p->wts = take(exp_bytes(d->C, p->op, 128));
+  }
+  if (grads & DCN_FP8_GRAD_W) {
+    p->xc = take(fp8_bytes(d->C, p->kt));
+    p->xcs = take(exp_bytes(d->C, p->kt, 1));
+  }
+  p->saved = at;
+  at = 0;
+  if (grads & DCN_FP8_GRAD_X) {
+    p->gq = take(fp8_bytes(p->T, p->op));
+    p->gs = take(exp_bytes(p->T, p->op, 1));
+  }
+  if (grads & DCN_FP8_GRAD_W) {
+    p->gc = take(fp8_bytes(d->O, p->kt));
+    p->gcs = take(exp_bytes(d->O, p->kt, 1));
+  }
+  p->mmb = take(std::max(grads & DCN_FP8_GRAD_X ? dcn::fp8_matmul_ws_bytes(p->gx) : 0,
+                         grads & DCN_FP8_GRAD_W ? dcn::fp8_matmul_ws_bytes(p->gw) : 0));
+  p->bwd = at;
+  return DCN_OK;
+}
+
+int buffer_ok(const void* p, size_t have, size_t need, const char* what) {
+  if (need && (!p || have < need))
+    return fail(DCN_ERR_WORKSPACE, (std::string(what) + " too small").c_str());
+  if (!aligned(p, 256))
+    return fail(DCN_ERR_INVALID, (std::string(what) + " must be 256-byte aligned").c_str());
+  return DCN_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int dcn_fp8_pointwise_workspace(const dcn_fp8_pointwise_desc* d, int grads, size_t* fwd_ws,
+                                size_t* saved, size_t* bwd_ws) {
+  Pointwise p{};
+  if (int rc = pointwise(d, grads, &p)) return rc;
+  if (!fwd_ws || !saved || !bwd_ws) return fail(DCN_ERR_INVALID, "null out pointer");
+  *fwd_ws = p.fwd;
+  *saved = p.saved;
+  *bwd_ws = p.bwd;
+  return DCN_OK;
+}
+
+int dcn_fp8_pointwise_fwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int grads, const void* x,
+                          const void* w, const void* q, const void* s, void* y, void* saved,
+                          size_t saved_bytes, void* ws, size_t ws_bytes) {
+  Pointwise p{};
+  if (int rc = pointwise(d, grads, &p)) return rc;
+  if (!x || !y || !(w || q)) return fail(DCN_ERR_INVALID, "null tensor");
+  if (w && (q || s)) return fail(DCN_ERR_INVALID, "one weight: as it is or in 8 bits");
+  if (int rc = fp8_pair(q, s, "weight")) return rc;
+  if (q && grads) return fail(DCN_ERR_INVALID, "a weight in 8 bits has no gradients");
+  if (int rc = buffer_ok(ws, ws_bytes, p.fwd, "pointwise workspace")) return rc;
+  if (int rc = buffer_ok(saved, saved_bytes, p.saved, "saved buffer")) return rc;
+  const size_t es = dtype_bytes(d->dtype);
+  const Span in[] = {{x, p.T * d->C * es}, {w, (size_t)d->O * d->C * es},
+                     {q, fp8_bytes(d->O, p.cp)}, {s, exp_bytes(d->O, p.cp, 128)}};
+  const Span out[] = {{y, p.T * d->O * es}, {p.saved ? saved : nullptr, p.saved}, {ws, p.fwd}};
+  for (const void* t : {x, w, static_cast<const void*>(y)})
+    if (!aligned(t, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
+  if (int rc = block_spans(in, 4, out, 3, 1, nullptr, nullptr)) return rc;
+  DeviceScope ds;
+  if (int rc = ds.bind(h)) return rc;
+  char *b = static_cast<char*>(ws), *k = static_cast<char*>(saved);
+  const bool gx = grads & DCN_FP8_GRAD_X, gw = grads & DCN_FP8_GRAD_W;
+  hipError_t e = hipSuccess;
+  if (w) {
+    e = dcn::launch_fp8_quantize_weight(d->O, d->C, d->dtype, w, b + p.wq, b + p.ws,
+                                        gx ? k + p.wt : nullptr, gx ? k + p.wts : nullptr, ds.stream);
+    q = b + p.wq;
+    s = b + p.ws;
+  }
+  if (e == hipSuccess)
+    e = dcn::launch_fp8_quantize(d->B, d->C, d->P, d->layout, d->dtype, x, b + p.xq, b + p.xs,
+                                 gw ? k + p.xc : nullptr, gw ? k + p.xcs : nullptr, ds.stream);
+  if (e == hipSuccess) {
+    const bool maps = d->layout == DCN_NCHW;
+    e = dcn::launch_fp8_matmul(p.y, maps ? q : b + p.xq, maps ? s : b + p.xs, maps ? b + p.xq : q,
+                               maps ? b + p.xs : s, y, b + p.mm, ds.stream);
+  }
+  return done(e, "fp8_pointwise forward");
+}
+
+int dcn_fp8_pointwise_bwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int grads,
+                          const void* grad_y, const void* saved, size_t saved_bytes, void* grad_x,
+                          void* grad_w, void* ws, size_t ws_bytes) {
+  Pointwise p{};
+  if (int rc = pointwise(d, grads, &p)) return rc;
+  if (!grad_y || !(grad_x || grad_w)) return fail(DCN_ERR_INVALID, "null tensor");
+  if ((grad_x && !(grads & DCN_FP8_GRAD_X)) || (grad_w && !(grads & DCN_FP8_GRAD_W)))
+    return fail(DCN_ERR_INVALID, "the forward kept nothing for this gradient");
+  if (int rc = buffer_ok(ws, ws_bytes, p.bwd, "pointwise workspace")) return rc;
+  if (int rc = buffer_ok(saved, saved_bytes, p.saved, "saved buffer")) return rc;
+  const size_t es = dtype_bytes(d->dtype);
+  for (const void* t : {grad_y, static_cast<const void*>(grad_x), static_cast<const void*>(grad_w)})
+    if (!aligned(t, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
+  const Span in[] = {{grad_y, p.T * d->O * es}, {saved, p.saved}};
+  const Span out[] = {{grad_x, p.T * d->C * es}, {grad_w, (size_t)d->O * d->C * es}, {ws, p.bwd}};
+  if (int rc = block_spans(in, 2, out, 3, 1, nullptr, nullptr)) return rc;
+  DeviceScope ds;
+  if (int rc = ds.bind(h)) return rc;
+  char* b = static_cast<char*>(ws);
+  const char* k = static_cast<const char*>(saved);
+  hipError_t e = dcn::launch_fp8_quantize(
+      d->B, d->O, d->P, d->layout, d->dtype, grad_y, grad_x ? b + p.gq : nullptr,
+      grad_x ? b + p.gs : nullptr, grad_w ? b + p.gc : nullptr, grad_w ? b + p.gcs : nullptr,
+      ds.stream);
+  const bool maps = d->layout == DCN_NCHW;
+  if (e == hipSuccess && grad_x)
+    e = dcn::launch_fp8_matmul(p.gx, maps ? k + p.wt : b + p.gq, maps ? k + p.wts : b + p.gs,
+                               maps ? b + p.gq : k + p.wt, maps ? b + p.gs : k + p.wts, grad_x,
+                               b + p.mmb, ds.stream);
+  if (e == hipSuccess && grad_w)
+    e = dcn::launch_fp8_matmul(p.gw, b + p.gc, b + p.gcs, k + p.xc, k + p.xcs, grad_w, b + p.mmb,
+                               ds.stream);
+  return done(e, "fp8_pointwise backward");
+}
 
 int dcn_fp8_quantize(dcn_handle* h, const dcn_fp8_desc* d, const void* v, void* q_tok, void* s_tok,
                      void* q_ch, void* s_ch) {

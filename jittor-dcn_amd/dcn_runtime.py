@@ -25,6 +25,7 @@ DCN_FWD_AUTO, DCN_FWD_UNFUSED, DCN_FWD_FUSED, DCN_FWD_FUSED_NOCOL = 0, 1, 2, 3
 DCN_NCHW, DCN_NHWC = 0, 1
 DCN_NORM_NONE, DCN_NORM_RMS, DCN_NORM_LAYER = 0, 1, 2
 DCN_GATE_NONE, DCN_GATE_FULL, DCN_GATE_IMAGE = 0, 1, 2
+DCN_FP8_GRAD_X, DCN_FP8_GRAD_W = 1, 2
 DCN_ACT_LINEAR, DCN_ACT_SIGMOID, DCN_ACT_SILU = 0, 1, 2
 DCN_MATH_F32, DCN_MATH_F32_BF16X3, DCN_MATH_F32_BF16X6, DCN_MATH_F32_BF16X9 = 0, 3, 6, 9
 KERNEL_IDS = {
@@ -81,6 +82,11 @@ class Fp8MatmulDesc(ctypes.Structure):
     """dcn_fp8_matmul_desc (include/dcn.h)."""
     _fields_ = [(n, ctypes.c_int) for n in ("M", "N", "K", "a_block", "b_block", "layout", "P",
                                             "out_dtype")]
+
+
+class Fp8PointwiseDesc(ctypes.Structure):
+    """dcn_fp8_pointwise_desc (include/dcn.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("B", "C", "P", "O", "layout", "dtype")]
 
 
 _vp = ctypes.c_void_p
@@ -162,6 +168,13 @@ SIGNATURES = {
                                 _vp],
     "dcn_fp8_matmul_workspace": [ctypes.POINTER(Fp8MatmulDesc), ctypes.POINTER(_sz)],
     "dcn_fp8_matmul": [_vp, ctypes.POINTER(Fp8MatmulDesc), _vp, _vp, _vp, _vp, _vp, _vp, _sz],
+    "dcn_fp8_pointwise_workspace": [ctypes.POINTER(Fp8PointwiseDesc), ctypes.c_int,
+                                    ctypes.POINTER(_sz), ctypes.POINTER(_sz),
+                                    ctypes.POINTER(_sz)],
+    "dcn_fp8_pointwise_fwd": [_vp, ctypes.POINTER(Fp8PointwiseDesc), ctypes.c_int, _vp, _vp, _vp,
+                              _vp, _vp, _vp, _sz, _vp, _sz],
+    "dcn_fp8_pointwise_bwd": [_vp, ctypes.POINTER(Fp8PointwiseDesc), ctypes.c_int, _vp, _vp, _sz,
+                              _vp, _vp, _vp, _sz],
 }
 _RESTYPES = {"dcn_last_error": ctypes.c_char_p}
 

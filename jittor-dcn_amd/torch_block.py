@@ -394,78 +394,96 @@ def fp8_quantize_weight(w):
     return Fp8Weight(q, e, w.shape[1])
 
 
-def _quantize(v, geo, tokens, channels):
-    """(bytes, exponents) by token and by channel of a map tensor in `geo`'s layout."""
-    layout, B, C, P, _ = geo
-    T, dev = B * P, v.device
+def fp8_quantize(x, tokens=True, channels=False):
+    """(bytes, exponents, bytes, exponents) of a map tensor by token and by channel (None where
+    not wanted), in the layouts of dcn_fp8_quantize (include/dcn.h)."""
+    dt = _dtype(x, "fp8_quantize")
+    layout, B, C, P, mf = _layout(x)
+    if not x.numel():
+        raise ValueError("fp8_quantize: an empty tensor")
+    x, T, dev = x.contiguous(memory_format=mf), B * P, x.device
     kt = B * _up(P) if layout == rt.DCN_NCHW else _up(T)
     q = e = qc = ec = None
     if tokens:
         q, e = _bytes(dev, T, _up(C)), _bytes(dev, _up(C) // 128, _up(T))
     if channels:
         qc, ec = _bytes(dev, C, kt), _bytes(dev, kt // 128, _up(C))
-    _call(dev, "dcn_fp8_quantize", rt.Fp8Desc(B, C, P, layout, _DT[v.dtype]), _ptr(v), _ptr(q),
-          _ptr(e), _ptr(qc), _ptr(ec))
+    _call(dev, "dcn_fp8_quantize", rt.Fp8Desc(B, C, P, layout, dt), _ptr(x), _ptr(q), _ptr(e),
+          _ptr(qc), _ptr(ec))
     return q, e, qc, ec
 
 
-def _matmul(desc, a, sa, b, sb, out):
-    nbytes = ctypes.c_size_t()
-    rt.check(_fn("dcn_fp8_matmul_workspace")(desc, nbytes), "dcn_fp8_matmul_workspace")
-    ws = _bytes(out.device, nbytes.value) if nbytes.value else None
-    _call(out.device, "dcn_fp8_matmul", desc, _ptr(a), _ptr(sa), _ptr(b), _ptr(sb), _ptr(out),
-          _ptr(ws), nbytes.value)
-
-
-def _pointwise(geo, O, q, e, wq, we, like):
-    """The map tensor [.., O, ..] of tokens q and a 128 x 128 blocked weight wq [O][K]."""
-    layout, B, _, P, mf = geo
-    T, K, dt = B * P, q.shape[1], _DT[like.dtype]
-    if like.dim() == 4:
-        shape = (B, O, *like.shape[2:])
-        out = torch.empty(shape, dtype=like.dtype, device=like.device, memory_format=mf)
-    else:
-        out = torch.empty((*like.shape[:-1], O), dtype=like.dtype, device=like.device)
-    if layout == rt.DCN_NCHW:
-        d = rt.Fp8MatmulDesc(O, T, K, 128, 1, layout, P, dt)
-        _matmul(d, wq, we, q, e, out)
-    else:
-        d = rt.Fp8MatmulDesc(T, O, K, 1, 128, layout, 0, dt)
-        _matmul(d, q, e, wq, we, out)
+def fp8_matmul(a, a_exponents, b, b_exponents, dtype=torch.float32):
+    """a · bᵀ of two matrices in 8 bits (fp8_quantize's or Fp8Weight's layouts; either may have
+    an exponent per row or per 128 rows), fp32 sums, as [a's rows, b's rows] of `dtype`."""
+    if dtype not in _DT:
+        raise TypeError(f"fp8_matmul gives float32 or bfloat16, not {dtype}")
+    K, blocks = a.shape[-1], []
+    for t, e in ((a, a_exponents), (b, b_exponents)):
+        if t.dim() != 2 or t.shape[1] != K or K % 128 or t.dtype != torch.uint8 or not t.is_cuda:
+            raise ValueError("fp8_matmul: operands are uint8 [rows, K] on a GPU, K a multiple of 128")
+        rows = t.shape[0]
+        shape = {(K // 128, _up(rows)): 1, (K // 128, -(-rows // 128)): 128}
+        if e.dtype != torch.uint8 or e.device != t.device or tuple(e.shape) not in shape:
+            raise ValueError(f"fp8_matmul: exponents of {rows} rows are uint8 {list(shape)}")
+        blocks.append(shape[tuple(e.shape)])
+    if b.device != a.device or not a.numel() or not b.numel():
+        raise ValueError("fp8_matmul: non-empty operands on one device")
+    a, a_exponents, b, b_exponents = (_at16(t) for t in (a, a_exponents, b, b_exponents))
+    out = torch.empty((a.shape[0], b.shape[0]), dtype=dtype, device=a.device)
+    d = rt.Fp8MatmulDesc(a.shape[0], b.shape[0], K, *blocks, rt.DCN_NHWC, 0, _DT[dtype])
+    n = ctypes.c_size_t()
+    rt.check(_fn("dcn_fp8_matmul_workspace")(d, n), "dcn_fp8_matmul_workspace")
+    ws = _bytes(out.device, n.value) if n.value else None
+    _call(out.device, "dcn_fp8_matmul", d, _ptr(a), _ptr(a_exponents), _ptr(b),
+          _ptr(b_exponents), _ptr(out), _ptr(ws), n.value)
     return out
+
+
+def _pointwise(x, w, kept, geo, grads):
+    """(y, what the backward needs) of x and a weight w [O, C] or an Fp8Weight `kept`."""
+    layout, B, C, P, mf = geo
+    x = x.contiguous(memory_format=mf)
+    O = kept.out_features if w is None else w.shape[0]
+    w = None if w is None else w.contiguous()
+    d = rt.Fp8PointwiseDesc(B, C, P, O, layout, _DT[x.dtype])
+    n_ws, n_saved, n_bwd = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
+    rt.check(_fn("dcn_fp8_pointwise_workspace")(d, grads, n_ws, n_saved, n_bwd),
+             "dcn_fp8_pointwise_workspace")
+    if x.dim() == 4:
+        y = torch.empty((B, O, *x.shape[2:]), dtype=x.dtype, device=x.device, memory_format=mf)
+    else:
+        y = torch.empty((*x.shape[:-1], O), dtype=x.dtype, device=x.device)
+    ws = _bytes(x.device, n_ws.value)
+    saved = _bytes(x.device, n_saved.value) if grads else None
+    q, e = (None, None) if kept is None else (kept.q.data_ptr(), kept.exponents.data_ptr())
+    _call(x.device, "dcn_fp8_pointwise_fwd", d, grads, x.data_ptr(), _ptr(w), q, e, y.data_ptr(),
+          _ptr(saved), n_saved.value, ws.data_ptr(), n_ws.value)
+    return y, (d, saved, n_saved.value, n_bwd.value)
 
 
 class _Fp8Pointwise(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, geo):
-        mf = geo[-1]
-        x = x.contiguous(memory_format=mf)
-        O = w.shape[0]
         need_x, need_w = ctx.needs_input_grad[:2]
-        wq, we, wqt, wet = _quantize_weight(w, True, need_x)
-        q, e, qc, ec = _quantize(x, geo, True, need_w)
-        y = _pointwise(geo, O, q, e, wq, we, x)
-        ctx.geo, ctx.shapes = geo, (x.shape, w.shape, x.dtype)
-        ctx.save_for_backward(wqt, wet, qc, ec)
+        grads = rt.DCN_FP8_GRAD_X * need_x | rt.DCN_FP8_GRAD_W * need_w
+        y, (d, saved, n_saved, n_bwd) = _pointwise(x, w, None, geo, grads)
+        ctx.args = d, grads, n_saved, n_bwd, geo[-1], x.shape, w.shape
+        ctx.save_for_backward(saved)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        (layout, B, C, P, mf), (xs, wshape, dt) = ctx.geo, ctx.shapes
-        wqt, wet, qc, ec = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad[:2]
+        d, grads, n_saved, n_bwd, mf, xshape, wshape = ctx.args
+        saved, = ctx.saved_tensors
         gy = gy.contiguous(memory_format=mf)
-        O = wshape[0]
-        geo = (layout, B, O, P, mf)
-        q, e, gc, gec = _quantize(gy, geo, need_x, need_w)
-        gx = gw = None
-        if need_x:
-            gx = _pointwise(geo, C, q, e, wqt, wet, gy)
-        if need_w:
-            gw = torch.empty(wshape, dtype=dt, device=gy.device)
-            d = rt.Fp8MatmulDesc(O, C, gc.shape[1], 1, 1, rt.DCN_NHWC, 0, _DT[dt])
-            _matmul(d, gc, gec, qc, ec, gw)
+        new = lambda shape, **kw: torch.empty(shape, dtype=gy.dtype, device=gy.device, **kw)
+        gx = new(xshape, memory_format=mf) if grads & rt.DCN_FP8_GRAD_X else None
+        gw = new(wshape) if grads & rt.DCN_FP8_GRAD_W else None
+        ws = _bytes(gy.device, n_bwd)
+        _call(gy.device, "dcn_fp8_pointwise_bwd", d, grads, gy.data_ptr(), saved.data_ptr(),
+              n_saved, _ptr(gx), _ptr(gw), ws.data_ptr(), n_bwd)
         return gx, gw, None
 
 
@@ -501,10 +519,10 @@ def fp8_pointwise(x, weight):
         y = x.new_empty(shape)
         return y if isinstance(weight, Fp8Weight) else y + 0 * (x.sum() + weight.sum())
     if isinstance(weight, Fp8Weight):
-        xc = x.contiguous(memory_format=geo[-1])
-        q, e, _, _ = _quantize(xc, geo, True, False)
-        return _pointwise(geo, O, q, e, weight.q, weight.exponents, xc)
-    return _Fp8Pointwise.apply(x, weight, geo)
+        return _pointwise(x, None, weight, geo, 0)[0]
+    if _wants_grad(x, weight):
+        return _Fp8Pointwise.apply(x, weight, geo)
+    return _pointwise(x, weight, None, geo, 0)[0]
 
 
 class Fp8Pointwise(torch.nn.Module):

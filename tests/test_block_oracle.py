@@ -223,3 +223,36 @@ def test_fp8_matmul_refusals(kw, ptr, msg):
     p = {**dict(a=A, sa=A * 2, b=A * 3, sb=A * 4, out=A * 5, ws=None, n=0), **ptr}
     assert rt.load().dcn_fp8_matmul(None, ctypes.byref(d), *p.values()) < 0
     assert msg in rt.last_error()
+
+
+def _pointwise(L, fwd, **kw):
+    d = rt.Fp8PointwiseDesc(**{**dict(B=2, C=20, P=6, O=30, layout=0, dtype=0),
+                               **{k: kw.pop(k) for k in list(kw) if k in "BCPO" or k in ("layout", "dtype")}})
+    if fwd:
+        p = {**dict(grads=0, x=A, w=A * 2, q=None, s=None, y=A * 3, saved=None, ns=0, ws=A * 4,
+                    n=1 << 19), **kw}
+        return L.dcn_fp8_pointwise_fwd(None, ctypes.byref(d), *p.values())
+    p = {**dict(grads=3, gy=A, saved=A * 2, ns=1 << 19, gx=A * 3, gw=A * 4, ws=A * 5, n=1 << 19), **kw}
+    return L.dcn_fp8_pointwise_bwd(None, ctypes.byref(d), *p.values())
+
+
+@pytest.mark.parametrize("fwd,kw,msg", [
+    (1, dict(O=0), "positive"), (1, dict(dtype=4), "dtype"), (1, dict(layout=5), "layout"),
+    (1, dict(grads=4), "unknown gradient"), (1, dict(x=None), "null tensor"),
+    (1, dict(w=None), "null tensor"), (1, dict(q=A * 7, s=A * 8), "one weight"),
+    (1, dict(w=None, q=A * 7), "come together"),
+    (1, dict(w=None, q=A * 7, s=A * 8, grads=1), "no gradients"),
+    (1, dict(n=100), "too small"), (1, dict(ws=A * 4 + 16), "256-byte"),
+    (1, dict(grads=1), "saved buffer too small"), (1, dict(y=A + 64), "overlaps"),
+    (1, dict(y=A * 3 + 2), "aligned"), (1, dict(ws=A * 3), "two outputs"),
+    (1, dict(B=1 << 15, P=1 << 16), "too large"), (1, {}, "null handle"),
+    (1, dict(w=None, q=A * 7, s=A * 8), "null handle"),
+    (1, dict(grads=3, saved=A * 9, ns=1 << 19), "null handle"),
+    (0, dict(gx=None, gw=None), "null tensor"), (0, dict(gy=None), "null tensor"),
+    (0, dict(grads=1), "kept nothing"), (0, dict(ns=4), "saved buffer too small"),
+    (0, dict(n=4), "too small"), (0, dict(gx=A), "overlaps"), (0, dict(gw=A * 3), "two outputs"),
+    (0, dict(gx=A * 3 + 1), "aligned"), (0, {}, "null handle"), (0, dict(gx=None), "null handle"),
+])
+def test_fp8_pointwise_refusals(fwd, kw, msg):
+    assert _pointwise(rt.load(), fwd, **dict(kw)) < 0
+    assert msg in rt.last_error()

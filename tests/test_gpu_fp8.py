@@ -63,8 +63,7 @@ def test_quantize(tb, dt, layout, B, C, P):
         f = x.view(-1)
         f[0], f[min(7, f.numel() - 1)] = float("inf"), float("nan")
         f[f.numel() // 2:f.numel() // 2 + 40] = 0.0
-    geo = tb._layout(x)
-    q, e, qc, ec = tb._quantize(x, geo, True, True)
+    q, e, qc, ec = tb.fp8_quantize(x, True, True)
     img = np64(x).reshape(B, C, P) if layout == "nchw" else np64(x).reshape(B, P, C).transpose(0, 2, 1)
     tok = np.zeros((B * P, up(C)))
     tok[:, :C] = img.transpose(0, 2, 1).reshape(B * P, C)
@@ -78,8 +77,8 @@ def test_quantize(tb, dt, layout, B, C, P):
         ch[:, :B * P] = tok[:, :C].T
     check_blocks(ch, qc, ec, ch.shape[1])
     # either alone gives the same bytes
-    assert torch.equal(tb._quantize(x, geo, True, False)[0], q)
-    assert torch.equal(tb._quantize(x, geo, False, True)[2], qc)
+    assert torch.equal(tb.fp8_quantize(x, True, False)[0], q)
+    assert torch.equal(tb.fp8_quantize(x, False, True)[2], qc)
 
 
 def test_rounding_of_every_half_step(tb):
@@ -100,7 +99,7 @@ def test_rounding_of_every_half_step(tb):
             r[127] = top
             rows.append(r)
     v = torch.from_numpy(np.stack(rows)).cuda()
-    q, e, _, _ = tb._quantize(v, tb._layout(v), True, False)
+    q, e, _, _ = tb.fp8_quantize(v)
     check_blocks(np64(v), q, e, 128)
 
 
@@ -190,6 +189,36 @@ def test_large_tiles(tb, dt, layout, B, P, C, O):
     with torch.no_grad():
         y = tb.fp8_pointwise(x, w)
     close(tok(y), BO.fp8_value(tok(x), 1, 128), BO.fp8_value(np64(w), 128, 128), dt, "y")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 128), (70, 300, 256), (200, 65, 1024), (300, 40, 384),
+                                   (129, 131, 2304)])
+@pytest.mark.parametrize("ab,bb", [(1, 1), (1, 128), (128, 1), (128, 128)])
+def test_matmul_blocks(tb, dt, M, N, K, ab, bb):
+    """Either operand with an exponent per row or per 128 rows, tile and few-row kernels."""
+    def operand(rows, block, seed):
+        v = make((rows, K), torch.float32, seed, 0.3)
+        if block == 1:
+            q, e, _, _ = tb.fp8_quantize(v)
+        else:
+            w = tb.fp8_quantize_weight(v)
+            q, e = w.q, w.exponents
+        return q, e, BO.fp8_value(np64(v), block, 128)
+
+    (a, ea, va), (b, eb, vb) = operand(M, ab, 1), operand(N, bb, 2)
+    close(np64(tb.fp8_matmul(a, ea, b, eb, dt)), va, vb, dt, "product")
+
+
+def test_only_one_gradient(tb):
+    """The gradient of one input alone is the one of both."""
+    x, w = make((50, 200), torch.bfloat16, 1, 0.2), make((70, 200), torch.bfloat16, 2, 0.2)
+    gy = make((50, 70), torch.bfloat16, 3, 0.2)
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    gx, gw = torch.autograd.grad(tb.fp8_pointwise(xr, wr), (xr, wr), gy)
+    assert torch.equal(torch.autograd.grad(tb.fp8_pointwise(xr, w), xr, gy)[0], gx)
+    assert torch.equal(torch.autograd.grad(tb.fp8_pointwise(x, wr), wr, gy)[0], gw)
+    assert torch.equal(torch.autograd.grad(tb.fp8_pointwise(xr, wr), wr, gy)[0], gw)
 
 
 def test_asymmetric_identity(tb):
@@ -302,6 +331,10 @@ def test_refusals_and_modules(tb):
         tb.fp8_pointwise(make((4, 11), torch.float32), qw)
     with pytest.raises(ValueError):
         tb.Fp8Weight(qw.q, qw.exponents, 200)
+    q, e, _, _ = tb.fp8_quantize(x)
+    for args in ((q, e, q[:, :64], e), (q, e[:, :4], q, e), (q.int(), e, q, e), (q, e, q.cpu(), e)):
+        with pytest.raises(ValueError):
+            tb.fp8_matmul(*args)
     with pytest.raises(ValueError):
         tb.fp8_quantize_weight(x[0])
     assert tb.fp8_pointwise(x[:0], w).shape == (0, 6)
