@@ -320,11 +320,14 @@ int dcn_fp8_pointwise_fwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int gr
     q = b + p.wq;
     s = b + p.ws;
   }
-  if (e == hipSuccess)
-    e = dcn::launch_fp8_quantize(d->B, d->C, d->P, d->layout, d->dtype, x, b + p.xq, b + p.xs,
-                                 gw ? k + p.xc : nullptr, gw ? k + p.xcs : nullptr, ds.stream);
-  if (e == hipSuccess) {
-    const bool maps = d->layout == DCN_NCHW;
+  const bool maps = d->layout == DCN_NCHW, few = !maps && dcn::fp8_few_tokens(p.T);
+  if (e == hipSuccess && (!few || gw))
+    e = dcn::launch_fp8_quantize(d->B, d->C, d->P, d->layout, d->dtype, x, few ? nullptr : b + p.xq,
+                                 few ? nullptr : b + p.xs, gw ? k + p.xc : nullptr,
+                                 gw ? k + p.xcs : nullptr, ds.stream);
+  if (e == hipSuccess && few) {
+    e = dcn::launch_fp8_few_tokens(p.y, d->C, x, q, s, y, ds.stream);
+  } else if (e == hipSuccess) {
     e = dcn::launch_fp8_matmul(p.y, maps ? q : b + p.xq, maps ? s : b + p.xs, maps ? b + p.xq : q,
                                maps ? b + p.xs : s, y, b + p.mm, ds.stream);
   }

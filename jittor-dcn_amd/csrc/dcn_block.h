@@ -34,5 +34,9 @@ hipError_t launch_fp8_quantize_weight(int O, int C, int dtype, const void* w, vo
 size_t fp8_matmul_ws_bytes(const dcn_fp8_matmul_desc& d);
 hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const void* sa,
                              const void* b, const void* sb, void* out, void* ws, hipStream_t s);
+// The product of few tokens x [d.M][cols] that are not rounded yet with b, in one launch.
+bool fp8_few_tokens(size_t tokens);
+hipError_t launch_fp8_few_tokens(const dcn_fp8_matmul_desc& d, int cols, const void* x,
+                                 const void* w, const void* sw, void* out, hipStream_t s);
 
 }  // namespace dcn

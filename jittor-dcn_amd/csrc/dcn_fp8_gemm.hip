@@ -20,7 +20,7 @@
 #include <type_traits>
 
 #include "dcn_block.h"
-#include "dcn_philox.h"
+#include "dcn_fp8.h"
 
 namespace dcn {
 
@@ -40,6 +40,8 @@ struct GemmArgs {
   int M, N, nkb, P, nchw, a_shift, b_shift;  // shift: log2 of rows per exponent
   long K, sa_str, sb_str;
   int kb_split;    // k blocks of a split
+  const void* x;   // the short side before its rounding, rows of x_cols
+  int x_cols;
   int tiles_m, tiles_n;
 };
 
@@ -313,9 +315,16 @@ __global__ __launch_bounds__(256) void fp8_gemm_join(GemmArgs g, int splits) {
 // A workgroup takes 16 rows of the long side and all of K; its waves take the k blocks in
 // turn, each lane loading its 32 bytes of a block straight into MFMA operands (whole 128-byte
 // lines per four lanes), AHEAD blocks in flight; the waves' sums meet in LDS, in wave order.
-template <int F, bool WIDE>  // F: fragments of the short side
+//
+// F: fragments (16 rows) of the short side. FUSED: the short side is not yet rounded; every
+// workgroup rounds its 16 rows of x [S][C] on the way in, four lanes to a block of 128, which
+// is cheaper than a launch for it (up to 16 tokens; 64 would cost each workgroup 12 us).
+template <int F, bool WIDE, bool FUSED>
 __global__ __launch_bounds__(512) void fp8_gemm_few(GemmArgs g, int swap) {
-  constexpr int NW = 8, AHEAD = F == 1 ? 4 : 2;
+  using T = std::conditional_t<WIDE, float, bf16_t>;
+  static_assert(!FUSED || F == 1, "one fragment");
+  constexpr int NW = 8, AHEAD = F > 1 || (FUSED && WIDE) ? 2 : 4;
+  constexpr int V = ElemVec<T>::N, XV = FUSED ? 32 / V : 1;  // vectors of x a lane and block
   __shared__ float sum[NW][F][256];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -335,6 +344,7 @@ __global__ __launch_bounds__(512) void fp8_gemm_few(GemmArgs g, int swap) {
     ssrc[f] = sp + (size_t)row * g.K + q * 16;
     sexp[f] = se + (row >> ssh);
   }
+  const T* xrow = FUSED ? static_cast<const T*>(g.x) + (size_t)min(r, S - 1) * g.x_cols : nullptr;
   f32x4 acc[F];
 #pragma unroll
   for (int f = 0; f < F; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -348,10 +358,19 @@ __global__ __launch_bounds__(512) void fp8_gemm_few(GemmArgs g, int swap) {
     constexpr int U = decltype(count)::value;
     i32x8 lv[U], sv[U][F];
     int el[U], es[U][F];
+    u32x4 xv[U][XV];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       lv[u] = ld(lsrc + (size_t)(kb0 + u) * 128);
       el[u] = lexp[(size_t)(kb0 + u) * lstr];
+      if constexpr (FUSED) {  // k 16q .. 16q + 15 of the block's lower half, then of its upper
+#pragma unroll
+        for (int i = 0; i < XV; ++i) {
+          const int c = (kb0 + u) * 128 + (i / (XV / 2)) * 64 + q * 16 + (i % (XV / 2)) * V;
+          xv[u][i] = c < g.x_cols ? ldv_raw(xrow + c, g.x_cols - c) : u32x4{0u, 0u, 0u, 0u};
+        }
+        continue;
+      }
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         sv[u][f] = ld(ssrc[f] + (size_t)(kb0 + u) * 128);
@@ -359,6 +378,31 @@ __global__ __launch_bounds__(512) void fp8_gemm_few(GemmArgs g, int swap) {
       }
     }
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (FUSED) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[32];
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < XV; ++i) {
+          float t[V];
+          unpack<T>(xv[u][i], t);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            v[i * V + j] = t[j];
+            m = mag_max(m, t[j]);
+          }
+        }
+        m = max(m, (unsigned)__shfl_xor((int)m, 16));
+        m = max(m, (unsigned)__shfl_xor((int)m, 32));
+        es[u][0] = (int)exp_byte(m);
+        const float inv = exp_inv((unsigned)es[u][0]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          sv[u][0][i] = (int)to_fp8x4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv,
+                                      v[4 * i + 3] * inv);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -444,34 +488,19 @@ hipError_t run_tiles(GemmArgs g, const Plan& p, bool wide, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int F>
+template <int F, bool FUSED>
 hipError_t run_few(const GemmArgs& g, bool wide, hipStream_t s) {
-  const int swap = g.N < g.M, longest = swap ? g.M : g.N;
+  const int swap = !FUSED && g.N < g.M, longest = swap ? g.M : g.N;
   const dim3 grid((longest + 15) / 16), block(512);
   if (wide)
-    hipLaunchKernelGGL((fp8_gemm_few<F, true>), grid, block, 0, s, g, swap);
+    hipLaunchKernelGGL((fp8_gemm_few<F, true, FUSED>), grid, block, 0, s, g, swap);
   else
-    hipLaunchKernelGGL((fp8_gemm_few<F, false>), grid, block, 0, s, g, swap);
+    hipLaunchKernelGGL((fp8_gemm_few<F, false, FUSED>), grid, block, 0, s, g, swap);
   return hipGetLastError();
 }
 
-}  // namespace
-
-size_t fp8_matmul_ws_bytes(const dcn_fp8_matmul_desc& d) {
-  const Plan p = plan(d);
-  return p.splits > 1 ? (size_t)p.splits * d.M * d.N * sizeof(float) : 0;
-}
-
-hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const void* sa,
-                             const void* b, const void* sb, void* out, void* ws, hipStream_t s) {
+GemmArgs gemm_args(const dcn_fp8_matmul_desc& d) {
   GemmArgs g{};
-  auto u8 = [](const void* p) { return static_cast<const unsigned char*>(p); };
-  g.a = u8(a);
-  g.sa = u8(sa);
-  g.b = u8(b);
-  g.sb = u8(sb);
-  g.out = out;
-  g.part = static_cast<float*>(ws);
   g.M = d.M;
   g.N = d.N;
   g.K = d.K;
@@ -482,16 +511,50 @@ hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const 
   g.b_shift = d.b_block == 128 ? 7 : 0;
   g.sa_str = d.a_block == 128 ? (d.M + 127) / 128 : (d.M + 127) / 128 * 128;
   g.sb_str = d.b_block == 128 ? (d.N + 127) / 128 : (d.N + 127) / 128 * 128;
+  return g;
+}
+
+const unsigned char* u8(const void* p) { return static_cast<const unsigned char*>(p); }
+
+}  // namespace
+
+size_t fp8_matmul_ws_bytes(const dcn_fp8_matmul_desc& d) {
+  const Plan p = plan(d);
+  return p.splits > 1 ? (size_t)p.splits * d.M * d.N * sizeof(float) : 0;
+}
+
+hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const void* sa,
+                             const void* b, const void* sb, void* out, void* ws, hipStream_t s) {
+  GemmArgs g = gemm_args(d);
+  g.a = u8(a);
+  g.sa = u8(sa);
+  g.b = u8(b);
+  g.sb = u8(sb);
+  g.out = out;
+  g.part = static_cast<float*>(ws);
   const bool wide = d.out_dtype == DCN_F32;
   const Plan p = plan(d);
   if (p.kind == Plan::FEW) {
     const int few = std::min(d.M, d.N);
-    return few <= 16 ? run_few<1>(g, wide, s) : few <= 32 ? run_few<2>(g, wide, s)
-                                                          : run_few<4>(g, wide, s);
+    return few <= 16 ? run_few<1, false>(g, wide, s) : few <= 32 ? run_few<2, false>(g, wide, s)
+                                                          : run_few<4, false>(g, wide, s);
   }
   if (p.kind == Plan::TILE256) return run_tiles<2, 1, 2, 4, 2, 2>(g, p, wide, s);
   if (p.kind == Plan::SHORT) return run_tiles<1, 1, 2, 2, 3, 1>(g, p, wide, s);
   return run_tiles<1, 1, 2, 2, 2, 2>(g, p, wide, s);
+}
+
+bool fp8_few_tokens(size_t tokens) { return tokens <= 16; }
+
+hipError_t launch_fp8_few_tokens(const dcn_fp8_matmul_desc& d, int cols, const void* x,
+                                 const void* w, const void* sw, void* out, hipStream_t s) {
+  GemmArgs g = gemm_args(d);
+  g.x = x;
+  g.x_cols = cols;
+  g.b = u8(w);
+  g.sb = u8(sw);
+  g.out = out;
+  return run_few<1, true>(g, d.out_dtype == DCN_F32, s);
 }
 
 }  // namespace dcn

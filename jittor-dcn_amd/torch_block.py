@@ -233,7 +233,10 @@ class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, desc, mf, dev_rng, *tensors):
         out, y, tensors, stats = _block(tensors, desc, mf, dev_rng, keep=True)
-        ctx.desc, ctx.mf = desc, mf
+        nbytes = ctypes.c_size_t()
+        if out is not None and out.numel() or y is not None and y.numel():
+            rt.check(_fn("dcn_block_norm_workspace")(desc, nbytes), "dcn_block_norm_workspace")
+        ctx.desc, ctx.mf, ctx.ws_bytes = desc, mf, nbytes.value
         ctx.save_for_backward(*tensors, dev_rng, stats)
         ctx.set_materialize_grads(False)
         return out, y
@@ -252,11 +255,9 @@ class _BlockNorm(torch.autograd.Function):
             return (None, None, None,
                     *(torch.zeros_like(t) if n else None for t, n in zip(inputs, need)))
         grads = [torch.empty_like(t) if n else None for t, n in zip(inputs, need)]
-        nbytes = ctypes.c_size_t()
-        rt.check(_fn("dcn_block_norm_workspace")(ctx.desc, nbytes), "dcn_block_norm_workspace")
-        ws = _bytes(ref.device, nbytes.value)
+        ws = _bytes(ref.device, ctx.ws_bytes)
         io = rt.BlockIO(*map(_ptr, (*inputs, dev_rng, None, None, grad_out, grad_y, *grads, stats)))
-        _call(ref.device, "dcn_block_norm_bwd", ctx.desc, io, ws.data_ptr(), nbytes.value)
+        _call(ref.device, "dcn_block_norm_bwd", ctx.desc, io, ws.data_ptr(), ctx.ws_bytes)
         return (None, None, None, *grads)
 
 
