@@ -90,8 +90,9 @@ int block_geo(const dcn_block_desc* d, dcn::BlockArgs* a) {
   if (d->B <= 0 || d->C <= 0 || d->P <= 0) return fail(DCN_ERR_INVALID, "B, C, P must be positive");
   if (!dtype_ok(d->dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
   if (d->layout != DCN_NCHW && d->layout != DCN_NHWC) return fail(DCN_ERR_INVALID, "unknown layout");
-  if ((double)d->B * d->C * d->P > (double)(1LL << 40) || (long long)d->B * d->P > (1LL << 34))
-    return fail(DCN_ERR_UNSUPPORTED, "more than 2^40 elements or 2^34 positions");
+  if ((double)d->B * d->C * d->P > (double)(1LL << 40) || (long long)d->B * d->P > (1LL << 34) ||
+      d->C > (1 << 30) || d->P > (1 << 30))
+    return fail(DCN_ERR_UNSUPPORTED, "more than 2^40 elements, 2^34 positions, or C or P above 2^30");
   for (int k : {d->post, d->pre})
     if (k < DCN_NORM_NONE || k > DCN_NORM_LAYER) return fail(DCN_ERR_INVALID, "unknown norm");
   if (d->gate < DCN_GATE_NONE || d->gate > DCN_GATE_IMAGE)

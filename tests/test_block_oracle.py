@@ -104,7 +104,8 @@ FAR = OK_PTR * 100
     (dict(), dict(out=OK_PTR + 64), "overlaps"), (dict(), dict(out=OK_PTR), "overlaps"),
     (dict(), dict(y=OK_PTR * 2), "overlaps"), (dict(), dict(y=OK_PTR * 3 + 380), "two outputs"),
     (dict(), dict(w_pre=OK_PTR * 4), "overlaps"),
-    (dict(B=1 << 20, C=1 << 20, P=2), {}, "2\\^40"),
+    (dict(B=1 << 20, C=1 << 20, P=2), {}, "2\\^40"), (dict(P=(1 << 30) + 1, C=1, B=1), {}, "2\\^30"),
+    (dict(P=1, C=(1 << 30) + 1, B=1), {}, "2\\^30"),
     (dict(), {}, "null handle"), (dict(), dict(out=OK_PTR * 2), "null handle"),
     (dict(post=0), dict(x=None, out=None), "null handle"),
 ])
