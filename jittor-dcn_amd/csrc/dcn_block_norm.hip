@@ -268,18 +268,23 @@ hipError_t any_bwd(const BlockArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// channels that the register-resident variants take
+constexpr int kMapChannels = 2048, kRowChannels = 16384;
+
 size_t block_norm_ws_floats(const BlockArgs& a) {
-  // partials of the parameters and of an image gate (interleaved where an image has
-  // kInterleave tiles, of 16 positions at least), or six numbers a position
+  const bool rows = a.layout == DCN_NHWC || a.P == 1;  // a one-position map is a row
+  // six numbers a position for the passes, or partials of the parameters and of an image gate
+  // (interleaved where an image has kInterleave tiles, of 16 positions at least)
+  if (a.C > (rows ? kRowChannels : kMapChannels)) return 6 * (size_t)a.B * a.P;
   size_t partials = (size_t)kMaxWgs * 5 * a.C;
   if (a.gate_kind == DCN_GATE_IMAGE)
     partials += (kMaxWgs + (size_t)a.B * (a.P > 16 * (kInterleave - 1) ? kInterleave : 1)) * a.C;
-  return std::max(6 * (size_t)a.B * a.P, partials);
+  return partials;
 }
 
 hipError_t launch_block_norm_fwd(const BlockArgs& a, hipStream_t s) {
   hipError_t e;
-  const bool rows = a.layout == DCN_NHWC || a.P == 1;  // a one-position map is a row
+  const bool rows = a.layout == DCN_NHWC || a.P == 1;
   if (rows ? block_row_fwd(a, s, &e) : block_map_fwd(a, s, &e)) return e;
   if (!rows) return a.dtype == DCN_BF16 ? any_fwd<bf16_t, 1>(a, s) : any_fwd<float, 1>(a, s);
   return a.dtype == DCN_BF16 ? any_fwd<bf16_t, 64>(a, s) : any_fwd<float, 64>(a, s);
