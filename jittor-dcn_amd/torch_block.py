@@ -51,6 +51,9 @@ def _call(dev: torch.device, name: str, *args):
     with _lock:
         h = _handles.get(idx)
         if h is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"torch_block: make one call on cuda:{idx} before capturing "
+                                   "(the library's handle is created by the first)")
             h = _handles[idx] = rt.Handle(idx)
             h.bound = None
         if h.bound != stream:
@@ -528,7 +531,8 @@ def fp8_pointwise(x, weight):
 
 class Fp8Pointwise(torch.nn.Module):
     """fp8_pointwise with its weight [out, in] (no bias: a norm or a residual scale follows it in
-    a block). serve() replaces the weight by its 8-bit form for inference."""
+    a block). serve() makes inference use the weight's 8-bit form, as it is at that moment, until
+    train(), a move or a load of other weights; call it again after changing the weight."""
 
     def __init__(self, in_channels, out_channels):
         super().__init__()
@@ -545,6 +549,14 @@ class Fp8Pointwise(torch.nn.Module):
         if mode:
             self.weight8 = None
         return super().train(mode)
+
+    def _apply(self, fn, *args, **kw):
+        self.weight8 = None
+        return super()._apply(fn, *args, **kw)
+
+    def _load_from_state_dict(self, *args, **kw):
+        self.weight8 = None
+        super()._load_from_state_dict(*args, **kw)
 
     def forward(self, x):
         if self.weight8 is not None and not (torch.is_grad_enabled() and x.requires_grad):

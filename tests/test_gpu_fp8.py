@@ -221,6 +221,18 @@ def test_only_one_gradient(tb):
     assert torch.equal(torch.autograd.grad(tb.fp8_pointwise(xr, wr), wr, gy)[0], gw)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+def test_few_tokens_equal_many(tb, dt):
+    """The first tokens of a long batch and the same tokens alone: another kernel, which rounds
+    them inside the product; with weights and values that make every partial sum exact."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.randint(-4, 5, (300, 1000), generator=g).to(dt).cuda()
+    w = torch.randint(-2, 3, (130, 1000), generator=g).to(dt).cuda()
+    want = (x.double() @ w.double().t())
+    for n in (1, 2, 15, 16, 17, 32, 33, 64, 65, 300):
+        assert torch.equal(tb.fp8_pointwise(x[:n], w).double(), want[:n].to(dt).double())
+
+
 def test_asymmetric_identity(tb):
     """Each weight row picks one channel: every output element is one input value, so a row, a
     column or an exponent out of place shows at once."""
@@ -252,13 +264,15 @@ def test_channels_last_and_strides(tb, dt):
         assert torch.equal(tb.fp8_pointwise(flat, wt), tb.fp8_pointwise(flat.clone(), w))
 
 
-def test_nan_stays_in_its_row(tb):
-    x, w = make((40, 300), torch.float32, 1), make((90, 300), torch.float32, 2, 0.1)
+@pytest.mark.parametrize("T", [12, 40, 200])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_nan_stays_in_its_row(tb, dt, T):
+    x, w = make((T, 300), dt, 1), make((90, 300), dt, 2, 0.1)
     clean = tb.fp8_pointwise(x, w)
-    x[7, 200], x[20, 3] = float("nan"), float("-inf")
+    x[7, 200], x[10, 3] = float("nan"), float("-inf")
     y = tb.fp8_pointwise(x, w)
-    bad = torch.zeros(40, dtype=torch.bool)
-    bad[7] = bad[20] = True
+    bad = torch.zeros(T, dtype=torch.bool)
+    bad[7] = bad[10] = True
     assert torch.isnan(y[bad]).all() and torch.equal(y[~bad], clean[~bad])
 
 
@@ -349,4 +363,8 @@ def test_refusals_and_modules(tb):
     assert m.weight.grad is not None
     with torch.no_grad():
         assert torch.equal(m.eval().serve()(x), y)
-    assert m.train().weight8 is None
+        m.load_state_dict({"weight": m.weight * 2})
+        assert torch.equal(m(x), y * 2)
+        m.serve().bfloat16()
+        assert m.weight8 is None
+    assert m.eval().serve().train().weight8 is None
