@@ -329,7 +329,9 @@ int dcn_dropout_bwd(dcn_handle* h, const dcn_dropout_desc* d, const void* grad_y
  *   y   = N_pre(out)
  *   N(v) = (v - m) / sqrt(var + eps) · w[c] + b[c];  DCN_NORM_LAYER: m = mean, var =
  *   mean((v - m)²); DCN_NORM_RMS: m = 0, var = mean(v²); DCN_NORM_NONE: N_post(x) = x, and
- *   no y. */
+ *   no y.
+ * A dropped element adds nothing to any gradient, whatever x and the gate hold there; with
+ * drop_image a dropped image's x and gate are not read at all and their gradients are 0. */
 typedef enum { DCN_NORM_NONE = 0, DCN_NORM_RMS = 1, DCN_NORM_LAYER = 2 } dcn_norm_kind;
 /* DCN_GATE_FULL: a gate of x's shape; DCN_GATE_IMAGE: gate[B][C], one per image and channel */
 typedef enum { DCN_GATE_NONE = 0, DCN_GATE_FULL = 1, DCN_GATE_IMAGE = 2 } dcn_gate_kind;

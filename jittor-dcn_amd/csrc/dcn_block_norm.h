@@ -8,6 +8,8 @@
 //   dt = keep ? G · drop scale : 0
 //   ∂gate = dt · N_post(x) · alpha · scale · act'(gate),  ∂scale = Σ dt · N_post(x) · alpha · act
 //   ∂x = N_post'(dt · alpha · scale · act)
+// What dropout drops reaches no gradient, NaN and infinities neither: x and the gate count as 0
+// in those products (a dropped image's are not even read).
 // out is computed again from x and the residual (the residual is read instead of out, so that
 // costs no bytes), which keeps the backward free of out's rounding. The statistics come from
 // the forward where the caller kept them: 16 bytes a position, against two of the four rounds
@@ -340,6 +342,7 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
   struct Raw {
     u32x4 x[CPT], r[CPT], g[CPT], y[CPT], o[CPT];
     float st[Sums::KEPT];
+    bool gone;  // the image is dropped
   } nx;
   const size_t rows = (size_t)a.B * a.P;
   auto load = [&](long t, Raw& w) {
@@ -349,13 +352,15 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
                  a.P - (int)(t % q.tpi) * TP, w.st);
     const size_t base = (size_t)(t / q.tpi) * a.C * a.P + p;
     const u32x4 zero = {0u, 0u, 0u, 0u};
+    w.gone = false;
+    if constexpr (DROP) w.gone = a.drop_image && !keep1(t / q.tpi, key, a.drop.thr);
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
       const bool ok = inc[i] && valid > 0;
       const size_t at = base + (size_t)(cg + CG * i) * a.P;
-      w.x[i] = ok && xp ? ldv_raw(xp + at, valid) : zero;
+      w.x[i] = ok && xp && !w.gone ? ldv_raw(xp + at, valid) : zero;
       w.r[i] = ok && rp ? ldv_raw(rp + at, valid) : zero;
-      if constexpr (FULL) w.g[i] = ok ? ldv_raw(gp + at, valid) : zero;
+      if constexpr (FULL) w.g[i] = ok && !w.gone ? ldv_raw(gp + at, valid) : zero;
       if constexpr (BWD) {
         w.y[i] = ok && a.gy ? ldv_raw(static_cast<const T*>(a.gy) + at, valid) : zero;
         w.o[i] = ok && a.go ? ldv_raw(static_cast<const T*>(a.go) + at, valid) : zero;
@@ -382,17 +387,21 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
     for (int i = 0; i < CPT; ++i) {
       gv[i] = 1.f;
       gd[i] = 0.f;
-      if (a.gate_kind == DCN_GATE_IMAGE && inc[i])
+      if (a.gate_kind == DCN_GATE_IMAGE && inc[i] && !in.gone)
         gate_act_grad(to_f32(gp[(size_t)b * a.C + cg + CG * i]), a.act, gv[i], gd[i]);
     }
     unsigned keep[CPT];
     if constexpr (DROP) {
-      const unsigned img = a.drop_image && keep1(b, key, a.drop.thr) ? 0xffu : 0u;
+      const unsigned img = in.gone ? 0u : 0xffu;
 #pragma unroll
       for (int i = 0; i < CPT; ++i) keep[i] = a.drop_image ? img : keepv<V>(at[i], key, a.drop.thr);
     }
+    auto kept = [&](int i, int e, float t) {
+      if constexpr (DROP) return (keep[i] >> e) & 1u ? t : 0.f;
+      return t;
+    };
     auto drop = [&](int i, int e, float t) {
-      if constexpr (DROP) return (keep[i] >> e) & 1u ? t * a.drop.scale : 0.f;
+      if constexpr (DROP) return kept(i, e, t * a.drop.scale);
       return t;
     };
 
@@ -400,13 +409,13 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
     const bool known = BWD && a.stats;
     if (known) sums.keep(in.st);
     auto post = [&](float (&m)[V], float (&r)[V]) {
-      if (a.post) {
+      if (a.post && !in.gone) {
         sums.get(0, m);
         sums.get(1, r);
         return;
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) {  // no post norm: N_post(x) = x
+      for (int e = 0; e < V; ++e) {  // no post norm: N_post(x) = x (a dropped image's x is 0)
         m[e] = 0.f;
         r[e] = 1.f;
       }
@@ -515,12 +524,12 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
           if constexpr (FULL) unpack<T>(in.g[i], fv);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float h = (xv[e] - m1[e]) * r1[e], v = fmaf(h, w1[i], b1[i]);
+            const float h = kept(i, e, (xv[e] - m1[e]) * r1[e]), v = fmaf(h, w1[i], b1[i]);
             const float dt = drop(i, e, o[i][e]), dtv = dt * v;
             float dv;
             if constexpr (FULL) {
               float av, ad;
-              gate_act_grad(fv[e], a.act, av, ad);
+              gate_act_grad(kept(i, e, fv[e]), a.act, av, ad);
               dv = dt * (sc[i] * av);
               gg[e] = dtv * (sc[i] * ad);
               acc[0][i] = fmaf(dtv, a.alpha * av, acc[0][i]);
@@ -762,6 +771,7 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
   struct Raw {
     u32x4 x[NV], r[NV], g[NV], y[NV], o[NV];
     float st[4];
+    bool gone;  // the row's image is dropped
   } nx;
   const size_t rows = (size_t)q.images * q.P;
   auto load = [&](long t, Raw& w) {
@@ -772,13 +782,20 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
       for (int k = 0; k < 4; ++k)  // 0 past the last row: nothing there may reach the sums
         w.st[k] = p < q.P ? a.stats[k * rows + (size_t)b * q.P + p] : 0.f;
     }
+    w.gone = false;
+    if constexpr (DROP) {
+      if (a.drop_image) {
+        const int image = q.images == a.B ? b : (int)(((size_t)b * q.P + p) / a.P);
+        w.gone = !keep1(image, key, a.drop.thr);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const bool ok = p < q.P && cv[j] > 0;
       const size_t at = base + (lane + LPR * j) * V;
-      w.x[j] = ok && a.x ? ldv_raw(ptr(a.x) + at, cv[j]) : zero;
+      w.x[j] = ok && a.x && !w.gone ? ldv_raw(ptr(a.x) + at, cv[j]) : zero;
       w.r[j] = ok && a.res ? ldv_raw(ptr(a.res) + at, cv[j]) : zero;
-      if constexpr (FULL) w.g[j] = ok ? ldv_raw(ptr(a.gate) + at, cv[j]) : zero;
+      if constexpr (FULL) w.g[j] = ok && !w.gone ? ldv_raw(ptr(a.gate) + at, cv[j]) : zero;
       if constexpr (BWD) {
         w.y[j] = ok && a.gy ? ldv_raw(ptr(a.gy) + at, cv[j]) : zero;
         w.o[j] = ok && a.go ? ldv_raw(ptr(a.go) + at, cv[j]) : zero;
@@ -796,15 +813,18 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
 
     unsigned keep[NV];
     if constexpr (DROP) {
-      const int image = q.images == a.B ? b : (int)(((size_t)b * q.P + p) / a.P);
-      const unsigned img = a.drop_image && keep1(image, key, a.drop.thr) ? 0xffu : 0u;
+      const unsigned img = in.gone ? 0u : 0xffu;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         keep[j] = a.drop_image ? img
                                : keepv<V>(base + (lane + LPR * j) * V, key, a.drop.thr);
     }
+    auto kept_or_0 = [&](int j, int e, float v) {
+      if constexpr (DROP) return (keep[j] >> e) & 1u ? v : 0.f;
+      return v;
+    };
     auto drop = [&](int j, int e, float v) {
-      if constexpr (DROP) return (keep[j] >> e) & 1u ? v * a.drop.scale : 0.f;
+      if constexpr (DROP) return kept_or_0(j, e, v * a.drop.scale);
       return v;
     };
     // the gate's value and slope; an image's gate is read here (the same row for all positions)
@@ -812,13 +832,17 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
       float f[V];
       if constexpr (FULL) {
         unpack<T>(in.g[j], f);
+        if constexpr (BWD) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) f[e] = kept_or_0(j, e, f[e]);
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           av[e] = 1.f;
           ad[e] = 0.f;
         }
-        if (a.gate_kind == DCN_GATE_NONE || cv[j] <= 0) return;
+        if (a.gate_kind == DCN_GATE_NONE || cv[j] <= 0 || in.gone) return;
         ldv(ptr(a.gate) + (size_t)b * a.C + (lane + LPR * j) * V, cv[j], f);
       }
 #pragma unroll
@@ -842,6 +866,10 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) unpack<T>(in.x[j], xv[j]);
         sums.moments(xv, a.post, a.eps1, live, m1, r1);
+      }
+      if (in.gone) {
+        m1 = 0.f;
+        r1 = 1.f;
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -941,7 +969,7 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
           gate(j, av, ad);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float h = (xv[e] - m1) * r1, v = fmaf(h, w1[e], b1[e]);
+            const float h = kept_or_0(j, e, (xv[e] - m1) * r1), v = fmaf(h, w1[e], b1[e]);
             const float dt = drop(j, e, o[j][e]), dtv = dt * v, k = a.alpha * sc[e];
             const float dv = dt * (k * av[e]);
             gg[e] = dtv * (k * ad[e]);

@@ -27,20 +27,21 @@ struct Pos {
   }
   __device__ float ld(const void* t, size_t i) const { return to_f32(static_cast<const T*>(t)[i]); }
   __device__ float par(const void* t, int c, float none) const { return t ? ld(t, c) : none; }
-  __device__ float x(int c) const { return ld(a.x, base + c * cs); }
+  __device__ float x(int c) const { return drop_all ? 0.f : ld(a.x, base + c * cs); }
   __device__ float h1(int c) const { return (x(c) - m1) * r1; }
   __device__ float v(int c) const {
     return a.post ? h1(c) * par(a.w1, c, 1.f) + par(a.b1, c, 0.f) : x(c);
   }
   __device__ float gate(int c) const {
-    return ld(a.gate, a.gate_kind == DCN_GATE_FULL ? base + c * cs : (size_t)b * a.C + c);
+    return drop_all ? 0.f : ld(a.gate, a.gate_kind == DCN_GATE_FULL ? base + c * cs : (size_t)b * a.C + c);
   }
   __device__ float act(int c) const { return a.gate_kind ? gate_act(gate(c), a.act) : 1.f; }
   __device__ float k(int c) const { return a.alpha * par(a.scale, c, 1.f) * act(c); }
+  __device__ bool kept(int c) const {
+    return !a.drop.thr || (a.drop_image ? !drop_all : keep1(base + c * cs, key, a.drop.thr));
+  }
   __device__ float drop(float t, int c) const {
-    if (!a.drop.thr) return t;
-    const bool keep = a.drop_image ? !drop_all : keep1(base + c * cs, key, a.drop.thr);
-    return keep ? t * a.drop.scale : 0.f;
+    return kept(c) ? (a.drop.thr ? t * a.drop.scale : t) : 0.f;
   }
   __device__ float out(int c) const {
     const float r = a.res ? ld(a.res, base + c * cs) : 0.f;
@@ -81,7 +82,7 @@ __device__ __forceinline__ void pos_moments(Pos<T>& q, int lane, size_t row, boo
   const BlockArgs& a = q.a;
   const size_t rows = (size_t)a.B * a.P;
   if (known) {
-    if (a.x && a.post) {
+    if (a.x && a.post && !q.drop_all) {
       q.m1 = a.stats[row];
       q.r1 = a.stats[rows + row];
     }
@@ -91,7 +92,7 @@ __device__ __forceinline__ void pos_moments(Pos<T>& q, int lane, size_t row, boo
     }
     return;
   }
-  if (a.x && a.post)
+  if (a.x && a.post && !q.drop_all)
     moments<LP>([&](int c) { return q.x(c); }, lane, a.C, a.post, a.eps1, q.m1, q.r1);
   if (a.pre) moments<LP>([&](int c) { return q.out(c); }, lane, a.C, a.pre, a.eps2, q.m2, q.r2);
 }
@@ -150,7 +151,9 @@ __global__ __launch_bounds__(kThreads) void block_any_bwd(BlockArgs a) {
     float s3 = 0.f, s4 = 0.f;
     if (a.x && a.post) {
       for (int c = lane; c < a.C; c += LP) {
-        const float w = q.drop(total(c), c) * q.k(c) * q.par(a.w1, c, 1.f);
+        if (!q.kept(c)) continue;
+        const float g = total(c), dt = a.drop.thr ? g * a.drop.scale : g;
+        const float w = dt * q.k(c) * q.par(a.w1, c, 1.f);
         s3 += w;
         s4 = fmaf(w, q.h1(c), s4);
       }
@@ -162,15 +165,16 @@ __global__ __launch_bounds__(kThreads) void block_any_bwd(BlockArgs a) {
       const float g = total(c);
       if (a.gr) static_cast<T*>(a.gr)[i] = from_f32(g, T());
       if (!a.x) continue;
-      const float dt = q.drop(g, c);
+      const bool kept = q.kept(c);
+      const float dt = a.drop.thr ? g * a.drop.scale : g;
       if (a.gg && a.gate_kind == DCN_GATE_FULL) {
         float av, ad;
         gate_act_grad(q.gate(c), a.act, av, ad);
-        static_cast<T*>(a.gg)[i] =
-            from_f32(dt * q.v(c) * (a.alpha * q.par(a.scale, c, 1.f)) * ad, T());
+        const float gg = dt * q.v(c) * (a.alpha * q.par(a.scale, c, 1.f)) * ad;
+        static_cast<T*>(a.gg)[i] = from_f32(kept ? gg : 0.f, T());
       }
       if (a.gx) {
-        const float dv = dt * q.k(c);
+        const float dv = kept ? dt * q.k(c) : 0.f;
         const float gx =
             a.post ? q.r1 * (dv * q.par(a.w1, c, 1.f) - s3 - q.h1(c) * s4) : dv;
         static_cast<T*>(a.gx)[i] = from_f32(gx, T());
@@ -209,8 +213,8 @@ __global__ __launch_bounds__(kThreads) void block_any_params(BlockArgs a) {
         sum[3] = fmaf(gy, h2, sum[3]);
         sum[4] += gy;
       }
-      if (!a.x) continue;
-      const float dt = q.drop(g, c), v = q.v(c);
+      if (!a.x || !q.kept(c)) continue;
+      const float dt = a.drop.thr ? g * a.drop.scale : g, v = q.v(c);
       float av = 1.f, ad = 0.f;
       if (a.gate_kind) gate_act_grad(q.gate(c), a.act, av, ad);
       sum[0] = fmaf(dt * v, a.alpha * av, sum[0]);

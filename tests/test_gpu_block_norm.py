@@ -238,6 +238,37 @@ def test_zero_rows_and_non_finite(tb, layout):
     assert torch.equal(ro[keep], rc[keep]) and torch.equal(ry[keep], rcy[keep])
 
 
+@pytest.mark.parametrize("drop", ["element", "image"])
+@pytest.mark.parametrize("gate", ["none", "full", "image"])
+@pytest.mark.parametrize("layout,C", [("nchw", 48), ("nchw", 2100), ("rows", 48), ("rows", 3000),
+                                      ("rows", 16500)])
+def test_dropped_values_reach_nothing(tb, layout, C, gate, drop):
+    """NaN and infinities where dropout drops give the bits that zeros there give. (Per element
+    without a norm after the block: with one, a NaN spreads over its position.)"""
+    B, P, p = 4, 6, 0.5
+    post = "layer" if drop == "image" else None
+    t, go, gy = tensors(layout, B, C, P, torch.float32, post, "layer", gate)
+    f = torch.from_numpy(BO.drop_factor(B * C * P, C * P if drop == "image" else 1, p, SEED, OFF))
+    f = f.reshape(B, C, P, 1) if layout == "nchw" else f.reshape(B, P, C)
+    dropped = (f == 0).cuda()
+    assert dropped.any() and not dropped.all()
+    names = ["x"] + (["gate"] if gate == "full" or (gate == "image" and drop == "image") else [])
+    results = []
+    for bad in (0.0, float("nan"), float("-inf")):
+        u = {k: v.clone() for k, v in t.items()}
+        for k in names:
+            m = dropped if u[k].shape == dropped.shape else dropped.flatten(1)[:, :1].expand(B, C)
+            u[k][m] = bad
+        for v in u.values():
+            v.requires_grad_()
+        o, y = call(tb, u, post, "layer", "silu", p=p, drop=drop)
+        results.append([o, y, *torch.autograd.grad((o, y), list(u.values()), (go, gy))])
+    assert all(torch.isfinite(v).all() for v in results[0])
+    for r in results[1:]:
+        for k, a, b in zip(["out", "y", *t], results[0], r):
+            assert torch.equal(a, b), k
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 def test_layouts_and_strides_agree(tb, dt):
     """Channels-last memory, transposed and sliced inputs give the results of dense copies (no
