@@ -91,8 +91,9 @@ int block_geo(const dcn_block_desc* d, dcn::BlockArgs* a) {
   if (!dtype_ok(d->dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
   if (d->layout != DCN_NCHW && d->layout != DCN_NHWC) return fail(DCN_ERR_INVALID, "unknown layout");
   if ((double)d->B * d->C * d->P > (double)(1LL << 40) || (long long)d->B * d->P > (1LL << 34) ||
-      d->C > (1 << 30) || d->P > (1 << 30))
-    return fail(DCN_ERR_UNSUPPORTED, "more than 2^40 elements, 2^34 positions, or C or P above 2^30");
+      d->C > (1 << 23) || d->P > (1 << 30))
+    return fail(DCN_ERR_UNSUPPORTED,
+                "more than 2^40 elements or 2^34 positions, C above 2^23 or P above 2^30");
   for (int k : {d->post, d->pre})
     if (k < DCN_NORM_NONE || k > DCN_NORM_LAYER) return fail(DCN_ERR_INVALID, "unknown norm");
   if (d->gate < DCN_GATE_NONE || d->gate > DCN_GATE_IMAGE)
@@ -138,7 +139,8 @@ struct Span {
   size_t bytes;
 };
 
-// Every output apart from every input and every other output; `same` may equal `inplace` whole.
+// Every output apart from every input and every other output; `inplace_out` may be `inplace_in`,
+// byte for byte.
 int block_spans(const Span* in, int nin, const Span* out, int nout, size_t es,
                 const void* inplace_out, const void* inplace_in) {
   for (int i = 0; i < nin; ++i)
@@ -146,7 +148,8 @@ int block_spans(const Span* in, int nin, const Span* out, int nout, size_t es,
   for (int i = 0; i < nout; ++i) {
     if (!aligned(out[i].p, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
     for (int j = 0; j < nin; ++j) {
-      if (out[i].p && out[i].p == inplace_out && in[j].p == inplace_in && out[i].p == in[j].p)
+      if (out[i].p && out[i].p == inplace_out && in[j].p == inplace_in && out[i].p == in[j].p &&
+          out[i].bytes == in[j].bytes)
         continue;
       if (overlap(out[i].p, out[i].bytes, in[j].p, in[j].bytes))
         return fail(DCN_ERR_INVALID, "an output overlaps an input");
@@ -175,9 +178,11 @@ int fp8_pair(const void* q, const void* s, const char* what) {
   return DCN_OK;
 }
 
-// At most 2^31 - 1 tiles of 128 x 128 (one workgroup each).
+// Below 2^24 tiles of 128 x 128, one workgroup of 256 threads each: a launch takes less than 2^32
+// threads. kMaxSide: the same for 512 threads per 16 rows of a product's long side.
+constexpr int kMaxSide = 1 << 26;
 bool tiles_ok(double a, double b, double images) {
-  return std::ceil(a / 128) * std::ceil(b / 128) * images < 2147483647.0;
+  return std::ceil(a / 128) * std::ceil(b / 128) * images < 16777216.0;
 }
 
 int fp8_matmul_check(const dcn_fp8_matmul_desc* d) {
@@ -190,8 +195,9 @@ int fp8_matmul_check(const dcn_fp8_matmul_desc* d) {
   if (d->layout == DCN_NCHW && (d->P <= 0 || d->N % d->P))
     return fail(DCN_ERR_INVALID, "DCN_NCHW needs N a multiple of P");
   if (!dtype_ok(d->out_dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
-  if (d->M > (1 << 30) || d->N > (1 << 30) || d->K > (1 << 30) || !tiles_ok(d->M, d->N, 1))
-    return fail(DCN_ERR_UNSUPPORTED, "M, N or K above 2^30, or 2^31 tiles of the product");
+  if (d->M > kMaxSide || d->N > kMaxSide || d->K > (1 << 30) || !tiles_ok(d->M, d->N, 1))
+    return fail(DCN_ERR_UNSUPPORTED,
+                "M or N above 2^26, K above 2^30, or 2^24 tiles of 128 x 128 of the product");
   return DCN_OK;
 }
 
@@ -219,7 +225,7 @@ int pointwise(const dcn_fp8_pointwise_desc* d, int grads, Pointwise* p) {
   p->op = up128(d->O);
   p->kt = maps ? d->B * up128(d->P) : up128(p->T);
   const double widest = std::max(d->C, d->O);
-  if (p->T > (1u << 30) || p->kt > (1u << 30) || widest > (1 << 30) ||
+  if (p->T > kMaxSide || p->kt > (1u << 30) || widest > kMaxSide ||
       !tiles_ok(maps ? widest : (double)p->T, maps ? d->P : widest, maps ? d->B : 1) ||
       !tiles_ok(d->O, d->C, 1) || !tiles_ok((double)p->T, widest, 1))
     return fail(DCN_ERR_UNSUPPORTED, "tensor too large");

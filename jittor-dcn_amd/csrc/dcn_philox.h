@@ -69,14 +69,6 @@ __device__ __forceinline__ bool keep1(uint64_t draw, const PhiloxKey& k, unsigne
   return (keep8(draw >> 3, k, thr) >> (draw & 7)) & 1u;
 }
 
-// bit j = element i + j is kept, for the eight elements from any i
-__device__ __forceinline__ unsigned keep8_from(uint64_t i, const PhiloxKey& k, unsigned thr) {
-  const unsigned s = (unsigned)(i & 7);
-  unsigned m = keep8(i >> 3, k, thr) >> s;
-  if (s) m |= keep8((i >> 3) + 1, k, thr) << (8 - s);
-  return m;
-}
-
 // Vectors of 16 bytes at any element alignment: global memory takes unaligned accesses, so rows
 // of odd length and sliced tensors need no scalar path (only their last partial vector does).
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));

@@ -105,7 +105,9 @@ FAR = OK_PTR * 100
     (dict(), dict(y=OK_PTR * 2), "overlaps"), (dict(), dict(y=OK_PTR * 3 + 380), "two outputs"),
     (dict(), dict(w_pre=OK_PTR * 4), "overlaps"),
     (dict(B=1 << 20, C=1 << 20, P=2), {}, "2\\^40"), (dict(P=(1 << 30) + 1, C=1, B=1), {}, "2\\^30"),
-    (dict(P=1, C=(1 << 30) + 1, B=1), {}, "2\\^30"),
+    (dict(P=1, C=(1 << 23) + 1, B=1), {}, "2\\^23"),
+    (dict(gate=2, P=6), dict(gate=OK_PTR * 2, out=OK_PTR * 2), "overlaps"),
+    (dict(gate=1), dict(gate=OK_PTR * 2, out=OK_PTR * 2), "null handle"),
     (dict(), {}, "null handle"), (dict(), dict(out=OK_PTR * 2), "null handle"),
     (dict(post=0), dict(x=None, out=None), "null handle"),
 ])
@@ -212,7 +214,7 @@ def test_fp8_quantize_weight_refusals(kw, msg):
     (dict(a_block=64), {}, "1 or 128"), (dict(b_block=0), {}, "1 or 128"),
     (dict(layout=2), {}, "layout"), (dict(layout=0, P=0), {}, "multiple of P"),
     (dict(layout=0, P=7), {}, "multiple of P"), (dict(out_dtype=9), {}, "dtype"),
-    (dict(M=1 << 30, N=1 << 30), {}, "2^31 tiles"),
+    (dict(M=1 << 26, N=1 << 26), {}, "2^24 tiles"), (dict(M=(1 << 26) + 1, N=1), {}, "2^26"),
     (dict(), dict(a=None), "null tensor"), (dict(), dict(sb=None), "come together"),
     (dict(), dict(b=A * 3 + 4), "16-byte"), (dict(), dict(sa=A * 2 + 1), "4-byte"),
     (dict(), dict(out=A * 5 + 2), "aligned"), (dict(), dict(out=A * 3), "overlaps"),
