@@ -11,6 +11,10 @@ a dense layout where they have another), and has no CPU fallback.
 Random numbers are arguments: `rng` is (seed, offset), or an int64 CUDA tensor of those two
 that is read when the kernel runs (a captured graph then draws a new mask per replay when the
 tensor is updated between replays). The backward draws the same mask again.
+
+Forward and backward may be captured into a graph. As with every torch operator, let go of the
+results of earlier eager passes over the same leaf tensors (and of their losses) first: a leaf's
+accumulation node lives as long as a graph that holds it and stays on the stream it was made on.
 """
 from __future__ import annotations
 
@@ -117,9 +121,15 @@ def _fresh_rng(rng):
     return int(torch.randint(1 << 62, ()).item()), 0
 
 
+def _ints(what, *sizes):
+    """The entry points count in 32-bit integers."""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError(f"{what}: a size above 2^31 - 1")
+
+
 # ---------------------------------------------------------------------------- dropout
 def _drop(x, residual, p, rng, group):
-    seed, offset, dev_rng = _rng(rng, x.device, "dropout")
+    seed, offset, dev_rng = _rng(rng, x.device, "dropout") if p > 0 else (0, 0, None)
     d = rt.DropoutDesc(x.numel(), group, seed, offset, _DT[x.dtype], p)
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None
@@ -204,14 +214,19 @@ _ACT = {"linear": rt.DCN_ACT_LINEAR, "sigmoid": rt.DCN_ACT_SIGMOID, "silu": rt.D
 def _layout(x):
     """(layout, B, C, P, memory format) of a map tensor: [B, C, H, W] (channels-last memory
     stays channels-last) or token rows [..., C]."""
+    if x.dim() == 0 or x.shape[1 if x.dim() == 4 else -1] == 0:
+        raise ValueError("torch_block: a tensor without channels")
     if x.dim() == 4:
         B, C, H, W = x.shape
+        _ints("a map tensor", B, C, H * W)
         if not x.is_contiguous() and x.is_contiguous(memory_format=torch.channels_last):
             return rt.DCN_NHWC, B, C, H * W, torch.channels_last
         return rt.DCN_NCHW, B, C, H * W, torch.contiguous_format
     C = x.shape[-1]
     B = x.shape[0] if x.dim() > 2 else 1
-    return rt.DCN_NHWC, B, C, x.numel() // max(B * C, 1), torch.contiguous_format
+    P = x.numel() // max(B * C, 1)
+    _ints("token rows", B, C, P)
+    return rt.DCN_NHWC, B, C, P, torch.contiguous_format
 
 
 def _block(tensors, desc, mf, dev_rng, keep=False):
@@ -288,8 +303,6 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     if drop not in ("element", "image") or not 0.0 <= drop_p <= 1.0:
         raise ValueError("block_norm: drop is 'element' or 'image' and 0 <= drop_p <= 1")
     layout, B, C, P, mf = _layout(ref)
-    if ref.dim() == 0 or C == 0:
-        raise ValueError("block_norm: no channels")
     kind = rt.DCN_GATE_NONE
     if gate is not None:
         image = gate.dim() == 2 and tuple(gate.shape) == (B, C) and gate.shape != ref.shape
@@ -394,6 +407,7 @@ def fp8_quantize_weight(w):
         w = w.flatten(1)
     if w.dim() != 2 or not w.numel():
         raise ValueError(f"fp8_quantize_weight: a weight is [O, C], not {tuple(w.shape)}")
+    _ints("fp8_quantize_weight", *w.shape)
     q, e, _, _ = _quantize_weight(w.detach(), True, False)
     return Fp8Weight(q, e, w.shape[1])
 
@@ -433,6 +447,7 @@ def fp8_matmul(a, a_exponents, b, b_exponents, dtype=torch.float32):
         blocks.append(shape[tuple(e.shape)])
     if b.device != a.device or not a.numel() or not b.numel():
         raise ValueError("fp8_matmul: non-empty operands on one device")
+    _ints("fp8_matmul", a.shape[0], b.shape[0], K)
     a, a_exponents, b, b_exponents = (_at16(t) for t in (a, a_exponents, b, b_exponents))
     out = torch.empty((a.shape[0], b.shape[0]), dtype=dtype, device=a.device)
     d = rt.Fp8MatmulDesc(a.shape[0], b.shape[0], K, *blocks, rt.DCN_NHWC, 0, _DT[dtype])
@@ -502,8 +517,6 @@ def fp8_pointwise(x, weight):
     dt = _dtype(x, "fp8_pointwise")
     geo = _layout(x)
     C = geo[2]
-    if x.dim() == 0 or C == 0:
-        raise ValueError("fp8_pointwise: no channels")
     if isinstance(weight, Fp8Weight):
         if weight.in_features != C or weight.q.device != x.device:
             raise ValueError(f"fp8_pointwise: the weight takes {weight.in_features} channels on "
@@ -518,6 +531,7 @@ def fp8_pointwise(x, weight):
         _same(x, weight, "fp8_pointwise", "weight", (O, C))
         if O == 0:
             raise ValueError("fp8_pointwise: no output channels")
+    _ints("fp8_pointwise", O)
     if not x.numel():  # no tokens
         shape = (x.shape[0], O, *x.shape[2:]) if x.dim() == 4 else (*x.shape[:-1], O)
         y = x.new_empty(shape)
@@ -531,8 +545,9 @@ def fp8_pointwise(x, weight):
 
 class Fp8Pointwise(torch.nn.Module):
     """fp8_pointwise with its weight [out, in] (no bias: a norm or a residual scale follows it in
-    a block). serve() makes inference use the weight's 8-bit form, as it is at that moment, until
-    train(), a move or a load of other weights; call it again after changing the weight."""
+    a block). serve() makes calls that want no gradient use the weight's 8-bit form, as it is at
+    that moment, until train(), a move or a load of other weights; call it again after changing
+    the weight. A call that wants a gradient, of x or of the weight, rounds the weight itself."""
 
     def __init__(self, in_channels, out_channels):
         super().__init__()
@@ -559,7 +574,7 @@ class Fp8Pointwise(torch.nn.Module):
         super()._load_from_state_dict(*args, **kw)
 
     def forward(self, x):
-        if self.weight8 is not None and not (torch.is_grad_enabled() and x.requires_grad):
+        if self.weight8 is not None and not _wants_grad(x, self.weight):
             return fp8_pointwise(x, self.weight8)
         return fp8_pointwise(x, self.weight)
 

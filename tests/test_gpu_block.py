@@ -175,3 +175,37 @@ def test_short_training_runs(tb):
         for n, p in net.named_parameters():
             assert p.grad is not None and bool(torch.isfinite(p.grad).all()), n
         opt.step()
+
+
+def test_captured_training_step(tb):
+    """The block's second half (join, channel MLP, leave) captured forward and backward in one
+    graph: every replay gives the eager step's bits, with the rng tensors' masks of the moment."""
+    m = make_block(tb, 32, torch.float32, 0.5)
+    x, h, g = (torch.randn(6, 32, 9, 7, device="cuda") for _ in range(3))
+    h.requires_grad_()
+    leaves = [h, *(p for k in ("join", "fc1", "fc2", "leave") for p in getattr(m, k).parameters())]
+
+    def step():
+        x1, y = m.join(h, x)
+        out = m.leave(m.fc2(m.act(m.fc1(y))), x1)[0]
+        return [out.detach(), *torch.autograd.grad(out, leaves, g)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    seen = []
+    for off in (5, 11, 23, 5):
+        for r in (m.join.rng, m.leave.rng):
+            r[1] = off
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), off
+        seen.append(got[0].clone())
+    assert torch.equal(seen[0], seen[3])
+    assert not (torch.equal(seen[0], seen[1]) and torch.equal(seen[0], seen[2]))

@@ -339,6 +339,91 @@ def test_bitwise_reproducible_and_graph(tb, layout):
             assert torch.equal(u, w) and torch.equal(v, w)
 
 
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+def test_more_than_2_31_elements(tb, layout):
+    """The last image of a large tensor gives the bits that it gives alone; its mask, drawn once per
+    image with p = 1/2, is an exact factor 2."""
+    B, C, P = 4, 256, 2_100_003
+    shape = (B, C, P, 1) if layout == "nchw" else (B, P, C)
+    assert B * C * P > 2 ** 31
+    make = lambda *s: torch.randn(s, device="cuda", dtype=torch.bfloat16)
+    t = {"x": make(*shape), "residual": make(*shape), "gate": make(*shape)}
+    vec = {"w_post": make(C), "w_pre": make(C)}
+    g = make(*shape)
+    seed = next(s for s in range(100) if BO.drop_factor(4, 1, 0.5, s, OFF)[3] > 0)
+
+    def step(t, g, **kw):
+        for v in t.values():
+            v.requires_grad_()
+        o, y = call(tb, {**t, **vec}, "rms", "rms", "silu", rng=(seed, OFF), **kw)
+        return [o.detach(), y.detach(), *torch.autograd.grad((o, y), list(t.values()), (g, g))]
+
+    whole = step(t, g, p=0.5, drop="image")
+    last = {k: v.detach()[3:].contiguous() for k, v in t.items()}
+    alone = step(last, g[3:].contiguous(), alpha=2.0)
+    for k, a, b in zip(("out", "y", *t), whole, alone):
+        assert torch.equal(a[3:], b), k
+
+
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+def test_image_gate_sums_over_2_31_elements(tb, layout):
+    """Small integers: every partial sum is exact in fp32, the result is rounded once."""
+    B, C, P = 3, 260, 2_800_001
+    shape = (B, C, P, 1) if layout == "nchw" else (B, P, C)
+    assert B * C * P > 2 ** 31
+    ints = lambda n, *s: torch.randint(-n, n + 1, s, device="cuda", dtype=torch.int8).bfloat16()
+    x, go, gate = ints(2, *shape), ints(1, *shape), ints(3, B, C).requires_grad_()
+    out, _ = tb.block_norm(x, gate=gate)
+    got, = torch.autograd.grad(out, gate, go)
+    dim = 2 if layout == "nchw" else 1
+    for b in range(B):
+        want = sum((x[b:b + 1].narrow(dim, i, min(700_000, P - i)).double() *
+                    go[b:b + 1].narrow(dim, i, min(700_000, P - i)).double()).sum(dim).reshape(C)
+                   for i in range(0, P, 700_000))
+        assert float(want.abs().max()) < 2 ** 24
+        assert torch.equal(got[b], want.bfloat16()), b
+
+
+def test_two_threads_two_streams(tb):
+    """Calls from two threads, each on its own stream, give the bits of one after the other."""
+    import threading
+    sets = []
+    for i in range(2):
+        t, go, gy = tensors("nchw" if i else "rows", 4, 128, 500 + i, torch.bfloat16, "layer",
+                            "rms", "full", seed=i)
+        for v in t.values():
+            v.requires_grad_()
+        sets.append((t, go, gy))
+
+    def step(i):
+        t, go, gy = sets[i]
+        o, y = call(tb, t, "layer", "rms", "silu", p=0.2)
+        return [o.detach(), y.detach(), *torch.autograd.grad((o, y), list(t.values()), (go, gy))]
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got[i] = step(i)
+            s.synchronize()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
+
+
 def test_in_place_out(tb):
     """dcn_block_norm_fwd with out = residual gives the bits of separate tensors."""
     import dcn_runtime as rt

@@ -368,3 +368,38 @@ def test_refusals_and_modules(tb):
         m.serve().bfloat16()
         assert m.weight8 is None
     assert m.eval().serve().train().weight8 is None
+    m.serve()  # a call that wants the weight's gradient gets it
+    m.weight.grad = None
+    m(x.to(m.weight.dtype)).sum().backward()
+    assert m.weight.grad is not None
+    for bad in (x[0, 0], x[:, :0]):
+        with pytest.raises(ValueError):
+            tb.fp8_pointwise(bad, w)
+        with pytest.raises(ValueError):
+            tb.fp8_quantize(bad)
+
+
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+def test_more_than_2_31_elements(tb, layout):
+    """Small integers, so that every product and sum is exact whatever its order."""
+    C, O = 2048, 130
+    n = 1_050_001
+    x = torch.randint(-2, 3, (3, C, 1000, 351) if layout == "nchw" else (n, C), device="cuda",
+                      dtype=torch.int8).float()
+    g = torch.Generator().manual_seed(1)
+    w = torch.randint(-2, 3, (O, C), generator=g).float().cuda()
+    assert x.numel() > 2 ** 31
+    x.requires_grad_(), w.requires_grad_()
+    y = tb.fp8_pointwise(x, w)
+    gy = torch.randint(-1, 2, y.shape, device="cuda", dtype=torch.int8).float()
+    gx, gw = torch.autograd.grad(y, (x, w), gy)
+    tok = lambda t: t.detach().permute(0, 2, 3, 1).flatten(0, 2) if layout == "nchw" else t.detach()
+    x, y, gy, gx, w = tok(x), tok(y), tok(gy), tok(gx), w.detach().double()
+    want = torch.zeros(O, C, dtype=torch.float64, device="cuda")
+    for i in range(0, x.shape[0], 150_000):
+        part = slice(i, i + 150_000)
+        a, b = x[part].double().contiguous(), gy[part].double().contiguous()
+        assert torch.equal(y[part].double(), a @ w.t()), i
+        assert torch.equal(gx[part].double(), b @ w), i
+        want += b.t() @ a
+    assert torch.equal(gw.double(), want)
