@@ -8,7 +8,10 @@
 // Memory is read once: a workgroup holds a 128 x 128 tile in registers (rows r of the tensor's
 // outer axis, columns s of its contiguous one), takes the maxima it needs (per row of the tile
 // for blocks along s, per column for blocks along r, over the tile for weights) and writes the
-// straight bytes from registers, the transposed ones through LDS.
+// straight bytes from registers, the transposed ones through LDS. bf16 values stay in pairs
+// throughout: maxima and conversions take two at a time.
+#include <type_traits>
+
 #include "dcn_block.h"
 #include "dcn_fp8.h"
 
@@ -29,15 +32,36 @@ struct QuantArgs {
   int tiles_s, tiles_r;
 };
 
+// max over aligned groups of LPR (16 or 32) lanes; JOIN: both halves apart, or whole
+template <int LPR, typename F>
+__device__ __forceinline__ unsigned lanes_max(unsigned v, F join) {
+  auto dpp = [](unsigned u, auto ctrl) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)u, decltype(ctrl)::value, 0xf, 0xf, false);
+  };
+  v = join(v, dpp(v, std::integral_constant<int, 0xB1>()));   // quad_perm [1,0,3,2]
+  v = join(v, dpp(v, std::integral_constant<int, 0x4E>()));   // quad_perm [2,3,0,1]
+  v = join(v, dpp(v, std::integral_constant<int, 0x141>()));  // row_half_mirror
+  v = join(v, dpp(v, std::integral_constant<int, 0x140>()));  // row_mirror
+  if constexpr (LPR == 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = join(r[0], r[1]);
+  }
+  return v;
+}
+
 // BLOCK2D: one exponent per tile, for both results (weights)
 template <typename T, bool BLOCK2D>
 __global__ __launch_bounds__(kThreads) void fp8_quantize(QuantArgs a) {
+  using M = Mag<T>;
+  constexpr bool PAIRS = sizeof(T) == 2;
   constexpr int V = ElemVec<T>::N, LPR = 128 / V;     // lanes across a row of the tile
   constexpr int GROUPS = kThreads / LPR;              // row groups of kRows rows at a time
   constexpr int PASS = 128 / (GROUPS * kRows);        // 1 (bf16), 2 (f32)
-  constexpr int PITCH = 136;                          // LDS row: 128 bytes of r, padded
+  // LDS row of the transposed tile: 16 chunks of 8 bytes, chunk c at c ^ 2 ((row >> 4) & 7), rows
+  // padded by 16 bytes: a wave's writes (rows V apart) meet every bank equally often
+  constexpr int PITCH = 144;
   __shared__ __attribute__((aligned(16))) unsigned char tile[128 * PITCH];
-  __shared__ unsigned colmax[GROUPS][128];
+  __shared__ __attribute__((aligned(16))) unsigned colmax[GROUPS][LPR][4];  // as raw: pairs, or one
   const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   const int ts = blockIdx.x % a.tiles_s, tr = (blockIdx.x / a.tiles_s) % a.tiles_r;
   const int img = blockIdx.x / (a.tiles_s * a.tiles_r);
@@ -53,45 +77,72 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize(QuantArgs a) {
       raw[p][i] = r < a.R ? ldv_raw(src + (size_t)r * a.S + s, a.S - s) : u32x4{0u, 0u, 0u, 0u};
     }
 
-  unsigned rowmax[PASS][kRows], cmax[V];
+  unsigned rmax[PASS][kRows], cmax[4];  // this thread's share of rows and columns
+  auto maxima = [&](auto clean) {
+    constexpr bool CLEAN = decltype(clean)::value;
 #pragma unroll
-  for (int j = 0; j < V; ++j) cmax[j] = 0;
+    for (int j = 0; j < 4; ++j) cmax[j] = 0;
 #pragma unroll
-  for (int p = 0; p < PASS; ++p)
+    for (int p = 0; p < PASS; ++p)
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      float v[V];
-      unpack<T>(raw[p][i], v);
-      unsigned m = 0;
+      for (int i = 0; i < kRows; ++i) {
+        unsigned m[4];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        m = mag_max(m, v[j]);
-        cmax[j] = mag_max(cmax[j], v[j]);
+        for (int j = 0; j < 4; ++j) {
+          m[j] = M::template of<CLEAN>(raw[p][i][j]);
+          cmax[j] = M::join(cmax[j], m[j]);
+        }
+        rmax[p][i] = M::join(M::join(m[0], m[1]), M::join(m[2], m[3]));
       }
-#pragma unroll
-      for (int o = 1; o < LPR; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));
-      rowmax[p][i] = m;
-    }
+  };
+  maxima(std::false_type());
+  if (__any(M::odd(M::join(M::join(cmax[0], cmax[1]), M::join(cmax[2], cmax[3])))))
+    maxima(std::true_type());
+
   if (BLOCK2D || a.qt) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) colmax[grp][lane * V + j] = cmax[j];
+    *reinterpret_cast<u32x4*>(colmax[grp][lane]) = u32x4{cmax[0], cmax[1], cmax[2], cmax[3]};
     __syncthreads();
-    if (threadIdx.x < 128) {
+    if (threadIdx.x < LPR * 4) {
+      unsigned* c = &colmax[0][0][0] + threadIdx.x;
       unsigned m = 0;
-      for (int g = 0; g < GROUPS; ++g) m = max(m, colmax[g][threadIdx.x]);
-      colmax[0][threadIdx.x] = m;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) m = M::join(m, c[g * LPR * 4]);
+      *c = m;
     }
     __syncthreads();
   }
   unsigned whole = 0;
   if (BLOCK2D) {
-    for (int j = threadIdx.x & 63; j < 128; j += 64) whole = max(whole, colmax[0][j]);
+    const unsigned* c = &colmax[0][0][0];
+    for (int j = threadIdx.x & 63; j < LPR * 4; j += 64) whole = M::join(whole, c[j]);
+    if (PAIRS) whole = max(whole >> 16, whole & 0xffffu);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) whole = max(whole, (unsigned)__shfl_xor((int)whole, o));
-    whole = exp_byte(whole);
+    whole = M::exp_byte(whole);
   }
 
   if (a.q) {
+    if constexpr (!BLOCK2D) {  // exponent bytes of the rows into rmax
+#pragma unroll
+      for (int p = 0; p < PASS; ++p) {
+        if constexpr (PAIRS) {  // two rows in one register
+#pragma unroll
+          for (int i = 0; i < kRows; i += 2) {
+            const unsigned x = rmax[p][i], y = rmax[p][i + 1];
+            const unsigned m = lanes_max<LPR>(
+                max2(__builtin_amdgcn_perm(y, x, 0x05040100u), __builtin_amdgcn_perm(y, x, 0x07060302u)),
+                max2);
+            rmax[p][i] = M::exp_byte(m & 0xffffu);
+            rmax[p][i + 1] = M::exp_byte(m >> 16);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kRows; ++i)
+            rmax[p][i] = M::exp_byte(lanes_max<LPR>(
+                rmax[p][i], [](unsigned u, unsigned v) { return max(u, v); }));
+        }
+      }
+    }
     const size_t k = (size_t)img * a.kimg + s;  // the row's tail up to the next 128 is zeros
 #pragma unroll
     for (int p = 0; p < PASS; ++p)
@@ -99,14 +150,17 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize(QuantArgs a) {
       for (int i = 0; i < kRows; ++i) {
         const int r = r0 + (p * GROUPS + grp) * kRows + i;
         if (r >= a.R) continue;
-        const unsigned e = BLOCK2D ? whole : exp_byte(rowmax[p][i]);
-        const float f = exp_inv(e);
-        float v[V];
-        unpack<T>(raw[p][i], v);
-        unsigned* dst = reinterpret_cast<unsigned*>(a.q + (size_t)r * a.qk + k);
-#pragma unroll
-        for (int j = 0; j < V; j += 4)
-          dst[j / 4] = to_fp8x4(v[j] * f, v[j + 1] * f, v[j + 2] * f, v[j + 3] * f);
+        const unsigned e = BLOCK2D ? whole : rmax[p][i];
+        const float sc = exp_scale(e);
+        const u32x4 v = raw[p][i];
+        unsigned char* dst = a.q + (size_t)r * a.qk + k;
+        if constexpr (PAIRS)
+          *reinterpret_cast<uint2*>(dst) =
+              make_uint2(to_fp8x4(v[0], v[1], sc), to_fp8x4(v[2], v[3], sc));
+        else
+          *reinterpret_cast<unsigned*>(dst) =
+              to_fp8x4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]),
+                       __uint_as_float(v[3]), sc);
         if (!BLOCK2D && lane == 0)
           a.s[(((size_t)img * a.kimg + s0) / 128) * a.sstr + r] = (unsigned char)e;
       }
@@ -115,34 +169,40 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize(QuantArgs a) {
   if (!a.qt) return;  // uniform
 
   float f[V];
+  const u32x4 cm = *reinterpret_cast<const u32x4*>(colmax[0][lane]);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const unsigned e = BLOCK2D ? whole : exp_byte(colmax[0][lane * V + j]);
-    f[j] = exp_inv(e);
+    const unsigned m = PAIRS ? (cm[j / 2] >> (16 * (j & 1))) & 0xffffu : cm[j % 4];
+    const unsigned e = BLOCK2D ? whole : M::exp_byte(m);
+    f[j] = exp_scale(e);
     if (!BLOCK2D && grp == 0 && s + j < a.S)
       a.st[(size_t)tr * a.tstr + (size_t)img * a.S + s + j] = (unsigned char)e;
   }
   if (BLOCK2D && threadIdx.x == 0) a.st[(size_t)tr * a.tstr + ts] = (unsigned char)whole;
 #pragma unroll
-  for (int p = 0; p < PASS; ++p) {
-    float v[kRows][V];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) unpack<T>(raw[p][i], v[i]);
+  for (int p = 0; p < PASS; ++p)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const uint2 b = make_uint2(
-          to_fp8x4(v[0][j] * f[j], v[1][j] * f[j], v[2][j] * f[j], v[3][j] * f[j]),
-          to_fp8x4(v[4][j] * f[j], v[5][j] * f[j], v[6][j] * f[j], v[7][j] * f[j]));
-      *reinterpret_cast<uint2*>(&tile[(lane * V + j) * PITCH + (p * GROUPS + grp) * kRows]) = b;
+      const u32x4(&v)[kRows] = raw[p];
+      uint2 b;
+      if constexpr (PAIRS) {  // column j of two rows, side by side
+        const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
+        auto two = [&](int i) { return __builtin_amdgcn_perm(v[i + 1][j / 2], v[i][j / 2], sel); };
+        b = make_uint2(to_fp8x4(two(0), two(2), f[j]), to_fp8x4(two(4), two(6), f[j]));
+      } else {
+        auto one = [&](int i) { return __uint_as_float(v[i][j % 4]); };
+        b = make_uint2(to_fp8x4(one(0), one(1), one(2), one(3), f[j]),
+                       to_fp8x4(one(4), one(5), one(6), one(7), f[j]));
+      }
+      const int row = lane * V + j, c = (p * GROUPS + grp) ^ (((row >> 4) & 7) << 1);
+      *reinterpret_cast<uint2*>(&tile[row * PITCH + c * 8]) = b;
     }
-  }
   __syncthreads();
   // 8 lanes of 16 bytes a row, 32 rows a pass
   for (int row = threadIdx.x / 8; row < 128 && s0 + row < a.S; row += kThreads / 8) {
-    const unsigned char* t = &tile[row * PITCH + (threadIdx.x % 8) * 16];
-    const uint2 lo = *reinterpret_cast<const uint2*>(t), hi = *reinterpret_cast<const uint2*>(t + 8);
-    *reinterpret_cast<uint4*>(a.qt + ((size_t)img * a.S + s0 + row) * a.tk + r0 +
-                              (threadIdx.x % 8) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    const int c = threadIdx.x % 8;
+    *reinterpret_cast<u32x4*>(a.qt + ((size_t)img * a.S + s0 + row) * a.tk + r0 + c * 16) =
+        *reinterpret_cast<const u32x4*>(&tile[row * PITCH + (c ^ ((row >> 4) & 7)) * 16]);
   }
 }
 
