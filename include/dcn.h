@@ -422,11 +422,13 @@ typedef struct {
 } dcn_fp8_pointwise_desc;
 #define DCN_FP8_GRAD_X 1
 #define DCN_FP8_GRAD_W 2
+#define DCN_FP8_SERVED 8 /* alone: the weight comes in 8 bits, the workspace holds no room for it */
 /* Bytes of the workspaces of the forward and the backward (one per call in flight) and of what
- * the forward leaves for a backward that computes `grads` (DCN_FP8_GRAD_* bits; 0: none). */
+ * the forward leaves for a backward that computes `grads` (DCN_FP8_GRAD_* bits; 0: none). A size
+ * of 0 needs no buffer. */
 int dcn_fp8_pointwise_workspace(const dcn_fp8_pointwise_desc* d, int grads, size_t* fwd_ws,
                                 size_t* saved, size_t* bwd_ws);
-/* w[O][C], or w NULL and its 8-bit form q[O][Cp], s (then grads is 0: a served weight). saved
+/* w[O][C], or w NULL and its 8-bit form q[O][Cp], s (then grads is DCN_FP8_SERVED, or 0). saved
  * holds the 8-bit forms that the backward multiplies: wᵀ for grad_x, x by channel for grad_w
  * (half of keeping bf16 x and w, a quarter of fp32). All buffers 256-byte aligned. */
 int dcn_fp8_pointwise_fwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int grads, const void* x,

@@ -207,6 +207,7 @@ struct Pointwise {
   size_t wq, ws, xq, xs, mm, fwd;             // forward workspace
   size_t wt, wts, xc, xcs, saved;             // saved
   size_t gq, gs, gc, gcs, mmb, bwd;           // backward workspace
+  bool few;
   dcn_fp8_matmul_desc y, gx, gw;
 };
 
@@ -218,7 +219,8 @@ int pointwise(const dcn_fp8_pointwise_desc* d, int grads, Pointwise* p) {
     return fail(DCN_ERR_INVALID, "B, C, P, O must be positive");
   if (!dtype_ok(d->dtype)) return fail(DCN_ERR_INVALID, "unknown dtype");
   if (d->layout != DCN_NCHW && d->layout != DCN_NHWC) return fail(DCN_ERR_INVALID, "unknown layout");
-  if (grads & ~(DCN_FP8_GRAD_X | DCN_FP8_GRAD_W)) return fail(DCN_ERR_INVALID, "unknown gradient");
+  if (grads != DCN_FP8_SERVED && (grads & ~(DCN_FP8_GRAD_X | DCN_FP8_GRAD_W)))
+    return fail(DCN_ERR_INVALID, "unknown gradient");
   const bool maps = d->layout == DCN_NCHW;
   p->T = (size_t)d->B * d->P;
   p->cp = up128(d->C);
@@ -244,11 +246,16 @@ int pointwise(const dcn_fp8_pointwise_desc* d, int grads, Pointwise* p) {
     at += up256(bytes);
     return o;
   };
-  p->wq = take(fp8_bytes(d->O, p->cp));
-  p->ws = take(exp_bytes(d->O, p->cp, 128));
-  p->xq = take(fp8_bytes(p->T, p->cp));
-  p->xs = take(exp_bytes(p->T, p->cp, 1));
-  p->mm = take(dcn::fp8_matmul_ws_bytes(p->y));
+  p->few = !maps && dcn::fp8_few_tokens(p->T);  // rounded inside the product
+  if (grads != DCN_FP8_SERVED) {
+    p->wq = take(fp8_bytes(d->O, p->cp));
+    p->ws = take(exp_bytes(d->O, p->cp, 128));
+  }
+  if (!p->few) {
+    p->xq = take(fp8_bytes(p->T, p->cp));
+    p->xs = take(exp_bytes(p->T, p->cp, 1));
+    p->mm = take(dcn::fp8_matmul_ws_bytes(p->y));
+  }
   p->fwd = at;
   at = 0;
   if (grads & DCN_FP8_GRAD_X) {
@@ -304,15 +311,18 @@ int dcn_fp8_pointwise_fwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int gr
   Pointwise p{};
   if (int rc = pointwise(d, grads, &p)) return rc;
   if (!x || !y || !(w || q)) return fail(DCN_ERR_INVALID, "null tensor");
-  if (w && (q || s)) return fail(DCN_ERR_INVALID, "one weight: as it is or in 8 bits");
+  if (w && (q || s || grads == DCN_FP8_SERVED))
+    return fail(DCN_ERR_INVALID, "one weight: as it is or in 8 bits");
   if (int rc = fp8_pair(q, s, "weight")) return rc;
-  if (q && grads) return fail(DCN_ERR_INVALID, "a weight in 8 bits has no gradients");
+  if (q && grads && grads != DCN_FP8_SERVED)
+    return fail(DCN_ERR_INVALID, "a weight in 8 bits has no gradients");
   if (int rc = buffer_ok(ws, ws_bytes, p.fwd, "pointwise workspace")) return rc;
   if (int rc = buffer_ok(saved, saved_bytes, p.saved, "saved buffer")) return rc;
   const size_t es = dtype_bytes(d->dtype);
   const Span in[] = {{x, p.T * d->C * es}, {w, (size_t)d->O * d->C * es},
                      {q, fp8_bytes(d->O, p.cp)}, {s, exp_bytes(d->O, p.cp, 128)}};
-  const Span out[] = {{y, p.T * d->O * es}, {p.saved ? saved : nullptr, p.saved}, {ws, p.fwd}};
+  const Span out[] = {{y, p.T * d->O * es}, {p.saved ? saved : nullptr, p.saved},
+                      {p.fwd ? ws : nullptr, p.fwd}};
   for (const void* t : {x, w, static_cast<const void*>(y)})
     if (!aligned(t, es)) return fail(DCN_ERR_INVALID, "tensor not aligned to its elements");
   if (int rc = block_spans(in, 4, out, 3, 1, nullptr, nullptr)) return rc;
@@ -327,7 +337,7 @@ int dcn_fp8_pointwise_fwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int gr
     q = b + p.wq;
     s = b + p.ws;
   }
-  const bool maps = d->layout == DCN_NCHW, few = !maps && dcn::fp8_few_tokens(p.T);
+  const bool maps = d->layout == DCN_NCHW, few = p.few;
   if (e == hipSuccess && (!few || gw))
     e = dcn::launch_fp8_quantize(d->B, d->C, d->P, d->layout, d->dtype, x, few ? nullptr : b + p.xq,
                                  few ? nullptr : b + p.xs, gw ? k + p.xc : nullptr,

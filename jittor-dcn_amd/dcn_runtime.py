@@ -25,7 +25,7 @@ DCN_FWD_AUTO, DCN_FWD_UNFUSED, DCN_FWD_FUSED, DCN_FWD_FUSED_NOCOL = 0, 1, 2, 3
 DCN_NCHW, DCN_NHWC = 0, 1
 DCN_NORM_NONE, DCN_NORM_RMS, DCN_NORM_LAYER = 0, 1, 2
 DCN_GATE_NONE, DCN_GATE_FULL, DCN_GATE_IMAGE = 0, 1, 2
-DCN_FP8_GRAD_X, DCN_FP8_GRAD_W = 1, 2
+DCN_FP8_GRAD_X, DCN_FP8_GRAD_W, DCN_FP8_SERVED = 1, 2, 8
 DCN_ACT_LINEAR, DCN_ACT_SIGMOID, DCN_ACT_SILU = 0, 1, 2
 DCN_MATH_F32, DCN_MATH_F32_BF16X3, DCN_MATH_F32_BF16X6, DCN_MATH_F32_BF16X9 = 0, 3, 6, 9
 KERNEL_IDS = {

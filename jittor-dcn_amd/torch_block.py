@@ -19,6 +19,7 @@ accumulation node lives as long as a graph that holds it and stays on the stream
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 
 import torch
@@ -92,9 +93,9 @@ def _same(x, t, what, name, shape=None):
     """t is of x's dtype, on its device, and of `shape` (None: x's)."""
     if t is None:
         return
-    shape = tuple(x.shape if shape is None else shape)
-    if t.dtype != x.dtype or t.device != x.device or tuple(t.shape) != shape:
-        raise ValueError(f"{what}: {name} must be {shape} {x.dtype} on {x.device}, not "
+    shape = x.shape if shape is None else shape
+    if t.shape != shape or t.dtype != x.dtype or t.device != x.device:
+        raise ValueError(f"{what}: {name} must be {tuple(shape)} {x.dtype} on {x.device}, not "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
 
 
@@ -229,21 +230,41 @@ def _layout(x):
     return rt.DCN_NHWC, B, C, P, torch.contiguous_format
 
 
+@functools.lru_cache(maxsize=1024)
+def _block_desc(*fields):
+    """The descriptor of a call without dropout (not written to by anyone)."""
+    return rt.BlockDesc(*fields)
+
+
+@functools.lru_cache(maxsize=1024)
+def _block_ws(*geometry):
+    """Bytes of workspace of a backward, by the descriptor's fields up to `gate`."""
+    nbytes = ctypes.c_size_t()
+    rt.check(_fn("dcn_block_norm_workspace")(rt.BlockDesc(*geometry), nbytes),
+             "dcn_block_norm_workspace")
+    return nbytes.value
+
+
+def _dense(t, mf):
+    return t if t is None else t.contiguous(memory_format=mf)
+
+
 def _block(tensors, desc, mf, dev_rng, keep=False):
     """(out, y), the dense tensors behind them and, with keep, the norms' statistics."""
-    x, residual, gate = tensors[:3]
-    full = (True, True, desc.gate == rt.DCN_GATE_FULL)
-    tensors = [t if t is None else t.contiguous(memory_format=mf) if i < 3 and full[i]
-               else t.contiguous() for i, t in enumerate(tensors)]
-    x, ref = tensors[0], tensors[1] if tensors[0] is None else tensors[0]
-    out = torch.empty_like(x, memory_format=mf) if x is not None else None
-    y = torch.empty_like(ref, memory_format=mf) if desc.pre else None
+    x, residual, gate, *vectors = tensors
+    x, residual = _dense(x, mf), _dense(residual, mf)
+    gate = _dense(gate, mf if desc.gate == rt.DCN_GATE_FULL else torch.contiguous_format)
+    tensors = (x, residual, gate, *[t if t is None else t.contiguous() for t in vectors])
+    ref = residual if x is None else x
+    out = None if x is None else torch.empty_like(x)  # as dense as x: in its memory format
+    y = torch.empty_like(ref) if desc.pre else None
     stats = None
     if ref.numel():
         if keep and (desc.post or desc.pre):
             stats = torch.empty(4 * desc.B * desc.P, dtype=torch.float32, device=ref.device)
         _call(ref.device, "dcn_block_norm_fwd", desc,
-              rt.BlockIO(*map(_ptr, (*tensors, dev_rng, out, y)), stats=_ptr(stats)))
+              rt.BlockIO(*[t if t is None else t.data_ptr()
+                           for t in (*tensors, dev_rng, out, y)], stats=_ptr(stats)))
     return out, y, tensors, stats
 
 
@@ -251,10 +272,7 @@ class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, desc, mf, dev_rng, *tensors):
         out, y, tensors, stats = _block(tensors, desc, mf, dev_rng, keep=True)
-        nbytes = ctypes.c_size_t()
-        if out is not None and out.numel() or y is not None and y.numel():
-            rt.check(_fn("dcn_block_norm_workspace")(desc, nbytes), "dcn_block_norm_workspace")
-        ctx.desc, ctx.mf, ctx.ws_bytes = desc, mf, nbytes.value
+        ctx.desc, ctx.mf = desc, mf
         ctx.save_for_backward(*tensors, dev_rng, stats)
         ctx.set_materialize_grads(False)
         return out, y
@@ -266,16 +284,18 @@ class _BlockNorm(torch.autograd.Function):
         need = ctx.needs_input_grad[3:]
         if grad_out is None and grad_y is None:
             return (None,) * 11
-        full = lambda t: None if t is None else t.contiguous(memory_format=ctx.mf)
-        grad_out, grad_y = full(grad_out), full(grad_y)
+        mf, d = ctx.mf, ctx.desc
+        grad_out, grad_y = _dense(grad_out, mf), _dense(grad_y, mf)
         ref = inputs[0] if inputs[0] is not None else inputs[1]
         if not ref.numel():
             return (None, None, None,
                     *(torch.zeros_like(t) if n else None for t, n in zip(inputs, need)))
         grads = [torch.empty_like(t) if n else None for t, n in zip(inputs, need)]
-        ws = _bytes(ref.device, ctx.ws_bytes)
-        io = rt.BlockIO(*map(_ptr, (*inputs, dev_rng, None, None, grad_out, grad_y, *grads, stats)))
-        _call(ref.device, "dcn_block_norm_bwd", ctx.desc, io, ws.data_ptr(), ctx.ws_bytes)
+        nbytes = _block_ws(d.B, d.C, d.P, d.layout, d.dtype, d.post, d.pre, d.gate)
+        ws = _bytes(ref.device, nbytes)
+        io = rt.BlockIO(*[t if t is None else t.data_ptr() for t in (
+            *inputs, dev_rng, None, None, grad_out, grad_y, *grads, stats)])
+        _call(ref.device, "dcn_block_norm_bwd", d, io, ws.data_ptr(), nbytes)
         return (None, None, None, *grads)
 
 
@@ -310,13 +330,20 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
         _same(ref, gate, "block_norm", "gate", (B, C) if image else None)
     if x is not None:
         _same(x, residual, "block_norm", "residual")
-    for name, t in (("scale", scale), ("post_weight", post_weight), ("post_bias", post_bias),
-                    ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
-        _same(ref, t, "block_norm", name, (C,))
+    shape = (C,)
+    _same(ref, scale, "block_norm", "scale", shape)
+    _same(ref, post_weight, "block_norm", "post_weight", shape)
+    _same(ref, post_bias, "block_norm", "post_bias", shape)
+    _same(ref, pre_weight, "block_norm", "pre_weight", shape)
+    _same(ref, pre_bias, "block_norm", "pre_bias", shape)
     e1, e2 = eps if isinstance(eps, (tuple, list)) else (eps, eps)
-    seed, offset, dev_rng = _rng(rng, ref.device, "block_norm") if drop_p > 0 else (0, 0, None)
-    desc = rt.BlockDesc(B, C, P, layout, dt, _NORM[post], _NORM[pre], kind, _ACT[gate_act], e1, e2,
-                        alpha, drop_p, int(drop == "image"), seed, offset)
+    fields = (B, C, P, layout, dt, _NORM[post], _NORM[pre], kind, _ACT[gate_act], e1, e2, alpha)
+    dev_rng = None
+    if drop_p > 0:
+        seed, offset, dev_rng = _rng(rng, ref.device, "block_norm")
+        desc = rt.BlockDesc(*fields, drop_p, int(drop == "image"), seed, offset)
+    else:
+        desc = _block_desc(*fields)
     tensors = (x, residual, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
     if _wants_grad(*tensors):
         out, y = _BlockNorm.apply(desc, mf, dev_rng, *tensors)
@@ -459,26 +486,32 @@ def fp8_matmul(a, a_exponents, b, b_exponents, dtype=torch.float32):
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _pointwise_plan(B, C, P, O, layout, dtype, grads):
+    """Descriptor and buffer sizes (forward workspace, kept, backward workspace) of a product."""
+    d = rt.Fp8PointwiseDesc(B, C, P, O, layout, dtype)
+    n = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
+    rt.check(_fn("dcn_fp8_pointwise_workspace")(d, grads, *n), "dcn_fp8_pointwise_workspace")
+    return d, *(v.value for v in n)
+
+
 def _pointwise(x, w, kept, geo, grads):
     """(y, what the backward needs) of x and a weight w [O, C] or an Fp8Weight `kept`."""
     layout, B, C, P, mf = geo
-    x = x.contiguous(memory_format=mf)
+    x, dev = x.contiguous(memory_format=mf), x.device
     O = kept.out_features if w is None else w.shape[0]
     w = None if w is None else w.contiguous()
-    d = rt.Fp8PointwiseDesc(B, C, P, O, layout, _DT[x.dtype])
-    n_ws, n_saved, n_bwd = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
-    rt.check(_fn("dcn_fp8_pointwise_workspace")(d, grads, n_ws, n_saved, n_bwd),
-             "dcn_fp8_pointwise_workspace")
+    d, n_ws, n_saved, n_bwd = _pointwise_plan(B, C, P, O, layout, _DT[x.dtype], grads)
     if x.dim() == 4:
-        y = torch.empty((B, O, *x.shape[2:]), dtype=x.dtype, device=x.device, memory_format=mf)
+        y = torch.empty((B, O, *x.shape[2:]), dtype=x.dtype, device=dev, memory_format=mf)
     else:
-        y = torch.empty((*x.shape[:-1], O), dtype=x.dtype, device=x.device)
-    ws = _bytes(x.device, n_ws.value)
-    saved = _bytes(x.device, n_saved.value) if grads else None
+        y = x.new_empty((*x.shape[:-1], O))
+    ws = _bytes(dev, n_ws) if n_ws else None
+    saved = _bytes(dev, n_saved) if n_saved else None
     q, e = (None, None) if kept is None else (kept.q.data_ptr(), kept.exponents.data_ptr())
-    _call(x.device, "dcn_fp8_pointwise_fwd", d, grads, x.data_ptr(), _ptr(w), q, e, y.data_ptr(),
-          _ptr(saved), n_saved.value, ws.data_ptr(), n_ws.value)
-    return y, (d, saved, n_saved.value, n_bwd.value)
+    _call(dev, "dcn_fp8_pointwise_fwd", d, grads, x.data_ptr(), _ptr(w), q, e, y.data_ptr(),
+          _ptr(saved), n_saved, _ptr(ws), n_ws)
+    return y, (d, saved, n_saved, n_bwd)
 
 
 class _Fp8Pointwise(torch.autograd.Function):
@@ -537,7 +570,7 @@ def fp8_pointwise(x, weight):
         y = x.new_empty(shape)
         return y if isinstance(weight, Fp8Weight) else y + 0 * (x.sum() + weight.sum())
     if isinstance(weight, Fp8Weight):
-        return _pointwise(x, None, weight, geo, 0)[0]
+        return _pointwise(x, None, weight, geo, rt.DCN_FP8_SERVED)[0]
     if _wants_grad(x, weight):
         return _Fp8Pointwise.apply(x, weight, geo)
     return _pointwise(x, weight, None, geo, 0)[0]

@@ -250,6 +250,11 @@ def _pointwise(L, fwd, **kw):
     (1, dict(y=A * 3 + 2), "aligned"), (1, dict(ws=A * 3), "two outputs"),
     (1, dict(B=1 << 15, P=1 << 16), "too large"), (1, {}, "null handle"),
     (1, dict(w=None, q=A * 7, s=A * 8), "null handle"),
+    (1, dict(grads=8), "one weight"), (1, dict(grads=9, w=None, q=A * 7, s=A * 8), "unknown"),
+    (1, dict(grads=8, w=None, q=A * 7, s=A * 8, n=100), "too small"),
+    (1, dict(grads=8, w=None, q=A * 7, s=A * 8), "null handle"),
+    (1, dict(grads=8, w=None, q=A * 7, s=A * 8, layout=1, ws=None, n=0), "null handle"),
+    (0, dict(grads=8), "kept nothing"),
     (1, dict(grads=3, saved=A * 9, ns=1 << 19), "null handle"),
     (0, dict(gx=None, gw=None), "null tensor"), (0, dict(gy=None), "null tensor"),
     (0, dict(grads=1), "kept nothing"), (0, dict(ns=4), "saved buffer too small"),
