@@ -54,8 +54,12 @@ __device__ __forceinline__ int slot_row(int slot) {
 __device__ __forceinline__ int exps4(const unsigned char* s, long str, int shift, int kb, int row0,
                                      int r) {
   const unsigned char* p = s + (size_t)kb * str;
-  if (shift) return (int)(p[min((long)(row0 >> shift), str - 1)] * 0x01010101u);
+  if (shift) return (int)p[min((long)(row0 >> shift), str - 1)];  // one for all four: spread()
   return *reinterpret_cast<const int*>(p + min((long)(row0 + 4 * r), str - 4));
+}
+// what exps4 loaded as four bytes (apart from the load, so that the load is waited for here)
+__device__ __forceinline__ int spread(int e, int shift) {
+  return shift ? (int)((unsigned)e * 0x01010101u) : e;
 }
 
 // eight bytes (dwords 2p, 2p + 1 of a fragment) as bf16, with the exponent `e`
@@ -224,9 +228,9 @@ __global__ __launch_bounds__(WM* WN * 64, WPE) void fp8_gemm(GemmArgs g) {
   auto step = [&](int kb, const char* cur, char* other) {
     __syncthreads();  // stage kb and its exponents landed; every wave is done with `other`
 #pragma unroll
-    for (int i = 0; i < GA; ++i) ea[i] = na[i];
+    for (int i = 0; i < GA; ++i) ea[i] = spread(na[i], g.a_shift);
 #pragma unroll
-    for (int j = 0; j < GB; ++j) eb[j] = nb[j];
+    for (int j = 0; j < GB; ++j) eb[j] = spread(nb[j], g.b_shift);
     if (kb + 1 < nkb) {
       exps(kb + 1);
       issue(kb + 1, other);
@@ -244,9 +248,9 @@ __global__ __launch_bounds__(WM* WN * 64, WPE) void fp8_gemm(GemmArgs g) {
     for (int kb = 0; kb < nkb; ++kb) {
       __syncthreads();  // the stage landed
 #pragma unroll
-      for (int i = 0; i < GA; ++i) ea[i] = na[i];
+      for (int i = 0; i < GA; ++i) ea[i] = spread(na[i], g.a_shift);
 #pragma unroll
-      for (int j = 0; j < GB; ++j) eb[j] = nb[j];
+      for (int j = 0; j < GB; ++j) eb[j] = spread(nb[j], g.b_shift);
       compute(ring0);
       if (kb + 1 == nkb) break;
       __syncthreads();  // every wave has read it
@@ -284,6 +288,135 @@ __global__ __launch_bounds__(WM* WN * 64, WPE) void fp8_gemm(GemmArgs g) {
           }
         }
     }
+}
+
+// ---- large tiles, two groups of waves in turn: 256 x 256, eight waves of 128 x 64. Waves 0..3 and
+// 4..7 (one of each on every SIMD) run half a stage apart: while one group's fragments come out of
+// LDS the other multiplies, so the matrix cores never wait for LDS; a barrier ends every half.
+//   phase 2k: group 0 reads stage k, group 1 multiplies stage k - 1; 2k + 1: the other way round.
+// Stage k + 1 replaces stage k - 1, which group 1 has read in phase 2k - 1: both groups fetch their
+// shares from phase 2k on and have waited for them by the end of phase 2k + 1.
+// A128, B128: an exponent per 128 rows (known here, so that the stages have no branches).
+template <bool A128, bool B128>
+__global__ __launch_bounds__(512, 2) void fp8_gemm_turns(GemmArgs g) {
+  constexpr int BM = 256, BN = 256, STAGE = (BM + BN) * 128, PER = STAGE / 1024 / 8;
+  __shared__ __attribute__((aligned(1024))) char ring0[STAGE], ring1[STAGE];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = w & 3;
+  const bool second = w >> 2;  // group, and which half of the rows
+  const int nwg = g.tiles_m * g.tiles_n, bid = blockIdx.x, xcd = bid & 7, q8 = nwg >> 3, r8 = nwg & 7;
+  const int lid = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (bid >> 3);
+  const int width = 8 * g.tiles_n, band = lid / width, in = lid % width;
+  const int rows = min(8, g.tiles_m - band * 8);
+  const int m0 = (band * 8 + in % rows) * BM, n0 = in / rows * BN;
+  const int nkb = g.nkb;
+
+  // Unit u fetches LDS rows 64 u + 8 w ..+ 7 (u < PER / 2: a's, else b's; laid out as in fp8_gemm),
+  // at 64 rows a unit from one lane offset. Through buffer descriptors that end with the matrix:
+  // rows past it read as zeros. (256 rows stay below 2^31 bytes: K <= 2^22.)
+  const auto ra = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(g.a) + (size_t)m0 * g.K, 0, (int)(min(g.M - m0, BM) * g.K), 0x00020000);
+  const auto rb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(g.b) + (size_t)n0 * g.K, 0, (int)(min(g.N - n0, BN) * g.K), 0x00020000);
+  const int t0 = w * 8 + (lane >> 3);
+  const unsigned off = (unsigned)slot_row(t0) * (unsigned)g.K + (((lane & 7) ^ ((t0 >> 1) & 7)) << 4);
+  auto issue = [&](int kb, char* slot) {
+    const int k = min(kb, nkb - 1) * 128;  // (past the end the last once more, unread)
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const unsigned at = off + (unsigned)(u % (PER / 2)) * 64u * (unsigned)g.K;
+      lvoid* to = (lvoid*)(slot + (u * 8 + w) * 1024);
+      if (u < PER / 2)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, to, 16, at, k, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, to, 16, at, k, 0, 0);
+    }
+  };
+  const int r = lane & 15, q = lane >> 4, x = (r >> 1) & 7;
+  const int lo = r * 128 + ((q ^ x) << 4), hi = r * 128 + (((q + 4) ^ x) << 4);
+  auto frag = [&](const char* base, int f) {
+    const i32x4 l = *reinterpret_cast<const i32x4*>(base + f * 2048 + lo);
+    const i32x4 h = *reinterpret_cast<const i32x4*>(base + f * 2048 + hi);
+    return __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  f32x4 acc[2][4][4];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) (&acc[0][0][0])[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int na[2], nb, ea[2], eb;
+  auto exps = [&](int kb) {
+    const int k = min(kb, nkb - 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      na[i] = exps4(g.sa, g.sa_str, A128 ? 7 : 0, k, m0 + (second * 2 + i) * 64, r);
+    nb = exps4(g.sb, g.sb_str, B128 ? 7 : 0, k, n0 + wn * 64, r);
+  };
+  auto landed = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+  auto turn = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto stage = [&](auto group, int kb, char* cur, char* other) {
+    constexpr bool SECOND = decltype(group)::value;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ea[i] = spread(na[i], A128);
+    eb = spread(nb, B128);
+    i32x8 fb[4], fa[2][4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) fb[f] = frag(cur + BM * 128, wn * 4 + f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) fa[i][f] = frag(cur, (SECOND * 2 + i) * 4 + f);
+    __builtin_amdgcn_sched_barrier(0);  // LDS first: the other group's turn waits for it
+    if (!SECOND) issue(kb + 1, other);
+    if (SECOND) landed();
+    exps(kb + 1);
+    turn();
+    if (SECOND) issue(kb + 2, cur);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) quad<false>(fa[i], fb, ea[i], eb, acc[i]);
+    if (!SECOND) landed();
+    turn();
+  };
+  auto stages = [&](auto group) {
+    for (int kb = 0; kb + 1 < nkb; kb += 2) {
+      stage(group, kb, ring0, ring1);
+      stage(group, kb + 1, ring1, ring0);
+    }
+    if (nkb & 1) stage(group, nkb - 1, ring0, ring1);
+  };
+  exps(0);
+  issue(0, ring0);
+  landed();
+  turn();
+  if (second) {
+    issue(1, ring1);
+    turn();
+    stages(std::true_type());
+  } else {
+    stages(std::false_type());
+    turn();
+  }
+  landed();  // nothing may arrive in LDS after the workgroup has ended
+
+#pragma unroll
+  for (int ga = 0; ga < 2; ++ga) {
+    const int n = n0 + wn * 64 + 4 * r;
+    const Column col = column(g, n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int m = m0 + (second * 2 + ga) * 64 + 4 * (4 * q + e) + i;
+        if (m >= g.M || n >= g.N) continue;
+        put4<false>(g, col, m, n, f32x4{acc[ga][i][0][e], acc[ga][i][1][e], acc[ga][i][2][e],
+                                        acc[ga][i][3][e]});
+      }
+  }
 }
 
 // the splits' partials, added in order, four columns a thread
@@ -548,6 +681,20 @@ hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const 
     const int few = std::min(d.M, d.N);
     return few <= 16 ? run_few<1, false>(g, wide, s) : few <= 32 ? run_few<2, false>(g, wide, s)
                                                           : run_few<4, false>(g, wide, s);
+  }
+  if (p.kind == Plan::TILE256 && !wide && d.K <= 1 << 22) {
+    g.tiles_m = (g.M + 255) / 256;
+    g.tiles_n = (g.N + 255) / 256;
+    const dim3 grid((unsigned)g.tiles_m * g.tiles_n), block(512);
+    if (g.a_shift && g.b_shift)
+      hipLaunchKernelGGL((fp8_gemm_turns<true, true>), grid, block, 0, s, g);
+    else if (g.a_shift)
+      hipLaunchKernelGGL((fp8_gemm_turns<true, false>), grid, block, 0, s, g);
+    else if (g.b_shift)
+      hipLaunchKernelGGL((fp8_gemm_turns<false, true>), grid, block, 0, s, g);
+    else
+      hipLaunchKernelGGL((fp8_gemm_turns<false, false>), grid, block, 0, s, g);
+    return hipGetLastError();
   }
   if (p.kind == Plan::TILE256) return run_tiles<2, 1, 2, 4, 2, 2>(g, p, wide, s);
   if (p.kind == Plan::SHORT) return run_tiles<1, 1, 2, 2, 3, 1>(g, p, wide, s);
