@@ -367,6 +367,15 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
       }
     }
   };
+  // an image gate's act and act', kept while the tiles stay in one image (read for every tile
+  // they cost 64x256x28x28 10 us of 45)
+  float gv[CPT], gd[CPT];
+  int gb = -1;
+#pragma unroll
+  for (int i = 0; i < CPT; ++i) {
+    gv[i] = 1.f;
+    gd[i] = 0.f;
+  }
   if (AHEAD && t0 < t1) load(t0, nx);
   for (long t = t0; t < t1; t += ts) {
     const int b = (int)(t / q.tpi), p = (int)(t % q.tpi) * TP + pl * V, valid = a.P - p;
@@ -382,13 +391,12 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
     if (!AHEAD) load(t, nx);
     const Raw in = nx;
     if (AHEAD && t + ts < t1) load(t + ts, nx);
-    float gv[CPT], gd[CPT];  // an image gate's act and act'
+    if (a.gate_kind == DCN_GATE_IMAGE && b != gb) {
+      gb = b;
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      gv[i] = 1.f;
-      gd[i] = 0.f;
-      if (a.gate_kind == DCN_GATE_IMAGE && inc[i] && !in.gone)
-        gate_act_grad(to_f32(gp[(size_t)b * a.C + cg + CG * i]), a.act, gv[i], gd[i]);
+      for (int i = 0; i < CPT; ++i)
+        if (inc[i] && !in.gone)
+          gate_act_grad(to_f32(gp[(size_t)b * a.C + cg + CG * i]), a.act, gv[i], gd[i]);
     }
     unsigned keep[CPT];
     if constexpr (DROP) {
@@ -802,6 +810,20 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
       }
     }
   };
+  // an image gate's act and act', kept while the rows stay in one image (with the registers for a
+  // prefetched row there are some for these); read for every row otherwise
+  constexpr bool KEEP = !FULL && AHEAD;
+  float gv[KEEP ? NV : 1][V], gd[KEEP && BWD ? NV : 1][V];
+  int gb = -1;
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        gv[j][e] = 1.f;
+        gd[BWD ? j : 0][e] = 0.f;
+      }
+  }
   if (AHEAD && t0 < t1) load(t0, nx);
   for (long t = t0; t < t1; ++t) {
     const int b = (int)(t / q.tpi), p = (int)(t % q.tpi) * GR + g;
@@ -827,8 +849,29 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
       if constexpr (DROP) return kept_or_0(j, e, v * a.drop.scale);
       return v;
     };
-    // the gate's value and slope; an image's gate is read here (the same row for all positions)
+    if constexpr (KEEP) {
+      if (a.gate_kind == DCN_GATE_IMAGE && b != gb) {
+        gb = b;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          if (cv[j] <= 0 || in.gone) continue;
+          float f[V];
+          ldv(ptr(a.gate) + (size_t)b * a.C + (lane + LPR * j) * V, cv[j], f);
+#pragma unroll
+          for (int e = 0; e < V; ++e) gate_act_grad(f[e], a.act, gv[j][e], gd[BWD ? j : 0][e]);
+        }
+      }
+    }
+    // the gate's value and slope
     auto gate = [&](int j, float (&av)[V], float (&ad)[V]) {
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          av[e] = gv[j][e];
+          ad[e] = gd[BWD ? j : 0][e];
+        }
+        return;
+      }
       float f[V];
       if constexpr (FULL) {
         unpack<T>(in.g[j], f);
