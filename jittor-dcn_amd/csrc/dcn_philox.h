@@ -35,13 +35,17 @@ __device__ __forceinline__ PhiloxKey philox_key(const DropArgs& a) {
   return PhiloxKey{(unsigned)seed, (unsigned)(seed >> 32), (unsigned)off, (unsigned)(off >> 32)};
 }
 
+__device__ __forceinline__ unsigned xor3(unsigned a, unsigned b, unsigned c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // one instruction
+}
+
 __device__ __forceinline__ uint4 philox10(uint64_t block, const PhiloxKey& k) {
   unsigned x0 = (unsigned)block, x1 = (unsigned)(block >> 32), x2 = k.o0, x3 = k.o1;
   unsigned k0 = k.k0, k1 = k.k1;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p0 = (uint64_t)x0 * 0xD2511F53u, p1 = (uint64_t)x2 * 0xCD9E8D57u;
-    const unsigned n0 = (unsigned)(p1 >> 32) ^ x1 ^ k0, n2 = (unsigned)(p0 >> 32) ^ x3 ^ k1;
+    const unsigned n0 = xor3((unsigned)(p1 >> 32), x1, k0), n2 = xor3((unsigned)(p0 >> 32), x3, k1);
     x1 = (unsigned)p1;
     x3 = (unsigned)p0;
     x0 = n0;
