@@ -2,7 +2,7 @@
 // of 128 along the contracted axis (include/dcn.h, 8-bit pointwise products).
 //
 // Power-of-two scales: v · 2^-e is exact, so a value is rounded once (round to nearest even,
-// v_cvt_pk_fp8_f32), and the MFMA applies the exponents itself (dcn_fp8_gemm.hip). A block
+// v_cvt_scalef32_pk_fp8), and the MFMA applies the exponents itself (dcn_fp8_gemm.hip). A block
 // loses no relative precision to that, at most one of e4m3's 18 binades of range.
 //
 // Memory is read once: a workgroup holds a 128 x 128 tile in registers (rows r of the tensor's

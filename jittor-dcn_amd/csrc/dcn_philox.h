@@ -4,10 +4,9 @@
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3",
 // 2011): ten rounds of two 32x32 -> 64-bit products. One call gives four words = eight 16-bit
 // draws, so eight neighbouring elements (one 16-byte bf16 vector) share a call. 16 bits per
-// draw instead of 32 halves the integer work, which at 32 bits would exceed what the memory
-// side of a bf16 stream takes (about 480 cycles a wave-call, 4 products of quarter rate a
-// round); the price is p in steps of 1/65536, with the kept values scaled by the exact
-// reciprocal of that p.
+// draw instead of 32 halves the integer work (ten dependent rounds of two 64-bit products a
+// call), which at 32 bits would exceed what the memory side of a bf16 stream takes; the price is
+// p in steps of 1/65536, with the kept values scaled by the exact reciprocal of that p.
 #pragma once
 #include "dcn_device.h"
 
