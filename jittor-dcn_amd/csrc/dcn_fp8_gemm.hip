@@ -596,10 +596,12 @@ Plan plan(const dcn_fp8_matmul_desc& d) {
   if (nkb <= 8 && tiles(128) >= 768) return {Plan::SHORT, 1, nkb};
   // 256 x 256: half the LDS reads per product (16384 x 8192 x 8192, bf16: 0.94 ms; 128 x 128 1.7 ms)
   if (tiles(256) >= 192) return {Plan::TILE256, 1, nkb};
-  // Too few tiles for the card: parts of K, at least four k blocks each, two workgroups a CU
-  // (2048 x 2048 x 2048 in two parts: 18 us, and 7 us to join them)
+  // Fewer tiles than CUs: parts of K, at least eight k blocks each, up to one workgroup a CU. (More
+  // parts cost more in the joining than they save: 2048 x 2048 x 2048, 256 tiles, whole 16 us, in two
+  // parts 16 + 7.5; 300 x 4096 x 4096, 96 tiles, whole 25, in two 17 + 4, in five 15 + 5.5;
+  // 1777 x 1500 x 1000 in fp32, 168 tiles, whole 14, in two 15 + 6.)
   const long t = tiles(128);
-  int splits = (int)std::min<long>(std::max<long>(1, 512 / t), std::max(1, nkb / 4));
+  int splits = (int)std::min<long>(std::max<long>(1, 256 / t), std::max(1, nkb / 8));
   const int kb = (nkb + splits - 1) / splits;
   splits = (nkb + kb - 1) / kb;
   return {Plan::TILE128, splits, kb};

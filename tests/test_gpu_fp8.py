@@ -210,6 +210,41 @@ def test_matmul_blocks(tb, dt, M, N, K, ab, bb):
     close(np64(tb.fp8_matmul(a, ea, b, eb, dt)), va, vb, dt, "product")
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("K", [128, 256, 384, 1152])
+@pytest.mark.parametrize("ab,bb", [(1, 1), (1, 128), (128, 1), (128, 128)])
+def test_wide_and_flat(tb, dt, K, ab, bb):
+    """One row of large tiles, any number of stages; small integers, so that the sums are exact."""
+    M, N = 100, 49500
+    g = torch.Generator(device="cuda").manual_seed(K)
+    v = [torch.randint(-4, 5, (rows, K), generator=g, device="cuda").float() for rows in (M, N)]
+    ops = []
+    for t, block in zip(v, (ab, bb)):
+        if block == 1:
+            ops += tb.fp8_quantize(t)[:2]
+        else:
+            w = tb.fp8_quantize_weight(t)
+            ops += [w.q, w.exponents]
+    assert torch.equal(tb.fp8_matmul(*ops, dt), (v[0].double() @ v[1].double().t()).to(dt))
+
+
+def test_k_beyond_the_tiles_offsets(tb):
+    """K above 2^22: rows too long for the 32-bit offsets of the large tiles. A few columns hold
+    values, the rest is zero."""
+    M, K = 3500, 2 ** 22 + 128
+    cols = torch.tensor([0, 127, 128, 2 ** 21, 2 ** 22 - 1, 2 ** 22, K - 1], device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    ops, vals = [], []
+    for _ in range(2):
+        v = torch.randint(-4, 5, (M, len(cols)), generator=g, device="cuda").float()
+        q = torch.zeros(M, K, dtype=torch.uint8, device="cuda")
+        q[:, cols] = v.to(torch.float8_e4m3fn).view(torch.uint8)
+        ops += [q, torch.full((K // 128, -(-M // 128) * 128), 127, dtype=torch.uint8, device="cuda")]
+        vals.append(v.double())
+    out = tb.fp8_matmul(*ops, torch.bfloat16)
+    assert torch.equal(out.double(), vals[0] @ vals[1].t())
+
+
 def test_only_one_gradient(tb):
     """The gradient of one input alone is the one of both."""
     x, w = make((50, 200), torch.bfloat16, 1, 0.2), make((70, 200), torch.bfloat16, 2, 0.2)
