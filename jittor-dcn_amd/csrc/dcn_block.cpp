@@ -228,8 +228,9 @@ int pointwise(const dcn_fp8_pointwise_desc* d, int grads, Pointwise* p) {
   p->kt = maps ? d->B * up128(d->P) : up128(p->T);
   const double widest = std::max(d->C, d->O);
   if (p->T > kMaxSide || p->kt > (1u << 30) || widest > kMaxSide ||
-      !tiles_ok(maps ? widest : (double)p->T, maps ? d->P : widest, maps ? d->B : 1) ||
-      !tiles_ok(d->O, d->C, 1) || !tiles_ok((double)p->T, widest, 1))
+      // (twice: the weight's tiles and x's go in one launch)
+      !tiles_ok(maps ? widest : (double)p->T, maps ? d->P : widest, maps ? 2.0 * d->B : 2) ||
+      !tiles_ok(d->O, d->C, 2) || !tiles_ok((double)p->T, widest, 1))
     return fail(DCN_ERR_UNSUPPORTED, "tensor too large");
   const int T = (int)p->T;
   if (maps) {
@@ -331,17 +332,20 @@ int dcn_fp8_pointwise_fwd(dcn_handle* h, const dcn_fp8_pointwise_desc* d, int gr
   char *b = static_cast<char*>(ws), *k = static_cast<char*>(saved);
   const bool gx = grads & DCN_FP8_GRAD_X, gw = grads & DCN_FP8_GRAD_W;
   hipError_t e = hipSuccess;
+  const bool maps = d->layout == DCN_NCHW, few = p.few, x8 = !few || gw;
+  char *xq = few ? nullptr : b + p.xq, *xs = few ? nullptr : b + p.xs;
+  char *xc = gw ? k + p.xc : nullptr, *xcs = gw ? k + p.xcs : nullptr;
   if (w) {
-    e = dcn::launch_fp8_quantize_weight(d->O, d->C, d->dtype, w, b + p.wq, b + p.ws,
-                                        gx ? k + p.wt : nullptr, gx ? k + p.wts : nullptr, ds.stream);
+    char *wt = gx ? k + p.wt : nullptr, *wts = gx ? k + p.wts : nullptr;
     q = b + p.wq;
     s = b + p.ws;
+    e = x8 ? dcn::launch_fp8_quantize_both(d->B, d->C, d->P, d->layout, d->dtype, x, xq, xs, xc, xcs,
+                                           d->O, w, b + p.wq, b + p.ws, wt, wts, ds.stream)
+           : dcn::launch_fp8_quantize_weight(d->O, d->C, d->dtype, w, b + p.wq, b + p.ws, wt, wts,
+                                             ds.stream);
+  } else if (x8) {
+    e = dcn::launch_fp8_quantize(d->B, d->C, d->P, d->layout, d->dtype, x, xq, xs, xc, xcs, ds.stream);
   }
-  const bool maps = d->layout == DCN_NCHW, few = p.few;
-  if (e == hipSuccess && (!few || gw))
-    e = dcn::launch_fp8_quantize(d->B, d->C, d->P, d->layout, d->dtype, x, few ? nullptr : b + p.xq,
-                                 few ? nullptr : b + p.xs, gw ? k + p.xc : nullptr,
-                                 gw ? k + p.xcs : nullptr, ds.stream);
   if (e == hipSuccess && few) {
     e = dcn::launch_fp8_few_tokens(p.y, d->C, x, q, s, y, ds.stream);
   } else if (e == hipSuccess) {

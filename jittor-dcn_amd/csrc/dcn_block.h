@@ -31,6 +31,11 @@ hipError_t launch_fp8_quantize(int B, int C, int P, int layout, int dtype, const
                                void* q_tok, void* s_tok, void* q_ch, void* s_ch, hipStream_t s);
 hipError_t launch_fp8_quantize_weight(int O, int C, int dtype, const void* w, void* q, void* sq,
                                       void* qT, void* sT, hipStream_t s);
+// both in one launch (x [B][C][P] or tokens, w [O][C])
+hipError_t launch_fp8_quantize_both(int B, int C, int P, int layout, int dtype, const void* v,
+                                    void* q_tok, void* s_tok, void* q_ch, void* s_ch, int O,
+                                    const void* w, void* q, void* sq, void* qT, void* sT,
+                                    hipStream_t s);
 size_t fp8_matmul_ws_bytes(const dcn_fp8_matmul_desc& d);
 hipError_t launch_fp8_matmul(const dcn_fp8_matmul_desc& d, const void* a, const void* sa,
                              const void* b, const void* sb, void* out, void* ws, hipStream_t s);

@@ -49,22 +49,29 @@ __device__ __forceinline__ unsigned lanes_max(unsigned v, F join) {
   return v;
 }
 
-// BLOCK2D: one exponent per tile, for both results (weights)
+// LDS row of the transposed tile: 16 chunks of 8 bytes, chunk c at c ^ 2 ((row >> 4) & 7), rows
+// padded by 16 bytes: a wave's writes (rows V apart) meet every bank equally often
+constexpr int PITCH = 144;
+template <typename T>
+struct QuantShared {
+  static constexpr int LPR = 128 / ElemVec<T>::N;
+  unsigned char tile[128 * PITCH];
+  unsigned colmax[kThreads / LPR][LPR][4];  // as raw: pairs, or one
+};
+
+// Tile `bid` of one matrix. BLOCK2D: one exponent per tile, for both results (weights)
 template <typename T, bool BLOCK2D>
-__global__ __launch_bounds__(kThreads) void fp8_quantize(QuantArgs a) {
+__device__ __forceinline__ void quantize_tile(const QuantArgs& a, int bid, QuantShared<T>& sh) {
   using M = Mag<T>;
   constexpr bool PAIRS = sizeof(T) == 2;
   constexpr int V = ElemVec<T>::N, LPR = 128 / V;     // lanes across a row of the tile
   constexpr int GROUPS = kThreads / LPR;              // row groups of kRows rows at a time
   constexpr int PASS = 128 / (GROUPS * kRows);        // 1 (bf16), 2 (f32)
-  // LDS row of the transposed tile: 16 chunks of 8 bytes, chunk c at c ^ 2 ((row >> 4) & 7), rows
-  // padded by 16 bytes: a wave's writes (rows V apart) meet every bank equally often
-  constexpr int PITCH = 144;
-  __shared__ __attribute__((aligned(16))) unsigned char tile[128 * PITCH];
-  __shared__ __attribute__((aligned(16))) unsigned colmax[GROUPS][LPR][4];  // as raw: pairs, or one
+  auto& tile = sh.tile;
+  auto& colmax = sh.colmax;
   const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
-  const int ts = blockIdx.x % a.tiles_s, tr = (blockIdx.x / a.tiles_s) % a.tiles_r;
-  const int img = blockIdx.x / (a.tiles_s * a.tiles_r);
+  const int ts = bid % a.tiles_s, tr = (bid / a.tiles_s) % a.tiles_r;
+  const int img = bid / (a.tiles_s * a.tiles_r);
   const int s0 = ts * 128, r0 = tr * 128, s = s0 + lane * V;
   const T* src = static_cast<const T*>(a.v) + (size_t)img * a.R * a.S;
 
@@ -206,13 +213,34 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize(QuantArgs a) {
   }
 }
 
+template <typename T, bool BLOCK2D>
+__global__ __launch_bounds__(kThreads) void fp8_quantize(QuantArgs a) {
+  __shared__ __attribute__((aligned(16))) QuantShared<T> sh;
+  quantize_tile<T, BLOCK2D>(a, blockIdx.x, sh);
+}
+
+// A weight's tiles and a tensor's in one launch (a launch and its gap are about 5 us, as long as
+// the rounding of 8 MB)
+template <typename T>
+__global__ __launch_bounds__(kThreads) void fp8_quantize_both(QuantArgs w, QuantArgs x, int w_tiles) {
+  __shared__ __attribute__((aligned(16))) QuantShared<T> sh;
+  if ((int)blockIdx.x < w_tiles)
+    quantize_tile<T, true>(w, blockIdx.x, sh);
+  else
+    quantize_tile<T, false>(x, blockIdx.x - w_tiles, sh);
+}
+
 long up128(long v) { return (v + 127) / 128 * 128; }
 
-hipError_t launch(QuantArgs a, int images, int dtype, bool block2d, hipStream_t s) {
+// fills in the tiles and gives their number
+unsigned tiles(QuantArgs& a, int images) {
   a.tiles_s = (a.S + 127) / 128;
   a.tiles_r = (a.R + 127) / 128;
-  const unsigned grid = (unsigned)((size_t)a.tiles_s * a.tiles_r * images);
-  const dim3 g(grid), t(kThreads);
+  return (unsigned)((size_t)a.tiles_s * a.tiles_r * images);
+}
+
+hipError_t launch(QuantArgs a, int images, int dtype, bool block2d, hipStream_t s) {
+  const dim3 g(tiles(a, images)), t(kThreads);
   if (dtype == DCN_BF16 && block2d)
     hipLaunchKernelGGL((fp8_quantize<bf16_t, true>), g, t, 0, s, a);
   else if (dtype == DCN_BF16)
@@ -224,10 +252,8 @@ hipError_t launch(QuantArgs a, int images, int dtype, bool block2d, hipStream_t 
   return hipGetLastError();
 }
 
-}  // namespace
-
-hipError_t launch_fp8_quantize(int B, int C, int P, int layout, int dtype, const void* v,
-                               void* q_tok, void* s_tok, void* q_ch, void* s_ch, hipStream_t s) {
+QuantArgs tensor_args(int B, int C, int P, int layout, const void* v, void* q_tok, void* s_tok,
+                      void* q_ch, void* s_ch) {
   QuantArgs a{};
   a.v = v;
   auto u8 = [](void* p) { return static_cast<unsigned char*>(p); };
@@ -243,7 +269,7 @@ hipError_t launch_fp8_quantize(int B, int C, int P, int layout, int dtype, const
     a.st = u8(s_ch);
     a.tk = up128(T);
     a.tstr = up128(C);
-    return launch(a, 1, dtype, false, s);
+    return a;
   }
   a.R = C;
   a.S = P;
@@ -256,11 +282,10 @@ hipError_t launch_fp8_quantize(int B, int C, int P, int layout, int dtype, const
   a.st = u8(s_tok);
   a.tk = up128(C);
   a.tstr = up128(T);
-  return launch(a, B, dtype, false, s);
+  return a;
 }
 
-hipError_t launch_fp8_quantize_weight(int O, int C, int dtype, const void* w, void* q, void* sq,
-                                      void* qT, void* sT, hipStream_t s) {
+QuantArgs weight_args(int O, int C, const void* w, void* q, void* sq, void* qT, void* sT) {
   QuantArgs a{};
   auto u8 = [](void* p) { return static_cast<unsigned char*>(p); };
   a.v = w;
@@ -274,7 +299,35 @@ hipError_t launch_fp8_quantize_weight(int O, int C, int dtype, const void* w, vo
   a.st = u8(sT);
   a.tk = up128(O);
   a.tstr = (C + 127) / 128;
-  return launch(a, 1, dtype, true, s);
+  return a;
+}
+
+}  // namespace
+
+hipError_t launch_fp8_quantize(int B, int C, int P, int layout, int dtype, const void* v,
+                               void* q_tok, void* s_tok, void* q_ch, void* s_ch, hipStream_t s) {
+  return launch(tensor_args(B, C, P, layout, v, q_tok, s_tok, q_ch, s_ch),
+                layout == DCN_NHWC ? 1 : B, dtype, false, s);
+}
+
+hipError_t launch_fp8_quantize_weight(int O, int C, int dtype, const void* w, void* q, void* sq,
+                                      void* qT, void* sT, hipStream_t s) {
+  return launch(weight_args(O, C, w, q, sq, qT, sT), 1, dtype, true, s);
+}
+
+hipError_t launch_fp8_quantize_both(int B, int C, int P, int layout, int dtype, const void* v,
+                                    void* q_tok, void* s_tok, void* q_ch, void* s_ch, int O,
+                                    const void* w, void* q, void* sq, void* qT, void* sT,
+                                    hipStream_t s) {
+  QuantArgs x = tensor_args(B, C, P, layout, v, q_tok, s_tok, q_ch, s_ch);
+  QuantArgs a = weight_args(O, C, w, q, sq, qT, sT);
+  const unsigned nw = tiles(a, 1), nx = tiles(x, layout == DCN_NHWC ? 1 : B);
+  const dim3 g(nw + nx), t(kThreads);
+  if (dtype == DCN_BF16)
+    hipLaunchKernelGGL((fp8_quantize_both<bf16_t>), g, t, 0, s, a, x, (int)nw);
+  else
+    hipLaunchKernelGGL((fp8_quantize_both<float>), g, t, 0, s, a, x, (int)nw);
+  return hipGetLastError();
 }
 
 }  // namespace dcn
