@@ -72,6 +72,7 @@ struct Plan {
   // [wgs][5][C], and a row of C for workgroup j of run g at image b in slot (g + b) · group + j
   // (g + b grows along the runs and their images, so no two share a slot)
   float *part, *gpart;
+  float* rowst;  // [6][rows]: m1, r1, m2, r2, mean(a2), mean(a2 h2) of long rows (N_pre's a and h)
 };
 
 __host__ __device__ __forceinline__ long first_tile(const Plan& q, int run) {
@@ -394,9 +395,12 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
     if (a.gate_kind == DCN_GATE_IMAGE && b != gb) {
       gb = b;
 #pragma unroll
-      for (int i = 0; i < CPT; ++i)
+      for (int i = 0; i < CPT; ++i) {
+        gv[i] = 1.f;  // (a dropped image's gate: nothing of another image's may stay)
+        gd[i] = 0.f;
         if (inc[i] && !in.gone)
           gate_act_grad(to_f32(gp[(size_t)b * a.C + cg + CG * i]), a.act, gv[i], gd[i]);
+      }
     }
     unsigned keep[CPT];
     if constexpr (DROP) {
@@ -706,12 +710,16 @@ struct RowSums {
   }
 };
 
-template <typename T, int NT, int LPR, int NV, int WPE, bool AHEAD, bool BWD, bool FULL, bool DROP>
+// PAR: the backward adds up the parameters' gradients here; without, it leaves each row's six
+// numbers (below) for block_row_params.
+template <typename T, int NT, int LPR, int NV, int WPE, bool AHEAD, bool BWD, bool FULL, bool DROP,
+          bool PAR>
 __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
   constexpr int V = ElemVec<T>::N, GR = NT / LPR;
   using Sums = RowSums<NT, LPR, V, NV>;
   __shared__ __attribute__((aligned(16))) typename Sums::Shared shared;
-  __shared__ float fold[BWD ? GR : 1][BWD ? LPR * NV * V : 1];
+  constexpr bool SUMS = BWD && PAR;
+  __shared__ float fold[SUMS ? GR : 1][SUMS ? LPR * NV * V : 1];
   const PhiloxKey key = philox_key(a.drop);
   Sums sums(shared, a.C);
   const int lane = sums.lane, g = threadIdx.x / LPR;
@@ -748,8 +756,8 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
       unpack<T>(fetch(k, j), v);
   };
   const u32x4 zero = {0u, 0u, 0u, 0u};
-  float acc[BWD ? 5 : 1][NV][V], accg[BWD && !FULL ? NV : 1][V];
-  if constexpr (BWD) {
+  float acc[SUMS ? 5 : 1][NV][V], accg[SUMS && !FULL ? NV : 1][V];
+  if constexpr (SUMS) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -854,11 +862,15 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
         gb = b;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          if (cv[j] <= 0 || in.gone) continue;
+          const bool read = cv[j] > 0 && !in.gone;
           float f[V];
-          ldv(ptr(a.gate) + (size_t)b * a.C + (lane + LPR * j) * V, cv[j], f);
+          if (read) ldv(ptr(a.gate) + (size_t)b * a.C + (lane + LPR * j) * V, cv[j], f);
 #pragma unroll
-          for (int e = 0; e < V; ++e) gate_act_grad(f[e], a.act, gv[j][e], gd[BWD ? j : 0][e]);
+          for (int e = 0; e < V; ++e) {
+            gv[j][e] = 1.f;  // (a dropped image's gate: nothing of another image's may stay)
+            gd[BWD ? j : 0][e] = 0.f;
+            if (read) gate_act_grad(f[e], a.act, gv[j][e], gd[BWD ? j : 0][e]);
+          }
         }
       }
     }
@@ -959,9 +971,9 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
       }
     } else {
       const float ic = 1.f / (float)a.C;
+      float s1 = 0.f, s2 = 0.f;
       // G into o
       if (a.pre) {
-        float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           float gy[V], w2[V];
@@ -973,8 +985,10 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
             o[j][e] = h;
             s1 += w;
             s2 = fmaf(w, h, s2);
-            acc[3][j][e] = fmaf(gy[e], h, acc[3][j][e]);
-            acc[4][j][e] += gy[e];
+            if constexpr (SUMS) {
+              acc[3][j][e] = fmaf(gy[e], h, acc[3][j][e]);
+              acc[4][j][e] += gy[e];
+            }
           }
         }
         sums.sum2(s1, s2);
@@ -993,6 +1007,13 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
       } else {
 #pragma unroll
         for (int j = 0; j < NV; ++j) unpack<T>(in.o[j], o[j]);
+      }
+      if constexpr (!PAR) {
+        if (q.rowst && live && lane == 0) {
+          const float st[6] = {m1, r1, m2, r2, s1, s2};
+#pragma unroll
+          for (int k = 0; k < 6; ++k) q.rowst[k * rows + (size_t)b * q.P + p] = st[k];
+        }
       }
       if (a.gr) {
 #pragma unroll
@@ -1016,10 +1037,12 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
             const float dt = drop(j, e, o[j][e]), dtv = dt * v, k = a.alpha * sc[e];
             const float dv = dt * (k * av[e]);
             gg[e] = dtv * (k * ad[e]);
-            acc[0][j][e] = fmaf(dtv, a.alpha * av[e], acc[0][j][e]);
-            acc[1][j][e] = fmaf(dv, h, acc[1][j][e]);
-            acc[2][j][e] += dv;
-            if constexpr (!FULL) accg[j][e] += gg[e];
+            if constexpr (SUMS) {
+              acc[0][j][e] = fmaf(dtv, a.alpha * av[e], acc[0][j][e]);
+              acc[1][j][e] = fmaf(dv, h, acc[1][j][e]);
+              acc[2][j][e] += dv;
+              if constexpr (!FULL) accg[j][e] += gg[e];
+            }
             o[j][e] = dv;
             const float w = dv * w1[e];
             s3 += w;
@@ -1050,7 +1073,7 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
             stv(static_cast<T*>(a.gx) + base + (lane + LPR * j) * V, cv[j], o[j]);
           }
         }
-        if constexpr (!FULL) {
+        if constexpr (SUMS && !FULL) {
           if (q.image_gate && (t + 1 == t1 || (t + 1) % q.tpi == 0)) {
             fold_groups(accg, q.gpart + (size_t)(wg + b) * a.C);
 #pragma unroll
@@ -1062,11 +1085,136 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
       }
     }
   }
-  if constexpr (BWD) {
+  if constexpr (SUMS) {
     if (!q.part) return;
 #pragma unroll
     for (int k = 0; k < 5; ++k) fold_groups(acc[k], q.part + ((size_t)wg * 5 + k) * a.C);
   }
+}
+
+// The parameters' gradients of long rows, in a second pass: with 16 channels a lane their five sums
+// do not fit beside the row (1024 x 8192 bf16, spilling, in one pass 65 us; in two 30 and 23, and 5
+// for the fold). A workgroup takes 64 vectors of channels and a run of rows, kParamRows / V of them
+// to a wave at a time; what a row needs besides its values are the six numbers that block_row left.
+constexpr int kParamRows = 16;  // channels times rows of a lane at a time
+template <typename T, bool FULL, bool DROP>
+__global__ __launch_bounds__(256) void block_row_params(BlockArgs a, Plan q) {
+  constexpr int V = ElemVec<T>::N, GR = 4, U = kParamRows / V;
+  __shared__ float fold[GR][64 * V];
+  const PhiloxKey key = philox_key(a.drop);
+  const int lane = threadIdx.x & 63, g = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = ((int)blockIdx.y * 64 + lane) * V, cv = a.C - c, wg = blockIdx.x;
+  auto ptr = [](const void* p) { return static_cast<const T*>(p); };
+  auto param = [&](const void* p, float none, float (&v)[V]) {
+    if (p && cv > 0) return ldv(ptr(p) + c, cv, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = none;
+  };
+  float sc[V], w1[V], b1[V], w2[V], gv[V], gd[V], acc[5][V], accg[V];
+  param(a.scale, 1.f, sc);
+  param(a.w1, 1.f, w1);
+  param(a.b1, 0.f, b1);
+  param(a.w2, 1.f, w2);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    gv[e] = 1.f;
+    gd[e] = accg[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) acc[k][e] = 0.f;
+  }
+  auto fold_waves = [&](const float (&v)[V], float* dst) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; ++e) fold[g][lane * V + e] = v[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * V; i += 256) {
+      const int at = (int)blockIdx.y * 64 * V + i;
+      if (at < a.C) dst[at] = (fold[0][i] + fold[1][i]) + (fold[2][i] + fold[3][i]);
+    }
+  };
+  int gb = -1;
+  const size_t rows = (size_t)q.images * q.P;
+  const long t1 = first_tile(q, wg + 1);
+  for (long t = first_tile(q, wg); t < t1; ++t) {
+    const int b = (int)(t / q.tpi), p0 = (int)(t % q.tpi) * GR * U + g * U;
+    // U rows' loads in flight at a time; a row behind the last is zeros and adds nothing
+    u32x4 x[U], o[U], f[U], gy[U], go[U];
+    float st[U][6];
+    unsigned keep[U];
+    bool gone = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool live = p0 + u < q.P && cv > 0;
+      const size_t row = (size_t)b * q.P + p0 + u, at = row * a.C + c;
+      keep[u] = 0xffu;
+      if constexpr (DROP) {
+        if (a.drop_image) {
+          gone = !keep1(q.images == a.B ? b : (int)(row / a.P), key, a.drop.thr);
+          keep[u] = gone ? 0u : 0xffu;
+        } else {
+          keep[u] = keepv<V>(at, key, a.drop.thr);
+        }
+      }
+      auto read = [&](const void* t) {
+        return t && live ? ldv_raw(ptr(t) + at, cv) : u32x4{0u, 0u, 0u, 0u};
+      };
+      x[u] = read(gone ? nullptr : a.x);
+      o[u] = read(a.res);
+      gy[u] = read(a.gy);
+      go[u] = read(a.go);
+      if constexpr (FULL) f[u] = read(gone ? nullptr : a.gate);
+#pragma unroll
+      for (int k = 0; k < 6; ++k) st[u][k] = live ? q.rowst[k * rows + row] : 0.f;
+    }
+    if (a.gate_kind == DCN_GATE_IMAGE && b != gb) {
+      gb = b;
+      float w[V];
+      if (!gone && cv > 0) ldv(ptr(a.gate) + (size_t)b * a.C + c, cv, w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        gv[e] = 1.f;
+        gd[e] = 0.f;
+        if (!gone && cv > 0) gate_act_grad(w[e], a.act, gv[e], gd[e]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float xv[V], ov[V], fv[V], gyv[V], gov[V];
+      unpack<T>(x[u], xv);
+      unpack<T>(o[u], ov);
+      unpack<T>(gy[u], gyv);
+      unpack<T>(go[u], gov);
+      if constexpr (FULL) unpack<T>(f[u], fv);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const bool kept = !DROP || (keep[u] >> e & 1u);
+        float av = gv[e], ad = gd[e];
+        if constexpr (FULL) gate_act_grad(kept ? fv[e] : 0.f, a.act, av, ad);
+        const float h = kept ? (xv[e] - st[u][0]) * st[u][1] : 0.f, v = fmaf(h, w1[e], b1[e]);
+        const float k = a.alpha * sc[e], ds = kept ? (DROP ? a.drop.scale : 1.f) : 0.f;
+        float G = gov[e];
+        if (a.pre) {
+          const float h2 = (ov[e] + (a.x && kept ? v * (k * av) * ds : 0.f) - st[u][2]) * st[u][3];
+          acc[3][e] = fmaf(gyv[e], h2, acc[3][e]);
+          acc[4][e] += gyv[e];
+          G = fmaf(st[u][3], gyv[e] * w2[e] - st[u][4] - h2 * st[u][5], G);
+        }
+        const float dt = kept ? G * ds : 0.f, dv = dt * (k * av);
+        acc[0][e] = fmaf(dt * v, a.alpha * av, acc[0][e]);
+        acc[1][e] = fmaf(dv, h, acc[1][e]);
+        acc[2][e] += dv;
+        if constexpr (!FULL) accg[e] = fmaf(dt * v, k * ad, accg[e]);
+      }
+    }
+    if (q.image_gate && (t + 1 == t1 || (t + 1) % q.tpi == 0)) {  // uniform
+      fold_waves(accg, q.gpart + (size_t)(wg + b) * a.C);
+#pragma unroll
+      for (int e = 0; e < V; ++e) accg[e] = 0.f;
+    }
+  }
+  if (!q.part) return;
+#pragma unroll
+  for (int k = 0; k < 5; ++k) fold_waves(acc[k], q.part + ((size_t)wg * 5 + k) * a.C);
 }
 
 // The partials of one parameter (k < 5) or of one image's gate (k = 5 + image), 64 channels
@@ -1108,8 +1256,23 @@ __global__ __launch_bounds__(1024) void block_fold(BlockArgs a, Plan q, int k0) 
   if (g == 0 && c < a.C) out[c] = from_f32(red[0][threadIdx.x], T());
 }
 
-constexpr int kMaxWgs = 1024;   // workgroups with partials
+constexpr int kMaxWgs = 1024;   // workgroups with partials, maps
+constexpr int kRowWgs = 512;    // and rows
+constexpr int kRowSums = 4096;  // channels of a row beside which the parameters' sums fit
 constexpr int kInterleave = 8;  // workgroups that share a run of map tiles
+
+// adds up the partials; a parameter without a destination ends at once
+template <typename T>
+hipError_t fold_partials(const BlockArgs& a, const Plan& q, hipStream_t s) {
+  const int rows = 5 + (q.image_gate ? a.B : 0);  // an image gate's start at 5
+  for (int k = q.part ? 0 : 5, n; k < rows; k += n) {
+    n = std::min(rows - k, 32768);
+    hipLaunchKernelGGL((block_fold<T>), dim3((a.C + 63) / 64, n), dim3(1024), 0, s, a, q, k);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
 
 // Fills the plan for tiles of `per` positions, launches `kernel(full gate, dropout)` and the fold.
 template <typename T, bool BWD, typename K>
@@ -1122,23 +1285,16 @@ hipError_t run_tiles(const BlockArgs& a, int images, int P, int per, int wgs, in
   q.tiles = (long)q.tpi * images;
   const bool params = BWD && (a.gs || a.gw1 || a.gb1 || a.gw2 || a.gb2);
   q.image_gate = BWD && a.gg && a.gate_kind == DCN_GATE_IMAGE;
-  // wgs: > 0 with a prefetch, < 0 without, 0 one a tile as far as partials allow
+  // wgs: 0 one a tile as far as partials allow
   q.wgs = (int)std::min<long>(
-      q.tiles, wgs ? std::abs(wgs) : params || q.image_gate ? kMaxWgs : 1 << 20);
+      q.tiles, wgs ? wgs : params || q.image_gate ? kMaxWgs : 1 << 20);
   q.group = maps && q.tpi >= kInterleave && q.wgs % kInterleave == 0 ? kInterleave : 1;
   if (params) q.part = a.ws;
-  if (q.image_gate) q.gpart = a.ws + (size_t)kMaxWgs * 5 * a.C;
+  if (q.image_gate) q.gpart = a.ws + (size_t)(maps ? kMaxWgs : kRowWgs) * 5 * a.C;
   auto* fn = kernel(a.gate_kind == DCN_GATE_FULL, a.drop.thr != 0);
   hipLaunchKernelGGL(fn, dim3(q.wgs), dim3(threads), 0, s, a, q);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !(params || q.image_gate)) return e;
-  // (a parameter without a destination ends at once; an image gate's rows start at 5)
-  for (int k = params ? 0 : 5, n; k < 5 + (q.image_gate ? a.B : 0); k += n) {
-    n = std::min(5 + (q.image_gate ? a.B : 0) - k, 32768);
-    hipLaunchKernelGGL((block_fold<T>), dim3((a.C + 63) / 64, n), dim3(1024), 0, s, a, q, k);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-  }
-  return hipSuccess;
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || !(params || q.image_gate) ? e : fold_partials<T>(a, q, s);
 }
 
 template <typename T, int NT, int PL, int CPT, int WPE, int WGS, bool BWD>
@@ -1152,18 +1308,72 @@ hipError_t run_map(const BlockArgs& a, hipStream_t s) {
   return run_tiles<T, BWD>(a, a.B, a.P, PL * ElemVec<T>::N, WGS, NT, true, pick, s);
 }
 
+// images matter to an image gate only; else all rows are one run (up to int)
+inline bool one_run(const BlockArgs& a) {
+  return a.gate_kind != DCN_GATE_IMAGE && (size_t)a.B * a.P < (1u << 30);
+}
+
 template <typename T, int NT, int LPR, int NV, int WPE, int WGS, bool BWD>
 hipError_t run_row(const BlockArgs& a, hipStream_t s) {
   auto pick = [](bool full, bool drop) {
-    return full ? (drop ? block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, true, true>
-                        : block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, true, false>)
-                : (drop ? block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, false, true>
-                        : block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, false, false>);
+    return full ? (drop ? block_row<T, NT, LPR, NV, WPE, true, BWD, true, true, true>
+                        : block_row<T, NT, LPR, NV, WPE, true, BWD, true, false, true>)
+                : (drop ? block_row<T, NT, LPR, NV, WPE, true, BWD, false, true, true>
+                        : block_row<T, NT, LPR, NV, WPE, true, BWD, false, false, true>);
   };
-  // images matter to an image gate only; else all rows are one run (up to int)
-  const bool one = a.gate_kind != DCN_GATE_IMAGE && (size_t)a.B * a.P < (1u << 30);
+  const bool one = one_run(a);
   return run_tiles<T, BWD>(a, one ? 1 : a.B, one ? a.B * a.P : a.P, NT / LPR, WGS, NT, false, pick,
                            s);
+}
+
+// A full gate's backward of rows of 16 channels a lane in one pass after all: with nothing fetched
+// ahead and the parameters read again for every row the sums fit (run_long_row).
+template <typename T, int NT, int NV, int WPE, int WGS>
+hipError_t run_gated_row(const BlockArgs& a, hipStream_t s) {
+  auto pick = [](bool, bool drop) {
+    return drop ? block_row<T, NT, NT, NV, WPE, false, true, true, true, true>
+                : block_row<T, NT, NT, NV, WPE, false, true, true, false, true>;
+  };
+  return run_tiles<T, true>(a, 1, a.B * a.P, 1, WGS, NT, false, pick, s);
+}
+
+// A backward in two passes: every row's gradients, then the parameters'.
+template <typename T, int NT, int NV, int WPE, bool AHEAD, int WGS>
+hipError_t run_long_row(const BlockArgs& a, hipStream_t s) {
+  Plan q{};
+  const bool one = one_run(a), image_gate = a.gg && a.gate_kind == DCN_GATE_IMAGE;
+  const bool params = a.gs || a.gw1 || a.gb1 || a.gw2 || a.gb2, full = a.gate_kind == DCN_GATE_FULL;
+  q.images = one ? 1 : a.B;
+  q.P = one ? a.B * a.P : a.P;
+  q.tpi = q.P;  // one row a tile
+  q.tiles = (long)q.tpi * q.images;
+  q.wgs = (int)std::min<long>(q.tiles, WGS);
+  q.group = 1;
+  if (params || image_gate) q.rowst = a.ws;
+  const bool drop = a.drop.thr != 0;
+  auto* fn = full ? (drop ? block_row<T, NT, NT, NV, WPE, AHEAD, true, true, true, false>
+                          : block_row<T, NT, NT, NV, WPE, AHEAD, true, true, false, false>)
+                  : (drop ? block_row<T, NT, NT, NV, WPE, AHEAD, true, false, true, false>
+                          : block_row<T, NT, NT, NV, WPE, AHEAD, true, false, false, false>);
+  if (a.gx || a.gr || (a.gg && full) || q.rowst) {
+    hipLaunchKernelGGL(fn, dim3(q.wgs), dim3(NT), 0, s, a, q);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !q.rowst) return e;
+  }
+  float* rest = a.ws + ((size_t)a.B * a.P * 6 + 63) / 64 * 64;
+  const int columns = (a.C + 64 * ElemVec<T>::N - 1) / (64 * ElemVec<T>::N);
+  const int per = 4 * kParamRows / ElemVec<T>::N;
+  q.tpi = (q.P + per - 1) / per;
+  q.tiles = (long)q.tpi * q.images;
+  q.wgs = (int)std::min<long>({q.tiles, kRowWgs, std::max(1, 1024 / columns)});
+  q.image_gate = image_gate;
+  if (params) q.part = rest;
+  if (image_gate) q.gpart = rest + (size_t)kRowWgs * 5 * a.C;
+  auto* pn = full ? (drop ? block_row_params<T, true, true> : block_row_params<T, true, false>)
+                  : (drop ? block_row_params<T, false, true> : block_row_params<T, false, false>);
+  hipLaunchKernelGGL(pn, dim3(q.wgs, columns), dim3(256), 0, s, a, q);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : fold_partials<T>(a, q, s);
 }
 
 }  // namespace

@@ -5,9 +5,12 @@ namespace dcn {
 
 // As forward, with 8 channels a lane: the five parameter sums of every channel stay in
 // registers beside the rows (8192 x 1024 bf16: 37 us; 75 us with 16 channels a lane, 83 us
-// with four waves per SIMD). Above 4096 bf16 channels (or 8192 fp32) 16 a lane are needed: without the
-// prefetch and the kept parameters (a negative count) less spills (1024 x 8192 bf16: 66 us
-// against 150, fp32 139 against 191). false: no variant.
+// with four waves per SIMD). Above 4096 channels the parameters' sums take a pass of their own
+// (us, one pass with its spills against two: bf16 2048 x 5120 92, 68, 1024 x 8192 65, 55,
+// 512 x 16384 253, 83; fp32 188, 118, 130, 99, 357, 171; the first pass prefetches in bf16, 68
+// against 86, and not in fp32, 118 against 125), save beside a full gate in bf16 up to 8192, which
+// adds a tensor to the second pass and spares the gate's sums in the first (76, 90 and 62, 72).
+// false: no variant.
 bool block_row_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
   const int C = a.C;
   if (a.dtype == DCN_BF16) {
@@ -17,8 +20,10 @@ bool block_row_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     else if (C <= 1024) *e = run_row<bf16_t, 256, 128, 1, 2, 512, true>(a, s);
     else if (C <= 2048) *e = run_row<bf16_t, 256, 256, 1, 2, 512, true>(a, s);
     else if (C <= 4096) *e = run_row<bf16_t, 512, 512, 1, 2, 256, true>(a, s);
-    else if (C <= 8192) *e = run_row<bf16_t, 512, 512, 2, 2, -256, true>(a, s);
-    else if (C <= 16384) *e = run_row<bf16_t, 1024, 1024, 2, 4, -256, true>(a, s);
+    else if (C <= 8192 && a.gate_kind == DCN_GATE_FULL && one_run(a))
+      *e = run_gated_row<bf16_t, 512, 2, 2, 256>(a, s);
+    else if (C <= 8192) *e = run_long_row<bf16_t, 512, 2, 2, true, 512>(a, s);
+    else if (C <= 16384) *e = run_long_row<bf16_t, 1024, 2, 4, false, 512>(a, s);
     else return false;
   } else {
     if (C <= 128) *e = run_row<float, 256, 16, 2, 2, 512, true>(a, s);
@@ -27,8 +32,8 @@ bool block_row_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     else if (C <= 1024) *e = run_row<float, 256, 128, 2, 2, 512, true>(a, s);
     else if (C <= 2048) *e = run_row<float, 256, 256, 2, 2, 512, true>(a, s);
     else if (C <= 4096) *e = run_row<float, 512, 512, 2, 2, 256, true>(a, s);
-    else if (C <= 8192) *e = run_row<float, 1024, 1024, 2, 4, -256, true>(a, s);
-    else if (C <= 16384) *e = run_row<float, 1024, 1024, 4, 4, -256, true>(a, s);
+    else if (C <= 8192) *e = run_long_row<float, 512, 4, 2, false, 512>(a, s);
+    else if (C <= 16384) *e = run_long_row<float, 1024, 4, 4, false, 512>(a, s);
     else return false;
   }
   return true;

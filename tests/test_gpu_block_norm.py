@@ -241,7 +241,7 @@ def test_zero_rows_and_non_finite(tb, layout):
 @pytest.mark.parametrize("drop", ["element", "image"])
 @pytest.mark.parametrize("gate", ["none", "full", "image"])
 @pytest.mark.parametrize("layout,C", [("nchw", 48), ("nchw", 2100), ("rows", 48), ("rows", 3000),
-                                      ("rows", 16500)])
+                                      ("rows", 8000), ("rows", 16500)])
 def test_dropped_values_reach_nothing(tb, layout, C, gate, drop):
     """NaN and infinities where dropout drops give the bits that zeros there give. (Per element
     without a norm after the block: with one, a NaN spreads over its position.)"""
@@ -267,6 +267,26 @@ def test_dropped_values_reach_nothing(tb, layout, C, gate, drop):
     for r in results[1:]:
         for k, a, b in zip(["out", "y", *t], results[0], r):
             assert torch.equal(a, b), k
+
+
+@pytest.mark.parametrize("layout,C", [("nchw", 48), ("nchw", 2100), ("rows", 48), ("rows", 3000),
+                                      ("rows", 8000), ("rows", 16500)])
+def test_a_bad_gate_stays_in_its_image(tb, layout, C):
+    """A NaN gate of a kept image leaves the dropped images' gate gradients 0 and their results
+    the residual's."""
+    B, P, p = 6, 5, 0.5
+    t, go, gy = tensors(layout, B, C, P, torch.float32, "rms", "rms", "image")
+    f = torch.from_numpy(BO.drop_factor(B * C * P, C * P, p, SEED, OFF)).reshape(B, -1)[:, 0]
+    assert (f > 0).any() and (f == 0).any()
+    t["gate"][f.cuda() > 0] = float("nan")
+    for v in t.values():
+        v.requires_grad_()
+    o, y = call(tb, t, "rms", "rms", "silu", p=p, drop="image")
+    gx, gg = torch.autograd.grad((o, y), (t["x"], t["gate"]), (go, gy))
+    gone = (f == 0).cuda()
+    assert torch.equal(o[gone], t["residual"][gone]) and torch.isfinite(y[gone]).all()
+    assert not gx[gone].any() and not gg[gone].any()
+    assert torch.isnan(gg[~gone]).all()
 
 
 @pytest.mark.parametrize("dt", DTYPES)
