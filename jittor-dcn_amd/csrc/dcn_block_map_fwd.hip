@@ -8,7 +8,9 @@ namespace dcn {
 // at 64 images (us, the best two):
 //   bf16  64x3136: 30, 44   128x784: 23, 25   256x784: 31, 34   512x196: 28, 36
 //   fp32  64x3136: 46, 55   128x784: 31, 34   256x3136: 178, 179   512x196: 35, 52
-// With dropout 256 bf16 channels want four waves per SIMD more than the prefetch (49 us, 55).
+// 256 bf16 channels want four waves per SIMD more than the prefetch with dropout (64x256x196 17 us,
+// 21; 64x200x784 36, 41) and where 256 workgroups would get three tiles of 32 positions or fewer
+// (64x256x196 12.4 us, 14.4; 32x256x784, 800 tiles, 17.6, 17.8; 64x256x784 34, 31).
 // More channels than a workgroup's registers hold take narrower tiles (32-byte runs of a
 // channel at 1024), which costs less than a second pass. false: no variant (C > 2048).
 bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
@@ -17,7 +19,8 @@ bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     if (C <= 32) *e = run_map<bf16_t, 256, 8, 1, 3, 0, false>(a, s);
     else if (C <= 64) *e = run_map<bf16_t, 256, 8, 2, 2, 512, false>(a, s);
     else if (C <= 128) *e = run_map<bf16_t, 256, 4, 2, 2, 512, false>(a, s);
-    else if (C <= 256 && a.drop.thr) *e = run_map<bf16_t, 512, 4, 2, 4, 0, false>(a, s);
+    else if (C <= 256 && (a.drop.thr || (long)a.B * ((a.P + 31) / 32) <= 3 * 256))
+      *e = run_map<bf16_t, 512, 4, 2, 4, 0, false>(a, s);
     else if (C <= 256) *e = run_map<bf16_t, 512, 4, 2, 2, 256, false>(a, s);
     else if (C <= 512) *e = run_map<bf16_t, 1024, 4, 2, 4, 0, false>(a, s);
     else if (C <= 1024) *e = run_map<bf16_t, 512, 2, 4, 2, 256, false>(a, s);
