@@ -4,11 +4,12 @@
 namespace dcn {
 
 // Threads, lanes along the positions, channels a thread, waves per SIMD and workgroups that
-// prefetch their next tile (0: up to 1024 that do not) by channels; the fastest of those tried
-// at 64 images (us, the best two, tiles not yet interleaved):
-//   bf16  64x3136: 52, 79   128x784: 42, 47   256x784: 72, 89   512x196: 62, 147
-//   fp32  64x3136: 83, 108  128x784: 61, 100  256x784: 112, 191  512x196: 103, 168
-// false: no variant (C > 2048).
+// prefetch their next tile (negative: that do not; 0: up to 1024 that do not) by channels; the
+// fastest of those tried at 64 images. The prefetch, us with and without (layer norms, no gate;
+// then a full gate): bf16 256x784 54, 67; 74, 88   512x196 46, 50; 63, 72   1024x196 130, 97;
+// 182, 134   fp32 128x784 50, 48; 70, 64   256x784 92, 86; 134, 117   512x196 61, 59; 84, 78
+// 1024x196 226, 184; 254, 214: a second tile in registers costs fp32 and wide maps spills that
+// cost more than the wait. false: no variant (C > 2048).
 bool block_map_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
   const int C = a.C;
   if (a.dtype == DCN_BF16) {
@@ -17,17 +18,17 @@ bool block_map_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     else if (C <= 128) *e = run_map<bf16_t, 256, 4, 2, 2, 512, true>(a, s);
     else if (C <= 256) *e = run_map<bf16_t, 512, 4, 2, 2, 256, true>(a, s);
     else if (C <= 512) *e = run_map<bf16_t, 512, 2, 2, 2, 256, true>(a, s);
-    else if (C <= 1024) *e = run_map<bf16_t, 512, 2, 4, 2, 256, true>(a, s);
-    else if (C <= 2048) *e = run_map<bf16_t, 1024, 2, 4, 4, 256, true>(a, s);
+    else if (C <= 1024) *e = run_map<bf16_t, 512, 2, 4, 2, -256, true>(a, s);
+    else if (C <= 2048) *e = run_map<bf16_t, 512, 2, 8, 2, 0, true>(a, s);
     else return false;
   } else {
     if (C <= 32) *e = run_map<float, 256, 8, 1, 3, 0, true>(a, s);
     else if (C <= 64) *e = run_map<float, 256, 8, 2, 4, 0, true>(a, s);
-    else if (C <= 128) *e = run_map<float, 256, 8, 4, 2, 512, true>(a, s);
-    else if (C <= 256) *e = run_map<float, 512, 8, 4, 2, 256, true>(a, s);
-    else if (C <= 512) *e = run_map<float, 512, 4, 4, 2, 256, true>(a, s);
-    else if (C <= 1024) *e = run_map<float, 1024, 4, 4, 4, 0, true>(a, s);
-    else if (C <= 2048) *e = run_map<float, 1024, 4, 8, 4, 256, true>(a, s);
+    else if (C <= 128) *e = run_map<float, 256, 8, 4, 2, -512, true>(a, s);
+    else if (C <= 256) *e = run_map<float, 512, 8, 4, 2, -256, true>(a, s);
+    else if (C <= 512) *e = run_map<float, 512, 4, 4, 2, -256, true>(a, s);
+    else if (C <= 1024) *e = run_map<float, 512, 4, 8, 2, -256, true>(a, s);
+    else if (C <= 2048) *e = run_map<float, 512, 4, 16, 2, -256, true>(a, s);
     else return false;
   }
   return true;

@@ -11,6 +11,8 @@ namespace dcn {
 // 256 bf16 channels want four waves per SIMD more than the prefetch with dropout (64x256x196 17 us,
 // 21; 64x200x784 36, 41) and where 256 workgroups would get three tiles of 32 positions or fewer
 // (64x256x196 12.4 us, 14.4; 32x256x784, 800 tiles, 17.6, 17.8; 64x256x784 34, 31).
+// Above 512 channels fp32, above 1024 bf16 spill beside a prefetched tile (64x1024x196 fp32 with a
+// full gate 143 us with it, 96 without; 64x2048x49 bf16 44, 30).
 // More channels than a workgroup's registers hold take narrower tiles (32-byte runs of a
 // channel at 1024), which costs less than a second pass. false: no variant (C > 2048).
 bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
@@ -24,7 +26,7 @@ bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     else if (C <= 256) *e = run_map<bf16_t, 512, 4, 2, 2, 256, false>(a, s);
     else if (C <= 512) *e = run_map<bf16_t, 1024, 4, 2, 4, 0, false>(a, s);
     else if (C <= 1024) *e = run_map<bf16_t, 512, 2, 4, 2, 256, false>(a, s);
-    else if (C <= 2048) *e = run_map<bf16_t, 1024, 2, 4, 4, 256, false>(a, s);
+    else if (C <= 2048) *e = run_map<bf16_t, 512, 2, 8, 2, 0, false>(a, s);
     else return false;
   } else {
     if (C <= 32) *e = run_map<float, 256, 8, 1, 3, 0, false>(a, s);
@@ -32,8 +34,8 @@ bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     else if (C <= 128) *e = run_map<float, 256, 8, 4, 2, 512, false>(a, s);
     else if (C <= 256) *e = run_map<float, 512, 8, 4, 2, 256, false>(a, s);
     else if (C <= 512) *e = run_map<float, 512, 4, 4, 2, 256, false>(a, s);
-    else if (C <= 1024) *e = run_map<float, 512, 4, 8, 2, 256, false>(a, s);
-    else if (C <= 2048) *e = run_map<float, 1024, 4, 8, 4, 256, false>(a, s);
+    else if (C <= 1024) *e = run_map<float, 512, 4, 8, 2, 0, false>(a, s);
+    else if (C <= 2048) *e = run_map<float, 512, 4, 16, 2, 0, false>(a, s);
     else return false;
   }
   return true;

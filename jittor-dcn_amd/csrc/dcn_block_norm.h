@@ -1285,9 +1285,9 @@ hipError_t run_tiles(const BlockArgs& a, int images, int P, int per, int wgs, in
   q.tiles = (long)q.tpi * images;
   const bool params = BWD && (a.gs || a.gw1 || a.gb1 || a.gw2 || a.gb2);
   q.image_gate = BWD && a.gg && a.gate_kind == DCN_GATE_IMAGE;
-  // wgs: 0 one a tile as far as partials allow
+  // wgs: > 0 with a prefetch, < 0 without, 0 without and one a tile as far as partials allow
   q.wgs = (int)std::min<long>(
-      q.tiles, wgs ? wgs : params || q.image_gate ? kMaxWgs : 1 << 20);
+      q.tiles, wgs ? std::abs(wgs) : params || q.image_gate ? kMaxWgs : 1 << 20);
   q.group = maps && q.tpi >= kInterleave && q.wgs % kInterleave == 0 ? kInterleave : 1;
   if (params) q.part = a.ws;
   if (q.image_gate) q.gpart = a.ws + (size_t)(maps ? kMaxWgs : kRowWgs) * 5 * a.C;
