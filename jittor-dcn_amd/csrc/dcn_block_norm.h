@@ -1316,10 +1316,10 @@ inline bool one_run(const BlockArgs& a) {
 template <typename T, int NT, int LPR, int NV, int WPE, int WGS, bool BWD>
 hipError_t run_row(const BlockArgs& a, hipStream_t s) {
   auto pick = [](bool full, bool drop) {
-    return full ? (drop ? block_row<T, NT, LPR, NV, WPE, true, BWD, true, true, true>
-                        : block_row<T, NT, LPR, NV, WPE, true, BWD, true, false, true>)
-                : (drop ? block_row<T, NT, LPR, NV, WPE, true, BWD, false, true, true>
-                        : block_row<T, NT, LPR, NV, WPE, true, BWD, false, false, true>);
+    return full ? (drop ? block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, true, true, true>
+                        : block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, true, false, true>)
+                : (drop ? block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, false, true, true>
+                        : block_row<T, NT, LPR, NV, WPE, (WGS > 0), BWD, false, false, true>);
   };
   const bool one = one_run(a);
   return run_tiles<T, BWD>(a, one ? 1 : a.B, one ? a.B * a.P : a.P, NT / LPR, WGS, NT, false, pick,

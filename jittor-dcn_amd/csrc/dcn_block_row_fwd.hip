@@ -4,8 +4,10 @@
 namespace dcn {
 
 // Threads, lanes a row, vectors a lane, waves per SIMD, workgroups (each prefetches its next
-// rows). 16 channels a lane and two waves per SIMD: with four, or 32 channels a lane, the
-// registers spill (8192 x 1024 bf16: 15.8 us against 20.7 and 25.4). false: no variant.
+// rows; negative: does not). 16 channels a lane and two waves per SIMD: with four, or 32 channels
+// a lane, the registers spill (8192 x 1024 bf16: 15.8 us against 20.7 and 25.4). Above 8192
+// channels a row leaves no room for the next (512 x 16384 bf16 58 us with the prefetch, 28
+// without, fp32 103, 80; 1024 x 8192 bf16 19, 24, fp32 37, 47). false: no variant.
 bool block_row_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
   const int C = a.C;
   if (a.dtype == DCN_BF16) {
@@ -15,7 +17,7 @@ bool block_row_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     else if (C <= 2048) *e = run_row<bf16_t, 256, 128, 2, 2, 512, false>(a, s);
     else if (C <= 4096) *e = run_row<bf16_t, 256, 256, 2, 2, 512, false>(a, s);
     else if (C <= 8192) *e = run_row<bf16_t, 512, 512, 2, 2, 256, false>(a, s);
-    else if (C <= 16384) *e = run_row<bf16_t, 1024, 1024, 2, 4, 256, false>(a, s);
+    else if (C <= 16384) *e = run_row<bf16_t, 1024, 1024, 2, 4, -512, false>(a, s);
     else return false;
   } else {
     if (C <= 256) *e = run_row<float, 256, 16, 4, 2, 512, false>(a, s);
@@ -24,7 +26,7 @@ bool block_row_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
     else if (C <= 2048) *e = run_row<float, 256, 128, 4, 2, 512, false>(a, s);
     else if (C <= 4096) *e = run_row<float, 256, 256, 4, 2, 512, false>(a, s);
     else if (C <= 8192) *e = run_row<float, 512, 512, 4, 2, 256, false>(a, s);
-    else if (C <= 16384) *e = run_row<float, 1024, 1024, 4, 4, 256, false>(a, s);
+    else if (C <= 16384) *e = run_row<float, 1024, 1024, 4, 4, -512, false>(a, s);
     else return false;
   }
   return true;
