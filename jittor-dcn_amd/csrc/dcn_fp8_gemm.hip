@@ -446,6 +446,39 @@ __global__ __launch_bounds__(256) void fp8_gemm_join(GemmArgs g, int splits) {
   }
 }
 
+// The same for many splits of a small result: 16 threads share four columns, each adds every 16th
+// split in order, then theirs are added in order (256 x 64 in 128 splits 12.6 -> 4 us).
+template <bool WIDE>
+__global__ __launch_bounds__(256) void fp8_gemm_join_many(GemmArgs g, int splits) {
+  __shared__ f32x4 part[16][16];
+  const unsigned quads = (g.N + 3) / 4;
+  const size_t total = (size_t)g.M * g.N, all = (size_t)g.M * quads;
+  const int l = threadIdx.x >> 4, c = threadIdx.x & 15;
+  for (size_t i0 = (size_t)blockIdx.x * 16; i0 < all; i0 += (size_t)gridDim.x * 16) {
+    const size_t i = i0 + c;
+    const int m = (int)(i / quads), n = 4 * (int)(i - (size_t)m * quads);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (i < all) {
+      const float* p = g.part + (size_t)m * g.N + n;
+      if (n + 4 <= g.N) {
+#pragma unroll 4
+        for (int k = l; k < splits; k += 16) s += *reinterpret_cast<const f32x4_any*>(p + k * total);
+      } else {
+        for (int j = 0; n + j < g.N; ++j)
+          for (int k = l; k < splits; k += 16) s[j] += p[j + k * total];
+      }
+    }
+    part[l][c] = s;
+    __syncthreads();
+    if (l == 0 && i < all) {
+#pragma unroll
+      for (int k = 1; k < 16; ++k) s += part[k][c];
+      put4<WIDE>(g, column(g, n), m, n, s);
+    }
+    __syncthreads();
+  }
+}
+
 // ---- few rows on one side (tokens being served): nothing to reuse, so no LDS for the operands.
 // A workgroup takes 16 rows of the long side and all of K; its waves take the k blocks in
 // turn, each lane loading its 32 bytes of a block straight into MFMA operands (whole 128-byte
@@ -588,14 +621,20 @@ struct Plan {
 
 Plan plan(const dcn_fp8_matmul_desc& d) {
   const int few = std::min(d.M, d.N), nkb = d.K / 128;
-  if (few <= 64) return {Plan::FEW, 1, nkb};
+  // One workgroup per 16 rows of the long side, all of K in it: up to 64 tokens through a weight.
+  // Not the weight gradient of few channels (few workgroups, the tokens as K) and not many tokens
+  // to few channels (a workgroup reads the short side whole, and up to eight k blocks keep one
+  // wave each): 64 x 256 channels over 200704 tokens, weight gradient 471 -> 27 us, input
+  // gradient 94 -> 18; 64 x 64 over 50176 132 -> 13, 24 -> 6.
+  const long wgs = (std::max(d.M, d.N) + 15L) / 16;
+  if (few <= 64 && wgs <= 1024 && (nkb <= 64 || wgs >= 256)) return {Plan::FEW, 1, nkb};
   auto tiles = [&](int b) { return (long)((d.M + b - 1) / b) * ((d.N + b - 1) / b); };
   // A short K is all prologue and epilogue: three small workgroups a CU that take turns at them
   // beat one large one that overlaps its own stages (50176 x 1024 bf16 results, K = 256 / 512 /
   // 1024: 30 / 40 / 64 us, one stage in LDS; two stages 35 / 49 / 78; 256 x 256 tiles 36 / 47 / 66).
   if (nkb <= 8 && tiles(128) >= 768) return {Plan::SHORT, 1, nkb};
   // 256 x 256: half the LDS reads per product (16384 x 8192 x 8192, bf16: 0.94 ms; 128 x 128 1.7 ms)
-  if (tiles(256) >= 192) return {Plan::TILE256, 1, nkb};
+  if (few > 128 && tiles(256) >= 192) return {Plan::TILE256, 1, nkb};
   // Fewer tiles than CUs: parts of K, at least eight k blocks each, up to one workgroup a CU. (More
   // parts cost more in the joining than they save: 2048 x 2048 x 2048, 256 tiles, whole 16 us, in two
   // parts 16 + 7.5; 300 x 4096 x 4096, 96 tiles, whole 25, in two 17 + 4, in five 15 + 5.5;
@@ -624,13 +663,22 @@ hipError_t run_tiles(GemmArgs g, const Plan& p, bool wide, hipStream_t s) {
     hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, STAGES, true, true>), grid, block, 0, s, g);
   else
     hipLaunchKernelGGL((fp8_gemm<GA, GB, WM, WN, WPE, STAGES, false, true>), grid, block, 0, s, g);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const unsigned n = (unsigned)std::min<size_t>(((size_t)g.M * ((g.N + 3) / 4) + 255) / 256, 4096);
-  if (wide)
-    hipLaunchKernelGGL(fp8_gemm_join<true>, dim3(n), dim3(256), 0, s, g, p.splits);
-  else
-    hipLaunchKernelGGL(fp8_gemm_join<false>, dim3(n), dim3(256), 0, s, g, p.splits);
+  const size_t quads = (size_t)g.M * ((g.N + 3) / 4);
+  if (p.splits > 16) {
+    const dim3 n((unsigned)std::min<size_t>((quads + 15) / 16, 4096));
+    if (wide)
+      hipLaunchKernelGGL(fp8_gemm_join_many<true>, n, dim3(256), 0, s, g, p.splits);
+    else
+      hipLaunchKernelGGL(fp8_gemm_join_many<false>, n, dim3(256), 0, s, g, p.splits);
+  } else {
+    const dim3 n((unsigned)std::min<size_t>((quads + 255) / 256, 4096));
+    if (wide)
+      hipLaunchKernelGGL(fp8_gemm_join<true>, n, dim3(256), 0, s, g, p.splits);
+    else
+      hipLaunchKernelGGL(fp8_gemm_join<false>, n, dim3(256), 0, s, g, p.splits);
+  }
   return hipGetLastError();
 }
 

@@ -228,6 +228,25 @@ def test_wide_and_flat(tb, dt, K, ab, bb):
     assert torch.equal(tb.fp8_matmul(*ops, dt), (v[0].double() @ v[1].double().t()).to(dt))
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+@pytest.mark.parametrize("C,O,B,P", [(40, 24, 5, 4000), (70, 130, 3, 20001), (16, 7, 1, 60000),
+                                     (300, 64, 40, 900), (64, 64, 9, 1024)])
+def test_few_channels_many_tokens(tb, dt, layout, C, O, B, P):
+    """Few tiles of a long K, many splits of a small result; small integers, sums exact."""
+    g = torch.Generator(device="cuda").manual_seed(C)
+    ints = lambda n, *s: torch.randint(-n, n + 1, s, generator=g, device="cuda").to(dt)
+    sh = lambda c: (B, c, P, 1) if layout == "nchw" else (B, P, c)
+    x, w, gy = ints(2, *sh(C)).requires_grad_(), ints(2, O, C).requires_grad_(), ints(1, *sh(O))
+    y = tb.fp8_pointwise(x, w)
+    gx, gw = torch.autograd.grad(y, (x, w), gy)
+    flat = lambda t: (t[..., 0].transpose(1, 2) if layout == "nchw" else t).detach().double().reshape(B * P, -1)
+    X, W, G = flat(x), w.detach().double(), flat(gy)
+    assert torch.equal(flat(y), (X @ W.t()).to(dt).double())
+    assert torch.equal(flat(gx), (G @ W).to(dt).double())
+    assert torch.equal(gw, (G.t() @ X).to(dt))
+
+
 def test_k_beyond_the_tiles_offsets(tb):
     """K above 2^22: rows too long for the 32-bit offsets of the large tiles. A few columns hold
     values, the rest is zero."""
