@@ -621,13 +621,18 @@ struct Plan {
 
 Plan plan(const dcn_fp8_matmul_desc& d) {
   const int few = std::min(d.M, d.N), nkb = d.K / 128;
-  // One workgroup per 16 rows of the long side, all of K in it: up to 64 tokens through a weight.
-  // Not the weight gradient of few channels (few workgroups, the tokens as K) and not many tokens
-  // to few channels (a workgroup reads the short side whole, and up to eight k blocks keep one
-  // wave each): 64 x 256 channels over 200704 tokens, weight gradient 471 -> 27 us, input
-  // gradient 94 -> 18; 64 x 64 over 50176 132 -> 13, 24 -> 6.
-  const long wgs = (std::max(d.M, d.N) + 15L) / 16;
-  if (few <= 64 && wgs <= 1024 && (nkb <= 64 || wgs >= 256)) return {Plan::FEW, 1, nkb};
+  // One workgroup per 16 rows of the long side, all of K in it: a few tokens through a weight, as
+  // long as fragments x k blocks x rounds of the card stay below 128. us, and in tiles: 16 tokens
+  // 4096 x 4096 6.6, 12.7, 8192 x 8192 18, 20; 32 tokens 4096 x 4096 8.7, 12.9, 8192 x 8192 25, 21;
+  // 64 tokens 4096 x 4096 12.7, 14.0, 4096 x 8192 22, 15.
+  // Nor the weight gradient of few channels (few workgroups, the tokens as K) nor many tokens to
+  // few channels (a workgroup reads the short side whole, and up to eight k blocks keep one wave
+  // each): 64 x 256 channels over 200704 tokens, weight gradient 471 -> 27 us, input gradient
+  // 94 -> 18; 64 x 64 over 50176 132 -> 13, 24 -> 6.
+  const long wgs = (std::max(d.M, d.N) + 15L) / 16, frags = few <= 16 ? 1 : few <= 32 ? 2 : 4;
+  if (few <= 64 && wgs <= 1024 && nkb <= 64 &&
+      frags * std::max(nkb, 8) * std::max(256L, wgs) <= 128 * 256)
+    return {Plan::FEW, 1, nkb};
   auto tiles = [&](int b) { return (long)((d.M + b - 1) / b) * ((d.N + b - 1) / b); };
   // A short K is all prologue and epilogue: three small workgroups a CU that take turns at them
   // beat one large one that overlaps its own stages (50176 x 1024 bf16 results, K = 256 / 512 /
