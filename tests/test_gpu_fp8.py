@@ -213,9 +213,10 @@ def test_matmul_blocks(tb, dt, M, N, K, ab, bb):
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("K", [128, 256, 384, 1152])
 @pytest.mark.parametrize("ab,bb", [(1, 1), (1, 128), (128, 1), (128, 128)])
-def test_wide_and_flat(tb, dt, K, ab, bb):
-    """One row of large tiles, any number of stages; small integers, so that the sums are exact."""
-    M, N = 100, 49500
+@pytest.mark.parametrize("M,N", [(100, 49500), (200, 49000)])
+def test_wide_and_flat(tb, dt, M, N, K, ab, bb):
+    """One row of tiles, at 200 x 49000 of the largest (fewer than 768 of 128 x 128), any number of
+    stages; small integers, so that the sums are exact."""
     g = torch.Generator(device="cuda").manual_seed(K)
     v = [torch.randint(-4, 5, (rows, K), generator=g, device="cuda").float() for rows in (M, N)]
     ops = []
