@@ -1258,7 +1258,8 @@ __global__ __launch_bounds__(1024) void block_fold(BlockArgs a, Plan q, int k0) 
 
 constexpr int kMaxWgs = 1024;   // workgroups with partials, maps
 constexpr int kRowWgs = 512;    // and rows
-constexpr int kRowSums = 4096;  // channels of a row beside which the parameters' sums fit
+constexpr int kLongWgs = 256;   // and rows of more than
+constexpr int kRowSums = 4096;  // channels: beside those the parameters' sums fit
 constexpr int kInterleave = 8;  // workgroups that share a run of map tiles
 
 // adds up the partials; a parameter without a destination ends at once
@@ -1290,7 +1291,7 @@ hipError_t run_tiles(const BlockArgs& a, int images, int P, int per, int wgs, in
       q.tiles, wgs ? std::abs(wgs) : params || q.image_gate ? kMaxWgs : 1 << 20);
   q.group = maps && q.tpi >= kInterleave && q.wgs % kInterleave == 0 ? kInterleave : 1;
   if (params) q.part = a.ws;
-  if (q.image_gate) q.gpart = a.ws + (size_t)(maps ? kMaxWgs : kRowWgs) * 5 * a.C;
+  if (q.image_gate) q.gpart = a.ws + (size_t)(maps ? kMaxWgs : kRowWgs) * 5 * a.C;  // (short rows)
   auto* fn = kernel(a.gate_kind == DCN_GATE_FULL, a.drop.thr != 0);
   hipLaunchKernelGGL(fn, dim3(q.wgs), dim3(threads), 0, s, a, q);
   const hipError_t e = hipGetLastError();
@@ -1330,6 +1331,7 @@ hipError_t run_row(const BlockArgs& a, hipStream_t s) {
 // ahead and the parameters read again for every row the sums fit (run_long_row).
 template <typename T, int NT, int NV, int WPE, int WGS>
 hipError_t run_gated_row(const BlockArgs& a, hipStream_t s) {
+  static_assert(WGS <= kLongWgs, "partials");
   auto pick = [](bool, bool drop) {
     return drop ? block_row<T, NT, NT, NV, WPE, false, true, true, true, true>
                 : block_row<T, NT, NT, NV, WPE, false, true, true, false, true>;
@@ -1365,10 +1367,10 @@ hipError_t run_long_row(const BlockArgs& a, hipStream_t s) {
   const int per = 4 * kParamRows / ElemVec<T>::N;
   q.tpi = (q.P + per - 1) / per;
   q.tiles = (long)q.tpi * q.images;
-  q.wgs = (int)std::min<long>({q.tiles, kRowWgs, std::max(1, 1024 / columns)});
+  q.wgs = (int)std::min<long>({q.tiles, kLongWgs, std::max(1, 1024 / columns)});
   q.image_gate = image_gate;
   if (params) q.part = rest;
-  if (image_gate) q.gpart = rest + (size_t)kRowWgs * 5 * a.C;
+  if (image_gate) q.gpart = rest + (size_t)kLongWgs * 5 * a.C;
   auto* pn = full ? (drop ? block_row_params<T, true, true> : block_row_params<T, true, false>)
                   : (drop ? block_row_params<T, false, true> : block_row_params<T, false, false>);
   hipLaunchKernelGGL(pn, dim3(q.wgs, columns), dim3(256), 0, s, a, q);
