@@ -728,7 +728,9 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
 
   int cv[NV];  // valid elements of a vector
   // The parameters of this lane's channels: kept beside a prefetched row, read again (from the
-  // caches) for every row where the registers are needed for the sums.
+  // caches) for every row where the registers are needed for the sums. Past the last channel they
+  // are 0, given or not: x is 0 there, but its normalised value -m r is not, and the factors' zeros
+  // keep it out of out, of N_pre's moments and of the backward's sums.
   const void* const pars[5] = {a.scale, a.w1, a.b1, a.w2, a.b2};
   u32x4 kept[AHEAD ? (BWD ? 4 : 5) : 1][NV];
   auto fetch = [&](int k, int j) {
@@ -737,7 +739,7 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
     if (pars[k]) return ldv_raw(ptr(pars[k]) + (lane + LPR * j) * V, cv[j]);
     float t[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) t[e] = k == 2 || k == 4 ? 0.f : 1.f;
+    for (int e = 0; e < V; ++e) t[e] = k == 2 || k == 4 || e >= cv[j] ? 0.f : 1.f;
     return pack<T>(t);
   };
 #pragma unroll

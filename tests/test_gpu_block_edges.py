@@ -1,0 +1,71 @@
+"""GPU: block norms where an argument is absent, a value is not finite or a channel count leaves
+a vector half filled, against the 64-bit oracle with the bounds of test_gpu_block_norm.py."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import block_oracle as BO  # noqa: E402
+import test_gpu_block_norm as N  # noqa: E402
+
+U, SEED, OFF = N.U, N.SEED, N.OFF
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def tb():
+    import torch_block
+    return torch_block
+
+
+NEUTRAL = {"scale": 1.0, "w_post": 1.0, "b_post": 0.0, "w_pre": 1.0, "b_pre": 0.0}
+
+
+def absent_equals_neutral(tb, layout, B, C, P, dt, post, pre, gate, act, keep=(), p=0.0):
+    """A call without the parameters that are not in `keep` gives the bits, results and gradients,
+    of one with ones for scale and weights and zeros for biases (which other tests hold against
+    the oracle)."""
+    t, go, gy = N.tensors(layout, B, C, P, dt, post, pre, gate, shift=3.0, seed=C)
+    got = []
+    for absent in (True, False):
+        u = {}
+        for k, v in t.items():
+            if k not in NEUTRAL or k in keep:
+                u[k] = v.clone()
+            elif not absent:
+                u[k] = torch.full_like(v, NEUTRAL[k])
+        for v in u.values():
+            v.requires_grad_()
+        out = N.call(tb, u, post, pre, act, p=p)
+        out = [(v, g) for v, g in zip(out, (go, gy)) if v is not None]
+        grads = torch.autograd.grad([v for v, _ in out], list(u.values()), [g for _, g in out])
+        got.append({**dict(zip(u, grads)), **dict(zip(("out", "y"), (v for v, _ in out)))})
+    for k, v in got[0].items():
+        assert torch.equal(v, got[1][k]), k
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layout", ["nchw", "rows"])
+@pytest.mark.parametrize("post,pre", [("layer", "rms"), ("layer", "layer"), ("layer", None),
+                                      ("rms", "layer"), ("rms", "rms"), (None, "layer")])
+@pytest.mark.parametrize("gate,act", [("none", "linear"), ("image", "sigmoid"), ("full", "sigmoid")])
+@pytest.mark.parametrize("keep", [(), ("scale",), ("w_post",), ("b_post",), ("w_pre", "b_pre")])
+def test_absent_parameters(tb, dt, layout, post, pre, gate, act, keep):
+    """50 channels, no whole number of vectors, and means that are not zero: a NULL weight is 1 for
+    the channels there are and adds nothing past the last."""
+    absent_equals_neutral(tb, layout, 3, 50, 13, dt, post, pre, gate, act, keep)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("C", [1, 3, 9, 33, 50, 100, 130, 257, 515, 1001, 2049, 4097, 8197, 16383,
+                               16387])
+@pytest.mark.parametrize("gate,p", [("none", 0.0), ("full", 0.0), ("image", 0.25)])
+def test_absent_parameters_at_every_row_variant(tb, dt, C, gate, p):
+    absent_equals_neutral(tb, "rows", 2, C, 3, dt, "layer", "layer", gate, "sigmoid", p=p)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("C", [3, 33, 65, 130, 257, 513, 1025, 2049])
+def test_absent_parameters_at_every_map_variant(tb, dt, C):
+    absent_equals_neutral(tb, "nchw", 2, C, 11, dt, "layer", "layer", "full", "sigmoid")
+    absent_equals_neutral(tb, "nchw", 5, C, 1, dt, "layer", "rms", "none", "linear")
