@@ -77,6 +77,18 @@ def _wants_grad(*tensors):
     return False
 
 
+def _number(v, what):
+    """v as it is now, as a float: the library takes numbers, and descriptors are kept by them."""
+    if type(v) is float:
+        return v
+    if isinstance(v, torch.Tensor):
+        if v.requires_grad and torch.is_grad_enabled():
+            raise TypeError(f"{what} is a number, which gets no gradient (a learnable factor per "
+                            "channel is block_norm's scale)")
+        v = v.detach()
+    return float(v)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -169,6 +181,7 @@ def dropout(x, p, rng, group="element", residual=None):
     x's logical order, whatever its strides."""
     _dtype(x, "dropout")
     _same(x, residual, "dropout", "residual")
+    p = _number(p, "dropout: p")
     if not 0.0 <= p <= 1.0:
         raise ValueError("dropout: p must be between 0 and 1")
     if isinstance(group, str):
@@ -180,7 +193,7 @@ def dropout(x, p, rng, group="element", residual=None):
             group *= s
     if group < 1 and x.numel():
         raise ValueError("dropout: group must be positive")
-    args = (x, residual, float(p), rng, max(int(group), 1))
+    args = (x, residual, p, rng, max(int(group), 1))
     return _Dropout.apply(*args) if _wants_grad(x, residual) else _drop(*args)[0]
 
 
@@ -312,7 +325,9 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     and channel, through gate_act "linear", "sigmoid" or "silu". scale, *_weight, *_bias: [C].
     drop: "element" (elements count in memory order) or "image". Without a residual out = t;
     without x the operator is the pre norm alone and out is the residual. All tensors have
-    x's dtype; everything but the rounding of the results is fp32."""
+    x's dtype; everything but the rounding of the results is fp32. alpha, eps and drop_p are
+    numbers: a tensor there counts with its value at the call, and one that wants a gradient is
+    refused."""
     ref = residual if x is None else x
     if ref is None:
         raise ValueError("block_norm: neither x nor a residual")
@@ -320,6 +335,7 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     if post not in _NORM or pre not in _NORM or gate_act not in _ACT:
         raise ValueError("block_norm: norms are None, 'rms' or 'layer'; gate_act is 'linear', "
                          "'sigmoid' or 'silu'")
+    drop_p = _number(drop_p, "block_norm: drop_p")
     if drop not in ("element", "image") or not 0.0 <= drop_p <= 1.0:
         raise ValueError("block_norm: drop is 'element' or 'image' and 0 <= drop_p <= 1")
     layout, B, C, P, mf = _layout(ref)
@@ -337,7 +353,9 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     _same(ref, pre_weight, "block_norm", "pre_weight", shape)
     _same(ref, pre_bias, "block_norm", "pre_bias", shape)
     e1, e2 = eps if isinstance(eps, (tuple, list)) else (eps, eps)
-    fields = (B, C, P, layout, dt, _NORM[post], _NORM[pre], kind, _ACT[gate_act], e1, e2, alpha)
+    fields = (B, C, P, layout, dt, _NORM[post], _NORM[pre], kind, _ACT[gate_act],
+              _number(e1, "block_norm: eps"), _number(e2, "block_norm: eps"),
+              _number(alpha, "block_norm: alpha"))
     dev_rng = None
     if drop_p > 0:
         seed, offset, dev_rng = _rng(rng, ref.device, "block_norm")
