@@ -15,6 +15,7 @@ tensor is updated between replays). The backward draws the same mask again.
 Forward and backward may be captured into a graph. As with every torch operator, let go of the
 results of earlier eager passes over the same leaf tensors (and of their losses) first: a leaf's
 accumulation node lives as long as a graph that holds it and stays on the stream it was made on.
+Refused are forward-mode derivatives (there are none) and torch.jit.trace.
 """
 from __future__ import annotations
 
@@ -23,6 +24,7 @@ import functools
 import threading
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch.autograd.function import once_differentiable
 
 import dcn_runtime as rt
@@ -48,6 +50,9 @@ def _fn(name):
 
 def _call(dev: torch.device, name: str, *args):
     """One libdcn call on torch's current stream of `dev`, whatever device is current."""
+    if torch._C._is_tracing():
+        raise RuntimeError("torch_block's calls cannot be traced: a trace would keep their empty "
+                           "results, or their sizes for tensors of others (capture a graph)")
     idx = dev.index
     if idx != torch._C._cuda_getDevice():
         with torch.cuda.device(idx):
@@ -70,6 +75,10 @@ def _call(dev: torch.device, name: str, *args):
 
 
 def _wants_grad(*tensors):
+    """Autograd has to see the call: for a gradient, or inside a forward-mode level, where it refuses
+    a tensor with a tangent (there are no forward-mode derivatives)."""
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -572,7 +581,8 @@ def fp8_pointwise(x, weight):
         if weight.in_features != C or weight.q.device != x.device:
             raise ValueError(f"fp8_pointwise: the weight takes {weight.in_features} channels on "
                              f"{weight.q.device}, x has {C} on {x.device}")
-        if torch.is_grad_enabled() and x.requires_grad:
+        if torch.is_grad_enabled() and x.requires_grad or \
+                forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError("fp8_pointwise: an Fp8Weight is for inference (no gradients)")
         O = weight.out_features
     else:

@@ -25,11 +25,12 @@ def tb(monkeypatch):
             view(a[0].out, n).copy_(d.alpha * view(a[0].x, n))
 
     calls = []
+    tb.real_call = tb._call
     monkeypatch.setattr(tb, "_call", call)
     monkeypatch.setattr(tb, "_dtype", lambda x, what: tb._DT[x.dtype])
     tb.calls = calls
     yield tb
-    del tb.calls
+    del tb.calls, tb.real_call
     tb._block_desc.cache_clear()
 
 
@@ -66,3 +67,53 @@ def test_a_learnable_alpha_is_refused(tb):
     m = tb.BlockNorm(4, post=None, pre=None, alpha=torch.nn.Parameter(torch.tensor(2.0)))
     with pytest.raises(TypeError, match="no gradient"):
         m(x)
+
+
+def test_forward_mode_is_refused(tb):
+    """A tangent is never dropped: the operators have no forward-mode derivative and say so."""
+    import torch.autograd.forward_ad as fa
+    x = torch.ones(2, 4)
+    with fa.dual_level():
+        dual = fa.make_dual(x, torch.ones(2, 4))
+        for f in (lambda: tb.dropout(dual, 0.5, (1, 2)),
+                  lambda: tb.dropout(x, 0.5, (1, 2), residual=dual),
+                  lambda: tb.block_norm(dual), lambda: tb.block_norm(x, dual),
+                  lambda: tb.block_norm(x, scale=fa.make_dual(torch.ones(4), torch.ones(4))),
+                  lambda: tb.fp8_pointwise(dual, torch.ones(3, 4))):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                f()
+        assert float(tb.dropout(x, 0.5, (1, 2))[0, 0]) == 2.0  # no tangent, nothing to refuse
+
+
+def _served(tb, o, c):
+    w = tb.Fp8Weight.__new__(tb.Fp8Weight)
+    w.q = torch.zeros(o, 128, dtype=torch.uint8)
+    w.exponents = torch.zeros(1, 1, dtype=torch.uint8)
+    w.out_features, w.in_features = o, c
+    return w
+
+
+def test_forward_mode_of_a_served_product_is_refused(tb):
+    import torch.autograd.forward_ad as fa
+    with fa.dual_level():
+        dual = fa.make_dual(torch.ones(2, 4), torch.ones(2, 4))
+        with pytest.raises(RuntimeError, match="inference"):
+            tb.fp8_pointwise(dual, _served(tb, 3, 4))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_tracing_is_refused(tb, monkeypatch):
+    """torch.jit.trace records torch's operations: it would keep the empty result that a call fills,
+    or the call with the sizes of the traced tensors. Nothing is recorded instead."""
+    monkeypatch.setattr(tb, "_call", tb.real_call)
+    x, w = torch.ones(2, 4), torch.ones(3, 4)
+    for f, args in ((lambda x: tb.dropout(x, 0.5, (1, 2)) + 1, (x,)),
+                    (lambda x: tb.dropout(x, 0.5, (1, 2)) + 1, (x.clone().requires_grad_(),)),
+                    (lambda x: tb.block_norm(x, alpha=3.0)[0] + 1, (x,)),
+                    (lambda x: tb.block_norm(x, alpha=3.0)[0] + 1, (x.clone().requires_grad_(),)),
+                    (lambda x: tb.fp8_pointwise(x, w), (x,)),
+                    (lambda x: tb.fp8_pointwise(x, _served(tb, 3, 4)), (x,)),
+                    (lambda x: tb.fp8_quantize(x)[0], (x,)),
+                    (lambda w: tb._quantize_weight(w, True, False)[0], (w,))):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, args, check_trace=False)
