@@ -332,8 +332,8 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     it is), else the last. post / pre: None, "rms" or "layer" (None: no norm after the block;
     no y); eps: one number, or (post, pre). gate: of x's shape, or [B, C] for one per image
     and channel, through gate_act "linear", "sigmoid" or "silu". scale, *_weight, *_bias: [C].
-    drop: "element" (elements count in memory order) or "image". Without a residual out = t;
-    without x the operator is the pre norm alone and out is the residual. All tensors have
+    drop: "element" (elements count in memory order) or "image", one draw per x[b] (stochastic
+    depth; a row of a 2-d tensor, as in dropout). Without a residual out = t; without x the operator is the pre norm alone and out is the residual. All tensors have
     x's dtype; everything but the rounding of the results is fp32. alpha, eps and drop_p are
     numbers: a tensor there counts with its value at the call, and one that wants a gradient is
     refused."""
@@ -348,6 +348,10 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     if drop not in ("element", "image") or not 0.0 <= drop_p <= 1.0:
         raise ValueError("block_norm: drop is 'element' or 'image' and 0 <= drop_p <= 1")
     layout, B, C, P, mf = _layout(ref)
+    if drop == "image" and drop_p > 0 and ref.dim() == 2:  # an image of one position per row
+        if gate is not None and gate.shape == (1, C):
+            gate = gate.expand(ref.shape)
+        B, P = P, 1
     kind = rt.DCN_GATE_NONE
     if gate is not None:
         image = gate.dim() == 2 and tuple(gate.shape) == (B, C) and gate.shape != ref.shape

@@ -117,3 +117,16 @@ def test_tracing_is_refused(tb, monkeypatch):
                     (lambda w: tb._quantize_weight(w, True, False)[0], (w,))):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, args, check_trace=False)
+
+
+def test_image_draws_of_flat_features(tb):
+    """drop="image" draws once per x[b], for features [N, C] too, as dropout(group="image")."""
+    x = torch.ones(6, 4)
+    tb.block_norm(x, drop_p=0.5, drop="image", rng=(1, 2))
+    d = tb.calls[-1][1]
+    assert (d.B, d.C, d.P, d.drop_image) == (6, 4, 1, 1)
+    tb.block_norm(x, drop_p=0.5, rng=(1, 2))  # per element: one run of tokens, as before
+    assert (tb.calls[-1][1].B, tb.calls[-1][1].P) == (1, 6)
+    tb.block_norm(x, torch.ones(6, 4), gate=torch.ones(1, 4), drop_p=0.5, drop="image", rng=(1, 2))
+    d = tb.calls[-1][1]
+    assert (d.B, d.P, d.gate) == (6, 1, rt.DCN_GATE_FULL)

@@ -69,3 +69,24 @@ def test_absent_parameters_at_every_row_variant(tb, dt, C, gate, p):
 def test_absent_parameters_at_every_map_variant(tb, dt, C):
     absent_equals_neutral(tb, "nchw", 2, C, 11, dt, "layer", "layer", "full", "sigmoid")
     absent_equals_neutral(tb, "nchw", 5, C, 1, dt, "layer", "rms", "none", "linear")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_image_draws_of_flat_features(tb, dt):
+    """drop="image" on [N, C] draws once per row, as DropPath does."""
+    n, C = 40, 36
+    t, go, gy = N.tensors("rows", n, C, 1, dt, "rms", "layer", "none")
+    t = {k: v.reshape(n, C) if v.dim() == 3 else v for k, v in t.items()}
+    f = torch.from_numpy(BO.drop_factor(n, 1, 0.5, SEED, OFF)).cuda()
+    assert (f == 0).any() and (f > 0).any()
+    out, y = N.call(tb, t, "rms", "layer", "linear", p=0.5, drop="image")
+    assert torch.equal(out[f == 0], t["residual"][f == 0])
+    kept = N.call(tb, t, "rms", "layer", "linear", alpha=2.0)  # (the factor of p = 1/2)
+    assert torch.equal(out[f > 0], kept[0][f > 0]) and torch.equal(y[f > 0], kept[1][f > 0])
+    d = tb.dropout(t["x"], 0.5, (SEED, OFF), group="image")
+    assert torch.equal((d != 0).any(1), f > 0)
+    g = torch.randn(1, C, device="cuda").to(dt).requires_grad_()
+    u = {**t, "gate": g}
+    o2, _ = N.call(tb, u, "rms", "layer", "silu", p=0.5, drop="image")
+    gg, = torch.autograd.grad(o2, g, go.reshape(n, C))
+    assert gg.shape == (1, C) and bool(torch.isfinite(gg).all())
