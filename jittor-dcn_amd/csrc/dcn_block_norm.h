@@ -8,8 +8,8 @@
 //   dt = keep ? G · drop scale : 0
 //   ∂gate = dt · N_post(x) · alpha · scale · act'(gate),  ∂scale = Σ dt · N_post(x) · alpha · act
 //   ∂x = N_post'(dt · alpha · scale · act)
-// What dropout drops reaches no gradient, NaN and infinities neither: x and the gate count as 0
-// in those products (a dropped image's are not even read).
+// What dropout drops reaches no gradient, NaN and infinities neither: x and a full gate count as 0
+// in those products, an image gate's are left out (a dropped image's are not even read).
 // out is computed again from x and the residual (the residual is read instead of out, so that
 // costs no bytes), which keeps the backward free of out's rounding. The statistics come from
 // the forward where the caller kept them: 16 bytes a position, against two of the four rounds
@@ -323,7 +323,10 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
   bool inc[CPT];
   float mk[CPT];
   float sc[CPT], w1[CPT], b1[CPT], w2[CPT], b2[CPT];
-  float acc[5][CPT], accg[CPT];
+  // accd: Σ dt · N_post(x) under one gate (an image's, or none), from which its ∂gate and ∂scale
+  // follow at its end; seen: channels of which anything was kept
+  float acc[5][CPT], accd[CPT];
+  unsigned seen = 0u;
 #pragma unroll
   for (int i = 0; i < CPT; ++i) {
     const int c = cg + CG * i;
@@ -336,7 +339,7 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
     b2[i] = inc[i] ? par<T>(a.b2, c, 0.f) : 0.f;
 #pragma unroll
     for (int k = 0; k < 5; ++k) acc[k][i] = 0.f;
-    accg[i] = 0.f;
+    accd[i] = 0.f;
   }
   const int run = wg / q.group, turn = wg % q.group;
   const long t0 = first_tile(q, run) + turn, t1 = first_tile(q, run + 1), ts = q.group;
@@ -404,9 +407,11 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
     }
     unsigned keep[CPT];
     if constexpr (DROP) {
-      const unsigned img = in.gone ? 0u : 0xffu;
+      // past the map's end nothing is kept (a gate that is not finite may not reach the sums there)
+      const unsigned img = in.gone ? 0u : 0xffu, in_map = valid < V ? (1u << max(valid, 0)) - 1u : ~0u;
 #pragma unroll
-      for (int i = 0; i < CPT; ++i) keep[i] = a.drop_image ? img : keepv<V>(at[i], key, a.drop.thr);
+      for (int i = 0; i < CPT; ++i)
+        keep[i] = (a.drop_image ? img : keepv<V>(at[i], key, a.drop.thr)) & in_map;
     }
     auto kept = [&](int i, int e, float t) {
       if constexpr (DROP) return (keep[i] >> e) & 1u ? t : 0.f;
@@ -416,7 +421,6 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
       if constexpr (DROP) return kept(i, e, t * a.drop.scale);
       return t;
     };
-
     float* st = a.stats && !BWD ? a.stats + (size_t)b * a.P + (t % q.tpi) * TP : nullptr;
     const bool known = BWD && a.stats;
     if (known) sums.keep(in.st);
@@ -531,8 +535,9 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
 #pragma unroll
         for (int i = 0; i < CPT; ++i) {
           float xv[V], fv[V], gg[V];
-          const float ka = a.alpha * gv[i], kd = sc[i] * gd[i], k = sc[i] * gv[i];
+          const float k = sc[i] * gv[i];
           unpack<T>(in.x[i], xv);
+          if constexpr (DROP && !FULL) seen |= (unsigned)(keep[i] != 0u) << i;
           if constexpr (FULL) unpack<T>(in.g[i], fv);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
@@ -546,9 +551,8 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
               gg[e] = dtv * (sc[i] * ad);
               acc[0][i] = fmaf(dtv, a.alpha * av, acc[0][i]);
             } else {
-              dv = dt * k;
-              accg[i] = fmaf(dtv, kd, accg[i]);
-              acc[0][i] = fmaf(dtv, ka, acc[0][i]);
+              dv = kept(i, e, dt * k);  // (0 times a gate that is not finite is not 0)
+              accd[i] += dtv;
             }
             acc[1][i] = fmaf(dv, h, acc[1][i]);
             acc[2][i] += dv;
@@ -580,14 +584,21 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
             stv(static_cast<T*>(a.gx) + at[i], valid, o[i]);
           }
         }
-        if (q.image_gate && (t + ts >= t1 || (t + ts) / q.tpi != b)) {
-          float* dst = q.gpart + ((size_t)(run + b) * q.group + turn) * a.C;
+        // the last tile of this gate
+        if (!FULL && (t + ts >= t1 || (a.gate_kind == DCN_GATE_IMAGE && (t + ts) / q.tpi != b))) {
+          float* dst =
+              q.image_gate ? q.gpart + ((size_t)(run + b) * q.group + turn) * a.C : nullptr;
 #pragma unroll
           for (int i = 0; i < CPT; ++i) {
-            const float g = group_sum<PL>(accg[i]);
-            if (inc[i] && pl == 0) dst[cg + CG * i] = g;
-            accg[i] = 0.f;
+            const bool any = !DROP || (seen >> i & 1u);
+            acc[0][i] = any ? fmaf(accd[i], a.alpha * gv[i], acc[0][i]) : acc[0][i];
+            if (q.image_gate) {
+              const float g = group_sum<PL>(any ? accd[i] * (sc[i] * gd[i]) : 0.f);
+              if (inc[i] && pl == 0) dst[cg + CG * i] = g;
+            }
+            accd[i] = 0.f;
           }
+          seen = 0u;
         }
       }
     }
@@ -845,11 +856,12 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
 
     unsigned keep[NV];
     if constexpr (DROP) {
-      const unsigned img = in.gone ? 0u : 0xffu;
+      // nothing of a row behind the last is kept, as past a map's end
+      const unsigned img = in.gone ? 0u : 0xffu, in_rows = live ? ~0u : 0u;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        keep[j] = a.drop_image ? img
-                               : keepv<V>(base + (lane + LPR * j) * V, key, a.drop.thr);
+        keep[j] = (a.drop_image ? img : keepv<V>(base + (lane + LPR * j) * V, key, a.drop.thr)) &
+                  in_rows;
     }
     auto kept_or_0 = [&](int j, int e, float v) {
       if constexpr (DROP) return (keep[j] >> e) & 1u ? v : 0.f;
@@ -1037,10 +1049,19 @@ __global__ __launch_bounds__(NT, WPE) void block_row(BlockArgs a, Plan q) {
           for (int e = 0; e < V; ++e) {
             const float h = kept_or_0(j, e, (xv[e] - m1) * r1), v = fmaf(h, w1[e], b1[e]);
             const float dt = drop(j, e, o[j][e]), dtv = dt * v, k = a.alpha * sc[e];
-            const float dv = dt * (k * av[e]);
+            // (selected: 0 times an image gate that is not finite is not 0; a full one counts as 0)
+            float dv = dt * (k * av[e]);
             gg[e] = dtv * (k * ad[e]);
+            if constexpr (!FULL) {
+              dv = kept_or_0(j, e, dv);
+              gg[e] = kept_or_0(j, e, gg[e]);
+            }
             if constexpr (SUMS) {
-              acc[0][j][e] = fmaf(dtv, a.alpha * av[e], acc[0][j][e]);
+              const float sum = fmaf(dtv, a.alpha * av[e], acc[0][j][e]);
+              if constexpr (DROP && !FULL)
+                acc[0][j][e] = (keep[j] >> e) & 1u ? sum : acc[0][j][e];
+              else
+                acc[0][j][e] = sum;
               acc[1][j][e] = fmaf(dv, h, acc[1][j][e]);
               acc[2][j][e] += dv;
               if constexpr (!FULL) accg[j][e] += gg[e];
@@ -1156,6 +1177,7 @@ __global__ __launch_bounds__(256) void block_row_params(BlockArgs a, Plan q) {
         } else {
           keep[u] = keepv<V>(at, key, a.drop.thr);
         }
+        if (!live) keep[u] = 0u;
       }
       auto read = [&](const void* t) {
         return t && live ? ldv_raw(ptr(t) + at, cv) : u32x4{0u, 0u, 0u, 0u};
@@ -1201,11 +1223,15 @@ __global__ __launch_bounds__(256) void block_row_params(BlockArgs a, Plan q) {
           acc[4][e] += gyv[e];
           G = fmaf(st[u][3], gyv[e] * w2[e] - st[u][4] - h2 * st[u][5], G);
         }
-        const float dt = kept ? G * ds : 0.f, dv = dt * (k * av);
-        acc[0][e] = fmaf(dt * v, a.alpha * av, acc[0][e]);
+        const float dt = kept ? G * ds : 0.f, dv = kept ? dt * (k * av) : 0.f;
+        const float s0 = fmaf(dt * v, a.alpha * av, acc[0][e]);
+        acc[0][e] = kept ? s0 : acc[0][e];
         acc[1][e] = fmaf(dv, h, acc[1][e]);
         acc[2][e] += dv;
-        if constexpr (!FULL) accg[e] = fmaf(dt * v, k * ad, accg[e]);
+        if constexpr (!FULL) {
+          const float sg = fmaf(dt * v, k * ad, accg[e]);
+          accg[e] = kept ? sg : accg[e];
+        }
       }
     }
     if (q.image_gate && (t + 1 == t1 || (t + 1) % q.tpi == 0)) {  // uniform

@@ -90,3 +90,31 @@ def test_image_draws_of_flat_features(tb, dt):
     o2, _ = N.call(tb, u, "rms", "layer", "silu", p=0.5, drop="image")
     gg, = torch.autograd.grad(o2, g, go.reshape(n, C))
     assert gg.shape == (1, C) and bool(torch.isfinite(gg).all())
+
+
+@pytest.mark.parametrize("act", ["linear", "sigmoid", "silu"])
+@pytest.mark.parametrize("p", [0.5, 1.0])
+@pytest.mark.parametrize("layout,C", [("nchw", 48), ("nchw", 300), ("nchw", 2100), ("rows", 48),
+                                      ("rows", 300), ("rows", 3000), ("rows", 8000),
+                                      ("rows", 16500)])
+def test_an_image_gate_of_dropped_elements(tb, layout, C, p, act):
+    """A gate[b, c] whose elements are all dropped reaches nothing, NaN and infinities neither:
+    the bits that 0 gives there, in the results and in every gradient."""
+    B, P = 6, 3
+    t, go, gy = N.tensors(layout, B, C, P, torch.float32, "layer", "layer", "image")
+    f = torch.from_numpy(BO.drop_factor(B * C * P, 1, p, SEED, OFF))
+    f = f.reshape(B, C, P).transpose(1, 2) if layout == "nchw" else f.reshape(B, P, C)
+    gone = (f == 0).all(1).cuda()
+    assert gone.any() and (p == 1.0 or not gone.all())
+    results = []
+    for bad in (0.0, float("nan"), float("inf"), float("-inf")):
+        u = {k: v.clone() for k, v in t.items()}
+        u["gate"][gone] = bad
+        for v in u.values():
+            v.requires_grad_()
+        o, y = N.call(tb, u, "layer", "layer", act, p=p)
+        results.append([o, y, *torch.autograd.grad((o, y), list(u.values()), (go, gy))])
+    assert all(torch.isfinite(v).all() for v in results[0])
+    for r in results[1:]:
+        for k, a, b in zip(["out", "y", *t], results[0], r):
+            assert torch.equal(a, b), k
