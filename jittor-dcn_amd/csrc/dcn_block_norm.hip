@@ -35,7 +35,7 @@ struct Pos {
   __device__ float gate(int c) const {
     return drop_all ? 0.f : ld(a.gate, a.gate_kind == DCN_GATE_FULL ? base + c * cs : (size_t)b * a.C + c);
   }
-  __device__ float act(int c) const { return a.gate_kind ? gate_act(gate(c), a.act) : 1.f; }
+  __device__ float act(int c) const { return a.gate_kind ? gate_act<T>(gate(c), a.act) : 1.f; }
   __device__ float k(int c) const { return a.alpha * par(a.scale, c, 1.f) * act(c); }
   __device__ bool kept(int c) const {
     return !a.drop.thr || (a.drop_image ? !drop_all : keep1(base + c * cs, key, a.drop.thr));
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(kThreads) void block_any_bwd(BlockArgs a) {
       const float dt = a.drop.thr ? g * a.drop.scale : g;
       if (a.gg && a.gate_kind == DCN_GATE_FULL) {
         float av, ad;
-        gate_act_grad(q.gate(c), a.act, av, ad);
+        gate_act_grad<T>(q.gate(c), a.act, av, ad);
         const float gg = dt * q.v(c) * (a.alpha * q.par(a.scale, c, 1.f)) * ad;
         static_cast<T*>(a.gg)[i] = from_f32(kept ? gg : 0.f, T());
       }
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void block_any_params(BlockArgs a) {
       if (!a.x || !q.kept(c)) continue;
       const float dt = a.drop.thr ? g * a.drop.scale : g, v = q.v(c);
       float av = 1.f, ad = 0.f;
-      if (a.gate_kind) gate_act_grad(q.gate(c), a.act, av, ad);
+      if (a.gate_kind) gate_act_grad<T>(q.gate(c), a.act, av, ad);
       sum[0] = fmaf(dt * v, a.alpha * av, sum[0]);
       sg = fmaf(dt * v * (a.alpha * q.par(a.scale, c, 1.f)), ad, sg);
       if (a.post) {

@@ -118,3 +118,43 @@ def test_an_image_gate_of_dropped_elements(tb, layout, C, p, act):
     for r in results[1:]:
         for k, a, b in zip(["out", "y", *t], results[0], r):
             assert torch.equal(a, b), k
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("layout,C", [("nchw", 16), ("nchw", 2064), ("rows", 16), ("rows", 16400)])
+@pytest.mark.parametrize("gate", ["full", "image"])
+def test_gate_values(tb, dt, act, layout, C, gate):
+    """act(g) and act'(g) alone (x = 1, nothing else) over the whole range of g.
+
+    With u = 2^-24: e = exp(-|g|) to 1 ulp (2 u) and 1 / (1 + e) to 2 u of a sum rounded once;
+    sigmoid = e or 1 times that: 2 + 2 + 1 + 2 + 1 = 8 u of its value, 1 - sigmoid the same; silu
+    one product more. sigmoid' = s (1 - s): 17 u. silu' = s (1 + g (1 - s)): 8 + 8 + 4 u of s (1 +
+    |g| (1 - s)). Each product with x, the scale of 1 and the incoming gradient of 1 is exact.
+    Results below 2^-126 are multiples of 2^-149, half of one off in each of up to four steps, the
+    silu's multiplied by |g| <= 110 after the first. In bf16 e's argument is a rounded product with a
+    rounded constant, 2 |g| u more in each of its two uses, the result has its half step, and what
+    lies below 110 times the smallest normal may be 0."""
+    n = C * 64
+    g = torch.cat([torch.linspace(-110, 110, n // 2), torch.linspace(-9, 9, n - n // 2)])
+    g = g[torch.randperm(n, generator=torch.Generator().manual_seed(1))]
+    if gate == "image":
+        B, P, gsh = 64, 1, (64, C)
+    else:
+        B, P, gsh = 1, 64, (1, C, 64, 1) if layout == "nchw" else (1, 64, C)
+    shape = (B, C, P, 1) if layout == "nchw" else (B, P, C)
+    x = torch.ones(shape, device="cuda", dtype=dt)
+    g = g.reshape(gsh).to("cuda", dt).requires_grad_()
+    out, _ = tb.block_norm(x, gate=g, gate_act=act)
+    d, = torch.autograd.grad(out, g, torch.ones_like(out))
+    G = g.detach().cpu().double()
+    s, t = torch.sigmoid(G), torch.sigmoid(-G)
+    bf = dt == torch.bfloat16
+    more, half, tiny = (2 * G.abs(), 2.0 ** -8, 110 * 2.0 ** -126) if bf else (0, 0, 110 * 2.0 ** -147)
+    want, slope = (s, s * t) if act == "sigmoid" else (G * s, s * (1 + G * t))
+    mag = s * t if act == "sigmoid" else s * (1 + G.abs() * t)
+    got = out.detach().cpu().double().reshape(G.shape)
+    err = (got - want).abs() / (((9 + more) * U + half) * want.abs() + tiny)
+    assert float(err.max()) <= 1, (float(err.max()), float(G.flatten()[err.argmax()]))
+    err = (d.cpu().double() - slope).abs() / ((20 + 2 * more) * U * mag + half * slope.abs() + tiny)
+    assert float(err.max()) <= 1, (float(err.max()), float(G.flatten()[err.argmax()]))
