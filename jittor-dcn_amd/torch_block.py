@@ -200,9 +200,9 @@ def dropout(x, p, rng, group="element", residual=None):
         group = 1
         for s in x.shape[skip:]:
             group *= s
-    if group < 1 and x.numel():
-        raise ValueError("dropout: group must be positive")
-    args = (x, residual, p, rng, max(int(group), 1))
+    if group != int(group) or (group < 1 and x.numel()):
+        raise ValueError("dropout: group must be a whole number of elements")
+    args = (x, residual, p, rng, max(min(int(group), x.numel()), 1))  # (all of them: one draw)
     return _Dropout.apply(*args) if _wants_grad(x, residual) else _drop(*args)[0]
 
 

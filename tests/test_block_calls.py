@@ -130,3 +130,15 @@ def test_image_draws_of_flat_features(tb):
     tb.block_norm(x, torch.ones(6, 4), gate=torch.ones(1, 4), drop_p=0.5, drop="image", rng=(1, 2))
     d = tb.calls[-1][1]
     assert (d.B, d.P, d.gate) == (6, 1, rt.DCN_GATE_FULL)
+
+
+def test_dropout_groups_of_any_size(tb):
+    """A group above the element count is one draw; it never wraps around in 64 bits."""
+    x = torch.ones(2, 4)
+    for g in (8, 9, 2 ** 63, 2 ** 64 + 1, 10 ** 30):
+        tb.dropout(x, 0.5, (1, 2), group=g)
+        assert tb.calls[-1][1].group >= 8
+    with pytest.raises(ValueError, match="group"):
+        tb.dropout(x, 0.5, (1, 2), group=2.5)
+    with pytest.raises(ValueError, match="group"):
+        tb.dropout(x, 0.5, (1, 2), group=0)
