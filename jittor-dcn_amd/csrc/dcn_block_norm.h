@@ -1301,6 +1301,24 @@ constexpr int kLongWgs = 256;   // and rows of more than
 constexpr int kRowSums = 4096;  // channels: beside those the parameters' sums fit
 constexpr int kInterleave = 8;  // workgroups that share a run of map tiles
 
+// Workgroups that leave partials, at most: those of the variant, and no more than a call has tiles
+// (of a row, or of 16 positions of a map, at least). The workspace's size and layout go by it.
+inline int long_columns(const BlockArgs& a) {  // workgroups across the channels in block_row_params
+  const int per = 64 * (a.dtype == DCN_BF16 ? ElemVec<bf16_t>::N : ElemVec<float>::N);
+  return (a.C + per - 1) / per;
+}
+inline int partial_wgs(const BlockArgs& a) {
+  const bool rows = a.layout == DCN_NHWC || a.P == 1;
+  const long tiles = (long)a.B * (rows ? a.P : (a.P + 15) / 16);
+  long wgs = kMaxWgs;
+  if (rows && a.C <= kRowSums) wgs = kRowWgs;
+  if (rows && a.C > kRowSums) {
+    const bool gated = a.dtype == DCN_BF16 && a.C <= 8192 && a.gate_kind == DCN_GATE_FULL;
+    wgs = gated ? kLongWgs : std::min(kLongWgs, std::max(1, 1024 / long_columns(a)));
+  }
+  return (int)std::min(wgs, tiles);
+}
+
 // adds up the partials; a parameter without a destination ends at once
 template <typename T>
 hipError_t fold_partials(const BlockArgs& a, const Plan& q, hipStream_t s) {
@@ -1330,7 +1348,7 @@ hipError_t run_tiles(const BlockArgs& a, int images, int P, int per, int wgs, in
       q.tiles, wgs ? std::abs(wgs) : params || q.image_gate ? kMaxWgs : 1 << 20);
   q.group = maps && q.tpi >= kInterleave && q.wgs % kInterleave == 0 ? kInterleave : 1;
   if (params) q.part = a.ws;
-  if (q.image_gate) q.gpart = a.ws + (size_t)(maps ? kMaxWgs : kRowWgs) * 5 * a.C;  // (short rows)
+  if (q.image_gate) q.gpart = a.ws + (size_t)partial_wgs(a) * 5 * a.C;
   auto* fn = kernel(a.gate_kind == DCN_GATE_FULL, a.drop.thr != 0);
   hipLaunchKernelGGL(fn, dim3(q.wgs), dim3(threads), 0, s, a, q);
   const hipError_t e = hipGetLastError();
@@ -1402,14 +1420,14 @@ hipError_t run_long_row(const BlockArgs& a, hipStream_t s) {
     if (e != hipSuccess || !q.rowst) return e;
   }
   float* rest = a.ws + ((size_t)a.B * a.P * 6 + 63) / 64 * 64;
-  const int columns = (a.C + 64 * ElemVec<T>::N - 1) / (64 * ElemVec<T>::N);
+  const int columns = long_columns(a);
   const int per = 4 * kParamRows / ElemVec<T>::N;
   q.tpi = (q.P + per - 1) / per;
   q.tiles = (long)q.tpi * q.images;
-  q.wgs = (int)std::min<long>({q.tiles, kLongWgs, std::max(1, 1024 / columns)});
+  q.wgs = (int)std::min<long>(q.tiles, partial_wgs(a));
   q.image_gate = image_gate;
   if (params) q.part = rest;
-  if (image_gate) q.gpart = rest + (size_t)kLongWgs * 5 * a.C;
+  if (image_gate) q.gpart = rest + (size_t)partial_wgs(a) * 5 * a.C;
   auto* pn = full ? (drop ? block_row_params<T, true, true> : block_row_params<T, true, false>)
                   : (drop ? block_row_params<T, false, true> : block_row_params<T, false, false>);
   hipLaunchKernelGGL(pn, dim3(q.wgs, columns), dim3(256), 0, s, a, q);

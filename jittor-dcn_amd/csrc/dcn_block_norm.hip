@@ -280,7 +280,7 @@ size_t block_norm_ws_floats(const BlockArgs& a) {
   // six numbers a position for the passes, or partials of the parameters and of an image gate
   // (interleaved where an image has kInterleave tiles, of 16 positions at least)
   if (a.C > (rows ? kRowChannels : kMapChannels)) return 6 * (size_t)a.B * a.P;
-  const int wgs = !rows ? kMaxWgs : a.C > kRowSums ? kLongWgs : kRowWgs;
+  const int wgs = partial_wgs(a);
   const int group = rows || a.P <= 16 * (kInterleave - 1) ? 1 : kInterleave;
   size_t partials = (size_t)wgs * 5 * a.C;
   if (a.gate_kind == DCN_GATE_IMAGE) partials += (wgs + (size_t)a.B * group) * a.C;

@@ -142,3 +142,25 @@ def test_dropout_groups_of_any_size(tb):
         tb.dropout(x, 0.5, (1, 2), group=2.5)
     with pytest.raises(ValueError, match="group"):
         tb.dropout(x, 0.5, (1, 2), group=0)
+
+
+def _workspace(**kw):
+    d = rt.BlockDesc(**{**dict(B=1, C=64, P=1, layout=rt.DCN_NHWC, dtype=rt.DCN_F32, post=1, pre=1,
+                               alpha=1.0), **kw})
+    n = ctypes.c_size_t()
+    rt.check(rt.load().dcn_block_norm_workspace(d, n))
+    return n.value
+
+
+@pytest.mark.parametrize("kw,floats", [
+    (dict(C=4096), 5 * 4096), (dict(C=4096, P=100), 100 * 5 * 4096),
+    (dict(C=4096, P=10000), 512 * 5 * 4096), (dict(C=8192), 64 + 5 * 8192),
+    (dict(C=16384, P=512, dtype=rt.DCN_BF16), 6 * 512 + 32 * 5 * 16384),
+    (dict(C=16384, P=512), 6 * 512 + 16 * 5 * 16384),
+    (dict(C=8192, P=512, dtype=rt.DCN_BF16, gate=rt.DCN_GATE_FULL), 6 * 512 + 256 * 5 * 8192),
+    (dict(B=2, C=256, P=49, layout=rt.DCN_NCHW), 8 * 5 * 256),
+    (dict(B=64, C=256, P=784, layout=rt.DCN_NCHW, gate=rt.DCN_GATE_IMAGE),
+     (1024 * 6 + 64 * 8) * 256)])
+def test_block_norm_workspace_holds_what_is_launched(kw, floats):
+    """Partials of no more workgroups than the call has tiles or its kernel launches."""
+    assert _workspace(**kw) == 4 * floats

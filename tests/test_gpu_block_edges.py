@@ -158,3 +158,35 @@ def test_gate_values(tb, dt, act, layout, C, gate):
     assert float(err.max()) <= 1, (float(err.max()), float(G.flatten()[err.argmax()]))
     err = (d.cpu().double() - slope).abs() / ((20 + 2 * more) * U * mag + half * slope.abs() + tiny)
     assert float(err.max()) <= 1, (float(err.max()), float(G.flatten()[err.argmax()]))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("gate", ["none", "full", "image"])
+@pytest.mark.parametrize("layout,B,C,P", [
+    ("rows", 1, 4096, 1), ("rows", 3, 4096, 300), ("rows", 5, 24, 7), ("rows", 2, 300, 2000),
+    ("rows", 1, 8192, 3), ("rows", 2, 6000, 700), ("rows", 2, 16384, 300), ("rows", 3, 16390, 5),
+    ("nchw", 2, 64, 5), ("nchw", 3, 48, 113), ("nchw", 70, 16, 130), ("nchw", 2, 256, 4000),
+    ("nchw", 3, 1500, 60), ("nchw", 2, 2050, 9), ("nchw", 9, 70, 1)])
+def test_backward_stays_in_its_workspace(tb, dt, gate, layout, B, C, P):
+    """With exactly dcn_block_norm_workspace bytes: what lies behind them stays, and the gradients are
+    those of a workspace of any contents."""
+    import ctypes
+
+    import dcn_runtime as rt
+    t, go, gy = N.tensors(layout, B, C, P, dt, "layer", "rms", gate, seed=P)
+    kind = {"none": rt.DCN_GATE_NONE, "full": rt.DCN_GATE_FULL, "image": rt.DCN_GATE_IMAGE}[gate]
+    d = rt.BlockDesc(B, C, P, rt.DCN_NCHW if layout == "nchw" else rt.DCN_NHWC, tb._DT[dt], 2, 1,
+                     kind, rt.DCN_ACT_SILU, 1e-6, 1e-6, 1.0, 0.0, 0, 0, 0)
+    n = ctypes.c_size_t()
+    rt.check(rt.load().dcn_block_norm_workspace(d, n))
+    behind, results = 1 << 22, []
+    for fill in (0, 255):
+        ws = torch.full((n.value + behind,), fill, dtype=torch.uint8, device="cuda")
+        g = {k: torch.empty_like(v) for k, v in t.items()}
+        io = rt.BlockIO(**{k: v.data_ptr() for k, v in t.items()}, grad_out=go.data_ptr(),
+                        grad_y=gy.data_ptr(), **{"grad_" + k: v.data_ptr() for k, v in g.items()})
+        tb._call(ws.device, "dcn_block_norm_bwd", d, io, ws.data_ptr(), n.value)
+        assert bool((ws[n.value:] == fill).all())
+        results.append(g)
+    for k, v in results[0].items():
+        assert torch.equal(v, results[1][k]) and bool(torch.isfinite(v).all()), k
