@@ -190,3 +190,39 @@ def test_backward_stays_in_its_workspace(tb, dt, gate, layout, B, C, P):
         results.append(g)
     for k, v in results[0].items():
         assert torch.equal(v, results[1][k]) and bool(torch.isfinite(v).all()), k
+
+
+# ---- the sums in 32 bits
+@pytest.mark.parametrize("layout,C,P", [("nchw", 64, 50), ("nchw", 256, 196), ("nchw", 512, 49),
+                                        ("nchw", 1024, 49), ("nchw", 2048, 33), ("rows", 64, 50),
+                                        ("rows", 256, 196), ("rows", 1024, 60), ("rows", 4096, 40),
+                                        ("rows", 8192, 24), ("rows", 16384, 24)])
+@pytest.mark.parametrize("post,pre", [("rms", "layer"), ("layer", "rms")])
+def test_sums_keep_fp32(tb, layout, C, P, post, pre):
+    """fp32 all the way: bounds of a few dozen roundings whatever the length (1e-4 of the magnitudes),
+    which half a bf16 step (2e-3) would pass many times over.
+
+    A sum over n values that each kernel takes as chains of at most m terms, joined by a tree
+    and a few partial sums, is off by at most (m + depth) u of its magnitudes: m <= 32 channels
+    of a thread, depth <= 6 lane steps + 16 waves. A parameter's gradient: at most 64 positions of a
+    thread here (4 images of P over the workgroups), the fold's 64 partials and 4 steps. So 96 u and
+    176 u of a sum's magnitudes in place of n u; two norms forward and two backward chain at most a
+    dozen such sums and products (16)."""
+    B = 4
+    t, go, gy = N.tensors(layout, B, C, P, torch.float32, post, pre, "full", seed=C)
+    for v in t.values():
+        v.requires_grad_()
+    out, y = N.call(tb, t, post, pre, "silu")
+    grads = torch.autograd.grad((out, y), list(t.values()), (go, gy))
+    ref = {k: N.rows(v, layout).requires_grad_() for k, v in t.items()}
+    kw = dict(post=post, pre=pre, act="silu")
+    ro, ry = BO.block_forward(ref, **kw)
+    rg = torch.autograd.grad((ro, ry), list(ref.values()), (N.rows(go, layout), N.rows(gy, layout)))
+    with torch.no_grad():
+        b = BO.block_bounds({k: v.detach() for k, v in ref.items()}, N.rows(go, layout),
+                            N.rows(gy, layout), **kw)
+    full = {"x", "residual", "gate"}
+    for k, a, r in [("out", out, ro), ("y", y, ry), *zip(t, grads, rg)]:
+        n = 96 if k in full or k in ("out", "y") else 176
+        err = (N.rows(a, layout) - r.detach()).abs() / (16 * n * U * b[k] + 1e-37)
+        assert float(err.max()) <= 1, (k, float(err.max()))
