@@ -292,7 +292,8 @@ int dcn_roi_pool_bwd_host(dcn_handle* h, const dcn_roi_desc* d, const float* fea
  * Tensors are dense, of the descriptor's dtype (parameters and gradients too), caller-owned
  * and on the handle's device. A map tensor is DCN_NCHW [B][C][P] or DCN_NHWC [B][P][C]
  * (token rows: B sequences of P tokens). Sums, statistics and everything between the loads
- * and the stores are fp32; each output is rounded once. Outputs are bitwise reproducible.
+ * and the stores are fp32 (8-bit products of bf16 results: dcn_fp8_matmul says what is not);
+ * each output is rounded once. Outputs are bitwise reproducible.
  * Every call may be captured into a graph. Unlike the entry points above, these leave the
  * thread's current device as they found it. */
 typedef enum { DCN_NCHW = 0, DCN_NHWC = 1 } dcn_layout;
@@ -378,7 +379,7 @@ int dcn_block_norm_bwd(dcn_handle* h, const dcn_block_desc* d, const dcn_block_i
 
 /* 8-bit pointwise products. A quantised matrix is q[rows][K] e4m3 bytes (OCP, 448 largest),
  * K a multiple of 128 (padded with zeros), 16-byte aligned, with exponent bytes
- * s[K / 128][stride], biased by 127: the value of q[r][k] is q · 2^(s[k / 128][r / block] - 127).
+ * s[K / 128][stride], biased by 127 (1 to 254): q[r][k] is worth q · 2^(s[k / 128][r / block] - 127).
  * block = 1: stride = rows rounded up to 128; block = 128: stride = rows / 128 rounded up;
  * s is 4-byte aligned. The exponent of a block is the smallest e >= -126 with max|v| <=
  * 448 · 2^e over its finite values; the bytes are round-to-nearest-even of v · 2^-e; an
@@ -391,7 +392,8 @@ typedef struct {
  *   by token:   q_tok[B*P][Cp], Cp = C rounded up to 128, s_tok[Cp/128][B*P up to 128]
  *   by channel: q_ch[C][Kt], the tokens as columns: DCN_NHWC Kt = B*P rounded up to 128;
  *               DCN_NCHW Kt = B * Pp, Pp = P rounded up to 128 (an image's blocks end with
- *               it), s_ch[Kt/128][C up to 128] */
+ *               it: at 7x7 positions 62 % of a weight gradient's K are zeros, at 14x14 23 %),
+ *               s_ch[Kt/128][C up to 128] */
 int dcn_fp8_quantize(dcn_handle* h, const dcn_fp8_desc* d, const void* v, void* q_tok,
                      void* s_tok, void* q_ch, void* s_ch);
 /* Quantise a weight w[O][C] in blocks of 128 x 128, as it stands (q[O][Cp], s[Cp/128][ceil(O/128)])
@@ -406,8 +408,14 @@ typedef struct {
   int P;                /* DCN_NCHW only */
   int out_dtype;        /* dcn_dtype */
 } dcn_fp8_matmul_desc;
-/* out = a · bᵀ with fp32 accumulation. ws: dcn_fp8_matmul_workspace bytes (may be 0, then
- * NULL), one per call in flight. */
+/* out = a · bᵀ. ws: dcn_fp8_matmul_workspace bytes (may be 0, then NULL), one per call in flight.
+ * out_dtype DCN_F32: products and sums are fp32, off by at most K · 2^-24 of Σ|a b|. The bytes are
+ * widened to bf16 for it: values count to multiples of 2^-133, and one that was rounded up to
+ * 2^128 is infinite.
+ * DCN_BF16: the 8-bit matrix instruction. Of every 8 neighbouring k's it cuts the products below
+ * 2^-13 of the largest one's power of two and adds what is left in fp32, so a result is off by up to
+ * 7 · 2^-13 of Σ|a b| (8.5e-4; the bytes themselves stand for their values to 2^-4) before it is
+ * rounded. Whoever wants fp32 sums there takes an fp32 result and rounds that. */
 int dcn_fp8_matmul_workspace(const dcn_fp8_matmul_desc* d, size_t* bytes);
 int dcn_fp8_matmul(dcn_handle* h, const dcn_fp8_matmul_desc* d, const void* a, const void* sa,
                    const void* b, const void* sb, void* out, void* ws, size_t ws_bytes);
@@ -415,7 +423,8 @@ int dcn_fp8_matmul(dcn_handle* h, const dcn_fp8_matmul_desc* d, const void* a, c
 /* A pointwise product of a map tensor in one call: y[.., O, ..] = w · x over the channels (a
  * linear layer of token rows, a 1x1 convolution of maps), both rounded as above (x by token,
  * w in 128 x 128 blocks), and its gradients
- *   grad_x = wᵀ · grad_y (grad_y by token),  grad_w = grad_y · xᵀ (both by channel). */
+ *   grad_x = wᵀ · grad_y (grad_y by token),  grad_w = grad_y · xᵀ (both by channel).
+ * Sums as in dcn_fp8_matmul for results of the descriptor's dtype. */
 typedef struct {
   int B, C, P, O;     /* x is a map tensor of C channels, y of O */
   int layout, dtype;

@@ -8,11 +8,13 @@
 //
 // The 8-bit MFMA does not add in 32 bits throughout: measured on the builtin, in every group of
 // 8 neighbouring k's the products are cut below 2^-13 of the largest one's power of two before
-// they are added (then fp32). An element is off by less than 7 · 2^-13 of its groups' largest
-// products, 1e-5 to 7e-5 of the result in practice: far inside the half step 2^-9 of a bf16
-// result, so those use it; an fp32 result (WIDE) multiplies the same bytes as bf16, which holds
-// every e4m3 value with its exponent, on the bf16 MFMA (fp32 sums, 1e-7), at half the rate and
-// a conversion per byte (v_cvt_scalef32_pk_bf16_fp8).
+// they are added (then fp32). A sum is off by less than 7 · 2^-13 = 8.5e-4 of its Σ|a b|, 1e-5 to
+// 7e-5 of the result in practice: inside the half step 2^-9 of a bf16 result unless the sum cancels
+// (and the bytes are worth their values to 2^-4 only), so those use it. An fp32 result (WIDE)
+// multiplies the same bytes as bf16 on the bf16 MFMA (fp32 sums, 1e-7), at half the rate and a
+// conversion per byte (v_cvt_scalef32_pk_bf16_fp8). bf16 holds every byte with its exponent but
+// for the ends of the range: below 2^-133 bits are lost (exponents under -124), and 448 · 2^120
+// covers values that e4m3 rounds up to 2^128, infinite there.
 //
 // Rows of a 64-row group are dealt to the fragments in turn (fragment f, lane r = row 4r + f):
 // one aligned dword of exponents then serves a lane's four fragments (the instruction picks the

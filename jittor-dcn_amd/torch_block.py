@@ -491,7 +491,10 @@ def fp8_quantize(x, tokens=True, channels=False):
 
 def fp8_matmul(a, a_exponents, b, b_exponents, dtype=torch.float32):
     """a · bᵀ of two matrices in 8 bits (fp8_quantize's or Fp8Weight's layouts; either may have
-    an exponent per row or per 128 rows), fp32 sums, as [a's rows, b's rows] of `dtype`."""
+    an exponent per row or per 128 rows), as [a's rows, b's rows] of `dtype`. float32: products and
+    sums in 32 bits. bfloat16: by the 8-bit matrix instruction, whose sums keep 13 bits below the
+    largest product of each 8 neighbouring k's (off by up to 8.5e-4 of Σ|a b|; include/dcn.h); where
+    that matters, take float32 and round it."""
     if dtype not in _DT:
         raise TypeError(f"fp8_matmul gives float32 or bfloat16, not {dtype}")
     K, blocks = a.shape[-1], []
@@ -573,8 +576,9 @@ class _Fp8Pointwise(torch.autograd.Function):
 def fp8_pointwise(x, weight):
     """x · weightᵀ over the channels (dim 1 of a 4-d tensor, else the last): a linear layer of
     token rows or a 1x1 convolution of maps, its products in 8 bits with one power-of-two scale
-    per 128 channels of a token (128 tokens of a channel in the weight's gradient; 128 x 128 of
-    the weight) and fp32 sums.
+    per 128 channels of a token (128 tokens of a channel in the weight's gradient, a map's blocks
+    ending with its image; 128 x 128 of the weight). Its sums are fp32 for float32 tensors, the
+    8-bit matrix instruction's for bfloat16 ones (fp8_matmul).
 
     weight: [O, C] (or [O, C, 1, 1]) of x's dtype, rounded in the call, gradients for both; or an
     Fp8Weight (no gradients), as a server keeps it."""

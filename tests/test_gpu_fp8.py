@@ -458,3 +458,38 @@ def test_more_than_2_31_elements(tb, layout):
         assert torch.equal(gx[part].double(), b @ w), i
         want += b.t() @ a
     assert torch.equal(gw.double(), want)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("T", [8, 300])
+@pytest.mark.parametrize("p", [-110, -118, -124, -126, -130, -134])
+def test_smallest_values(tb, dt, T, p):
+    """Blocks near the smallest exponent against a large weight: fp32 results take the values to
+    multiples of 2^-133 (half of one off), bf16 results as they are."""
+    g = torch.Generator().manual_seed(0)
+    x = (torch.rand((T, 256), generator=g) + 0.5) * \
+        torch.exp2(torch.randint(-8, 1, (T, 256), generator=g).float() + p)
+    x, w = x.to(dt), (torch.rand((200, 256), generator=g) * 2.0 ** 90).to(dt)
+    got = np64(tb.fp8_pointwise(x.cuda(), w.cuda()))
+    a, b = BO.fp8_value(np64(x), 1, 128), BO.fp8_value(np64(w), 128, 128)
+    if dt == torch.bfloat16:
+        return close(got, a, b, dt, "y")
+    ref, mag = a @ b.T, np.abs(a) @ np.abs(b).T
+    tol = (256 + 128) * U * mag + 2.0 ** -134 * np.abs(b).sum(1)
+    assert (np.abs(got - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("T", [8, 300])
+def test_largest_values(tb, T):
+    """The type's largest magnitude is worth 2^128 in e4m3 (its neighbour below it is 240 / 256 of
+    that): infinite in fp32's products, finite in bf16's; what rounds down stays finite in both."""
+    w = torch.eye(128)[:100] * 0.25
+    x = torch.full((T, 128), torch.finfo(torch.float32).min)
+    y = tb.fp8_pointwise(x.cuda(), w.cuda())
+    assert not bool(torch.isfinite(y[:, :100]).any())
+    x = torch.full((T, 128), torch.finfo(torch.bfloat16).min, dtype=torch.bfloat16)
+    y = tb.fp8_pointwise(x.cuda(), w.bfloat16().cuda())
+    assert bool((y == -2.0 ** 126).all())
+    for dt in DTYPES:
+        x = torch.full((T, 128), -247.0 * 2.0 ** 120, dtype=dt)
+        assert bool((tb.fp8_pointwise(x.cuda(), w.to(dt).cuda()) == -240.0 * 2.0 ** 118).all())
