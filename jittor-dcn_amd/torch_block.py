@@ -15,7 +15,7 @@ tensor is updated between replays). The backward draws the same mask again.
 Forward and backward may be captured into a graph. As with every torch operator, let go of the
 results of earlier eager passes over the same leaf tensors (and of their losses) first: a leaf's
 accumulation node lives as long as a graph that holds it and stays on the stream it was made on.
-Refused are forward-mode derivatives (there are none) and torch.jit.trace.
+Refused are forward-mode derivatives (there are none), torch.jit.trace and make_fx.
 """
 from __future__ import annotations
 
@@ -33,6 +33,8 @@ _DT = {torch.float32: rt.DCN_F32, torch.bfloat16: rt.DCN_BF16}
 _handles = {}
 _lock = threading.Lock()  # a handle takes one caller at a time: stream and launch belong together
 _fns = {}
+_is_tracing, _mode = torch._C._is_tracing, torch._C._get_dispatch_mode
+_PROXY = torch._C._TorchDispatchModeKey.PROXY  # the mode under which torch.fx's make_fx records
 
 
 def _fn(name):
@@ -50,7 +52,7 @@ def _fn(name):
 
 def _call(dev: torch.device, name: str, *args):
     """One libdcn call on torch's current stream of `dev`, whatever device is current."""
-    if torch._C._is_tracing():
+    if _is_tracing() or _mode(_PROXY) is not None:
         raise RuntimeError("torch_block's calls cannot be traced: a trace would keep their empty "
                            "results, or their sizes for tensors of others (capture a graph)")
     idx = dev.index

@@ -103,8 +103,9 @@ def test_forward_mode_of_a_served_product_is_refused(tb):
 
 @pytest.mark.filterwarnings("ignore")
 def test_tracing_is_refused(tb, monkeypatch):
-    """torch.jit.trace records torch's operations: it would keep the empty result that a call fills,
-    or the call with the sizes of the traced tensors. Nothing is recorded instead."""
+    """torch.jit.trace and make_fx record torch's operations: they would keep the empty result that a
+    call fills, or the call with the sizes of the traced tensors. Nothing is recorded instead."""
+    from torch.fx.experimental.proxy_tensor import make_fx
     monkeypatch.setattr(tb, "_call", tb.real_call)
     x, w = torch.ones(2, 4), torch.ones(3, 4)
     for f, args in ((lambda x: tb.dropout(x, 0.5, (1, 2)) + 1, (x,)),
@@ -117,6 +118,8 @@ def test_tracing_is_refused(tb, monkeypatch):
                     (lambda w: tb._quantize_weight(w, True, False)[0], (w,))):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, args, check_trace=False)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f)(*args)
 
 
 def test_image_draws_of_flat_features(tb):
