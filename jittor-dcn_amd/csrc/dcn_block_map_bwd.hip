@@ -7,8 +7,8 @@ namespace dcn {
 // prefetch their next tile (negative: that do not; 0: up to 1024 that do not) by channels; the
 // fastest of those tried at 64 images. The prefetch, us with and without (layer norms, no gate;
 // then a full gate): bf16 256x784 54, 67; 74, 88   512x196 46, 50; 63, 72   1024x196 130, 97;
-// 182, 134   fp32 128x784 50, 48; 70, 64   256x784 92, 86; 134, 117   512x196 61, 59; 84, 78
-// 1024x196 226, 184; 254, 214: a second tile in registers costs fp32 and wide maps spills that
+// 182, 136   fp32 128x784 50, 48; 70, 66   256x784 92, 86; 134, 122   512x196 61, 59; 84, 82
+// 1024x196 226, 159; 254, 224: a second tile in registers costs fp32 and wide maps spills that
 // cost more than the wait. false: no variant (C > 2048).
 bool block_map_bwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {
   const int C = a.C;

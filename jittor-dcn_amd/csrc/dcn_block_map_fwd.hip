@@ -12,7 +12,7 @@ namespace dcn {
 // 21; 64x200x784 36, 41) and where 256 workgroups would get three tiles of 32 positions or fewer
 // (64x256x196 12.4 us, 14.4; 32x256x784, 800 tiles, 17.6, 17.8; 64x256x784 34, 31).
 // Above 512 channels fp32, above 1024 bf16 spill beside a prefetched tile (64x1024x196 fp32 with a
-// full gate 143 us with it, 96 without; 64x2048x49 bf16 44, 30).
+// full gate 143 us with it, 103 without; 64x2048x49 bf16 44, 30).
 // More channels than a workgroup's registers hold take narrower tiles (32-byte runs of a
 // channel at 1024), which costs less than a second pass. false: no variant (C > 2048).
 bool block_map_fwd(const BlockArgs& a, hipStream_t s, hipError_t* e) {

@@ -7,8 +7,8 @@ namespace dcn {
 // registers beside the rows (8192 x 1024 bf16: 37 us; 75 us with 16 channels a lane, 83 us
 // with four waves per SIMD). Few channels take fewer lanes (64 x 3136 x 32 bf16 64 us on 16 lanes a
 // row, 28 on 4; fp32 64, 41). Above 4096 channels the parameters' sums take a pass of their own
-// (us, one pass with its spills against two: bf16 2048 x 5120 92, 68, 1024 x 8192 65, 55,
-// 512 x 16384 253, 83; fp32 188, 118, 130, 99, 357, 171; the first pass prefetches in bf16, 68
+// (us, one pass with its spills against two: bf16 2048 x 5120 92, 66, 1024 x 8192 65, 57,
+// 512 x 16384 253, 91; fp32 188, 118, 130, 101, 357, 182; the first pass prefetches in bf16, 68
 // against 86, and not in fp32, 118 against 125), save beside a full gate in bf16 up to 8192, which
 // adds a tensor to the second pass and spares the gate's sums in the first (76, 90 and 62, 72).
 // false: no variant.

@@ -6,8 +6,8 @@ namespace dcn {
 // Threads, lanes a row, vectors a lane, waves per SIMD, workgroups (each prefetches its next
 // rows; negative: does not). 16 channels a lane and two waves per SIMD: with four, or 32 channels
 // a lane, the registers spill (8192 x 1024 bf16: 15.8 us against 20.7 and 25.4). Above 8192
-// channels a row leaves no room for the next (512 x 16384 bf16 58 us with the prefetch, 28
-// without, fp32 103, 80; 1024 x 8192 bf16 19, 24, fp32 37, 47). Up to 128 channels fewer lanes,
+// channels a row leaves no room for the next (512 x 16384 bf16 58 us with the prefetch, 32
+// without, fp32 103, 76; 1024 x 8192 bf16 19, 24, fp32 37, 47). Up to 128 channels fewer lanes,
 // or one vector a lane: those without a channel cost more than the width saves (50176 x 64 bf16
 // 20 us on 16 lanes of two vectors, 10 on 8 of one; 200704 x 32 58, 15 on 4; 50176 x 128 20, 16 on
 // 16 of one; fp32 23, 12 and 67, 26). false: no variant.
