@@ -432,6 +432,7 @@ __global__ __launch_bounds__(NT, WPE) void block_map(BlockArgs a, Plan q) {
       if constexpr (DROP) return kept(i, e, t * a.drop.scale);
       return t;
     };
+
     float* st = a.stats && !BWD ? a.stats + (size_t)b * a.P + (t % q.tpi) * TP : nullptr;
     const bool known = BWD && a.stats;
     if (known) sums.keep(in.st);

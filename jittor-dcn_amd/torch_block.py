@@ -335,10 +335,10 @@ def block_norm(x=None, residual=None, *, gate=None, gate_act="linear", scale=Non
     no y); eps: one number, or (post, pre). gate: of x's shape, or [B, C] for one per image
     and channel, through gate_act "linear", "sigmoid" or "silu". scale, *_weight, *_bias: [C].
     drop: "element" (elements count in memory order) or "image", one draw per x[b] (stochastic
-    depth; a row of a 2-d tensor, as in dropout). Without a residual out = t; without x the operator is the pre norm alone and out is the residual. All tensors have
-    x's dtype; everything but the rounding of the results is fp32. alpha, eps and drop_p are
-    numbers: a tensor there counts with its value at the call, and one that wants a gradient is
-    refused."""
+    depth; a row of a 2-d tensor, as in dropout). Without a residual out = t; without x the
+    operator is the pre norm alone and out is the residual. All tensors have x's dtype;
+    everything but the rounding of the results is fp32. alpha, eps and drop_p are numbers: a
+    tensor there counts with its value at the call, and one that wants a gradient is refused."""
     ref = residual if x is None else x
     if ref is None:
         raise ValueError("block_norm: neither x nor a residual")
